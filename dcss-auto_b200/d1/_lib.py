@@ -8,6 +8,7 @@ ERR_BAD_ARGUMENT = 9002
 ERR_TOO_LARGE = 9003
 
 _P, _I, _U64, _F = C.c_void_p, C.c_int, C.c_uint64, C.c_float
+_I64, _D = C.c_int64, C.c_double
 # name -> argtypes; every export returns int.
 SIGNATURES = {
     'learn_state_bytes': [], 'learn_obs_size': [], 'learn_action_size': [], 'learn_out_size': [],
@@ -95,6 +96,13 @@ SIGNATURES = {
     'd1_route_observe': [_P, _I, _P, _P, _P, _P, _P, _P],
     'd1_route_compact': [_P, _I, _P, _P],
     'd1_route_memory': [_P, _I, _P, _P, _P],
+    'd1_layer_norm': [_P, _I64, _I, _I64, _I, _P, _P, _F, _P, _I64, _P, _P, _P],
+    'd1_layer_norm_parts': [_I64, _I],
+    'd1_layer_norm_backward': [_P, _I64, _P, _I64, _I, _I64, _I, _P, _P, _P, _P, _I64, _P, _P, _P, _P],
+    'd1_token_logprob': [_P, _I64, _I, _I64, _I, _P, _P, _I64, _F, _I, _P, _P, _P, _P, _P, _P],
+    'd1_token_logprob_backward': [_P, _I64, _I, _I64, _I, _P, _P, _I64, _F, _P, _P, _P, _P, _P, _I64, _P],
+    'd1_adamw_work_bytes': [],
+    'd1_adamw': [_P, _I, _I64, _I, _P, _P, _P, _P, _D, _D, _D, _D, _D, _P, _U64, _P, _P, _P],
 }
 
 _LIB = None

@@ -1,0 +1,101 @@
+"""Log-probabilities of given tokens (actions), with the distribution's entropy
+and its likeliest alternatives, and their gradient (d1_token_logprob).
+
+    r = token_logprob(logits, tokens, legal=legal, top=8)
+    dlogits = token_logprob_backward(logits, tokens, r.stats, r.entropy, dlogp, dentropy, legal=legal)
+
+logits are float32, bfloat16 or float16 [..., vocab] with one row pitch; tokens
+int64 [...], negative where a row has none. `legal` holds a bit per token, as
+the environments' legal masks do: an integer tensor [...] or [..., words], bit
+j of a row (counted from its lowest byte) for token j; a mask shared by all
+rows may be expanded. A token whose bit is clear counts for nothing, whatever
+its logit holds. The calls launch on the current stream of the logits' device
+and can be captured in a CUDA graph.
+"""
+from typing import NamedTuple
+
+import torch
+
+from ._lib import check, launch_stream, library
+from ._rows import like, matrix, on_gpu, type_of, vector
+
+MAX_TOP = 32
+
+
+class TokenLogprob(NamedTuple):
+    logp: torch.Tensor                 # float32 [...]; 0 where a row has no token, -inf where it is left out
+    entropy: torch.Tensor              # float32 [...]
+    stats: torch.Tensor                # float32 [..., 2], for the backward pass
+    top_tokens: torch.Tensor = None    # int64 [..., top], likeliest first, -1 where no token is left
+    top_logp: torch.Tensor = None      # float32 [..., top]
+
+
+def _legal(legal, lead, vocab, device):
+    """(address, row pitch in bytes) of the mask."""
+    if legal is None:
+        return None, 0
+    if legal.is_floating_point() or legal.is_complex() or legal.dtype == torch.bool:
+        raise ValueError('legal must be an integer tensor of bits')
+    if legal.shape == lead:
+        legal = legal.unsqueeze(-1)
+    if legal.shape[:-1] != lead or legal.device != device:
+        raise ValueError(f'legal {tuple(legal.shape)} on {legal.device} does not match rows {tuple(lead)} on {device}')
+    m = matrix(legal, 'legal')
+    size = m.element_size()
+    if m.shape[1] * size * 8 < vocab:
+        raise ValueError(f'legal has {m.shape[1] * size * 8} bits a row for {vocab} tokens')
+    return m.data_ptr(), m.stride(0) * size
+
+
+def _common(logits, tokens, legal, temperature):
+    dev, kind, m = on_gpu(logits, 'logits'), type_of(logits, 'logits'), matrix(logits, 'logits')
+    if not temperature > 0:
+        raise ValueError('temperature must be positive')
+    lead, (rows, vocab) = logits.shape[:-1], m.shape
+    if tokens.shape != lead:
+        raise ValueError(f'tokens {tuple(tokens.shape)} do not match rows {tuple(lead)}')
+    t = vector(tokens, rows, torch.int64, dev, 'tokens')
+    return dev, kind, m, lead, rows, vocab, t, _legal(legal, lead, vocab, dev)
+
+
+def token_logprob(logits, tokens, legal=None, temperature=1.0, top=0):
+    """TokenLogprob of softmax(logits / temperature) over the legal tokens."""
+    dev, kind, m, lead, rows, vocab, t, (bits, pitch) = _common(logits, tokens, legal, temperature)
+    if not 0 <= top <= MAX_TOP:
+        raise ValueError(f'top must be between 0 and {MAX_TOP}')
+    logp, entropy = torch.empty((2,) + lead, device=dev).unbind()
+    stats = torch.empty(lead + (2,), device=dev)
+    top_tokens = top_logp = None
+    if top:
+        top_tokens = torch.empty(lead + (top,), dtype=torch.int64, device=dev)
+        top_logp = torch.empty(lead + (top,), device=dev)
+    check(library().d1_token_logprob(m.data_ptr(), m.stride(0), kind, rows, vocab, t, bits, pitch, temperature, top,
+                                     logp.data_ptr(), entropy.data_ptr(), stats.data_ptr(),
+                                     top_tokens.data_ptr() if top else None, top_logp.data_ptr() if top else None,
+                                     launch_stream(dev)), 'd1_token_logprob')
+    return TokenLogprob(logp, entropy, stats, top_tokens, top_logp)
+
+
+def token_logprob_backward(logits, tokens, stats, entropy, dlogp, dentropy=None, legal=None, temperature=1.0,
+                           out=None):
+    """dlogits (the logits' shape and type) from the gradients of logp and of the
+    entropy (float32 of the rows' shape; None: zero). `out` may be the logits."""
+    dev, kind, m, lead, rows, vocab, t, (bits, pitch) = _common(logits, tokens, legal, temperature)
+    f32 = torch.float32
+    s = vector(stats, 2 * rows, f32, dev, 'stats')
+    if dentropy is not None and entropy is None:
+        raise ValueError('dentropy needs the entropy')
+    h, dl = vector(entropy, rows, f32, dev, 'entropy'), vector(dlogp, rows, f32, dev, 'dlogp')
+    dh = vector(dentropy, rows, f32, dev, 'dentropy')
+    if out is None:
+        d = out = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+        ldd = vocab
+    else:
+        d = like(out, logits, 'out')
+        ldd = d.stride(0)
+        if out.data_ptr() == logits.data_ptr() and rows > 1 and ldd != m.stride(0):
+            raise ValueError('out shares its first element with logits but not its row pitch')
+    check(library().d1_token_logprob_backward(m.data_ptr(), m.stride(0), kind, rows, vocab, t, bits, pitch,
+                                              temperature, s, h, dl, dh, d.data_ptr(), ldd, launch_stream(dev)),
+          'd1_token_logprob_backward')
+    return out

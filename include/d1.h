@@ -642,6 +642,94 @@ int d1_peer_error(void);
 int d1_ppo_gather_x(const void *obs, int F, const int64_t *idx, int n, void *x, int ldx, int ones_col,
                     void *stream);
 
+/* ======================================================================
+ * Operators for training policies with named parameter tensors: layer norm,
+ * token log-probabilities and AdamW. No counterpart in the reference.
+ * Rows are given by a base, a pitch in elements and a type; the last
+ * dimension is contiguous. Any pitch and any alignment of the element type is
+ * taken (16-byte aligned rows are the fast case). Sums are held in fp32; a
+ * 16-bit result is rounded once, to nearest.
+ * ====================================================================== */
+#define D1_TYPE_F32 0
+#define D1_TYPE_BF16 1
+#define D1_TYPE_F16 2
+
+/* y[r] = (x[r] - mean_r) rstd_r weight + bias, with rstd_r = 1 / sqrt(var_r + eps)
+ * over the n elements of row r. weight and bias are f32 [n] (NULL: 1 and 0);
+ * mean and rstd (f32 [rows], NULL: not wanted) are what the backward pass takes.
+ * x and y have type `type`; y may be x itself. eps >= 0, n >= 1. */
+int d1_layer_norm(const void *x, int64_t ldx, int type, int64_t rows, int n, const float *weight, const float *bias,
+                  float eps, void *y, int64_t ldy, float *mean, float *rstd, void *stream);
+/* Number of partial sums d1_layer_norm_backward makes for each weight: its
+ * `work` holds 2 * n floats for each. */
+int d1_layer_norm_parts(int64_t rows, int n);
+/* The gradients of d1_layer_norm from dy (type `type`): dx (same type; NULL: not
+ * wanted), dweight and dbias (f32 [n]; NULL: not wanted). work: f32
+ * [d1_layer_norm_parts(rows, n) * 2 * n], 16-byte aligned, needed for dweight or
+ * dbias. The partial sums are added in a fixed order: the same inputs give the
+ * same bits. rows == 0 gives zero dweight and dbias. dx overlaps no input. */
+int d1_layer_norm_backward(const void *dy, int64_t lddy, const void *x, int64_t ldx, int type, int64_t rows, int n,
+                           const float *weight, const float *mean, const float *rstd, void *dx, int64_t lddx,
+                           float *dweight, float *dbias, float *work, void *stream);
+
+/* The log-probabilities of given tokens under softmax(logits / temperature), row
+ * by row: logp[r] of token tokens[r] (0 for a negative token, a row that has
+ * none; NaN for a token >= vocab), the distribution's entropy[r] and
+ * stats[r] = (largest logit, log of the sum of e^((logit - largest) /
+ * temperature)), which the backward pass takes. legal: bit j & 7 of byte
+ * j >> 3 of row r (at r * ldlegal bytes; ldlegal 0: one mask for all rows) says
+ * whether token j may be drawn; NULL: all may. A token without its bit is left
+ * out whatever its logit holds (a NaN too), and so is a logit of -inf: its
+ * log-probability is -inf. A row with nothing left has logp -inf, entropy 0 and
+ * stats (-inf, -inf). top (0..32) > 0: top_tokens[r][k] and top_logp[r][k] are
+ * the k-th likeliest token (the lower one first where logits are equal) and its
+ * log-probability, -1 and -inf where no token is left. Any of logp, entropy and
+ * stats may be NULL. */
+int d1_token_logprob(const void *logits, int64_t ld, int type, int64_t rows, int vocab, const int64_t *tokens,
+                     const void *legal, int64_t ldlegal, float temperature, int top, float *logp, float *entropy,
+                     float *stats, int64_t *top_tokens, float *top_logp, void *stream);
+/* dlogits (type `type`) from dlogp and dentropy (f32 [rows], NULL: zero), with
+ * the forward pass' logits, tokens, legal, temperature, stats and entropy
+ * (entropy may be NULL when dentropy is):
+ *   dlogits_j = ([j == token] dlogp - p_j (dlogp + dentropy (log p_j + entropy))) / temperature
+ * A token that is left out gets 0; a row without a token, or whose token is left
+ * out, has no dlogp; a row with nothing left gets zeros. dlogits may be logits
+ * itself (same pitch) and overlaps nothing else. */
+int d1_token_logprob_backward(const void *logits, int64_t ld, int type, int64_t rows, int vocab,
+                              const int64_t *tokens, const void *legal, int64_t ldlegal, float temperature,
+                              const float *stats, const float *entropy, const float *dlogp, const float *dentropy,
+                              void *dlogits, int64_t ldd, void *stream);
+
+/* One parameter tensor of d1_adamw: `count` fp32 elements at param, its gradient
+ * (fp32 or bf16), the bf16 compute copy that each step refreshes (or NULL),
+ * decay = its weight decay. first_block = number of 128-element blocks of the
+ * tensors before it (each has (count + 127) / 128). */
+typedef struct {
+    float *param;
+    const void *grad;
+    void *copy;
+    int64_t count, first_block;
+    double decay;
+    int grad_type, reserved;
+} D1AdamWTensor;
+/* Bytes of d1_adamw's work buffer, which the caller zeroes once. */
+int d1_adamw_work_bytes(void);
+/* One AdamW step over all tensors (`tensors`: a DEVICE array of ntensors, whose
+ * blocks come to nblocks) in one launch, or two with clipping:
+ *   g = grad * min(1, max_norm / (norm + 1e-6))   (norm over all tensors; max_norm <= 0: no clipping)
+ *   m = beta1 m + (1 - beta1) g,   v = beta2 v + (1 - beta2) g^2
+ *   p = p (1 - lr decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * with t = *step + 1 (device), which the call stores back. The moments are flat
+ * over the blocks, zero at the start: state_bits 32: m and v f32 [nblocks * 128];
+ * state_bits 8: m e4m3 and v e5m2 codes [nblocks * 128] times the block scales
+ * m_scale and v_scale (f32 [nblocks], powers of two), rounded stochastically,
+ * unbiased in m and in v, by 16 bits per element that depend on (seed, step,
+ * element) alone. m, v and work are 16-byte aligned. norm goes to *grad_norm
+ * (unless NULL) when clipping. Calls that share state or work must not overlap. */
+int d1_adamw(const D1AdamWTensor *tensors, int ntensors, int64_t nblocks, int state_bits, void *m, void *v,
+             float *m_scale, float *v_scale, double lr, double beta1, double beta2, double eps, double max_norm,
+             int64_t *step, uint64_t seed, void *work, float *grad_norm, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
