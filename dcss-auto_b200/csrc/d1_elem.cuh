@@ -27,6 +27,9 @@ __device__ __forceinline__ float warp_sum(float x) {
     return x;
 }
 
+inline bool element_aligned(const void *p, int type) {
+    return (reinterpret_cast<uintptr_t>(p) & (type == D1_TYPE_F32 ? 3 : 1)) == 0;
+}
 inline bool type_ok(int type) { return type == D1_TYPE_F32 || type == D1_TYPE_BF16 || type == D1_TYPE_F16; }
 
 }  // namespace d1

@@ -50,3 +50,13 @@ def on_gpu(t, name):
     if not t.is_cuda:
         raise ValueError(f'{name} must be on a CUDA device (there is no CPU path)')
     return t.device
+
+
+def apart(a, b, name, other):
+    """Refuses two matrices whose spans of memory overlap."""
+    ends = []
+    for t in (a, b):
+        span = ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size() if t.shape[0] else 0
+        ends.append((t.data_ptr(), t.data_ptr() + span))
+    if ends[0][0] < ends[1][1] and ends[1][0] < ends[0][1]:
+        raise ValueError(f'{name} overlaps {other}')

@@ -12,7 +12,7 @@ in a CUDA graph.
 import torch
 
 from ._lib import check, launch_stream, library
-from ._rows import like, matrix, on_gpu, type_of, vector
+from ._rows import apart, like, matrix, on_gpu, type_of, vector
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, out=None):
@@ -50,6 +50,8 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, out=None):
     else:
         dx = like(out, x, 'out')
         lddx = dx.stride(0)
+        apart(dx, m, 'out', 'x')
+        apart(dx, d, 'out', 'dy')
     lib = library()
     dweight, dbias = torch.empty((2, n), device=dev).unbind()
     work = torch.empty(lib.d1_layer_norm_parts(rows, n) * 2 * n, device=dev)

@@ -17,7 +17,7 @@ from typing import NamedTuple
 import torch
 
 from ._lib import check, launch_stream, library
-from ._rows import like, matrix, on_gpu, type_of, vector
+from ._rows import apart, like, matrix, on_gpu, type_of, vector
 
 MAX_TOP = 32
 
@@ -79,7 +79,8 @@ def token_logprob(logits, tokens, legal=None, temperature=1.0, top=0):
 def token_logprob_backward(logits, tokens, stats, entropy, dlogp, dentropy=None, legal=None, temperature=1.0,
                            out=None):
     """dlogits (the logits' shape and type) from the gradients of logp and of the
-    entropy (float32 of the rows' shape; None: zero). `out` may be the logits."""
+    entropy (float32 of the rows' shape; None: zero), written to `out` when given,
+    which overlaps no input."""
     dev, kind, m, lead, rows, vocab, t, (bits, pitch) = _common(logits, tokens, legal, temperature)
     f32 = torch.float32
     s = vector(stats, 2 * rows, f32, dev, 'stats')
@@ -93,8 +94,7 @@ def token_logprob_backward(logits, tokens, stats, entropy, dlogp, dentropy=None,
     else:
         d = like(out, logits, 'out')
         ldd = d.stride(0)
-        if out.data_ptr() == logits.data_ptr() and rows > 1 and ldd != m.stride(0):
-            raise ValueError('out shares its first element with logits but not its row pitch')
+        apart(d, m, 'out', 'logits')
     check(library().d1_token_logprob_backward(m.data_ptr(), m.stride(0), kind, rows, vocab, t, bits, pitch,
                                               temperature, s, h, dl, dh, d.data_ptr(), ldd, launch_stream(dev)),
           'd1_token_logprob_backward')
