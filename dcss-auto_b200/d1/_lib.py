@@ -153,6 +153,16 @@ def launch_stream(device):
     return torch.cuda.current_stream(dev).cuda_stream
 
 
+def stream_of(t):
+    """launch_stream for a CUDA tensor, at the cost of a microsecond less: the
+    row operators are called on batches small enough for that to count."""
+    import torch
+    index = t.get_device()
+    if torch._C._cuda_getDevice() != index:
+        return launch_stream(t.device)  # raises
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def check(code, what='libd1 call'):
     if code:
         raise D1Error(f'{what} failed with error {code}')

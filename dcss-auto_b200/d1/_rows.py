@@ -46,6 +46,22 @@ def like(t, of, name):
     return matrix(t, name)
 
 
+_F32 = {}
+
+
+def empty_f32(device, shape):
+    """torch.empty of float32 on `device`, by the cheapest route (new_empty of a kept tensor)."""
+    kept = _F32.get(device)
+    if kept is None:
+        kept = _F32[device] = torch.empty(0, device=device)
+    return kept.new_empty(shape)
+
+
+def empty_like(t):
+    """A contiguous tensor of t's shape, type and device."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def on_gpu(t, name):
     if not t.is_cuda:
         raise ValueError(f'{name} must be on a CUDA device (there is no CPU path)')

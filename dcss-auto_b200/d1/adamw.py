@@ -20,7 +20,7 @@ import ctypes as C
 
 import torch
 
-from ._lib import check, launch_stream, library
+from ._lib import check, library, stream_of
 from ._rows import on_gpu
 
 BLOCK = 128
@@ -99,7 +99,7 @@ class AdamW:
                                 None if self.v_scale is None else self.v_scale.data_ptr(),
                                 self.lr if lr is None else lr, self.betas[0], self.betas[1], self.eps, self.max_norm,
                                 self.step_dev.data_ptr(), self.seed, self._work.data_ptr(), self.grad_norm.data_ptr(),
-                                launch_stream(self.device)), 'd1_adamw')
+                                stream_of(self.m)), 'd1_adamw')
 
     def moments(self, i):
         """(m, v) of parameter i as float32 in its shape (decoded copies where the state is in 8 bits)."""

@@ -11,8 +11,8 @@ in a CUDA graph.
 """
 import torch
 
-from ._lib import check, launch_stream, library
-from ._rows import apart, like, matrix, on_gpu, type_of, vector
+from ._lib import check, library, stream_of
+from ._rows import apart, empty_f32, empty_like, like, matrix, on_gpu, type_of, vector
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, out=None):
@@ -24,14 +24,15 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, out=None):
         raise ValueError('eps must not be negative')
     w, b = vector(weight, n, torch.float32, dev, 'weight'), vector(bias, n, torch.float32, dev, 'bias')
     if out is None:
-        y = out = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        y = out = empty_like(x)
         ldy = n
     else:
         y = like(out, x, 'out')
         ldy = y.stride(0)
-    mean, rstd = torch.empty((2,) + x.shape[:-1], device=dev).unbind()
+    lead = x.shape[:-1]
+    mean, rstd = empty_f32(dev, lead), empty_f32(dev, lead)
     check(library().d1_layer_norm(m.data_ptr(), m.stride(0), kind, rows, n, w, b, eps, y.data_ptr(), ldy,
-                                  mean.data_ptr(), rstd.data_ptr(), launch_stream(dev)), 'd1_layer_norm')
+                                  mean.data_ptr(), rstd.data_ptr(), stream_of(x)), 'd1_layer_norm')
     return out, mean, rstd
 
 
@@ -45,7 +46,7 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, out=None):
     w = vector(weight, n, torch.float32, dev, 'weight')
     mu, rs = vector(mean, rows, torch.float32, dev, 'mean'), vector(rstd, rows, torch.float32, dev, 'rstd')
     if out is None:
-        dx = out = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        dx = out = empty_like(x)
         lddx = n
     else:
         dx = like(out, x, 'out')
@@ -53,9 +54,9 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, out=None):
         apart(dx, m, 'out', 'x')
         apart(dx, d, 'out', 'dy')
     lib = library()
-    dweight, dbias = torch.empty((2, n), device=dev).unbind()
-    work = torch.empty(lib.d1_layer_norm_parts(rows, n) * 2 * n, device=dev)
+    dweight, dbias = empty_f32(dev, n), empty_f32(dev, n)
+    work = empty_f32(dev, lib.d1_layer_norm_parts(rows, n) * 2 * n)
     check(lib.d1_layer_norm_backward(d.data_ptr(), d.stride(0), m.data_ptr(), m.stride(0), kind, rows, n, w, mu, rs,
                                      dx.data_ptr(), lddx, dweight.data_ptr(), dbias.data_ptr(), work.data_ptr(),
-                                     launch_stream(dev)), 'd1_layer_norm_backward')
+                                     stream_of(x)), 'd1_layer_norm_backward')
     return out, dweight, dbias

@@ -16,8 +16,8 @@ from typing import NamedTuple
 
 import torch
 
-from ._lib import check, launch_stream, library
-from ._rows import apart, like, matrix, on_gpu, type_of, vector
+from ._lib import check, library, stream_of
+from ._rows import apart, empty_f32, empty_like, like, matrix, on_gpu, type_of, vector
 
 MAX_TOP = 32
 
@@ -63,16 +63,15 @@ def token_logprob(logits, tokens, legal=None, temperature=1.0, top=0):
     dev, kind, m, lead, rows, vocab, t, (bits, pitch) = _common(logits, tokens, legal, temperature)
     if not 0 <= top <= MAX_TOP:
         raise ValueError(f'top must be between 0 and {MAX_TOP}')
-    logp, entropy = torch.empty((2,) + lead, device=dev).unbind()
-    stats = torch.empty(lead + (2,), device=dev)
+    logp, entropy, stats = empty_f32(dev, lead), empty_f32(dev, lead), empty_f32(dev, lead + (2,))
     top_tokens = top_logp = None
     if top:
-        top_tokens = torch.empty(lead + (top,), dtype=torch.int64, device=dev)
-        top_logp = torch.empty(lead + (top,), device=dev)
+        top_tokens = tokens.new_empty(lead + (top,))
+        top_logp = empty_f32(dev, lead + (top,))
     check(library().d1_token_logprob(m.data_ptr(), m.stride(0), kind, rows, vocab, t, bits, pitch, temperature, top,
                                      logp.data_ptr(), entropy.data_ptr(), stats.data_ptr(),
                                      top_tokens.data_ptr() if top else None, top_logp.data_ptr() if top else None,
-                                     launch_stream(dev)), 'd1_token_logprob')
+                                     stream_of(logits)), 'd1_token_logprob')
     return TokenLogprob(logp, entropy, stats, top_tokens, top_logp)
 
 
@@ -89,13 +88,13 @@ def token_logprob_backward(logits, tokens, stats, entropy, dlogp, dentropy=None,
     h, dl = vector(entropy, rows, f32, dev, 'entropy'), vector(dlogp, rows, f32, dev, 'dlogp')
     dh = vector(dentropy, rows, f32, dev, 'dentropy')
     if out is None:
-        d = out = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+        d = out = empty_like(logits)
         ldd = vocab
     else:
         d = like(out, logits, 'out')
         ldd = d.stride(0)
         apart(d, m, 'out', 'logits')
     check(library().d1_token_logprob_backward(m.data_ptr(), m.stride(0), kind, rows, vocab, t, bits, pitch,
-                                              temperature, s, h, dl, dh, d.data_ptr(), ldd, launch_stream(dev)),
+                                              temperature, s, h, dl, dh, d.data_ptr(), ldd, stream_of(logits)),
           'd1_token_logprob_backward')
     return out
