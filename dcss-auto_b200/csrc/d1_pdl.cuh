@@ -14,6 +14,9 @@ namespace d1 {
 
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// Lets the next kernel of the stream start (up to its pdl_wait()) from here on.
+__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // A launch configuration whose single attribute allows the programmatic
 // overlap; `attr` must outlive the launch call.
 inline cudaLaunchConfig_t pdl_config(dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
