@@ -23,6 +23,8 @@
 // or a NaN gets a NaN scale.
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "d1_common.cuh"
 #include "d1_elem.cuh"
 #include "d1_pdl.cuh"
@@ -30,22 +32,26 @@
 namespace d1 {
 namespace adamw {
 
-__device__ __forceinline__ int64_t imin64(int64_t a, int64_t b) { return a < b ? a : b; }
+constexpr int BLOCK = 128, THREADS = 256, WARPS = THREADS / 32, SMS = 148, NORM_GRID = SMS * 8;
 
-constexpr int BLOCK = 128, THREADS = 256, WARPS = THREADS / 32, GRID = 148 * 4;
+// Below this eps (2^-63, the root of the smallest normal fp32 number) the square
+// root of a subnormal v, which is taken as zero, would show.
+constexpr double EPS_FLOOR = 1.0842021724855044e-19;
 
 struct Args {
     const D1AdamWTensor *tensors;
     int ntensors;
-    int64_t nblocks;
+    int nblocks;
+    int tile;  // blocks that a warp takes at a time: 8, handed out, or 2 at fixed places
     void *m, *v;
     float *m_scale, *v_scale;
     double lr, beta1, beta2, log2_beta1, log2_beta2;
     float b1, c1, b2, c2, eps, max_norm;
     int64_t *step;
     uint64_t seed;
-    double *partials;       // GRID sums of squares, then the arrival count
-    unsigned *arrived;
+    double *partials;            // the norm's sums, one for each of its blocks
+    unsigned *arrived, *taken;   // blocks that are done, tiles handed out beyond the first of each warp; both left at 0
+    int norm_parts;
     float *grad_norm;
 };
 
@@ -53,15 +59,15 @@ struct Args {
 // addresses, moved so that element i of all blocks is at index i.
 struct Place {
     uintptr_t param, grad, copy;  // copy 0: none
-    int64_t stop, end;            // first element past the tensor; first block past its blocks
+    int full, rest;               // first block that is not whole, and how many elements it has
+    int vectors, end;             // first block that is not whole or not aligned for vectors of four; first block past the tensor
     float keep;                   // 1 - lr decay
     int grad_shift;               // 2: fp32, 1: bf16
-    bool wide;                    // every address allows vectors of four
 };
 
 // The place of block `b`: the last tensor that starts at or before it, found by
 // the whole warp (32 tensors looked at in one round trip).
-__device__ __forceinline__ Place locate(const Args &a, int64_t b) {
+__device__ __forceinline__ Place locate(const Args &a, int b) {
     const int lane = threadIdx.x & 31;
     int lo = 0, hi = a.ntensors;
     while (hi - lo > 1) {
@@ -77,12 +83,13 @@ __device__ __forceinline__ Place locate(const Args &a, int64_t b) {
     p.param = reinterpret_cast<uintptr_t>(t.param) - 4 * start;
     p.grad = reinterpret_cast<uintptr_t>(t.grad) - (start << p.grad_shift);
     p.copy = t.copy ? reinterpret_cast<uintptr_t>(t.copy) - 2 * start : 0;
-    p.stop = start + t.count;
-    p.end = lo + 1 < a.ntensors ? a.tensors[lo + 1].first_block : a.nblocks;
+    p.full = (int)(t.first_block + t.count / BLOCK);
+    p.rest = (int)(t.count % BLOCK);
+    p.end = lo + 1 < a.ntensors ? (int)a.tensors[lo + 1].first_block : a.nblocks;
     p.keep = (float)(1. - a.lr * t.decay);
     const uintptr_t odd = (reinterpret_cast<uintptr_t>(t.param) & 15) | (reinterpret_cast<uintptr_t>(t.copy) & 7) |
                           (reinterpret_cast<uintptr_t>(t.grad) & ((4 << p.grad_shift) - 1));
-    p.wide = odd == 0;
+    p.vectors = odd == 0 ? p.full : 0;
     return p;
 }
 
@@ -117,44 +124,36 @@ template <bool WIDE> __device__ __forceinline__ void load_grad(const Place &t, i
         load4<__nv_bfloat16, WIDE>(reinterpret_cast<const __nv_bfloat16 *>(at), left, g);
 }
 
-// Blocks [lo, hi) of block `blockIdx.x`'s share; its warps take pairs of blocks
-// in turn. f(place, b, two): blocks b and b + 1 whole and in vectors of one
-// tensor (two), or block b alone.
-template <class F> __device__ __forceinline__ void for_blocks(const Args &a, F f) {
-    const int64_t lo = a.nblocks * blockIdx.x / gridDim.x, hi = a.nblocks * (blockIdx.x + 1) / gridDim.x;
-    int64_t b = lo + 2 * (threadIdx.x >> 5);
-    if (b >= hi) return;
-    Place p = locate(a, b);
-    for (; b < hi; b += 2 * WARPS) {
-        if (b >= p.end) p = locate(a, b);
-        if (b + 1 < hi && p.wide && (b + 2) * BLOCK <= p.stop) {
-            f(p, b, true);
-        } else {
-            f(p, b, false);
-            if (b + 1 < hi) {
-                if (b + 1 >= p.end) p = locate(a, b + 1);
-                f(p, b + 1, false);
-            }
-        }
-    }
+// Elements of block b from the lane's first on, up to four (b lies in the place's tensor).
+__device__ __forceinline__ int left_at(const Place &p, int b) {
+    return b < p.full ? 4 : imin(p.rest - 4 * (int)(threadIdx.x & 31), 4);
 }
+// Whether blocks b and b + 1 are whole and aligned (b or an earlier block lies in the place's tensor).
+__device__ __forceinline__ bool pair_at(const Place &p, int b) { return b + 2 <= p.vectors; }
 
 __global__ void __launch_bounds__(THREADS) norm_kernel(Args a) {
     __shared__ double part[WARPS];
     pdl_launch();
     const int lane = threadIdx.x & 31;
     float s = 0.f;
-    for_blocks(a, [&](const Place &t, int64_t b, bool two) {
-        const int64_t i = b * BLOCK + 4 * lane;
-        float g[4], h[4] = {0.f, 0.f, 0.f, 0.f};
-        if (two) {
-            load_grad<true>(t, i, 4, g);
-            load_grad<true>(t, i + BLOCK, 4, h);
+    // a fixed share of the blocks, for a fixed order of the sum
+    const int lo = (int)((int64_t)a.nblocks * blockIdx.x / gridDim.x), hi = (int)((int64_t)a.nblocks * (blockIdx.x + 1) / gridDim.x);
+    Place t;
+    t.end = 0;
+    for (int b = lo + 2 * (threadIdx.x >> 5); b < hi; b += 2 * WARPS) {
+        float g[2][4] = {};
+        if (b >= t.end) t = locate(a, b);
+        if (b + 1 < hi && pair_at(t, b)) {
+            load_grad<true>(t, (int64_t)b * BLOCK + 4 * lane, 4, g[0]);
+            load_grad<true>(t, (int64_t)(b + 1) * BLOCK + 4 * lane, 4, g[1]);
         } else
-            load_grad<false>(t, i, (int)imin64(t.stop - i, 4), g);
-        s += (g[0] * g[0] + g[1] * g[1]) + (g[2] * g[2] + g[3] * g[3]);
-        s += (h[0] * h[0] + h[1] * h[1]) + (h[2] * h[2] + h[3] * h[3]);
-    });
+            for (int c = b; c < hi && c < b + 2; c++) {
+                if (c >= t.end) t = locate(a, c);
+                load_grad<false>(t, (int64_t)c * BLOCK + 4 * lane, left_at(t, c), g[c - b]);
+            }
+#pragma unroll
+        for (int k = 0; k < 2; k++) s += (g[k][0] * g[k][0] + g[k][1] * g[k][1]) + (g[k][2] * g[k][2] + g[k][3] * g[k][3]);
+    }
     double d = s;
 #pragma unroll
     for (int o = 16; o; o >>= 1) d += __shfl_xor_sync(FULL, d, o);
@@ -167,13 +166,6 @@ __global__ void __launch_bounds__(THREADS) norm_kernel(Args a) {
     }
 }
 
-// 2^e for -149 <= e <= 127.
-__device__ __forceinline__ float pow2(int e) { return e >= -126 ? __int_as_float((e + 127) << 23) : __int_as_float(1 << (e + 149)); }
-
-// The block's exponent for a largest magnitude `top` (its bits), never below
-// -100; the scale then is 2^(exponent - field).
-__device__ __forceinline__ int block_exponent(uint32_t top) { return imax((int)(top >> 23) - 127, -100); }
-
 __device__ __forceinline__ float max_nan(float a, float b) {
     float y;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
@@ -181,134 +173,222 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 __device__ __forceinline__ float sqrt_approx(float x) {
     float y;
-    asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ float rcp_approx(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 
 // Four codes as numbers (exact: both formats are within fp16), before their scale.
-template <bool E4M3> __device__ __forceinline__ void decode4(uint32_t codes, float (&x)[4]) {
+template <bool E4M3> __device__ __forceinline__ void decode4(uint32_t codes, float2 (&x)[2]) {
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-        const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes >> (16 * h)), E4M3 ? __NV_E4M3 : __NV_E5M2);
-        const float2 f = __half22float2(__half2(r));
-        x[2 * h] = f.x;
-        x[2 * h + 1] = f.y;
-    }
+    for (int h = 0; h < 2; h++)
+        x[h] = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes >> (16 * h)), E4M3 ? __NV_E4M3 : __NV_E5M2)));
 }
 
-// x times a power of two that brings the block's top to `field` of an 8-bit
-// float of bias `bias`, at the exponent where an fp32 number's bits from
-// position 23 - mantissa on are that float's. One product where the factor is a
-// normal number, else two: both exact but for the last, subnormal rounding.
-__device__ __forceinline__ void code_factors(int exponent, int field, int bias, float &first, float &second) {
-    const int e = field - exponent + bias - 127;
-    first = e >= -126 ? pow2(e) : pow2(field - exponent);
-    second = e >= -126 ? 1.f : pow2(bias - 127);
-}
+// A block's scale is 2^(E - FIELD), with E the exponent of its largest
+// magnitude (not below -100). A magnitude times 2^(FIELD - E + BIAS - 127) is an
+// fp32 number whose bits from position 23 - mantissa on are its 8-bit code: it
+// is held at the exponents where both formats have the same field, subnormal
+// where the code is. `top`: the largest magnitude's bits; factor 2 is 1 unless
+// the first alone would not be a normal number.
+template <int FIELD, int BIAS> struct Scale {
+    float first, second, scale;
+    __device__ __forceinline__ explicit Scale(uint32_t top) {
+        const int e = imax((int)(top & 0x7f800000u), 27 << 23);  // E + 127, in place
+        const int bits = ((FIELD + BIAS + 127) << 23) - e;
+        first = __int_as_float(bits);
+        second = 1.f;
+        scale = __int_as_float(e - (FIELD << 23));
+        if (bits < 1 << 23) {
+            const bool bad = top >= 0x7f800000u;  // an infinity or a NaN in the block
+            first = bad ? 0.f : __int_as_float(((FIELD + 127) << 23) - e + (127 << 23));
+            second = __int_as_float(BIAS << 23);
+            if (bad) scale = __int_as_float(0x7fc00000);
+        }
+    }
+};
 
 struct Step {
     float clip, rate, inv_bc2, eps, b1, c1, b2, c2;
     uint64_t key;
 };
 
-// One block of 128: p and both moments, four elements a lane.
+// One block of 128, four elements a lane; the gradient as it is stored.
 template <int BITS> struct Held {
-    float p[4], g[4];
-    float m32[BITS == 32 ? 4 : 1], v32[BITS == 32 ? 4 : 1];
-    uint32_t mc, vc;
+    float4 p;
+    uint4 g;
+    typename std::conditional<BITS == 32, float4, uint32_t>::type m, v;
     float ms, vs;
 };
+
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
+// The step of one block, stored where its elements belong. at: the lane's first element.
 template <int BITS, bool WIDE>
-__device__ __forceinline__ void load_block(const Args &a, const Place &t, int64_t b, Held<BITS> &h) {
+__device__ __forceinline__ void step_block(const Args &a, const Step &s, const Place &t, int b, const Held<BITS> &h) {
     const int lane = threadIdx.x & 31;
-    const int64_t at = b * BLOCK + 4 * lane;
-    const int left = WIDE ? 4 : (int)imin64(t.stop - at, 4);
-    load4<float, WIDE>(reinterpret_cast<const float *>(t.param) + at, left, h.p);
-    load_grad<WIDE>(t, at, left, h.g);
+    const int64_t at = (int64_t)b * BLOCK + 4 * lane;
+    const int left = WIDE ? 4 : left_at(t, b);
+    float2 m[2], v[2];
     if constexpr (BITS == 32) {
-        load4<float, true>((const float *)a.m + at, 4, h.m32);
-        load4<float, true>((const float *)a.v + at, 4, h.v32);
+        m[0] = make_float2(h.m.x, h.m.y), m[1] = make_float2(h.m.z, h.m.w);
+        v[0] = make_float2(h.v.x, h.v.y), v[1] = make_float2(h.v.z, h.v.w);
     } else {
-        h.mc = ((const uint32_t *)a.m)[at >> 2];
-        h.vc = ((const uint32_t *)a.v)[at >> 2];
-        h.ms = a.m_scale[b];
-        h.vs = a.v_scale[b];
+        decode4<true>(h.m, m);
+        decode4<false>(h.v, v);
+#pragma unroll
+        for (int k = 0; k < 2; k++) m[k] = __fmul2_rn(m[k], both(h.ms)), v[k] = __fmul2_rn(v[k], both(h.vs));
     }
-}
-template <int BITS, bool WIDE>
-__device__ __forceinline__ void step_block(const Args &a, const Step &s, const Place &t, int64_t b, Held<BITS> &h) {
-    const int lane = threadIdx.x & 31;
-    const int64_t at = b * BLOCK + 4 * lane;
-    const int left = WIDE ? 4 : (int)imin64(t.stop - at, 4);
-    float m[4], v[4];
+    float2 g2[2];
+    if (t.grad_shift == 2) {
+        g2[0] = make_float2(__uint_as_float(h.g.x), __uint_as_float(h.g.y));
+        g2[1] = make_float2(__uint_as_float(h.g.z), __uint_as_float(h.g.w));
+    } else {
+        g2[0] = make_float2(__uint_as_float(h.g.x << 16), __uint_as_float(h.g.x & 0xffff0000u));
+        g2[1] = make_float2(__uint_as_float(h.g.y << 16), __uint_as_float(h.g.y & 0xffff0000u));
+    }
+    const float2 p2[2] = {make_float2(h.p.x, h.p.y), make_float2(h.p.z, h.p.w)};
+    float p[4];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const float2 g = __fmul2_rn(g2[k], both(s.clip)), kept = __fmul2_rn(p2[k], both(t.keep));
+        m[k] = __fadd2_rn(__fmul2_rn(m[k], both(s.b1)), __fmul2_rn(g, both(s.c1)));
+        v[k] = __fadd2_rn(__fmul2_rn(v[k], both(s.b2)), __fmul2_rn(__fmul2_rn(g, g), both(s.c2)));
+        const float2 d = __ffma2_rn(make_float2(sqrt_approx(v[k].x), sqrt_approx(v[k].y)), both(s.inv_bc2), both(s.eps));
+        const float2 ratio = __fmul2_rn(m[k], make_float2(rcp_approx(d.x), rcp_approx(d.y)));
+        const float2 new_p = __ffma2_rn(both(-s.rate), ratio, kept);
+        p[2 * k] = new_p.x;
+        p[2 * k + 1] = new_p.y;
+    }
+    store4<float, WIDE>(reinterpret_cast<float *>(t.param) + at, left, p);
+    if (t.copy) store4<__nv_bfloat16, WIDE>(reinterpret_cast<__nv_bfloat16 *>(t.copy) + at, left, p);
     if constexpr (BITS == 32) {
-#pragma unroll
-        for (int k = 0; k < 4; k++) m[k] = h.m32[k], v[k] = h.v32[k];
+        *reinterpret_cast<float4 *>((float *)a.m + at) = make_float4(m[0].x, m[0].y, m[1].x, m[1].y);
+        *reinterpret_cast<float4 *>((float *)a.v + at) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
     } else {
-        decode4<true>(h.mc, m);
-        decode4<false>(h.vc, v);
+        const float mtop = max_nan(max_nan(fabsf(m[0].x), fabsf(m[0].y)), max_nan(fabsf(m[1].x), fabsf(m[1].y)));
+        const float vtop = max_nan(max_nan(v[0].x, v[0].y), max_nan(v[1].x, v[1].y));
+        const Scale<7, 7> sm(__reduce_max_sync(FULL, __float_as_uint(mtop)));
+        const Scale<14, 15> sv(__reduce_max_sync(FULL, __float_as_uint(vtop)));
+        const uint64_t word = mix64(s.key + ((uint64_t)b * 32 + lane));
+        float ym[4], yv[4];
 #pragma unroll
-        for (int k = 0; k < 4; k++) m[k] *= h.ms, v[k] *= h.vs;
-    }
-    float mtop = 0.f, vtop = 0.f;
+        for (int k = 0; k < 4; k++) {
+            ym[k] = __fmul_rn(fabsf(k & 1 ? m[k / 2].y : m[k / 2].x), sm.first);
+            yv[k] = __fmul_rn(k & 1 ? v[k / 2].y : v[k / 2].x, sv.first);
+        }
+        if (sm.second != 1.f || sv.second != 1.f) {
 #pragma unroll
-    for (int k = 0; k < 4; k++) {
-        const float g = __fmul_rn(h.g[k], s.clip);
-        m[k] = __fadd_rn(__fmul_rn(m[k], s.b1), __fmul_rn(g, s.c1));
-        v[k] = __fadd_rn(__fmul_rn(v[k], s.b2), __fmul_rn(__fmul_rn(g, g), s.c2));
-        h.p[k] = fmaf(-s.rate, __fdividef(m[k], fmaf(sqrt_approx(v[k]), s.inv_bc2, s.eps)), h.p[k] * t.keep);
-        mtop = max_nan(mtop, fabsf(m[k]));
-        vtop = max_nan(vtop, v[k]);
-    }
-    store4<float, WIDE>(reinterpret_cast<float *>(t.param) + at, left, h.p);
-    if (t.copy) store4<__nv_bfloat16, WIDE>(reinterpret_cast<__nv_bfloat16 *>(t.copy) + at, left, h.p);
-    if constexpr (BITS == 32) {
-        store4<float, true>((float *)a.m + at, 4, m);
-        store4<float, true>((float *)a.v + at, 4, v);
-    } else {
-        const uint32_t mbits = __reduce_max_sync(FULL, __float_as_uint(mtop));
-        const uint32_t vbits = __reduce_max_sync(FULL, __float_as_uint(vtop));
-        const int em = block_exponent(mbits), ev = block_exponent(vbits);
-        float mf, mg, vf, vg;
-        code_factors(em, 7, 7, mf, mg);
-        code_factors(ev, 14, 15, vf, vg);
-        const uint64_t word = mix64(s.key + (uint64_t)(b * 32 + lane));
+            for (int k = 0; k < 4; k++) ym[k] = __fmul_rn(ym[k], sm.second), yv[k] = __fmul_rn(yv[k], sv.second);
+        }
         uint32_t mc[4], vc[4];  // the codes in the top byte
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            const uint32_t w = (uint32_t)(word >> (k < 2 ? 0 : 32)), d = k & 1 ? w >> 16 : w & 0xffffu;
-            const float ym = __fmul_rn(__fmul_rn(fabsf(m[k]), mf), mg), yv = __fmul_rn(__fmul_rn(v[k], vf), vg);
-            mc[k] = ((__float_as_uint(ym) + (d << 4 | 8u)) << 4 & 0x7f000000u) | (__float_as_uint(m[k]) & 0x80000000u);
-            vc[k] = max(__float_as_uint(yv) + (d << 5 | 16u), v[k] > 0.f ? 1u << 21 : 0u) << 3;
+            const uint32_t w = k < 2 ? (uint32_t)word : (uint32_t)(word >> 32);
+            const uint32_t d = 2 * (k & 1 ? w >> 16 : w & 0xffffu) + 1;  // 16 random bits and a half
+            mc[k] = ((__float_as_uint(ym[k]) + 8 * d) << 4 & 0x7f000000u) | (__float_as_uint(k & 1 ? m[k / 2].y : m[k / 2].x) & 0x80000000u);
+            vc[k] = (__float_as_uint(yv[k]) + 16 * d) << 3;
         }
-        const uint32_t mw = __byte_perm(__byte_perm(mc[0], mc[1], 0x0073), __byte_perm(mc[2], mc[3], 0x0073), 0x5410);
-        const uint32_t vw = __byte_perm(__byte_perm(vc[0], vc[1], 0x0073), __byte_perm(vc[2], vc[3], 0x0073), 0x5410);
-        const bool mbad = mbits >= 0x7f800000u, vbad = vbits >= 0x7f800000u;
-        ((uint32_t *)a.m)[at >> 2] = mbad ? 0u : mw;
-        ((uint32_t *)a.v)[at >> 2] = vbad ? 0u : vw;
+        if (__any_sync(FULL, min(min(vc[0], vc[1]), min(vc[2], vc[3])) < 1u << 24)) {  // a code of zero: only for v = 0
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if ((k & 1 ? v[k / 2].y : v[k / 2].x) > 0.f) vc[k] = max(vc[k], 1u << 24);
+        }
+        ((uint32_t *)a.m)[at >> 2] = __byte_perm(__byte_perm(mc[0], mc[1], 0x0073), __byte_perm(mc[2], mc[3], 0x0073), 0x5410);
+        ((uint32_t *)a.v)[at >> 2] = __byte_perm(__byte_perm(vc[0], vc[1], 0x0073), __byte_perm(vc[2], vc[3], 0x0073), 0x5410);
         if (lane == 0) {
-            a.m_scale[b] = mbad ? __uint_as_float(0x7fc00000u) : pow2(em - 7);
-            a.v_scale[b] = vbad ? __uint_as_float(0x7fc00000u) : pow2(ev - 14);
+            a.m_scale[b] = sm.scale;
+            a.v_scale[b] = sv.scale;
         }
     }
 }
 
-template <int BITS> __global__ void __launch_bounds__(THREADS, 4) step_kernel(Args a) {
+template <int BITS, bool WIDE>
+__device__ __forceinline__ void load_block(const Args &a, const Place &t, int b, Held<BITS> &h) {
+    const int64_t at = (int64_t)b * BLOCK + 4 * (threadIdx.x & 31);
+    const int left = WIDE ? 4 : left_at(t, b);
+    const uintptr_t g = t.grad + (at << t.grad_shift);
+    if (WIDE) {
+        h.p = *(reinterpret_cast<const float4 *>(t.param) + (at >> 2));
+        if (t.grad_shift == 2)
+            h.g = *reinterpret_cast<const uint4 *>(g);
+        else
+            *reinterpret_cast<uint2 *>(&h.g) = *reinterpret_cast<const uint2 *>(g);
+    } else {
+        float p[4];
+        load4<float, false>(reinterpret_cast<const float *>(t.param) + at, left, p);
+        h.p = make_float4(p[0], p[1], p[2], p[3]);
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            w[k] = k >= left ? 0u : t.grad_shift == 2 ? reinterpret_cast<const uint32_t *>(g)[k] : reinterpret_cast<const uint16_t *>(g)[k];
+        h.g = t.grad_shift == 2 ? make_uint4(w[0], w[1], w[2], w[3]) : make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, 0u, 0u);
+    }
+    if constexpr (BITS == 32) {
+        h.m = *reinterpret_cast<const float4 *>((const float *)a.m + at);
+        h.v = *reinterpret_cast<const float4 *>((const float *)a.v + at);
+    } else {
+        h.m = ((const uint32_t *)a.m)[at >> 2];
+        h.v = ((const uint32_t *)a.v)[at >> 2];
+        h.ms = a.m_scale[b];
+        h.vs = a.v_scale[b];
+    }
+}
+
+// The tiles of a warp: its own number first, then the next ones that nobody has
+// (asked for one tile ahead). They are handed out, not shared out, because the
+// SMs differ in how fast they get at memory: 128 Mi parameters in 32 bits took
+// 624 us in equal shares and 563 us so. A few thousand tiles would spend more
+// time at the counter than they take, so smaller steps have fixed places.
+struct Tiles {
+    int block, left;  // the next pair; pairs left in the tile
+    unsigned next;    // lane 0's
+    __device__ __forceinline__ void ask(const Args &a) {
+        left = a.tile / 2;
+        if (a.tile > 2 && (threadIdx.x & 31) == 0) next = atomicAdd(a.taken, 1u);
+    }
+    __device__ __forceinline__ explicit Tiles(const Args &a) : next(0u) {
+        block = (blockIdx.x * WARPS + (threadIdx.x >> 5)) * a.tile;
+        ask(a);
+    }
+    __device__ __forceinline__ void advance(const Args &a) {
+        block += 2;
+        if (--left == 0) {
+            const int warps = gridDim.x * WARPS;
+            const int64_t far = a.tile > 2 ? ((int64_t)warps + __shfl_sync(FULL, next, 0)) * a.tile : block + 2 * (warps - 1);
+            block = far < a.nblocks ? (int)far : a.nblocks;
+            ask(a);
+        }
+    }
+};
+
+constexpr int per_sm(int) { return 3; }  // blocks of step_kernel
+
+template <int BITS> __global__ void __launch_bounds__(THREADS, per_sm(BITS)) step_kernel(Args a) {
     __shared__ double part[WARPS];
     __shared__ float coef[2];
     __shared__ int64_t now;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (threadIdx.x < 2) {  // the two bias corrections, side by side
-        const int64_t t = *a.step + 1;
-        const double left = 1. - exp2((double)t * (lane ? a.log2_beta2 : a.log2_beta1));
+        const int64_t n = *a.step + 1;
+        const double left = 1. - exp2((double)n * (lane ? a.log2_beta2 : a.log2_beta1));
         coef[lane] = lane ? (float)(1. / sqrt(left)) : (float)(a.lr / left);
-        now = t;
+        now = n;
     }
+    Tiles tiles(a);
+    Place t;
+    t.end = 0;
+    if (tiles.block < a.nblocks) t = locate(a, tiles.block);
     Step s{1.f, 0.f, 0.f, a.eps, a.b1, a.c1, a.b2, a.c2, 0u};
     if (a.max_norm > 0.f) {
         pdl_wait();  // for the norm's partial sums
         double d = 0.;
-        for (int i = threadIdx.x; i < gridDim.x; i += THREADS) d += a.partials[i];
+        for (int i = threadIdx.x; i < a.norm_parts; i += THREADS) d += a.partials[i];
 #pragma unroll
         for (int o = 16; o; o >>= 1) d += __shfl_xor_sync(FULL, d, o);
         if (lane == 0) part[warp] = d;
@@ -323,56 +403,85 @@ template <int BITS> __global__ void __launch_bounds__(THREADS, 4) step_kernel(Ar
     s.rate = coef[0];
     s.inv_bc2 = coef[1];
     s.key = mix64(mix64(a.seed) + (uint64_t)now);
-    // the step was read before each block's arrival: the last one advances it
+    while (tiles.block < a.nblocks) {
+        const int b = tiles.block;
+        if (b >= t.end) t = locate(a, b);
+        if (!pair_at(t, b)) {
+            for (int c = b; c < a.nblocks && c < b + 2; c++) {
+                Held<BITS> h;
+                if (c >= t.end) t = locate(a, c);
+                load_block<BITS, false>(a, t, c, h);
+                step_block<BITS, false>(a, s, t, c, h);
+            }
+            tiles.advance(a);
+            continue;
+        }
+        Held<BITS> h[2];
+        load_block<BITS, true>(a, t, b, h[0]);
+        load_block<BITS, true>(a, t, b + 1, h[1]);
+        for (bool more = true; more;) {
+            const int c = tiles.block;
+            tiles.advance(a);
+            more = pair_at(t, tiles.block);
+            if constexpr (BITS == 32) {
+                step_block<BITS, true>(a, s, t, c, h[0]);
+                step_block<BITS, true>(a, s, t, c + 1, h[1]);
+                if (more) {
+                    load_block<BITS, true>(a, t, tiles.block, h[0]);
+                    load_block<BITS, true>(a, t, tiles.block + 1, h[1]);
+                }
+            } else {  // 8 bits take long to compute: the next blocks' loads are under way meanwhile
+                Held<BITS> n = h[0];
+                if (more) load_block<BITS, true>(a, t, tiles.block, h[0]);
+                step_block<BITS, true>(a, s, t, c, n);
+                n = h[1];
+                if (more) load_block<BITS, true>(a, t, tiles.block + 1, h[1]);
+                step_block<BITS, true>(a, s, t, c + 1, n);
+            }
+        }
+    }
+    __syncthreads();
+    // every block has read the step when the last one arrives here
     if (threadIdx.x == 0) {
         __threadfence();
         if (atomicAdd(a.arrived, 1u) == gridDim.x - 1) {
-            *a.arrived = 0u;
+            *a.arrived = *a.taken = 0u;
             *a.step = now;
         }
     }
-    for_blocks(a, [&](const Place &t, int64_t b, bool two) {
-        if (two) {
-            Held<BITS> h, k;
-            load_block<BITS, true>(a, t, b, h);
-            load_block<BITS, true>(a, t, b + 1, k);
-            step_block<BITS, true>(a, s, t, b, h);
-            step_block<BITS, true>(a, s, t, b + 1, k);
-        } else {
-            Held<BITS> h;
-            load_block<BITS, false>(a, t, b, h);
-            step_block<BITS, false>(a, s, t, b, h);
-        }
-    });
 }
 
 }  // namespace adamw
 }  // namespace d1
 
-extern "C" int d1_adamw_work_bytes(void) { return d1::adamw::GRID * (int)sizeof(double) + 16; }
+extern "C" int d1_adamw_work_bytes(void) { return d1::adamw::NORM_GRID * (int)sizeof(double) + 16; }
 
 extern "C" int d1_adamw(const D1AdamWTensor *tensors, int ntensors, int64_t nblocks, int state_bits, void *m, void *v,
                         float *m_scale, float *v_scale, double lr, double beta1, double beta2, double eps,
                         double max_norm, int64_t *step, uint64_t seed, void *work, float *grad_norm, void *stream) {
     using namespace d1::adamw;
+    if (nblocks > INT32_MAX - 8) return D1_ERR_TOO_LARGE;
     if (!tensors || ntensors < 1 || nblocks < 1 || (state_bits != 32 && state_bits != 8) || !m || !v || !step ||
         !work || (state_bits == 8 && (!m_scale || !v_scale)) || !(beta1 >= 0. && beta1 < 1.) ||
         !(beta2 >= 0. && beta2 < 1.) || !(eps >= 0.) || (reinterpret_cast<uintptr_t>(m) & 15) ||
         (reinterpret_cast<uintptr_t>(v) & 15) || (reinterpret_cast<uintptr_t>(work) & 15))
         return D1_ERR_BAD_ARGUMENT;
-    Args a{tensors, ntensors, nblocks, m, v, m_scale, v_scale, lr, beta1, beta2, log2(beta1), log2(beta2),
-           (float)beta1, (float)(1. - beta1), (float)beta2, (float)(1. - beta2), (float)eps, (float)max_norm, step,
-           seed, (double *)work, (unsigned *)((double *)work + GRID), grad_norm};
-    const int64_t want = (nblocks + 2 * WARPS - 1) / (2 * WARPS);
-    const int grid = (int)(want < GRID ? want : GRID);
+    const int tile = nblocks >= SMS * 32 * 4 * 8 ? 8 : 2;  // 8 where that makes four tiles for each warp
+    Args a{tensors, ntensors, (int)nblocks, tile, m, v, m_scale, v_scale, lr, beta1, beta2, log2(beta1), log2(beta2),
+           (float)beta1, (float)(1. - beta1), (float)beta2, (float)(1. - beta2), (float)(eps > EPS_FLOOR ? eps : EPS_FLOOR), (float)max_norm, step,
+           seed, (double *)work, (unsigned *)((double *)work + NORM_GRID), (unsigned *)((double *)work + NORM_GRID) + 1,
+           0, grad_norm};
     const cudaStream_t s = (cudaStream_t)stream;
+    const int64_t norm_want = (nblocks + 2 * WARPS - 1) / (2 * WARPS), want = (nblocks + tile * WARPS - 1) / (tile * WARPS);
+    const int most = SMS * per_sm(state_bits);
     cudaLaunchAttribute attr;
-    cudaLaunchConfig_t cfg = d1::pdl_config(dim3(grid), dim3(THREADS), 0, s, &attr);
+    cudaLaunchConfig_t cfg = d1::pdl_config(dim3((unsigned)(want < most ? want : most)), dim3(THREADS), 0, s, &attr);
     if (a.max_norm > 0.f) {
-        norm_kernel<<<grid, THREADS, 0, s>>>(a);
+        a.norm_parts = (int)(norm_want < NORM_GRID ? norm_want : NORM_GRID);
+        norm_kernel<<<a.norm_parts, THREADS, 0, s>>>(a);
         if (cudaError_t e = cudaGetLastError()) return (int)e;
     } else
         cfg.numAttrs = 0;
-    return (int)(state_bits == 32 ? cudaLaunchKernelEx(&cfg, step_kernel<32>, a)
-                                  : cudaLaunchKernelEx(&cfg, step_kernel<8>, a));
+    const auto kernel = state_bits == 32 ? step_kernel<32> : step_kernel<8>;
+    return (int)cudaLaunchKernelEx(&cfg, kernel, a);
 }

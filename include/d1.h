@@ -719,7 +719,7 @@ int d1_adamw_work_bytes(void);
  *   g = grad * min(1, max_norm / (norm + 1e-6))   (norm over all tensors; max_norm <= 0: no clipping)
  *   m = beta1 m + (1 - beta1) g,   v = beta2 v + (1 - beta2) g^2
  *   p = p (1 - lr decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
- * with t = *step + 1 (device), which the call stores back. The moments are flat
+ * with t = *step + 1 (device), which the call stores back, and eps not below 2^-63. The moments are flat
  * over the blocks, zero at the start: state_bits 32: m and v f32 [nblocks * 128];
  * state_bits 8: m e4m3 and v e5m2 codes [nblocks * 128] times the block scales
  * m_scale and v_scale (f32 [nblocks], powers of two), rounded stochastically,
