@@ -6,17 +6,18 @@
 //   dw_j = sum_r dy xhat       db_j = sum_r dy
 //
 // Both passes are bound by memory. A row is read once and held in registers, P
-// elements a thread, by 8 or 32 lanes (short rows, joined by shuffles) or by a
-// block (joined through shared memory); the variance is the mean square of the
-// held x - mean, not a difference of sums. A block keeps taking rows, and loads
-// the next one before it joins the sums of this one, so that loads are in
-// flight all the time. In the backward pass a thread owns the same columns in
-// every row, so that the weights' gradients are sums in its registers; a block
-// writes one partial sum for each column, and a second, small launch adds the
-// blocks' in a fixed order.
+// elements a thread, by a team of 8 or 32 lanes (short rows, joined by shuffles)
+// or by a block (joined through shared memory); the variance is the mean square
+// of the held x - mean, not a difference of sums. In the backward pass a thread
+// owns the same columns in every row, so that the weights' gradients are sums in
+// its registers; a block writes one partial sum for each column, and a second,
+// small launch adds the blocks' in a fixed order.
 //
-// Rows are read as 16-byte vectors where base, pitch and n allow, else element
-// by element (still coalesced).
+// Rows are read as 16-byte vectors (VEC = 16 / size) where base, pitch and n
+// allow. Else 16-bit types are taken in pairs of columns (VEC = 2; a pair at an
+// odd place is two loads) and fp32 column by column (VEC = 1). A warp's columns
+// are 32 P in a row, so that a thread's lie at fixed distances, and only the
+// last warp has to look where the row ends.
 #include "d1_elem.cuh"
 #include "d1_pdl.cuh"
 
@@ -24,238 +25,609 @@ namespace d1 {
 namespace ln {
 
 constexpr int SMS = 148;
-constexpr int HELD_FORWARD = 32768, HELD_BACKWARD = 8192;  // longest rows held in registers
+constexpr int HELD_FORWARD = 32768;  // longest rows held in registers
 
-// P elements of a row as P / VEC vectors, `threads` apart.
-template <class T, int VEC, int P> struct Held {
+template <class T> __device__ __forceinline__ float2 pair_f32(const T *e) { return make_float2(to_f32(e[0]), to_f32(e[1])); }
+template <> __device__ __forceinline__ float2 pair_f32<__nv_bfloat16>(const __nv_bfloat16 *e) {
+    const uint32_t w = *reinterpret_cast<const uint32_t *>(e);
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <> __device__ __forceinline__ float2 pair_f32<__half>(const __half *e) {
+    return __half22float2(*reinterpret_cast<const __half2 *>(e));
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
+// Loads from and stores to shared memory by its own addresses (32 bits), so
+// that none of them becomes a generic access.
+template <int BYTES> struct Word;
+template <> struct Word<2> {
+    using U = uint16_t;
+    static __device__ __forceinline__ U load(uint32_t at) {
+        U v;
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
+        return v;
+    }
+    static __device__ __forceinline__ void store(uint32_t at, U v) { asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"(v) : "memory"); }
+};
+template <> struct Word<4> {
+    using U = uint32_t;
+    static __device__ __forceinline__ U load(uint32_t at) {
+        U v;
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+        return v;
+    }
+    static __device__ __forceinline__ void store(uint32_t at, U v) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory"); }
+};
+template <> struct Word<8> {
+    using U = uint2;
+    static __device__ __forceinline__ U load(uint32_t at) {
+        U v;
+        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
+        return v;
+    }
+};
+template <> struct Word<16> {
+    using U = uint4;
+    static __device__ __forceinline__ U load(uint32_t at) {
+        U v;
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+        return v;
+    }
+    static __device__ __forceinline__ void store(uint32_t at, U v) {
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+    }
+};
+__device__ __forceinline__ uint32_t shared_address(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+template <class E> __device__ __forceinline__ E load_shared(uint32_t at) {
+    const auto w = Word<sizeof(E)>::load(at);
+    return *reinterpret_cast<const E *>(&w);
+}
+
+// A thread's columns: element k of its P is column start + (k / VEC) STEP + k % VEC.
+template <int VEC, int P, int G> struct Columns {
+    static constexpr int LANES = G ? G : 32, STEP = LANES * VEC;
+    int start, left;  // left: columns of the row from `start` on
+    bool full;        // every column of the warp is in the row
+    __device__ __forceinline__ explicit Columns(int n) {
+        const int warp = G ? 0 : threadIdx.x >> 5, lane = threadIdx.x % LANES;
+        start = warp * 32 * P + lane * VEC;
+        left = n - start;
+        full = G ? n == G * P : n >= (warp + 1) * 32 * P;
+    }
+    static __device__ __forceinline__ int offset(int k) { return k / VEC * STEP + k % VEC; }
+};
+
+// P elements of a row in registers, as P / VEC vectors.
+template <class T, int VEC, int P, int G> struct Held {
+    using C = Columns<VEC, P, G>;
     Elems<T, VEC> v[P / VEC];
-    __device__ __forceinline__ void load(const T *row, int t, int threads, int n) {
+    // From a row in shared memory, padded with zeros.
+    __device__ __forceinline__ void load_staged(uint32_t at) {
+        if (VEC == 2 && (at & 3)) {
+#pragma unroll
+            for (int i = 0; i < P / VEC; i++) {
+                v[i].v[0] = load_shared<T>(at + i * C::STEP * (int)sizeof(T));
+                v[i].v[VEC - 1] = load_shared<T>(at + (i * C::STEP + 1) * (int)sizeof(T));
+            }
+        } else
+#pragma unroll
+            for (int i = 0; i < P / VEC; i++) v[i] = load_shared<Elems<T, VEC>>(at + i * C::STEP * (int)sizeof(T));
+    }
+    __device__ __forceinline__ void load_all(const T *at) {
+        if (VEC == 2 && (reinterpret_cast<uintptr_t>(at) & 3)) {
+#pragma unroll
+            for (int i = 0; i < P / VEC; i++) {
+                v[i].v[0] = at[i * C::STEP];
+                v[i].v[VEC - 1] = at[i * C::STEP + 1];
+            }
+        } else
+#pragma unroll
+            for (int i = 0; i < P / VEC; i++) v[i] = *reinterpret_cast<const Elems<T, VEC> *>(at + i * C::STEP);
+    }
+    // From a row in global memory; zeros past its end.
+    __device__ __forceinline__ void load(const T *at, const C &c) {
+        if (c.full) {
+            load_all(at);
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < P / VEC; i++) {
-            const int j = (t + i * threads) * VEC;
-            if (j < n)
-                v[i] = *reinterpret_cast<const Elems<T, VEC> *>(row + j);
-            else
+            const int left = c.left - i * C::STEP;
+            if (VEC > 2 && left > 0) {
+                v[i] = *reinterpret_cast<const Elems<T, VEC> *>(at + i * C::STEP);
+            } else
 #pragma unroll
-                for (int e = 0; e < VEC; e++) v[i].v[e] = from_f32<T>(0.f);
+                for (int e = 0; e < VEC; e++) v[i].v[e] = VEC <= 2 && e < left ? at[i * C::STEP + e] : from_f32<T>(0.f);
         }
     }
-    __device__ __forceinline__ float at(int k) const { return to_f32(v[k / VEC].v[k % VEC]); }
+    // Elements 2k and 2k + 1 of the P.
+    __device__ __forceinline__ float2 pair(int k) const {
+        if constexpr (VEC == 1)
+            return make_float2(to_f32(v[2 * k].v[0]), to_f32(v[2 * k + 1].v[0]));
+        else
+            return pair_f32<T>(&v[2 * k / VEC].v[2 * k % VEC]);
+    }
 };
-template <class T, int VEC, int P>
-__device__ __forceinline__ void store_row(T *row, int t, int threads, int n, const float (&y)[P]) {
+template <class T, int VEC, int P, int G>
+__device__ __forceinline__ void store_row(T *at, const Columns<VEC, P, G> &c, const float2 (&y)[P / 2]) {
+    constexpr int STEP = Columns<VEC, P, G>::STEP;
+    Elems<T, VEC> o[P / VEC];
 #pragma unroll
-    for (int i = 0; i < P / VEC; i++) {
-        const int j = (t + i * threads) * VEC;
-        if (j < n) {
-            Elems<T, VEC> o;
+    for (int k = 0; k < P; k++) o[k / VEC].v[k % VEC] = from_f32<T>(k & 1 ? y[k / 2].y : y[k / 2].x);
+    if (VEC == 2 && (reinterpret_cast<uintptr_t>(at) & 3)) {
 #pragma unroll
-            for (int e = 0; e < VEC; e++) o.v[e] = from_f32<T>(y[i * VEC + e]);
-            *reinterpret_cast<Elems<T, VEC> *>(row + j) = o;
+        for (int k = 0; k < P; k++)
+            if (c.full || k / VEC * STEP + k % VEC < c.left) at[k / VEC * STEP + k % VEC] = o[k / VEC].v[k % VEC];
+    } else if (c.full) {
+#pragma unroll
+        for (int i = 0; i < P / VEC; i++) *reinterpret_cast<Elems<T, VEC> *>(at + i * STEP) = o[i];
+    } else
+#pragma unroll
+        for (int i = 0; i < P / VEC; i++) {
+            if (i * STEP + VEC <= c.left)
+                *reinterpret_cast<Elems<T, VEC> *>(at + i * STEP) = o[i];
+            else if (VEC == 2 && i * STEP < c.left)
+                at[i * STEP] = o[i].v[0];
         }
-    }
 }
-// The columns' weights (`other` where there are none, 0 past the row).
-template <int VEC, int P>
-__device__ __forceinline__ void load_weights(const float *w, int t, int threads, int n, float other, float (&x)[P]) {
+// The columns' weights from global memory, `other` where there are none, 0 past the row.
+template <int VEC, int P, int G>
+__device__ __forceinline__ void load_weights(const float *w, const Columns<VEC, P, G> &c, float other, float2 (&x)[P / 2]) {
 #pragma unroll
     for (int k = 0; k < P; k++) {
-        const int j = (t + k / VEC * threads) * VEC + k % VEC;
-        x[k] = j < n ? (w ? __ldg(w + j) : other) : 0.f;
+        const int o = Columns<VEC, P, G>::offset(k);
+        const float v = o < c.left ? w ? __ldg(w + c.start + o) : other : 0.f;
+        if (k & 1)
+            x[k / 2].y = v;
+        else
+            x[k / 2].x = v;
     }
 }
 
-// Sums over the G threads of a row, which all get them: by shuffles (G <= 32),
-// or over the block (G = 0) through `part`, of which calls in turn take turns.
-template <int G, int K> __device__ __forceinline__ void row_sums(float (&s)[K], float (*part)[32]) {
+// Weights in shared memory, zeros past the row: padded, and for vectors of eight
+// with the halves apart, so that a warp's loads of four have no bank conflicts.
+template <int VEC, int P> struct SharedWeights {
+    static __host__ __device__ constexpr int floats(int warps) { return warps * 32 * P; }
+    static __device__ __forceinline__ int place(int j, int total) {
+        return VEC == 8 ? (j & 4 ? total / 2 : 0) + j / 8 * 4 + j % 4 : j;
+    }
+    static __device__ __forceinline__ void fill(float *s, const float *w, float other, int n, int total) {
+        for (int j = threadIdx.x; j < total; j += blockDim.x) s[place(j, total)] = j < n ? w ? __ldg(w + j) : other : 0.f;
+    }
+    // Elements 2k and 2k + 1 of the thread's P.
+    static __device__ __forceinline__ float2 pair(const float *s, int start, int k, int total) {
+        constexpr int STEP = 32 * VEC;
+        if constexpr (VEC == 8)
+            return *reinterpret_cast<const float2 *>(s + (k & 2 ? total / 2 : 0) + start / 2 + 2 * k / VEC * (STEP / 2) + 2 * (k & 1));
+        else if constexpr (VEC == 1)
+            return make_float2(s[start + 2 * k * STEP], s[start + (2 * k + 1) * STEP]);
+        else
+            return *reinterpret_cast<const float2 *>(s + start + 2 * k / VEC * STEP + 2 * k % VEC);
+    }
+};
+
+// The sum over a team of G lanes, or over the block through `part` (32 floats,
+// zeros past the warps); every thread gets it. Calls in turn take turns at it.
+template <int G> __device__ __forceinline__ float team_sum(float s, float *part) {
 #pragma unroll
-    for (int o = (G ? G : 32) / 2; o; o >>= 1)
-#pragma unroll
-        for (int k = 0; k < K; k++) s[k] += __shfl_xor_sync(0xffffffffu, s[k], o);
-    if (G) return;
-    const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
-    if (lane == 0)
-#pragma unroll
-        for (int k = 0; k < K; k++) part[k][threadIdx.x >> 5] = s[k];
+    for (int o = (G ? G : 32) / 2; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (G) return s;
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
     __syncthreads();
-#pragma unroll
-    for (int k = 0; k < K; k++) {
-        s[k] = lane < warps ? part[k][lane] : 0.f;
-        s[k] = warp_sum(s[k]);
+    float2 sum = both(0.f);
+    for (int w = 0; w < (int)blockDim.x; w += 256) {  // eight warps at a time
+        const float4 a = *reinterpret_cast<const float4 *>(part + w / 32), b = *reinterpret_cast<const float4 *>(part + w / 32 + 4);
+        sum = __fadd2_rn(sum, __fadd2_rn(__fadd2_rn(make_float2(a.x, a.y), make_float2(a.z, a.w)), __fadd2_rn(make_float2(b.x, b.y), make_float2(b.z, b.w))));
     }
+    return sum.x + sum.y;
+}
+// The sums of a and b: the halves of the team share the work of all steps but
+// the first. part: 64 floats.
+template <int G> __device__ __forceinline__ void team_sums(float &a, float &b, float *part) {
+    constexpr int HALF = (G ? G : 32) / 2;
+    const int lane = threadIdx.x & 31;
+    const bool upper = lane & HALF;
+    float s = upper ? b : a;
+    s += __shfl_xor_sync(0xffffffffu, upper ? a : b, HALF);
+#pragma unroll
+    for (int o = HALF / 2; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (G) {
+        a = __shfl_sync(0xffffffffu, s, 0, G ? G : 32);
+        b = __shfl_sync(0xffffffffu, s, HALF, G ? G : 32);
+        return;
+    }
+    if ((lane & 15) == 0) part[(threadIdx.x >> 5) * 2 + (lane >> 4)] = s;
+    __syncthreads();
+    float2 sum = both(0.f);
+    for (int w = 0; w < (int)blockDim.x; w += 128) {  // four warps at a time
+        const float4 p = *reinterpret_cast<const float4 *>(part + w / 16), q = *reinterpret_cast<const float4 *>(part + w / 16 + 4);
+        sum = __fadd2_rn(sum, __fadd2_rn(__fadd2_rn(make_float2(p.x, p.y), make_float2(p.z, p.w)), __fadd2_rn(make_float2(q.x, q.y), make_float2(q.z, q.w))));
+    }
+    a = sum.x;
+    b = sum.y;
 }
 
+// The sum of (x - mu)^2 over the columns that are in the row.
 template <class T, int VEC, int P, int G>
-__global__ void __launch_bounds__(G ? 256 : P == 32 ? 1024 : 512)
+__device__ __forceinline__ float square_sum(const Held<T, VEC, P, G> &h, const Columns<VEC, P, G> &c, float mu) {
+    float2 s = both(0.f);
+    if (c.full) {
+#pragma unroll
+        for (int k = 0; k < P / 2; k++) {
+            const float2 d = __fadd2_rn(h.pair(k), both(-mu));
+            s = __ffma2_rn(d, d, s);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < P / 2; k++) {
+            const float2 d = __fadd2_rn(h.pair(k), both(-mu));
+            if (Columns<VEC, P, G>::offset(2 * k) < c.left) s.x = fmaf(d.x, d.x, s.x);
+            if (Columns<VEC, P, G>::offset(2 * k + 1) < c.left) s.y = fmaf(d.y, d.y, s.y);
+        }
+    }
+    return s.x + s.y;
+}
+template <class T, int VEC, int P, int G> __device__ __forceinline__ float plain_sum(const Held<T, VEC, P, G> &h) {
+    float2 s = both(0.f);  // elements past the row are zeros
+#pragma unroll
+    for (int k = 0; k < P / 2; k++) s = __fadd2_rn(s, h.pair(k));
+    return s.x + s.y;
+}
+
+// Forward, R rows at a time by each team of G lanes (or the block), once. The
+// rows' loads are issued together and their sums joined together; blocks are
+// many and small, so that others load while one adds.
+template <class T, int VEC, int P, int G, int R>
+__global__ void __launch_bounds__(G ? 256 : 1024, G == 32 && P == 16 ? 4 : 1)
     forward_kernel(const T *__restrict__ x, int64_t ldx, int64_t rows, int n, const float *__restrict__ w,
                    const float *__restrict__ b, float eps, T *__restrict__ y, int64_t ldy, float *__restrict__ mean,
                    float *__restrict__ rstd) {
-    constexpr bool KEEP = P <= 16;  // the weights stay in registers too
-    __shared__ float part[4][1][32];
-    const int threads = G ? G : blockDim.x, t = G ? threadIdx.x % G : threadIdx.x;
-    const int per_block = G ? 256 / (G ? G : 1) : 1;
-    const int64_t step = (int64_t)gridDim.x * per_block;
-    const int64_t base = (int64_t)blockIdx.x * per_block, mine = G ? threadIdx.x / (G ? G : 1) : 0;
-    float wk[KEEP ? P : 1], bk[KEEP ? P : 1];
-    if (KEEP) {
-        load_weights<VEC>(w, t, threads, n, 1.f, wk);
-        load_weights<VEC>(b, t, threads, n, 0.f, bk);
+    __shared__ __align__(16) float part[2][R][32];
+    const Columns<VEC, P, G> c(n);
+    constexpr int STEP = Columns<VEC, P, G>::STEP;
+    if (!G) {
+        for (int i = threadIdx.x; i < 2 * R * 32; i += blockDim.x) (&part[0][0][0])[i] = 0.f;
+        __syncthreads();
+    }
+    const int64_t first = G ? ((int64_t)blockIdx.x * (256 / (G ? G : 1)) + threadIdx.x / (G ? G : 1)) * R : (int64_t)blockIdx.x * R;
+    const float inv_n = 1.f / n;
+    Held<T, VEC, P, G> h[R];
+#pragma unroll
+    for (int q = 0; q < R; q++) {
+        const int64_t r = first + q < rows ? first + q : rows - 1;  // past the end: the last row again, not stored
+        h[q].load(x + r * ldx + c.start, c);
+    }
+    float mu[R], rs[R];
+#pragma unroll
+    for (int q = 0; q < R; q++) mu[q] = team_sum<G>(plain_sum(h[q]), part[0][q]) * inv_n;
+#pragma unroll
+    for (int q = 0; q < R; q++) rs[q] = 1.f / sqrtf(team_sum<G>(square_sum(h[q], c, mu[q]), part[1][q]) * inv_n + eps);
+#pragma unroll
+    for (int i = 0; i < P / VEC; i++) {  // vector by vector, for few registers
+        const int left = c.left - i * STEP, j = c.start + i * STEP;
+        if (left <= 0) break;
+        float wv[VEC], bv[VEC];
+        if constexpr (VEC % 4 == 0) {
+#pragma unroll
+            for (int e = 0; e < VEC; e += 4) {
+                *reinterpret_cast<float4 *>(wv + e) = w ? __ldg(reinterpret_cast<const float4 *>(w + j + e)) : make_float4(1.f, 1.f, 1.f, 1.f);
+                *reinterpret_cast<float4 *>(bv + e) = b ? __ldg(reinterpret_cast<const float4 *>(b + j + e)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; e++) {
+                wv[e] = w && e < left ? __ldg(w + j + e) : 1.f;
+                bv[e] = b && e < left ? __ldg(b + j + e) : 0.f;
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < R; q++) {
+            if (first + q >= rows) break;
+            Elems<T, VEC> o;
+            if constexpr (VEC > 1) {
+#pragma unroll
+                for (int e = 0; e < VEC; e += 2) {
+                    const float2 c = __fmul2_rn(__fadd2_rn(h[q].pair((i * VEC + e) / 2), both(-mu[q])), both(rs[q]));
+                    const float2 f = __ffma2_rn(c, make_float2(wv[e], wv[e + 1]), make_float2(bv[e], bv[e + 1]));
+                    o.v[e] = from_f32<T>(f.x);
+                    o.v[e + 1] = from_f32<T>(f.y);
+                }
+            } else
+                o.v[0] = from_f32<T>(fmaf((to_f32(h[q].v[i].v[0]) - mu[q]) * rs[q], wv[0], bv[0]));
+            T *const at = y + (first + q) * ldy + j;
+            if (VEC == 2 && (left == 1 || (reinterpret_cast<uintptr_t>(at) & 3))) {
+                at[0] = o.v[0];
+                if (left > 1) at[1] = o.v[VEC - 1];
+            } else
+                *reinterpret_cast<Elems<T, VEC> *>(at) = o;
+        }
+    }
+    if ((G ? threadIdx.x % (G ? G : 1) : threadIdx.x) == 0)
+#pragma unroll
+        for (int q = 0; q < R; q++)
+            if (first + q < rows) {
+                if (mean) mean[first + q] = mu[q];
+                if (rstd) rstd[first + q] = rs[q];
+            }
+}
+
+// ---------------------------------------------------------------- rows on their way through shared memory
+
+__device__ __forceinline__ void copy_async16(uint32_t to, const void *from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+// 16 bytes, of which the first `size` are read and the others zero.
+__device__ __forceinline__ void copy_async16(uint32_t to, const void *from, int size) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(size) : "memory");
+}
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_group %0;" ::"n"(N < 0 ? 0 : N) : "memory"); }
+
+// A team's rows of x (row, row + step, ...) on their way to shared memory, DEPTH
+// of them with the present one, each padded with zeros to the team's columns.
+// Where rows are vectors (VECTOR) a thread copies what it will use itself and
+// needs no barrier to see it. Else the team copies the row's 16-byte pieces,
+// the row keeping its offset within 16 bytes, and a barrier makes them visible;
+// the first piece then brings the end of the row before, but where that would
+// reach out of the matrix the piece is copied element by element.
+template <class T, int VEC, int P, int G> struct Rows {
+    static constexpr bool VECTOR = VEC * sizeof(T) == 16;
+    using C = Columns<VEC, P, G>;
+    const T *at;  // the next row to fetch
+    int64_t pitch;
+    int left;  // rows
+    uintptr_t origin;  // where the matrix begins
+    __device__ __forceinline__ Rows(const T *x, int64_t ld, int64_t rows, int64_t row, int64_t step)
+        : at(x + row * ld), pitch(step * ld), left(row < rows ? (int)((rows - row + step - 1) / step) : 0),
+          origin(reinterpret_cast<uintptr_t>(x)) {}
+    static __host__ __device__ constexpr int bytes(int warps) { return (G ? G : warps * 32) * P * (int)sizeof(T) + (VECTOR ? 0 : 16); }
+    __device__ __forceinline__ void fetch(uint32_t stage, const C &c, int n) {
+        if (left <= 0) return;
+        if (VECTOR) {
+            const uint32_t to = stage + c.start * (int)sizeof(T);
+#pragma unroll
+            for (int i = 0; i < P / VEC; i++)
+                if (c.full || i * C::STEP < c.left) copy_async16(to + i * C::STEP * (int)sizeof(T), at + c.start + i * C::STEP);
+        } else {
+            const int threads = G ? G : blockDim.x, t = G ? threadIdx.x % (G ? G : 1) : threadIdx.x;
+            const uintptr_t base = reinterpret_cast<uintptr_t>(at) & ~(uintptr_t)15;
+            const int from = (int)(reinterpret_cast<uintptr_t>(at) & 15), to = from + n * (int)sizeof(T);
+            // as far as a row at any offset goes, with zeros past this one's end
+            for (int p = 16 * t; p < n * (int)sizeof(T) + 15; p += 16 * threads) {
+                if (p < from && base < origin)
+                    for (int e = from; e < 16; e += sizeof(T)) {
+                        using U = typename Word<sizeof(T)>::U;
+                        Word<sizeof(T)>::store(stage + e, e < to ? *reinterpret_cast<const U *>(base + e) : U(0));
+                    }
+                else
+                    copy_async16(stage + p, p < to ? reinterpret_cast<const void *>(base + p) : at, to - p < 0 ? 0 : to - p < 16 ? to - p : 16);
+            }
+        }
+        left--;
+        at += pitch;
+    }
+    // Zeros past the rows' ends in `count` places, before the first copies.
+    static __device__ __forceinline__ void clear(uint32_t stage, int count, int bytes, int n) {
+        const int threads = G ? G : blockDim.x, t = G ? threadIdx.x % (G ? G : 1) : threadIdx.x;
+        for (int s = 0; s < count; s++)
+            for (int p = n * (int)sizeof(T) / 16 * 16 + 16 * t; p < bytes; p += 16 * threads)
+                Word<16>::store(stage + s * bytes + p, make_uint4(0u, 0u, 0u, 0u));
+    }
+    // Where the thread's first element of the row at `row` is in its place.
+    static __device__ __forceinline__ uint32_t staged(uint32_t stage, const T *row, const C &c) {
+        return stage + (VECTOR ? 0 : (uint32_t)(reinterpret_cast<uintptr_t>(row) & 15)) + c.start * (int)sizeof(T);
+    }
+};
+
+// Forward of long rows: a block takes row after row.
+template <class T, int VEC, int DEPTH>
+__global__ void __launch_bounds__(1024, 1)
+    long_forward_kernel(const T *__restrict__ x, int64_t ldx, int64_t rows, int n, const float *__restrict__ w,
+                        const float *__restrict__ b, float eps, T *__restrict__ y, int64_t ldy,
+                        float *__restrict__ mean, float *__restrict__ rstd) {
+    constexpr int P = 16;
+    using R = Rows<T, VEC, P, 0>;
+    using W = SharedWeights<VEC, P>;
+    extern __shared__ __align__(16) unsigned char space[];
+    __shared__ __align__(16) float part[4][32];
+    const Columns<VEC, P, 0> c(n);
+    const int warps = blockDim.x >> 5, bytes = R::bytes(warps), total = W::floats(warps);
+    float *const sw = reinterpret_cast<float *>(space), *const sb = sw + total;
+    const uint32_t ring = shared_address(space) + 8 * total;
+    R::clear(ring, DEPTH, bytes, n);
+    for (int i = threadIdx.x; i < 128; i += blockDim.x) (&part[0][0])[i] = 0.f;
+    W::fill(sw, w, 1.f, n, total);
+    W::fill(sb, b, 0.f, n, total);
+    __syncthreads();
+    const int64_t step = gridDim.x;
+    int64_t r = blockIdx.x;
+    R next(x, ldx, rows, r, step);
+#pragma unroll
+    for (int d = 0; d < DEPTH - 1; d++) {
+        next.fetch(ring + d * bytes, c, n);
+        commit_copies();
+    }
+    if (!R::VECTOR) {
+        wait_copies<DEPTH - 2>();
+        __syncthreads();
     }
     const float inv_n = 1.f / n;
-    Held<T, VEC, P> now, next;
-    if (base + mine < rows) now.load(x + (base + mine) * ldx, t, threads, n);
-    int turn = 0;
-    for (int64_t first = base; first < rows; first += step) {  // the lanes of a warp stay together
-        const int64_t r = first + mine;
-        const bool live = r < rows;
-        if (r + step < rows) next.load(x + (r + step) * ldx, t, threads, n);
-        float s[1] = {0.f};
-#pragma unroll
-        for (int k = 0; k < P; k++) s[0] += now.at(k);  // zeros past the row
-        row_sums<G>(s, part[turn]);
-        const float mu = s[0] * inv_n;
-        s[0] = 0.f;
-#pragma unroll
-        for (int k = 0; k < P; k++) {
-            const float c = now.at(k) - mu;
-            if ((t + k / VEC * threads) * VEC < n) s[0] += c * c;
-        }
-        row_sums<G>(s, part[turn + 1]);
+    const T *row = x + r * ldx;
+    T *out = y + r * ldy + c.start;
+    int slot = 0, turn = 0;
+    for (; r < rows; r += step) {
+        if (R::VECTOR) wait_copies<DEPTH - 2>();
+        Held<T, VEC, P, 0> h;
+        h.load_staged(R::staged(ring + slot * bytes, row, c));
+        const float mu = team_sum<0>(plain_sum(h), part[turn]) * inv_n;
+        const float mine = square_sum(h, c, mu);
+        // every thread has read the row before this one: its place takes the next
+        next.fetch(ring + (slot == 0 ? DEPTH - 1 : slot - 1) * bytes, c, n);
+        commit_copies();
+        if (!R::VECTOR) wait_copies<DEPTH - 2>();
+        const float rs = 1.f / sqrtf(team_sum<0>(mine, part[turn + 1]) * inv_n + eps);
         turn ^= 2;
-        const float rs = 1.f / sqrtf(s[0] * inv_n + eps);
-        if (live) {
-            float o[P];
-            if (KEEP) {
+        float2 o[P / 2];
 #pragma unroll
-                for (int k = 0; k < P; k++) o[k] = (now.at(k) - mu) * rs * wk[k] + bk[k];
-            } else {
-#pragma unroll
-                for (int k = 0; k < P; k++) {
-                    const int j = (t + k / VEC * threads) * VEC + k % VEC;
-                    o[k] = (now.at(k) - mu) * rs;
-                    if (j < n) o[k] = o[k] * (w ? __ldg(w + j) : 1.f) + (b ? __ldg(b + j) : 0.f);
-                }
-            }
-            store_row<T, VEC, P>(y + r * ldy, t, threads, n, o);
-            if (t == 0) {
-                if (mean) mean[r] = mu;
-                if (rstd) rstd[r] = rs;
-            }
+        for (int k = 0; k < P / 2; k++)
+            o[k] = __ffma2_rn(__fmul2_rn(__fadd2_rn(h.pair(k), both(-mu)), both(rs)), W::pair(sw, c.start, k, total), W::pair(sb, c.start, k, total));
+        store_row<T, VEC, P, 0>(out, c, o);
+        if (threadIdx.x == 0) {
+            if (mean) mean[r] = mu;
+            if (rstd) rstd[r] = rs;
         }
-        now = next;
+        row += step * ldx;
+        out += step * ldy;
+        slot = slot == DEPTH - 1 ? 0 : slot + 1;
     }
 }
 
-// dx of the rows that a block takes, and its partial sums of dw and db in work[blockIdx.x].
-template <class T, int VEC, int P, int G>
-__global__ void __launch_bounds__(G ? 256 : 512)
+// dx of the rows that a team (8 or 32 lanes, or the block) takes, and the
+// block's partial sums of dw and db in work[blockIdx.x]. Up to P = 16 the weights
+// and dy w stay in registers; with 32 the weights are in shared memory and dy w
+// is taken again.
+template <class T, int VEC, int P, int G, int DEPTH, int MOST>
+__global__ void __launch_bounds__(MOST, P == 8 && G ? 3 : P == 8 || MOST == 256 ? 2 : 1)
     backward_kernel(const T *__restrict__ dy, int64_t lddy, const T *__restrict__ x, int64_t ldx, int64_t rows, int n,
                     const float *__restrict__ w, const float *__restrict__ mean, const float *__restrict__ rstd,
                     T *__restrict__ dx, int64_t lddx, float *__restrict__ work) {
-    constexpr bool KEEP = P <= 16;
-    constexpr int GROUPS = G ? 256 / (G ? G : 1) : 1;
-    __shared__ float part[2][2][32];
-    __shared__ float joined[G ? 256 * P : 1];
-    const int threads = G ? G : blockDim.x, t = G ? threadIdx.x % G : threadIdx.x;
-    const int64_t step = (int64_t)gridDim.x * GROUPS;
-    const int64_t base = (int64_t)blockIdx.x * GROUPS, mine = G ? threadIdx.x / (G ? G : 1) : 0;
-    float wk[KEEP ? P : 1], aw[P], ab[P];
-    if (KEEP) load_weights<VEC>(w, t, threads, n, 1.f, wk);
-#pragma unroll
-    for (int k = 0; k < P; k++) aw[k] = ab[k] = 0.f;
-    const float inv_n = 1.f / n;
-    Held<T, VEC, P> xv, dv, xn, dn;
-    float mu = 0.f, rs = 0.f, mun = 0.f, rsn = 0.f;
-    auto fetch = [&](int64_t r, Held<T, VEC, P> &a, Held<T, VEC, P> &d, float &m, float &s) {
-        a.load(x + r * ldx, t, threads, n);
-        d.load(dy + r * lddy, t, threads, n);
-        m = __ldg(mean + r);
-        s = __ldg(rstd + r);
+    constexpr int TEAMS = G ? 256 / (G ? G : 1) : 1;
+    using C = Columns<VEC, P, G>;
+    using R = Rows<T, VEC, P, G>;
+    using W = SharedWeights<VEC, P>;
+    constexpr bool KEEP = P <= 16, EARLY = R::VECTOR && DEPTH > 2;
+    extern __shared__ __align__(16) unsigned char space[];
+    __shared__ __align__(16) float part[2][64];
+    __shared__ float stats[TEAMS][DEPTH][2];  // mean and rstd of the rows in their places
+    pdl_launch();
+    const C c(n);
+    const int warps = blockDim.x >> 5, team = G ? threadIdx.x / (G ? G : 1) : 0, bytes = R::bytes(warps), total = W::floats(warps);
+    const uint32_t ring = shared_address(space) + team * (DEPTH * 2 * bytes);
+    float *const sw = reinterpret_cast<float *>(space + TEAMS * DEPTH * 2 * bytes);
+    R::clear(ring, 2 * DEPTH, bytes, n);
+    for (int i = threadIdx.x; i < 128; i += blockDim.x) (&part[0][0])[i] = 0.f;
+    if (!KEEP) W::fill(sw, w, 1.f, n, total);
+    __syncthreads();
+    const int64_t step = (int64_t)gridDim.x * TEAMS, first = (int64_t)blockIdx.x * TEAMS + team;
+    R next_x(x, ldx, rows, first, step), next_dy(dy, lddy, rows, first, step);
+    const int t = G ? threadIdx.x % (G ? G : 1) : threadIdx.x;
+    const float *next_stat = (t == 0 ? mean : rstd) + first;
+    const uint32_t stat_at = shared_address(&stats[team][0][0]);
+    auto fetch = [&](int slot) {
+        if (t < 2 && next_x.left > 0) {
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(stat_at + 8 * slot + 4 * t), "l"(next_stat) : "memory");
+            next_stat += step;
+        }
+        next_x.fetch(ring + slot * 2 * bytes, c, n);
+        next_dy.fetch(ring + slot * 2 * bytes + bytes, c, n);
+        commit_copies();
     };
-    if (base + mine < rows) fetch(base + mine, xv, dv, mu, rs);
-    int turn = 0;
-    for (int64_t first = base; first < rows; first += step) {
-        const int64_t r = first + mine;
-        const bool live = r < rows;
-        if (r + step < rows) fetch(r + step, xn, dn, mun, rsn);
-        float s[2] = {0.f, 0.f};
-        if (live) {
 #pragma unroll
-            for (int k = 0; k < P; k++) {
-                const int j = (t + k / VEC * threads) * VEC + k % VEC;
-                const float d = dv.at(k), xhat = (xv.at(k) - mu) * rs;
-                const float g = d * (KEEP ? wk[KEEP ? k : 0] : w && j < n ? __ldg(w + j) : 1.f);  // d is zero past the row
-                s[0] += g;
-                s[1] += g * xhat;
-                aw[k] += d * xhat;
-                ab[k] += d;
+    for (int d = 0; d < DEPTH - 1; d++) fetch(d);
+    float2 wk[P / 2], aw[P / 2], ab[P / 2];
+    if (KEEP) load_weights<VEC, P, G>(w, c, 1.f, wk);
+#pragma unroll
+    for (int k = 0; k < P / 2; k++) aw[k] = ab[k] = both(0.f);
+    auto weight = [&](int k) { return KEEP ? wk[k] : W::pair(sw, c.start, k, total); };
+    const float inv_n = 1.f / n;
+    wait_copies<DEPTH - 2>();
+    __syncthreads();
+    float2 stat = load_shared<float2>(stat_at);
+    const T *xr = x + first * ldx, *dr = dy + first * lddy;
+    T *out_row = dx + first * lddx + c.start;
+    int slot = 0, turn = 0;
+    const int rounds = (int)((rows - (int64_t)blockIdx.x * TEAMS + step - 1) / step);  // of the block's first team
+    int64_t r = first;
+    for (int round = 0; round < rounds; round++) {
+        const bool live = r < rows;  // the teams of a warp stay together
+        const float mu = stat.x, rs = stat.y;
+        // the place of the row before this one takes the next: at once where it was the thread's
+        // own, else when the team has done with it
+        if (EARLY) fetch(slot == 0 ? DEPTH - 1 : slot - 1);
+        const uint32_t stage = ring + slot * 2 * bytes, ds = R::staged(stage + bytes, dr, c);
+        float2 xhat[P / 2], g[KEEP ? P / 2 : 1], sum1 = both(0.f), sum2 = both(0.f);
+        if (TEAMS == 1 || live) {
+            Held<T, VEC, P, G> xv, dv;  // zeros past the row
+            xv.load_staged(R::staged(stage, xr, c));
+            dv.load_staged(ds);
+#pragma unroll
+            for (int k = 0; k < P / 2; k++) {
+                const float2 d = dv.pair(k), h = __fmul2_rn(__fadd2_rn(xv.pair(k), both(-mu)), both(rs)), gk = __fmul2_rn(d, weight(k));
+                sum1 = __fadd2_rn(sum1, gk);
+                sum2 = __ffma2_rn(gk, h, sum2);
+                aw[k] = __ffma2_rn(d, h, aw[k]);
+                ab[k] = __fadd2_rn(ab[k], d);
+                xhat[k] = h;
+                if (KEEP) g[KEEP ? k : 0] = gk;
             }
         }
-        row_sums<G>(s, part[turn]);
+        float s1 = sum1.x + sum1.y, s2 = sum2.x + sum2.y;
+        wait_copies<EARLY ? DEPTH - 2 : DEPTH - 3>();  // for the row after this one
+        team_sums<G>(s1, s2, part[turn]);
         turn ^= 1;
-        if (live && dx) {
-            const float s1 = s[0] * inv_n, s2 = s[1] * inv_n;
-            float o[P];
+        if (G) __syncwarp();
+        stat = load_shared<float2>(stat_at + 8 * (slot == DEPTH - 1 ? 0 : slot + 1));
+        if (!EARLY) fetch(slot == 0 ? DEPTH - 1 : slot - 1);
+        if ((TEAMS == 1 || live) && dx) {
+            const float2 c1 = both(-rs * s1 * inv_n), c2 = both(-rs * s2 * inv_n);
+            Held<T, VEC, P, G> dv;
+            if (!KEEP) dv.load_staged(ds);
 #pragma unroll
-            for (int k = 0; k < P; k++) {
-                const int j = (t + k / VEC * threads) * VEC + k % VEC;
-                const float g = dv.at(k) * (KEEP ? wk[KEEP ? k : 0] : w && j < n ? __ldg(w + j) : 1.f);
-                o[k] = rs * (g - s1 - (xv.at(k) - mu) * rs * s2);
-            }
-            store_row<T, VEC, P>(dx + r * lddx, t, threads, n, o);
+            for (int k = 0; k < P / 2; k++)
+                xhat[k] = __ffma2_rn(xhat[k], c2, __ffma2_rn(KEEP ? g[KEEP ? k : 0] : __fmul2_rn(dv.pair(k), weight(k)), both(rs), c1));
+            store_row<T, VEC, P, G>(out_row, c, xhat);
         }
-        xv = xn;
-        dv = dn;
-        mu = mun;
-        rs = rsn;
+        r += step;
+        xr += step * ldx;
+        dr += step * lddy;
+        out_row += step * lddx;
+        slot = slot == DEPTH - 1 ? 0 : slot + 1;
     }
     if (!work) return;
-    float *out = work + (int64_t)blockIdx.x * 2 * n;
+    wait_copies<0>();
+    float *out = work + (int64_t)blockIdx.x * 2 * n + c.start, *joined = reinterpret_cast<float *>(space);
 #pragma unroll
     for (int half = 0; half < 2; half++) {
-        float(&a)[P] = half ? ab : aw;
-        if (G) {  // the groups' sums, added in their order
+        float2(&a)[P / 2] = half ? ab : aw;
+        if (G) {  // the teams' sums, added in their order
             __syncthreads();
 #pragma unroll
-            for (int k = 0; k < P; k++) joined[threadIdx.x * P + k] = a[k];
+            for (int k = 0; k < P / 2; k++) *reinterpret_cast<float2 *>(joined + (k * 256 + threadIdx.x) * 2) = a[k];
             __syncthreads();
-            if (mine == 0)
+            if (team == 0)
 #pragma unroll
-                for (int k = 0; k < P; k++) {
-                    a[k] = 0.f;
-                    for (int g = 0; g < GROUPS; g++) a[k] += joined[(g * threads + t) * P + k];
+                for (int k = 0; k < P / 2; k++) {
+                    a[k] = both(0.f);
+                    for (int q = 0; q < TEAMS; q++) a[k] = __fadd2_rn(a[k], *reinterpret_cast<float2 *>(joined + (k * 256 + q * G + threadIdx.x) * 2));
                 }
         }
-        if (mine == 0)
+        if (team == 0)
 #pragma unroll
-            for (int k = 0; k < P; k++) {
-                const int j = (t + k / VEC * threads) * VEC + k % VEC;
-                if (j < n) out[half * n + j] = a[k];
-            }
+            for (int k = 0; k < P; k++)
+                if (C::offset(k) < c.left) out[half * n + C::offset(k)] = k & 1 ? a[k / 2].y : a[k / 2].x;
     }
 }
 
-// dw and db from the blocks' partial sums: 32 columns a block, in 8 slices of the parts.
-__global__ void __launch_bounds__(256)
+// dw and db from the blocks' partial sums: 32 columns a block, in 32 slices of the parts.
+__global__ void __launch_bounds__(1024)
     reduce_kernel(const float *__restrict__ work, int parts, int n, float *__restrict__ dw, float *__restrict__ db) {
-    __shared__ float sums[8][32];
+    __shared__ float sums[32][33];
     pdl_wait();
     const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, j = blockIdx.x * 32 + lane;
     float s = 0.f;
     if (j < 2 * n) {
 #pragma unroll 8
-        for (int p = slice; p < parts; p += 8) s += work[(int64_t)p * 2 * n + j];
+        for (int p = slice; p < parts; p += 32) s += work[(int64_t)p * 2 * n + j];
     }
     sums[slice][lane] = s;
     __syncthreads();
-    if (slice || j >= 2 * n) return;
-    s = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; i++) s += sums[i][lane];
-    if (j < n) {
-        if (dw) dw[j] = s;
+    s = warp_sum(sums[lane][slice]);  // warp `slice` adds the slices of its column
+    const int c = blockIdx.x * 32 + slice;
+    if (lane || c >= 2 * n) return;
+    if (c < n) {
+        if (dw) dw[c] = s;
     } else if (db)
-        db[j - n] = s;
+        db[c - n] = s;
 }
 
 // ---------------------------------------------------------------- rows too long for registers
@@ -267,20 +639,18 @@ __global__ void __launch_bounds__(WIDE)
     wide_forward_kernel(const T *__restrict__ x, int64_t ldx, int64_t rows, int n, const float *__restrict__ w,
                         const float *__restrict__ b, float eps, T *__restrict__ y, int64_t ldy,
                         float *__restrict__ mean, float *__restrict__ rstd) {
-    __shared__ float part[2][1][32];
+    __shared__ __align__(16) float part[2][32];
     for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
         const T *xr = x + r * ldx;
-        float s[1] = {0.f};
-        for (int j = threadIdx.x; j < n; j += WIDE) s[0] += to_f32(xr[j]);
-        row_sums<0>(s, part[0]);
-        const float mu = s[0] / n;
-        s[0] = 0.f;
+        float s = 0.f;
+        for (int j = threadIdx.x; j < n; j += WIDE) s += to_f32(xr[j]);
+        const float mu = team_sum<0>(s, part[0]) / n;
+        s = 0.f;
         for (int j = threadIdx.x; j < n; j += WIDE) {
             const float c = to_f32(xr[j]) - mu;
-            s[0] += c * c;
+            s += c * c;
         }
-        row_sums<0>(s, part[1]);
-        const float rs = 1.f / sqrtf(s[0] / n + eps);
+        const float rs = 1.f / sqrtf(team_sum<0>(s, part[1]) / n + eps);
         for (int j = threadIdx.x; j < n; j += WIDE)
             y[r * ldy + j] = from_f32<T>((to_f32(xr[j]) - mu) * rs * (w ? w[j] : 1.f) + (b ? b[j] : 0.f));
         if (threadIdx.x == 0) {
@@ -295,19 +665,20 @@ __global__ void __launch_bounds__(WIDE)
     wide_rows_kernel(const T *__restrict__ dy, int64_t lddy, const T *__restrict__ x, int64_t ldx, int64_t rows, int n,
                      const float *__restrict__ w, const float *__restrict__ mean, const float *__restrict__ rstd,
                      T *__restrict__ dx, int64_t lddx) {
-    __shared__ float part[2][2][32];
+    __shared__ __align__(16) float part[2][64];
     int turn = 0;
     for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
         const float mu = mean[r], rs = rstd[r];
-        float s[2] = {0.f, 0.f};
+        float s1 = 0.f, s2 = 0.f;
         for (int j = threadIdx.x; j < n; j += WIDE) {
             const float g = to_f32(dy[r * lddy + j]) * (w ? w[j] : 1.f);
-            s[0] += g;
-            s[1] += g * ((to_f32(x[r * ldx + j]) - mu) * rs);
+            s1 += g;
+            s2 += g * ((to_f32(x[r * ldx + j]) - mu) * rs);
         }
-        row_sums<0>(s, part[turn]);
+        team_sums<0>(s1, s2, part[turn]);
         turn ^= 1;
-        const float s1 = s[0] / n, s2 = s[1] / n;
+        s1 /= n;
+        s2 /= n;
         for (int j = threadIdx.x; j < n; j += WIDE) {
             const float g = to_f32(dy[r * lddy + j]) * (w ? w[j] : 1.f);
             dx[r * lddx + j] = from_f32<T>(rs * (g - s1 - (to_f32(x[r * ldx + j]) - mu) * rs * s2));
@@ -340,54 +711,39 @@ __global__ void __launch_bounds__(256)
 // Threads of a block that holds rows of n, P elements each.
 static int block_threads(int n, int p) { return ((n + p - 1) / p + 31) / 32 * 32; }
 
-// Rows at a time and blocks of the backward pass. More blocks hide more latency
-// but write more partial sums: about 768 threads an SM.
-static void backward_shape(int64_t rows, int n, int *threads, int *grid) {
-    int per_block = 1;
-    if (n <= 64)
-        *threads = 256, per_block = 32;
-    else if (n <= 512)
-        *threads = 256, per_block = 8;
-    else
-        *threads = block_threads(n, n <= 2048 ? 8 : 16);
-    const int64_t want = (rows + per_block - 1) / per_block;
-    const int full = SMS * (*threads >= 384 ? 2 : 768 / *threads);
-    *grid = (int)(want < 1 ? 1 : want < full ? want : full);
-}
-static int parts_of(int64_t rows, int n) {
-    if (n > HELD_BACKWARD) return (int)(rows < 1 ? 1 : rows < 16 ? rows : 16);
-    int threads, grid;
-    backward_shape(rows, n, &threads, &grid);
-    return grid;
-}
-
 template <class T> static bool vectors_of(const void *p, int64_t ld) {
     return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld * (int64_t)sizeof(T) % 16 == 0;
+}
+static bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+constexpr size_t SPACE = 225 * 1024;  // shared memory of an SM that blocks can have
+
+template <class K> static int allow_space(K kernel, size_t smem) {
+    return smem > 40 * 1024 ? (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) : 0;
 }
 
 template <class T, int VEC>
 static int forward(const T *x, int64_t ldx, int64_t rows, int n, const float *w, const float *b, float eps, T *y,
                    int64_t ldy, float *mean, float *rstd, cudaStream_t s) {
-#define D1_LN_FORWARD(P, G, threads, per_block, resident)                                                             \
-    forward_kernel<T, VEC, P, G>                                                                                      \
-        <<<(int)((rows + per_block - 1) / per_block < SMS * (resident) ? (rows + per_block - 1) / per_block           \
-                                                                       : SMS * (resident)),                          \
-           threads, 0, s>>>(x, ldx, rows, n, w, b, eps, y, ldy, mean, rstd)
-    if (n <= 64)
-        D1_LN_FORWARD(8, 8, 256, 32, 6);
-    else if (n <= 256)
-        D1_LN_FORWARD(8, 32, 256, 8, 6);
-    else if (n <= 512)
-        D1_LN_FORWARD(16, 32, 256, 8, 4);
-    else if (n <= 1024)
-        D1_LN_FORWARD(32, 32, 256, 8, 4);
-    else if (n <= 8192) {
-        const int threads = block_threads(n, 16);
-        D1_LN_FORWARD(16, 0, threads, 1, 1024 / threads);
-    } else {
-        const int threads = block_threads(n, 32);
-        D1_LN_FORWARD(32, 0, threads, 1, threads <= 512 ? 2 : 1);
-    }
+#define D1_LN_FORWARD(P, G, R, threads)                                                                               \
+    do {                                                                                                              \
+        const int64_t per_block = (int64_t)R * ((G) ? 256 / ((G) ? (G) : 1) : 1), blocks = (rows + per_block - 1) / per_block; \
+        if (blocks > INT32_MAX) return D1_ERR_TOO_LARGE;                                                              \
+        forward_kernel<T, VEC, P, G, R><<<(int)blocks, threads, 0, s>>>(x, ldx, rows, n, w, b, eps, y, ldy, mean, rstd); \
+        return (int)cudaGetLastError();                                                                               \
+    } while (0)
+    if (n <= 64) D1_LN_FORWARD(8, 8, 2, 256);
+    if (n <= 256) D1_LN_FORWARD(8, 32, 2, 256);
+    if (n <= 512) D1_LN_FORWARD(16, 32, 2, 256);
+    if (n <= 1024) D1_LN_FORWARD(32, 32, 1, 256);
+    const int threads = block_threads(n, 16), warps = threads / 32, depth = n <= 8192 ? 4 : 3;
+    const size_t smem = (size_t)depth * Rows<T, VEC, 16, 0>::bytes(warps) + 8 * (size_t)SharedWeights<VEC, 16>::floats(warps);
+    if (threads > 1024 || smem + 2048 > SPACE) D1_LN_FORWARD(32, 0, 1, block_threads(n, 32));
+    const auto kernel = depth == 4 ? long_forward_kernel<T, VEC, 4> : long_forward_kernel<T, VEC, 3>;
+    if (const int e = allow_space(kernel, smem)) return e;
+    const int by_threads = 1024 / threads, by_space = (int)(SPACE / (smem + 2048));
+    const int64_t full = (int64_t)SMS * (by_threads < by_space ? by_threads : by_space);
+    kernel<<<(int)(rows < full ? rows : full), threads, smem, s>>>(x, ldx, rows, n, w, b, eps, y, ldy, mean, rstd);
     return (int)cudaGetLastError();
 }
 
@@ -400,28 +756,59 @@ static int forward_any(const void *x, int64_t ldx, int64_t rows, int n, const fl
             (const T *)x, ldx, rows, n, w, b, eps, (T *)y, ldy, mean, rstd);
         return (int)cudaGetLastError();
     }
-    if (n % VEC == 0 && vectors_of<T>(x, ldx) && vectors_of<T>(y, ldy))
+    if (n % VEC == 0 && vectors_of<T>(x, ldx) && vectors_of<T>(y, ldy) && aligned16(w) && aligned16(b))
         return forward<T, VEC>((const T *)x, ldx, rows, n, w, b, eps, (T *)y, ldy, mean, rstd, s);
-    return forward<T, 1>((const T *)x, ldx, rows, n, w, b, eps, (T *)y, ldy, mean, rstd, s);
+    return forward<T, sizeof(T) == 2 ? 2 : 1>((const T *)x, ldx, rows, n, w, b, eps, (T *)y, ldy, mean, rstd, s);
+}
+
+// How the backward pass runs: teams of 8 or 32 lanes, or blocks (lanes = 0),
+// with P elements a thread, DEPTH rows in shared memory and as many blocks as
+// the SMs hold at once (more would only write more partial sums).
+struct Backward {
+    int lanes, p, depth, threads, grid;
+    size_t smem;
+};
+static Backward backward_shape(int64_t rows, int n, int size, bool vector) {
+    Backward o;
+    o.lanes = n <= 64 ? 8 : n <= 512 ? 32 : 0;
+    o.p = n <= 256 || (n > 512 && n <= 1024) ? 8 : n <= 8192 ? 16 : 32;
+    o.threads = o.lanes ? 256 : block_threads(n, o.p);
+    const int teams = o.lanes ? 256 / o.lanes : 1;
+    const size_t pair = 2 * (size_t)((o.lanes ? o.lanes : o.threads) * o.p * size + (vector ? 0 : 16));  // a row of x and one of dy
+    o.depth = o.p == 32 ? 2 : 4 * pair > 160 * 1024 ? 3 : 4;
+    o.smem = o.depth * pair * teams + (o.p == 32 ? 4 * (size_t)o.threads * 32 : 0);
+    if (o.lanes && o.smem < (size_t)256 * o.p * 4) o.smem = (size_t)256 * o.p * 4;  // the teams' sums, joined at the end
+    const int by_threads = (o.p == 8 ? o.lanes ? 768 : 1024 : 512) / o.threads, by_space = (int)(SPACE / (o.smem + 2048));
+    const int resident = by_threads < by_space ? by_threads : by_space;
+    const int64_t want = (rows + teams - 1) / teams, full = (int64_t)SMS * (resident < 1 ? 1 : resident);
+    o.grid = (int)(want < 1 ? 1 : want < full ? want : full);
+    return o;
+}
+// Rows that the backward pass holds: over 8,192 elements only 16-bit vectors are.
+static bool held_backward(int n, int size, bool vector) { return n <= 8192 || (n <= 16384 && size == 2 && vector); }
+static int parts_of(int64_t rows, int n, int size, bool vector) {
+    if (!held_backward(n, size, vector)) return (int)(rows < 1 ? 1 : rows < 16 ? rows : 16);
+    return backward_shape(rows, n, size, vector).grid;
 }
 
 template <class T, int VEC>
 static int backward(const T *dy, int64_t lddy, const T *x, int64_t ldx, int64_t rows, int n, const float *w,
                     const float *mean, const float *rstd, T *dx, int64_t lddx, float *work, cudaStream_t s) {
-    int threads, grid;
-    backward_shape(rows, n, &threads, &grid);
-#define D1_LN_BACKWARD(P, G) \
-    backward_kernel<T, VEC, P, G><<<grid, threads, 0, s>>>(dy, lddy, x, ldx, rows, n, w, mean, rstd, dx, lddx, work)
-    if (n <= 64)
-        D1_LN_BACKWARD(8, 8);
-    else if (n <= 256)
-        D1_LN_BACKWARD(8, 32);
-    else if (n <= 512)
-        D1_LN_BACKWARD(16, 32);
-    else if (n <= 2048)
-        D1_LN_BACKWARD(8, 0);
-    else
-        D1_LN_BACKWARD(16, 0);
+    constexpr bool VECTOR = VEC * sizeof(T) == 16;
+    const Backward o = backward_shape(rows, n, sizeof(T), VECTOR);
+    auto kernel = backward_kernel<T, VEC, 8, 0, 4, 512>;
+    if (o.lanes == 8)
+        kernel = backward_kernel<T, VEC, 8, 8, 4, 256>;
+    else if (o.lanes == 32)
+        kernel = o.p == 8 ? backward_kernel<T, VEC, 8, 32, 4, 256> : backward_kernel<T, VEC, 16, 32, 4, 256>;
+    else if (o.p == 16)
+        kernel = o.threads <= 256 ? backward_kernel<T, VEC, 16, 0, 4, 256>
+                 : o.depth == 4   ? backward_kernel<T, VEC, 16, 0, 4, 512>
+                                  : backward_kernel<T, VEC, 16, 0, 3, 512>;
+    if constexpr (VECTOR && sizeof(T) == 2)
+        if (o.p == 32) kernel = backward_kernel<T, VEC, 32, 0, 2, 512>;
+    if (const int e = allow_space(kernel, o.smem)) return e;
+    kernel<<<o.grid, o.threads, o.smem, s>>>(dy, lddy, x, ldx, rows, n, w, mean, rstd, dx, lddx, work);
     return (int)cudaGetLastError();
 }
 
@@ -430,10 +817,11 @@ static int backward_any(const void *dy, int64_t lddy, const void *x, int64_t ldx
                         const float *mean, const float *rstd, void *dx, int64_t lddx, float *dw, float *db,
                         float *work, cudaStream_t s) {
     constexpr int VEC = 16 / sizeof(T);
-    const int parts = parts_of(rows, n);
-    const bool sums = dw || db;
+    const bool sums = dw || db, vector = n % VEC == 0 && vectors_of<T>(x, ldx) && vectors_of<T>(dy, lddy) &&
+                                         (!dx || vectors_of<T>(dx, lddx)) && aligned16(w);
+    const int parts = parts_of(rows, n, sizeof(T), vector);
     int e = 0;
-    if (n > HELD_BACKWARD) {
+    if (!held_backward(n, sizeof(T), vector)) {
         if (dx && rows)
             wide_rows_kernel<T><<<(int)(rows < SMS * 2 ? rows : SMS * 2), WIDE, 0, s>>>(
                 (const T *)dy, lddy, (const T *)x, ldx, rows, n, w, mean, rstd, (T *)dx, lddx);
@@ -442,15 +830,14 @@ static int backward_any(const void *dy, int64_t lddy, const void *x, int64_t ldx
             wide_columns_kernel<T><<<dim3((n + 255) / 256, parts), 256, 0, s>>>((const T *)dy, lddy, (const T *)x, ldx,
                                                                                 rows, n, mean, rstd, work);
         e = (int)cudaGetLastError();
-    } else if (n % VEC == 0 && vectors_of<T>(x, ldx) && vectors_of<T>(dy, lddy) && (!dx || vectors_of<T>(dx, lddx)))
-        e = backward<T, VEC>((const T *)dy, lddy, (const T *)x, ldx, rows, n, w, mean, rstd, (T *)dx, lddx,
-                             sums ? work : nullptr, s);
+    } else if (vector)
+        e = backward<T, VEC>((const T *)dy, lddy, (const T *)x, ldx, rows, n, w, mean, rstd, (T *)dx, lddx, sums ? work : nullptr, s);
     else
-        e = backward<T, 1>((const T *)dy, lddy, (const T *)x, ldx, rows, n, w, mean, rstd, (T *)dx, lddx,
-                           sums ? work : nullptr, s);
+        e = backward<T, sizeof(T) == 2 ? 2 : 1>((const T *)dy, lddy, (const T *)x, ldx, rows, n, w, mean, rstd, (T *)dx, lddx,
+                                                sums ? work : nullptr, s);
     if (e || !sums) return e;
     cudaLaunchAttribute attr;
-    const cudaLaunchConfig_t cfg = pdl_config(dim3((2 * n + 31) / 32), dim3(256), 0, s, &attr);
+    const cudaLaunchConfig_t cfg = pdl_config(dim3((2 * n + 31) / 32), dim3(1024), 0, s, &attr);
     return (int)cudaLaunchKernelEx(&cfg, reduce_kernel, (const float *)work, parts, n, dw, db);
 }
 
@@ -474,7 +861,12 @@ extern "C" int d1_layer_norm(const void *x, int64_t ldx, int type, int64_t rows,
 
 extern "C" int d1_layer_norm_parts(int64_t rows, int n) {
     if (rows < 0 || n < 1) return D1_ERR_BAD_ARGUMENT;
-    return d1::ln::parts_of(rows, n);
+    int most = 0;  // of either size of element and either alignment
+    for (int k = 0; k < 4; k++) {
+        const int parts = d1::ln::parts_of(rows, n, k & 1 ? 4 : 2, k & 2);
+        if (parts > most) most = parts;
+    }
+    return most;
 }
 
 extern "C" int d1_layer_norm_backward(const void *dy, int64_t lddy, const void *x, int64_t ldx, int type, int64_t rows,
