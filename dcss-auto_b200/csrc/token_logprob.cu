@@ -32,6 +32,7 @@ namespace d1 {
 namespace lp {
 
 constexpr int THREADS = 256, WARPS = THREADS / 32, MAX_TOP = 32, MAX_CLUSTER = 8, CAP = 768;
+constexpr int SMS = 148;
 constexpr int UNROLL = 4;           // vectors a thread has in flight
 constexpr int SHORT_VOCAB = 1024;   // rows up to here are held in the registers of 8 or 32 lanes
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
@@ -68,23 +69,34 @@ struct Acc {
     float m, s, t;
 };
 
-template <int N> __device__ __forceinline__ void take(Acc &a, const float (&x)[N], float c) {
-    float top = a.m;
-#pragma unroll
-    for (int k = 0; k < N; k++) top = max_nan(top, x[k]);
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
+// top: the largest of x (a NaN if there is one).
+template <int N> __device__ __forceinline__ void take(Acc &a, const float2 (&x)[N], float top, float c) {
+    top = max_nan(top, a.m);
     if (!(top <= a.m)) {
         const float d = fmaxf((a.m - top) * c, -1e4f), f = ex2(d);
         a.t = f * fmaf(d, a.s, a.t);
         a.s *= f;
         a.m = top;
     }
+    float2 s = make_float2(a.s, 0.f), t = make_float2(a.t, 0.f);
 #pragma unroll
     for (int k = 0; k < N; k++) {
         // below 2^-200 the term is zero; the bound also takes in -inf (and -inf - -inf)
-        const float z = fmaxf((x[k] - a.m) * c, -200.f), e = ex2(z);
-        a.s += e;
-        a.t = fmaf(z, e, a.t);
+        float2 z = __fmul2_rn(__fadd2_rn(x[k], both(-a.m)), both(c));
+        z.x = fmaxf(z.x, -200.f);
+        z.y = fmaxf(z.y, -200.f);
+        const float2 e = make_float2(ex2(z.x), ex2(z.y));
+        s = __fadd2_rn(s, e);
+        t = __ffma2_rn(z, e, t);
     }
+    a.s = s.x + s.y;
+    a.t = t.x + t.y;
+}
+__device__ __forceinline__ void take_one(Acc &a, float x, float c) {
+    const float2 v[1] = {make_float2(x, -CUDART_INF_F)};
+    take(a, v, x, c);
 }
 
 __device__ __forceinline__ Acc join(const Acc &a, const Acc &b, float c) {
@@ -144,66 +156,81 @@ __device__ __forceinline__ float logit_at(const T *x, const uint8_t *legal, int 
 template <class T> struct Wide;
 template <> struct Wide<float> {
     static constexpr int N = 4, LOW_BIT = 0;
-    static __device__ __forceinline__ void unpack(const uint4 &v, float *x) {
-        x[0] = __uint_as_float(v.x), x[1] = __uint_as_float(v.y), x[2] = __uint_as_float(v.z), x[3] = __uint_as_float(v.w);
+    static __device__ __forceinline__ void unpack(const uint4 &v, float2 *x) {
+        x[0] = make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
+        x[1] = make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
     }
-    static __device__ __forceinline__ uint4 pack(const float *x) {
-        return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+    static __device__ __forceinline__ uint4 pack(const float2 *x) {
+        return make_uint4(__float_as_uint(x[0].x), __float_as_uint(x[0].y), __float_as_uint(x[1].x), __float_as_uint(x[1].y));
     }
     static __device__ __forceinline__ uint4 mask(uint4 v, uint32_t bits) {
         const uint32_t none = 0xff800000u;
         return make_uint4(bits & 1 ? v.x : none, bits & 2 ? v.y : none, bits & 4 ? v.z : none, bits & 8 ? v.w : none);
     }
+    template <int U> static __device__ __forceinline__ float top(const uint4 (&v)[U]) {
+        float m = -CUDART_INF_F;
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            m = max_nan(m, max_nan(max_nan(__uint_as_float(v[u].x), __uint_as_float(v[u].y)), max_nan(__uint_as_float(v[u].z), __uint_as_float(v[u].w))));
+        return m;
+    }
 };
-template <class T> struct Wide16 {
+// Two 16-bit types: NONE is -inf.
+template <class H2, uint32_t NONE> struct Wide16 {
     static constexpr int N = 8;
-    static __device__ __forceinline__ uint32_t halves(uint32_t v, uint32_t bits, uint32_t none) {
-        const uint32_t keep = (bits & 1 ? 0xffffu : 0u) | (bits & 2 ? 0xffff0000u : 0u);
-        return (v & keep) | (none & ~keep);
+    // The 8 bits spread to the top bits of 8 bytes, then a byte's top bit over a half.
+    template <int SELECT> static __device__ __forceinline__ uint32_t signs(uint32_t v) {
+        uint32_t w;
+        asm("prmt.b32 %0, %1, 0, %2;" : "=r"(w) : "r"(v), "n"(SELECT));
+        return w;
     }
-    static __device__ __forceinline__ uint4 mask_with(uint4 v, uint32_t bits, uint32_t none) {
-        return make_uint4(halves(v.x, bits, none), halves(v.y, bits >> 2, none), halves(v.z, bits >> 4, none),
-                          halves(v.w, bits >> 6, none));
+    static __device__ __forceinline__ uint4 mask(uint4 v, uint32_t bits) {
+        const uint32_t lo = (bits & 15u) * 0x10204080u, hi = (bits >> 4 & 15u) * 0x10204080u, none = NONE | NONE << 16;
+        const uint32_t a = signs<0x9988>(lo), b = signs<0xbbaa>(lo), c = signs<0x9988>(hi), d = signs<0xbbaa>(hi);
+        return make_uint4((v.x & a) | (none & ~a), (v.y & b) | (none & ~b), (v.z & c) | (none & ~c), (v.w & d) | (none & ~d));
     }
+    static __device__ __forceinline__ H2 as(const uint32_t &v) { return *reinterpret_cast<const H2 *>(&v); }
+    template <int U> static __device__ __forceinline__ float top(const uint4 (&v)[U]) {
+        H2 m = __hmax2_nan(__hmax2_nan(as(v[0].x), as(v[0].y)), __hmax2_nan(as(v[0].z), as(v[0].w)));
+#pragma unroll
+        for (int u = 1; u < U; u++)
+            m = __hmax2_nan(m, __hmax2_nan(__hmax2_nan(as(v[u].x), as(v[u].y)), __hmax2_nan(as(v[u].z), as(v[u].w))));
+        return max_nan(to_f32(low_of(m)), to_f32(high_of(m)));
+    }
+    static __device__ __forceinline__ __nv_bfloat16 low_of(__nv_bfloat162 h) { return h.x; }
+    static __device__ __forceinline__ __nv_bfloat16 high_of(__nv_bfloat162 h) { return h.y; }
+    static __device__ __forceinline__ __half low_of(__half2 h) { return __low2half(h); }
+    static __device__ __forceinline__ __half high_of(__half2 h) { return __high2half(h); }
 };
-template <> struct Wide<__nv_bfloat16> : Wide16<__nv_bfloat16> {
+template <> struct Wide<__nv_bfloat16> : Wide16<__nv_bfloat162, 0xff80u> {
     static constexpr int LOW_BIT = 16;
-    static __device__ __forceinline__ void unpack(const uint4 &v, float *x) {
+    static __device__ __forceinline__ void unpack(const uint4 &v, float2 *x) {
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            x[2 * k] = __uint_as_float(w[k] << 16);
-            x[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
-        }
+        for (int k = 0; k < 4; k++) x[k] = make_float2(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u));
     }
-    static __device__ __forceinline__ uint4 pack(const float *x) {
+    static __device__ __forceinline__ uint4 pack(const float2 *x) {
         uint4 v;
         __nv_bfloat162 *h = reinterpret_cast<__nv_bfloat162 *>(&v);
 #pragma unroll
-        for (int k = 0; k < 4; k++) h[k] = __floats2bfloat162_rn(x[2 * k], x[2 * k + 1]);
+        for (int k = 0; k < 4; k++) h[k] = __float22bfloat162_rn(x[k]);
         return v;
     }
-    static __device__ __forceinline__ uint4 mask(uint4 v, uint32_t bits) { return mask_with(v, bits, 0xff80ff80u); }
 };
-template <> struct Wide<__half> : Wide16<__half> {
+template <> struct Wide<__half> : Wide16<__half2, 0xfc00u> {
     static constexpr int LOW_BIT = 13;
-    static __device__ __forceinline__ void unpack(const uint4 &v, float *x) {
+    static __device__ __forceinline__ void unpack(const uint4 &v, float2 *x) {
         const __half2 *h = reinterpret_cast<const __half2 *>(&v);
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const float2 f = __half22float2(h[k]);
-            x[2 * k] = f.x;
-            x[2 * k + 1] = f.y;
-        }
+        for (int k = 0; k < 4; k++) x[k] = __half22float2(h[k]);
     }
-    static __device__ __forceinline__ uint4 pack(const float *x) {
+    static __device__ __forceinline__ uint4 pack(const float2 *x) {
         uint4 v;
         __half2 *h = reinterpret_cast<__half2 *>(&v);
 #pragma unroll
-        for (int k = 0; k < 4; k++) h[k] = __floats2half2_rn(x[2 * k], x[2 * k + 1]);
+        for (int k = 0; k < 4; k++) h[k] = __float22half2_rn(x[k]);
         return v;
     }
-    static __device__ __forceinline__ uint4 mask(uint4 v, uint32_t bits) { return mask_with(v, bits, 0xfc00fc00u); }
 };
 
 // A row as 16-byte vectors from its first aligned element `head` on, and the
@@ -235,6 +262,7 @@ template <class T> struct Row {
 struct Shared {
     Acc warp[WARPS], block;
     uint64_t list[CAP], best[MAX_TOP];
+    uint32_t keys[THREADS], bound;
     uint16_t column[THREADS];
     int columns, count;
     uint64_t round[WARPS];
@@ -267,26 +295,44 @@ __device__ __forceinline__ void order_list(Shared &sh, int n, int top) {
 // elements, if they are its), into sh.best. m: the thread's largest logit.
 template <class T, bool MASK>
 __device__ __forceinline__ void select_top(Shared &sh, const Row<T> &row, int lo, int hi, bool own_loose, float m, int top) {
-    constexpr int N = Wide<T>::N;
+    constexpr int N = Wide<T>::N, EACH = THREADS / 32;
     const int tid = threadIdx.x;
-    const uint32_t key = order_key(m);
-    uint32_t bound = 1u;
-    if (__syncthreads_count(key >= 1u) >= top) {
-        bound = 0u;
-        for (int bit = 31; bit >= Wide<T>::LOW_BIT; bit--) {
-            const uint32_t next = bound | 1u << bit;
-            const int n = __syncthreads_count(key >= next);
-            if (n >= top) {
-                bound = next;
-                if (n <= top + top / 4) break;
+    sh.keys[tid] = order_key(m);
+    __syncthreads();
+    if (tid < 32) {  // one warp looks for the bound: the others would only wait for one another more often
+        uint32_t key[EACH];
+        int some = 0;
+#pragma unroll
+        for (int i = 0; i < EACH; i++) some += (key[i] = sh.keys[tid + 32 * i]) >= 1u;
+        uint32_t bound = 0u;
+        if (__reduce_add_sync(0xffffffffu, some) >= top)
+            for (int bit = 31; bit >= Wide<T>::LOW_BIT; bit--) {
+                const uint32_t next = bound | 1u << bit;
+                int n = 0;
+#pragma unroll
+                for (int i = 0; i < EACH; i++) n += key[i] >= next;
+                n = __reduce_add_sync(0xffffffffu, n);
+                if (n >= top) {
+                    bound = next;
+                    if (n <= top + top / 4) break;
+                }
             }
-        }
         bound = max(bound, 1u);
+        int columns = 0;
+#pragma unroll
+        for (int i = 0; i < EACH; i++) {
+            const uint32_t in = __ballot_sync(0xffffffffu, key[i] >= bound);
+            if (key[i] >= bound) sh.column[columns + __popc(in & ((1u << tid) - 1u))] = (uint16_t)(tid + 32 * i);
+            columns += __popc(in);
+        }
+        if (tid == 0) {
+            sh.bound = bound;
+            sh.columns = columns;
+            sh.count = 0;
+        }
     }
-    if (tid == 0) sh.columns = sh.count = 0;
     __syncthreads();
-    if (key >= bound) sh.column[atomicAdd(&sh.columns, 1)] = (uint16_t)tid;
-    __syncthreads();
+    const uint32_t bound = sh.bound;
     auto offer = [&](float x, int j) {
         const uint32_t k = order_key(x);
         if (k >= bound) {
@@ -300,10 +346,10 @@ __device__ __forceinline__ void select_top(Shared &sh, const Row<T> &row, int lo
         if (i >= hi) continue;
         uint4 v = row.load(i);
         if (MASK) v = Wide<T>::mask(v, row.bits(i));
-        float x[N];
+        float2 x[N / 2];
         Wide<T>::unpack(v, x);
 #pragma unroll
-        for (int k = 0; k < N; k++) offer(x[k], row.first(i) + k);
+        for (int k = 0; k < N; k++) offer(k & 1 ? x[k / 2].y : x[k / 2].x, row.first(i) + k);
     }
     if (own_loose && tid < row.loose) {
         const int j = row.loose_index(tid);
@@ -324,10 +370,10 @@ __device__ __forceinline__ void select_top(Shared &sh, const Row<T> &row, int lo
         for (int i = lo + tid; i < hi; i += THREADS) {
             uint4 v = row.load(i);
             if (MASK) v = Wide<T>::mask(v, row.bits(i));
-            float x[N];
+            float2 x[N / 2];
             Wide<T>::unpack(v, x);
 #pragma unroll
-            for (int k = 0; k < N; k++) consider(x[k], row.first(i) + k);
+            for (int k = 0; k < N; k++) consider(k & 1 ? x[k / 2].y : x[k / 2].x, row.first(i) + k);
         }
         if (own_loose && tid < row.loose) {
             const int j = row.loose_index(tid);
@@ -367,40 +413,38 @@ __global__ void __launch_bounds__(THREADS, 4)
         int i = lo + tid;
         for (; i + (UNROLL - 1) * THREADS < hi; i += UNROLL * THREADS) {
             uint4 v[UNROLL];
-            float x[UNROLL * N];
+            float2 x[UNROLL * N / 2];
 #pragma unroll
             for (int u = 0; u < UNROLL; u++) v[u] = row.load(i + u * THREADS);
 #pragma unroll
             for (int u = 0; u < UNROLL; u++) {
                 if (MASK) v[u] = Wide<T>::mask(v[u], row.bits(i + u * THREADS));
-                Wide<T>::unpack(v[u], x + u * N);
+                Wide<T>::unpack(v[u], x + u * N / 2);
             }
-            take(a, x, c);
+            take(a, x, Wide<T>::top(v), c);
         }
         for (; i < hi; i += THREADS) {
-            uint4 v = row.load(i);
-            float x[N];
-            if (MASK) v = Wide<T>::mask(v, row.bits(i));
-            Wide<T>::unpack(v, x);
-            take(a, x, c);
+            uint4 v[1] = {row.load(i)};
+            float2 x[N / 2];
+            if (MASK) v[0] = Wide<T>::mask(v[0], row.bits(i));
+            Wide<T>::unpack(v[0], x);
+            take(a, x, Wide<T>::top(v), c);
         }
         const float seen = a.m;  // of the vectors alone
         if (rank == 0 && tid < row.loose) {
-            const float x[1] = {logit_at(row.x, row.legal, row.loose_index(tid))};
-            take(a, x, c);
+            take_one(a, logit_at(row.x, row.legal, row.loose_index(tid)), c);
         }
         a = group_join<32>(a, c);
         if ((tid & 31) == 0) sh.warp[tid >> 5] = a;
         if (out.top) select_top<T, MASK>(sh, row, lo, hi, rank == 0, seen, out.top);
         __syncthreads();
-        a = sh.warp[0];
-#pragma unroll
-        for (int w = 1; w < WARPS; w++) a = join(a, sh.warp[w], c);
+        if (tid < 32) a = group_join<WARPS>(sh.warp[tid % WARPS], c);
         if (cluster > 1) {
             if (tid == 0) sh.block = a;
             cluster_sync();
             if (rank == 0) {
-                for (int p = 1; p < cluster; p++) a = join(a, *peer(&sh.block, p), c);
+                if (tid < 32)
+                    for (int p = 1; p < cluster; p++) a = join(a, *peer(&sh.block, p), c);
                 if (out.top) {
                     for (int q = tid; q < cluster * out.top; q += THREADS) {
                         const int p = q / out.top;
@@ -412,9 +456,11 @@ __global__ void __launch_bounds__(THREADS, 4)
             }
         }
         if (rank == 0) {
-            const float log_sum = tid < 32 ? a.m == -CUDART_INF_F ? -CUDART_INF_F : a.m < CUDART_INF_F ? logf(a.s) : CUDART_NAN_F : 0.f;
-            if (tid == 0) write_row(out, r, vocab, a, token, tv, inv_t);
-            if (tid < out.top) write_top(out, r, tid, sh.best[tid], a.m, log_sum, inv_t);
+            if (tid < 32) {
+                const float log_sum = a.m == -CUDART_INF_F ? -CUDART_INF_F : a.m < CUDART_INF_F ? logf(a.s) : CUDART_NAN_F;
+                if (tid == 0) write_row(out, r, vocab, a, token, tv, inv_t);
+                if (tid < out.top) write_top(out, r, tid, sh.best[tid], a.m, log_sum, inv_t);
+            }
         }
         if (cluster > 1)
             cluster_sync();  // the other blocks' shared memory has been read
@@ -441,14 +487,17 @@ __global__ void __launch_bounds__(THREADS)
         const bool live = r < rows;
         const T *row = logits + (live ? r : 0) * ld;
         const uint8_t *bits = legal ? legal + (live ? r : 0) * ldlegal : nullptr;
-        float x[NV];
+        float x[NV], largest = -CUDART_INF_F;
+        float2 pairs[NV / 2];
 #pragma unroll
         for (int i = 0; i < NV; i++) {
             const int j = lane + G * i;
             x[i] = live && j < vocab ? logit_at(row, bits, j) : -CUDART_INF_F;
+            largest = max_nan(largest, x[i]);
+            if (i & 1) pairs[i / 2] = make_float2(x[i - 1], x[i]);
         }
         Acc a{-CUDART_INF_F, 0.f, 0.f};
-        take(a, x, c);
+        take(a, pairs, largest, c);
         const float seen = a.m;
         a = group_join<G>(a, c);
         int64_t token = -1;
@@ -521,7 +570,7 @@ struct Grads {
     const float *stats, *entropy, *dlogp, *dentropy;
 };
 
-// A row's constants: with z2 = (x - m) c - l2 = log2 p, dlogits = -p (w0 + w1 z2), plus `hit` at the token.
+// A row's constants: with z2 = (x - m) c - l2 = log2 p, dlogits = p (w0 + w1 z2), plus `hit` at the token.
 struct RowGrad {
     float m, l2, w0, w1, hit;
     int token;
@@ -544,65 +593,67 @@ __device__ __forceinline__ RowGrad row_grad(const Grads &g, const T *x, const ui
         k.token = (int)token;
     }
     k.hit = a * inv_t;
-    k.w0 = (a + b * h) * inv_t;
-    k.w1 = b * inv_t * LN2;
+    k.w0 = -(a + b * h) * inv_t;
+    k.w1 = -b * inv_t * LN2;
     return k;
 }
-__device__ __forceinline__ float grad_of(const RowGrad &k, float x, float c) {
-    // z2 is bounded so that p = 0 times it is 0
-    const float z2 = max_nan(fmaf(x - k.m, c, -k.l2), -1e30f);
-    return x == -CUDART_INF_F ? 0.f : -ex2(z2) * fmaf(z2, k.w1, k.w0);
+// Of two logits; where p is 0 (a token that is left out, for one) 0 whatever the factor.
+__device__ __forceinline__ float2 grad_of(const RowGrad &k, float2 x, float c) {
+    const float2 z2 = __ffma2_rn(__fadd2_rn(x, both(-k.m)), both(c), both(-k.l2));
+    const float2 p = make_float2(ex2(z2.x), ex2(z2.y)), d = __fmul2_rn(p, __ffma2_rn(z2, both(k.w1), both(k.w0)));
+    return make_float2(p.x == 0.f ? 0.f : d.x, p.y == 0.f ? 0.f : d.y);
+}
+template <class T> __device__ __forceinline__ T grad_one(const RowGrad &k, float x, int j, float c) {
+    return from_f32<T>(k.zero ? 0.f : grad_of(k, make_float2(x, x), c).x + (j == k.token ? k.hit : 0.f));
 }
 
-constexpr int TILE = THREADS * UNROLL;  // vectors of one block
-
-// Long rows: a block takes a tile of one row. The vectors are the logits'
-// aligned ones; the gradient is stored as vectors where its rows are aligned
-// alike, else element by element.
+// Long rows: a block takes rows (or, where they are few, shares of them). The
+// vectors are the logits' aligned ones; the gradient is stored as vectors where
+// its rows are aligned alike, else element by element.
 template <class T, bool MASK>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, 6)
     long_backward_kernel(const T *__restrict__ logits, int64_t ld, int64_t rows, int vocab,
                          const uint8_t *__restrict__ legal, int64_t ldlegal, float inv_t, Grads g,
-                         T *__restrict__ dlogits, int64_t ldd, int tiles) {
+                         T *__restrict__ dlogits, int64_t ldd) {
     constexpr int N = Wide<T>::N;
     const float c = inv_t * LOG2E;
-    for (int64_t b = blockIdx.x; b < rows * tiles; b += gridDim.x) {
-        const int64_t r = b / tiles;
-        const int tile = (int)(b - r * tiles);
+    for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
         const Row<T> row(logits + r * ld, MASK ? legal + r * ldlegal : nullptr, vocab);
         T *d = dlogits + r * ldd;
         const bool alike = ((reinterpret_cast<uintptr_t>(d) ^ reinterpret_cast<uintptr_t>(row.x)) & 15) == 0;
-        const int i0 = tile * TILE + threadIdx.x;
-        uint4 v[UNROLL];
-#pragma unroll
-        for (int u = 0; u < UNROLL; u++)
-            if (i0 + u * THREADS < row.vectors) v[u] = row.load(i0 + u * THREADS);
+        const int lo = (int)((int64_t)row.vectors * blockIdx.x / gridDim.x), hi = (int)((int64_t)row.vectors * (blockIdx.x + 1) / gridDim.x);
         const RowGrad k = row_grad(g, row.x, row.legal, r, vocab, inv_t);
+        for (int i0 = lo + threadIdx.x; i0 < hi; i0 += UNROLL * THREADS) {
+            uint4 v[UNROLL];
 #pragma unroll
-        for (int u = 0; u < UNROLL; u++) {
-            const int i = i0 + u * THREADS, j = row.first(i);
-            if (i >= row.vectors) continue;
-            float x[N];
-            if (MASK) v[u] = Wide<T>::mask(v[u], row.bits(i));
-            Wide<T>::unpack(v[u], x);
+            for (int u = 0; u < UNROLL; u++)
+                if (i0 + u * THREADS < hi) v[u] = row.load(i0 + u * THREADS);
 #pragma unroll
-            for (int e = 0; e < N; e++) x[e] = k.zero ? 0.f : grad_of(k, x[e], c);
-            if ((unsigned)(k.token - j) < (unsigned)N) {
+            for (int u = 0; u < UNROLL; u++) {
+                const int i = i0 + u * THREADS, j = row.first(i);
+                if (i >= hi) break;
+                float2 x[N / 2];
+                if (MASK) v[u] = Wide<T>::mask(v[u], row.bits(i));
+                Wide<T>::unpack(v[u], x);
 #pragma unroll
-                for (int e = 0; e < N; e++)
-                    if (k.token - j == e) x[e] += k.hit;
+                for (int e = 0; e < N / 2; e++) x[e] = grad_of(k, x[e], c);
+                if ((unsigned)(k.token - j) < (unsigned)N) {
+#pragma unroll
+                    for (int e = 0; e < N; e++)
+                        if (k.token - j == e) (e & 1 ? x[e / 2].y : x[e / 2].x) += k.hit;
+                }
+                uint4 o = Wide<T>::pack(x);
+                if (k.zero) o = make_uint4(0u, 0u, 0u, 0u);
+                if (alike)
+                    *reinterpret_cast<uint4 *>(d + j) = o;
+                else
+#pragma unroll
+                    for (int e = 0; e < N; e++) d[j + e] = reinterpret_cast<const T *>(&o)[e];
             }
-            if (alike)
-                *reinterpret_cast<uint4 *>(d + j) = Wide<T>::pack(x);
-            else
-#pragma unroll
-                for (int e = 0; e < N; e++) d[j + e] = from_f32<T>(x[e]);
         }
-        if (tile == 0 && threadIdx.x < row.loose) {
+        if (blockIdx.x == 0 && threadIdx.x < row.loose) {
             const int j = row.loose_index(threadIdx.x);
-            float x = logit_at(row.x, row.legal, j);
-            x = k.zero ? 0.f : grad_of(k, x, c) + (j == k.token ? k.hit : 0.f);
-            d[j] = from_f32<T>(x);
+            d[j] = grad_one<T>(k, logit_at(row.x, row.legal, j), j, c);
         }
     }
 }
@@ -622,8 +673,7 @@ __global__ void __launch_bounds__(THREADS)
         const RowGrad k = row_grad(g, row, bits, r, vocab, inv_t);
 #pragma unroll 4
         for (int j = lane; j < vocab; j += G) {
-            const float x = logit_at(row, bits, j);
-            dlogits[r * ldd + j] = from_f32<T>(k.zero ? 0.f : grad_of(k, x, c) + (j == k.token ? k.hit : 0.f));
+            dlogits[r * ldd + j] = grad_one<T>(k, logit_at(row, bits, j), j, c);
         }
     }
 }
@@ -632,7 +682,7 @@ __global__ void __launch_bounds__(THREADS)
 
 static int blocks_of(int64_t rows, int per_block) {
     const int64_t want = (rows + per_block - 1) / per_block;
-    return (int)(want < 148 * 64 ? want : 148 * 64);
+    return (int)(want < SMS * 64 ? want : SMS * 64);
 }
 
 template <class T>
@@ -651,7 +701,7 @@ static int forward(const void *logits, int64_t ld, int64_t rows, int vocab, cons
     // a row is split over a cluster while there are too few rows for the 148 SMs (two blocks each) and a
     // block's share stays above two vectors a thread
     int cluster = 1;
-    while (cluster < MAX_CLUSTER && rows * cluster < 2 * 148 && vocab / (2 * cluster) >= 2 * THREADS * Wide<T>::N) cluster *= 2;
+    while (cluster < MAX_CLUSTER && rows * cluster < 2 * SMS && vocab / (2 * cluster) >= 2 * THREADS * Wide<T>::N) cluster *= 2;
     const int64_t most = (1 << 20) / cluster;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
@@ -679,13 +729,14 @@ static int backward(const void *logits, int64_t ld, int64_t rows, int vocab, con
             short_backward_kernel<T, 32><<<blocks_of(rows, 8), THREADS, 0, s>>>(x, ld, rows, vocab, legal, ldlegal, inv_t, g, d, ldd);
         return (int)cudaGetLastError();
     }
-    const int tiles = (vocab / Wide<T>::N + TILE - 1) / TILE;
-    const int64_t want = rows * tiles, most = 1 << 30;
-    const int grid = (int)(want < most ? want : most);
+    // blocks for each row: one, or enough of them for the 148 SMs where rows are few
+    const int tiles = vocab / (Wide<T>::N * THREADS * UNROLL) + 1;
+    const int64_t want = (SMS * 6 + rows - 1) / rows;
+    const dim3 grid((unsigned)(want < tiles ? want : tiles), (unsigned)(rows < 65535 ? rows : 65535));
     if (legal)
-        long_backward_kernel<T, true><<<grid, THREADS, 0, s>>>(x, ld, rows, vocab, legal, ldlegal, inv_t, g, d, ldd, tiles);
+        long_backward_kernel<T, true><<<grid, THREADS, 0, s>>>(x, ld, rows, vocab, legal, ldlegal, inv_t, g, d, ldd);
     else
-        long_backward_kernel<T, false><<<grid, THREADS, 0, s>>>(x, ld, rows, vocab, legal, ldlegal, inv_t, g, d, ldd, tiles);
+        long_backward_kernel<T, false><<<grid, THREADS, 0, s>>>(x, ld, rows, vocab, legal, ldlegal, inv_t, g, d, ldd);
     return (int)cudaGetLastError();
 }
 
