@@ -34,7 +34,8 @@ namespace lp {
 constexpr int THREADS = 256, WARPS = THREADS / 32, MAX_TOP = 32, MAX_CLUSTER = 8, CAP = 768;
 constexpr int SMS = 148;
 constexpr int UNROLL = 4;           // vectors a thread has in flight
-constexpr int SHORT_VOCAB = 1024;   // rows up to here are held in the registers of 8 or 32 lanes
+constexpr int SHORT_VOCAB = 64;     // rows up to here are held in the registers of 8 lanes
+constexpr int MIDDLE_VOCAB = 8192;  // rows up to here are a warp's
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 __device__ __forceinline__ float ex2(float x) {
@@ -71,26 +72,29 @@ struct Acc {
 
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 
-// top: the largest of x (a NaN if there is one).
-template <int N> __device__ __forceinline__ void take(Acc &a, const float2 (&x)[N], float top, float c) {
-    top = max_nan(top, a.m);
+__device__ __forceinline__ void rescale(Acc &a, float top, float c) {
     if (!(top <= a.m)) {
         const float d = fmaxf((a.m - top) * c, -1e4f), f = ex2(d);
         a.t = f * fmaf(d, a.s, a.t);
         a.s *= f;
         a.m = top;
     }
+}
+__device__ __forceinline__ void add_pair(float2 &s, float2 &t, float2 x, float m, float c) {
+    // below 2^-200 the term is zero; the bound also takes in -inf (and -inf - -inf)
+    float2 z = __fmul2_rn(__fadd2_rn(x, both(-m)), both(c));
+    z.x = fmaxf(z.x, -200.f);
+    z.y = fmaxf(z.y, -200.f);
+    const float2 e = make_float2(ex2(z.x), ex2(z.y));
+    s = __fadd2_rn(s, e);
+    t = __ffma2_rn(z, e, t);
+}
+// top: the largest of x (a NaN if there is one).
+template <int N> __device__ __forceinline__ void take(Acc &a, const float2 (&x)[N], float top, float c) {
+    rescale(a, max_nan(top, a.m), c);
     float2 s = make_float2(a.s, 0.f), t = make_float2(a.t, 0.f);
 #pragma unroll
-    for (int k = 0; k < N; k++) {
-        // below 2^-200 the term is zero; the bound also takes in -inf (and -inf - -inf)
-        float2 z = __fmul2_rn(__fadd2_rn(x[k], both(-a.m)), both(c));
-        z.x = fmaxf(z.x, -200.f);
-        z.y = fmaxf(z.y, -200.f);
-        const float2 e = make_float2(ex2(z.x), ex2(z.y));
-        s = __fadd2_rn(s, e);
-        t = __ffma2_rn(z, e, t);
-    }
+    for (int k = 0; k < N; k++) add_pair(s, t, x[k], a.m, c);
     a.s = s.x + s.y;
     a.t = t.x + t.y;
 }
@@ -249,15 +253,394 @@ template <class T> struct Row {
     __device__ __forceinline__ int first(int i) const { return head + i * N; }
     __device__ __forceinline__ int loose_index(int k) const { return k < head ? k : k + vectors * N; }
     __device__ __forceinline__ uint4 load(int i) const { return __ldg(reinterpret_cast<const uint4 *>(x + first(i))); }
-    // The legal bits of vector i: its N bits lie in one byte or in two.
+    // The legal bits of vector i: its N bits lie in one byte (in all of a row's
+    // vectors, where the first starts at a multiple of N) or in two.
     __device__ __forceinline__ uint32_t bits(int i) const {
-        const int j = first(i), at = j >> 3, last = (j + N - 1) >> 3;
-        const uint32_t lo = __ldg(legal + at), hi = __ldg(legal + last);
-        return (lo | hi << 8) >> (j & 7);  // hi is lo itself where one byte holds them all
+        const int j = first(i), at = j >> 3;
+        uint32_t b = __ldg(legal + at);
+        if (head % N) b |= __ldg(legal + ((j + N - 1) >> 3)) << 8;  // the same byte again where one holds them all
+        return b >> (j & 7);
     }
 };
 
-// ---------------------------------------------------------------- long rows: a cluster of 1 to 8 blocks each
+template <class T, int U> __device__ __forceinline__ float take_vectors(Acc &a, const uint4 (&v)[U], float c) {
+    constexpr int N = Wide<T>::N;
+    const float top = Wide<T>::top(v);
+    rescale(a, max_nan(top, a.m), c);
+    float2 s = make_float2(a.s, 0.f), t = make_float2(a.t, 0.f);
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        float2 x[N / 2];
+        Wide<T>::unpack(v[u], x);
+#pragma unroll
+        for (int k = 0; k < N / 2; k++) add_pair(s, t, x[k], a.m, c);
+    }
+    a.s = s.x + s.y;
+    a.t = t.x + t.y;
+    return top;
+}
+// The thread's vectors first, first + step, ... below `hi`. cell (or not): the
+// largest logit of each `group` batches of U vectors, a place every `step` floats.
+template <class T, bool MASK, int U>
+__device__ __forceinline__ void take_range(Acc &a, const Row<T> &row, int first, int step, int hi, float c, float *cell = nullptr, int group = 1) {
+    int i = first, batch = 0;
+    float largest = -CUDART_INF_F;
+    auto seen = [&](float top, bool end) {
+        if (!cell) return;
+        largest = max_nan(largest, top);
+        if (end && ++batch == group) {
+            *cell = largest;
+            cell += step;
+            largest = -CUDART_INF_F;
+            batch = 0;
+        }
+    };
+    for (; i + (U - 1) * step < hi; i += U * step) {
+        uint4 v[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) v[u] = row.load(i + u * step);
+        if (MASK) {
+            uint32_t bits[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) bits[u] = row.bits(i + u * step);
+#pragma unroll
+            for (int u = 0; u < U; u++) v[u] = Wide<T>::mask(v[u], bits[u]);
+        }
+        seen(take_vectors<T>(a, v, c), true);
+    }
+    for (; i < hi; i += step) {
+        uint4 v[1] = {row.load(i)};
+        if (MASK) v[0] = Wide<T>::mask(v[0], row.bits(i));
+        seen(take_vectors<T>(a, v, c), false);
+    }
+    if (cell) *cell = largest;
+}
+
+// ---------------------------------------------------------------- one warp's share of the work on a row
+
+constexpr int WARP_CAP = 512;
+struct WarpShared {
+    uint64_t list[WARP_CAP], best[MAX_TOP];
+    uint16_t column[THREADS];
+    int count, cells;
+};
+constexpr int CELLS = 12, CELL_CAP = 512;  // cells of a thread's vectors in a long row; cells that a warp looks at
+struct CellShared {
+    uint16_t cell[CELL_CAP];
+};
+
+// The join of EACH accumulators of each lane: the largest maximum first, then
+// the sums at its scale. Every lane gets it.
+template <int EACH> __device__ __forceinline__ Acc warp_join(const Acc (&a)[EACH], float c) {
+    float m = a[0].m;
+#pragma unroll
+    for (int i = 1; i < EACH; i++) m = max_nan(m, a[i].m);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float s = 0.f, t = 0.f;
+#pragma unroll
+    for (int i = 0; i < EACH; i++) {
+        const float d = fmaxf((a[i].m - m) * c, -1e4f), f = ex2(d);
+        s = fmaf(a[i].s, f, s);
+        t = fmaf(f, fmaf(d, a[i].s, a[i].t), t);
+    }
+    return Acc{m, warp_sum(s), warp_sum(t)};
+}
+
+// A bound that at least `top` of the warp's keys reach, and seldom many more (or
+// 1, which every token reaches): bisection, by ballots where a lane has one key,
+// else two bits at a time with three counts (below 1,024) in one sum.
+template <int EACH, int LOW_BIT> __device__ __forceinline__ uint32_t bound_of(const uint32_t (&key)[EACH], int top) {
+    uint32_t bound = 0u;
+    if constexpr (EACH == 1) {
+        for (int bit = 31; bit >= LOW_BIT; bit--) {
+            const uint32_t next = bound | 1u << bit;
+            const int n = __popc(__ballot_sync(0xffffffffu, key[0] >= next));
+            if (n < top) continue;
+            bound = next;
+            if (n <= top + top / 4) break;
+        }
+    } else {
+        auto reach = [&](uint32_t b) {
+            int n = 0;
+#pragma unroll
+            for (int i = 0; i < EACH; i++) n += key[i] >= b;
+            return n;
+        };
+        for (int bit = 30; bit >= (LOW_BIT & ~1); bit -= 2) {
+            const uint32_t b1 = bound | 1u << bit, b2 = bound | 2u << bit, b3 = bound | 3u << bit;
+            const int n = __reduce_add_sync(0xffffffffu, reach(b1) | reach(b2) << 10 | reach(b3) << 20);
+            const int n1 = n & 1023, n2 = n >> 10 & 1023, n3 = n >> 20;
+            if (n1 < top) continue;
+            bound = n3 >= top ? b3 : n2 >= top ? b2 : b1;
+            if ((n3 >= top ? n3 : n2 >= top ? n2 : n1) <= top + top / 4) break;
+        }
+    }
+    return max(bound, 1u);
+}
+
+// The row's best `top` candidates, into w.best, by one warp. seen[i]: the largest
+// logit among vectors lane + 32 i, lane + 32 i + 32 EACH, ... of the row; cell
+// (long rows): the same for each `group` batches of them.
+template <class T, bool MASK, int EACH>
+__device__ __forceinline__ void warp_select(WarpShared &w, const Row<T> &row, const float (&seen)[EACH], int top, const float *cell, int group,
+                                            CellShared *cs) {
+    constexpr int N = Wide<T>::N, STEP = 32 * EACH;
+    const int lane = threadIdx.x & 31;
+    uint32_t key[EACH];
+#pragma unroll
+    for (int i = 0; i < EACH; i++) key[i] = order_key(seen[i]);
+    const uint32_t bound = bound_of<EACH, Wide<T>::LOW_BIT>(key, top);
+    // as a logit: not below it is what reaches the bound (and a NaN)
+    const float least = bound < 0x00800000u ? -3.402823466e38f : logit_of((uint64_t)bound << 32);
+    int columns = 0;
+#pragma unroll
+    for (int i = 0; i < EACH; i++) {
+        const uint32_t in = __ballot_sync(0xffffffffu, key[i] >= bound);
+        if (key[i] >= bound) w.column[columns + __popc(in & ((1u << lane) - 1u))] = (uint16_t)(lane + 32 * i);
+        columns += __popc(in);
+    }
+    if (lane == 0) w.count = 0;
+    w.best[lane] = 0u;
+    __syncwarp();
+    auto put = [&](uint32_t k, int j) {
+        const int at = atomicAdd(&w.count, 1);
+        if (at < WARP_CAP) w.list[at] = candidate(k, j);
+    };
+    auto vector = [&](int i, float2 (&x)[N / 2]) {
+        uint4 v = row.load(i);
+        if (MASK) v = Wide<T>::mask(v, row.bits(i));
+        Wide<T>::unpack(v, x);
+    };
+    auto element = [&](const float2 (&x)[N / 2], int k) { return order_key(k & 1 ? x[k / 2].y : x[k / 2].x); };
+    auto loose = [&](int k) { return order_key(logit_at(row.x, MASK ? row.legal : nullptr, row.loose_index(k))); };
+    auto look = [&](int i, uint4 v) {
+        if (MASK) v = Wide<T>::mask(v, row.bits(i));
+        const uint4 one[1] = {v};
+        if (Wide<T>::top(one) < least) return;
+        float2 x[N / 2];
+        Wide<T>::unpack(v, x);
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            const uint32_t e = element(x, k);
+            if (e >= bound) put(e, row.first(i) + k);
+        }
+    };
+    bool many = false;
+    int deep = (row.vectors + STEP - 1) / STEP, cells = columns;
+    if (EACH > 1) {  // of the columns' cells, those that reach the bound
+        if (lane == 0) w.cells = 0;
+        __syncwarp();
+        const int span = UNROLL * group, parts = (deep + span - 1) / span;
+        for (int i = lane / 8; i < columns; i += 4)
+            for (int p = lane % 8; p < parts; p += 8) {
+                const int col = w.column[i];
+                if (cell[p * THREADS + col] < least) continue;
+                const int at = atomicAdd(&w.cells, 1);
+                if (at < CELL_CAP) cs->cell[at] = (uint16_t)(p << 8 | col);
+            }
+        __syncwarp();
+        cells = w.cells;
+        many = cells > CELL_CAP;
+        deep = span;
+    }
+    if (!many)
+        for (int it0 = 0; it0 < cells * deep; it0 += 64) {
+            uint4 v[2];
+            int i[2];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int it = it0 + 32 * u + lane, k = it / deep, q = it - k * deep;
+                i[u] = row.vectors;
+                if (it < cells * deep) {
+                    if (EACH > 1) {
+                        const int id = cs->cell[k];
+                        i[u] = (id & 255) + ((id >> 8) * deep + q) * STEP;
+                    } else
+                        i[u] = w.column[k] + q * STEP;
+                }
+                if (i[u] < row.vectors) v[u] = row.load(i[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+                if (i[u] < row.vectors) look(i[u], v[u]);
+        }
+    if (lane < row.loose) {
+        const uint32_t e = loose(lane);
+        if (e >= bound) put(e, row.loose_index(lane));
+    }
+    __syncwarp();
+    if (many || w.count > WARP_CAP) {
+        // Many equal logits: the row once more from its start, with what is above the bound and the first that equal it.
+        __syncwarp();
+        if (lane == 0) w.count = 0;
+        __syncwarp();
+        int equal = 0;  // of those, how many are in the list
+        auto more = [&](uint32_t e, int j) {
+            const bool in = e > bound || (e == bound && equal < top);
+            if (in) put(e, j);
+        };
+        const int tail = row.loose - row.head;
+        {
+            const uint32_t e = lane < row.head ? loose(lane) : 0u;
+            more(e, lane);
+            equal += __popc(__ballot_sync(0xffffffffu, e == bound));
+        }
+        for (int i0 = 0; i0 < row.vectors; i0 += 32) {
+            const int i = i0 + lane;
+            int here = 0;
+            if (i < row.vectors) {
+                float2 x[N / 2];
+                vector(i, x);
+#pragma unroll
+                for (int k = 0; k < N; k++) {
+                    const uint32_t e = element(x, k);
+                    more(e, row.first(i) + k);
+                    here += e == bound;
+                }
+            }
+            equal += __reduce_add_sync(0xffffffffu, here);
+        }
+        const uint32_t e = lane < tail ? loose(row.head + lane) : 0u;
+        more(e, row.loose_index(row.head + lane));
+        __syncwarp();
+    }
+    const int n = w.count;
+    if (n <= WARP_CAP) {
+        for (int i = lane; i < n; i += 32) {  // a candidate's place is the number of better ones
+            const uint64_t d = w.list[i];
+            int place = 0;
+            for (int q = 0; q < n; q++) place += w.list[q] > d;
+            if (place < top) w.best[place] = d;
+        }
+    } else {  // hundreds above the bound: round by round
+        uint64_t last = ~0ull;
+        for (int q = 0; q < top; q++) {
+            uint64_t b = 0u;
+            auto consider = [&](uint32_t e, int j) {
+                const uint64_t d = candidate(e, j);
+                if (d < last && d > b) b = d;
+            };
+            for (int i = lane; i < row.vectors; i += 32) {
+                float2 x[N / 2];
+                vector(i, x);
+#pragma unroll
+                for (int k = 0; k < N; k++) consider(element(x, k), row.first(i) + k);
+            }
+            if (lane < row.loose) consider(loose(lane), row.loose_index(lane));
+#pragma unroll
+            for (int o = 16; o; o >>= 1) b = max(b, (uint64_t)__shfl_xor_sync(0xffffffffu, b, o));
+            if (lane == 0) w.best[q] = b;
+            last = b;
+        }
+    }
+    __syncwarp();
+}
+
+// All of a row's outputs, by one warp. tv: the token's masked logit.
+template <class T, bool MASK, int EACH>
+__device__ __forceinline__ void warp_finish(WarpShared &w, const Row<T> &row, const Acc (&own)[EACH], const float (&seen)[EACH], const Out &out,
+                                            int64_t r, int64_t token, float tv, float inv_t, const float *cell = nullptr, int group = 1,
+                                            CellShared *cs = nullptr) {
+    const Acc a = warp_join(own, inv_t * LOG2E);
+    const int lane = threadIdx.x & 31;
+    const float log_sum = a.m == -CUDART_INF_F ? -CUDART_INF_F : a.m < CUDART_INF_F ? logf(a.s) : CUDART_NAN_F;
+    if (lane == 0) write_row(out, r, row.vocab, a, token, tv, inv_t);
+    if (out.top) {
+        warp_select<T, MASK, EACH>(w, row, seen, out.top, cell, group, cs);
+        if (lane < out.top) write_top(out, r, lane, w.best[lane], a.m, log_sum, inv_t);
+        __syncwarp();
+    }
+}
+template <class T> __device__ __forceinline__ void token_of(const Out &out, const Row<T> &row, int64_t r, int64_t &token, float &tv) {
+    token = out.logp ? out.tokens[r] : -1;
+    tv = token >= 0 && token < row.vocab ? logit_at(row.x, row.legal, (int)token) : -CUDART_INF_F;
+}
+
+// Middling rows: a warp each.
+template <class T, bool MASK>
+__global__ void __launch_bounds__(THREADS, 5)
+    warp_forward_kernel(const T *__restrict__ logits, int64_t ld, int64_t rows, int vocab,
+                        const uint8_t *__restrict__ legal, int64_t ldlegal, float inv_t, Out out) {
+    __shared__ WarpShared shared[WARPS];
+    WarpShared &w = shared[threadIdx.x >> 5];
+    const int lane = threadIdx.x & 31;
+    const float c = inv_t * LOG2E;
+    for (int64_t r = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.x * WARPS) {
+        const Row<T> row(logits + r * ld, MASK ? legal + r * ldlegal : nullptr, vocab);
+        int64_t token;
+        float tv;
+        token_of(out, row, r, token, tv);
+        Acc a[1] = {{-CUDART_INF_F, 0.f, 0.f}};
+        take_range<T, MASK, UNROLL>(a[0], row, lane, 32, row.vectors, c);
+        const float seen[1] = {a[0].m};
+        if (lane < row.loose) take_one(a[0], logit_at(row.x, row.legal, row.loose_index(lane)), c);
+        warp_finish<T, MASK, 1>(w, row, a, seen, out, r, token, tv, inv_t);
+    }
+}
+
+// Long rows: eight warps of a block read row after row and leave each thread's
+// sums in shared memory, where two more join them and find the alternatives while
+// the eight read on. Each of the two has a place for one row's sums, and a pair
+// of barriers that hand it over and back. (Without them the blocks' reading
+// stopped for each row's alternatives: 4,096 rows of 32,768 in bf16 took 87 us.)
+struct LongShared {
+    float m[2][THREADS], s[2][THREADS], t[2][THREADS], seen[2][THREADS], cell[2][CELLS + 1][THREADS];
+    WarpShared warp[2];
+    CellShared cells[2];
+};
+__device__ __forceinline__ void bar_sync(int id) { asm volatile("barrier.sync %0, %1;" ::"r"(id), "n"(THREADS + 32) : "memory"); }
+__device__ __forceinline__ void bar_arrive(int id) { asm volatile("barrier.arrive %0, %1;" ::"r"(id), "n"(THREADS + 32) : "memory"); }
+
+template <class T, bool MASK>
+__global__ void __launch_bounds__(THREADS + 64, 4)
+    long_forward_kernel(const T *__restrict__ logits, int64_t ld, int64_t rows, int vocab,
+                        const uint8_t *__restrict__ legal, int64_t ldlegal, float inv_t, Out out) {
+    extern __shared__ __align__(16) unsigned char space[];
+    LongShared &sh = *reinterpret_cast<LongShared *>(space);
+    const int tid = threadIdx.x, lane = tid & 31;
+    const float c = inv_t * LOG2E;
+    // batches to a cell, so that a thread has at most CELLS whole ones
+    const int group = vocab / (Wide<T>::N * THREADS * UNROLL * CELLS) + 1;
+    int turn = 0;
+    if (tid < THREADS) {
+        for (int64_t r = blockIdx.x; r < rows; r += gridDim.x, turn ^= 1) {
+            const Row<T> row(logits + r * ld, MASK ? legal + r * ldlegal : nullptr, vocab);
+            Acc a{-CUDART_INF_F, 0.f, 0.f};
+            if (r >= blockIdx.x + 2 * (int64_t)gridDim.x) bar_sync(3 + turn);  // the row before the last is done with
+            take_range<T, MASK, UNROLL>(a, row, tid, THREADS, row.vectors, c, out.top ? &sh.cell[turn][0][tid] : nullptr, group);
+            const float seen = a.m;
+            if (tid < row.loose) take_one(a, logit_at(row.x, row.legal, row.loose_index(tid)), c);
+            sh.m[turn][tid] = a.m;
+            sh.s[turn][tid] = a.s;
+            sh.t[turn][tid] = a.t;
+            sh.seen[turn][tid] = seen;
+            __threadfence_block();
+            bar_arrive(1 + turn);
+        }
+    } else {
+        turn = (tid - THREADS) >> 5;
+        for (int64_t r = blockIdx.x + (int64_t)turn * gridDim.x; r < rows; r += 2 * (int64_t)gridDim.x) {
+            const Row<T> row(logits + r * ld, MASK ? legal + r * ldlegal : nullptr, vocab);
+            int64_t token;
+            float tv;
+            token_of(out, row, r, token, tv);
+            bar_sync(1 + turn);
+            Acc a[WARPS];
+            float seen[WARPS];
+#pragma unroll
+            for (int i = 0; i < WARPS; i++) {
+                a[i] = Acc{sh.m[turn][lane + 32 * i], sh.s[turn][lane + 32 * i], sh.t[turn][lane + 32 * i]};
+                seen[i] = sh.seen[turn][lane + 32 * i];
+            }
+            warp_finish<T, MASK, WARPS>(sh.warp[turn], row, a, seen, out, r, token, tv, inv_t, &sh.cell[turn][0][0], group, &sh.cells[turn]);
+            __syncwarp();
+            if (r + 2 * (int64_t)gridDim.x < rows) bar_arrive(3 + turn);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- few long rows: a cluster of 2 to 8 blocks each
 
 struct Shared {
     Acc warp[WARPS], block;
@@ -394,9 +777,8 @@ __device__ __forceinline__ void select_top(Shared &sh, const Row<T> &row, int lo
 
 template <class T, bool MASK>
 __global__ void __launch_bounds__(THREADS, 4)
-    long_forward_kernel(const T *__restrict__ logits, int64_t ld, int64_t rows, int vocab,
-                        const uint8_t *__restrict__ legal, int64_t ldlegal, float inv_t, int cluster, Out out) {
-    constexpr int N = Wide<T>::N;
+    cluster_forward_kernel(const T *__restrict__ logits, int64_t ld, int64_t rows, int vocab,
+                           const uint8_t *__restrict__ legal, int64_t ldlegal, float inv_t, int cluster, Out out) {
     __shared__ Shared sh;
     const int tid = threadIdx.x, rank = blockIdx.x % cluster;
     const float c = inv_t * LOG2E;
@@ -410,26 +792,7 @@ __global__ void __launch_bounds__(THREADS, 4)
             if (token >= 0 && token < vocab) tv = logit_at(row.x, row.legal, (int)token);
         }
         Acc a{-CUDART_INF_F, 0.f, 0.f};
-        int i = lo + tid;
-        for (; i + (UNROLL - 1) * THREADS < hi; i += UNROLL * THREADS) {
-            uint4 v[UNROLL];
-            float2 x[UNROLL * N / 2];
-#pragma unroll
-            for (int u = 0; u < UNROLL; u++) v[u] = row.load(i + u * THREADS);
-#pragma unroll
-            for (int u = 0; u < UNROLL; u++) {
-                if (MASK) v[u] = Wide<T>::mask(v[u], row.bits(i + u * THREADS));
-                Wide<T>::unpack(v[u], x + u * N / 2);
-            }
-            take(a, x, Wide<T>::top(v), c);
-        }
-        for (; i < hi; i += THREADS) {
-            uint4 v[1] = {row.load(i)};
-            float2 x[N / 2];
-            if (MASK) v[0] = Wide<T>::mask(v[0], row.bits(i));
-            Wide<T>::unpack(v[0], x);
-            take(a, x, Wide<T>::top(v), c);
-        }
+        take_range<T, MASK, UNROLL>(a, row, lo + tid, THREADS, hi, c);
         const float seen = a.m;  // of the vectors alone
         if (rank == 0 && tid < row.loose) {
             take_one(a, logit_at(row.x, row.legal, row.loose_index(tid)), c);
@@ -439,20 +802,18 @@ __global__ void __launch_bounds__(THREADS, 4)
         if (out.top) select_top<T, MASK>(sh, row, lo, hi, rank == 0, seen, out.top);
         __syncthreads();
         if (tid < 32) a = group_join<WARPS>(sh.warp[tid % WARPS], c);
-        if (cluster > 1) {
-            if (tid == 0) sh.block = a;
-            cluster_sync();
-            if (rank == 0) {
-                if (tid < 32)
-                    for (int p = 1; p < cluster; p++) a = join(a, *peer(&sh.block, p), c);
-                if (out.top) {
-                    for (int q = tid; q < cluster * out.top; q += THREADS) {
-                        const int p = q / out.top;
-                        sh.list[q] = *peer(&sh.best[q - p * out.top], p);
-                    }
-                    __syncthreads();
-                    order_list(sh, cluster * out.top, out.top);
+        if (tid == 0) sh.block = a;
+        cluster_sync();
+        if (rank == 0) {
+            if (tid < 32)
+                for (int p = 1; p < cluster; p++) a = join(a, *peer(&sh.block, p), c);
+            if (out.top) {
+                for (int q = tid; q < cluster * out.top; q += THREADS) {
+                    const int p = q / out.top;
+                    sh.list[q] = *peer(&sh.best[q - p * out.top], p);
                 }
+                __syncthreads();
+                order_list(sh, cluster * out.top, out.top);
             }
         }
         if (rank == 0) {
@@ -462,24 +823,20 @@ __global__ void __launch_bounds__(THREADS, 4)
                 if (tid < out.top) write_top(out, r, tid, sh.best[tid], a.m, log_sum, inv_t);
             }
         }
-        if (cluster > 1)
-            cluster_sync();  // the other blocks' shared memory has been read
-        else
-            __syncthreads();
+        cluster_sync();  // the other blocks' shared memory has been read
     }
 }
 
-// ---------------------------------------------------------------- short rows: G lanes each, in registers
+// ---------------------------------------------------------------- short rows: eight lanes each, in registers
 
-template <class T, int G, int NV>
+template <class T>
 __global__ void __launch_bounds__(THREADS)
     short_forward_kernel(const T *__restrict__ logits, int64_t ld, int64_t rows, int vocab,
                          const uint8_t *__restrict__ legal, int64_t ldlegal, float inv_t, Out out) {
-    constexpr int GROUPS = THREADS / G, LIST = G * NV < 256 ? G * NV : 256;
-    __shared__ uint64_t lists[GROUPS][LIST], bests[GROUPS][MAX_TOP];
+    constexpr int G = 8, NV = SHORT_VOCAB / G, GROUPS = THREADS / G;
+    __shared__ uint64_t lists[GROUPS][SHORT_VOCAB], bests[GROUPS][MAX_TOP];
     __shared__ int counts[GROUPS];
     const int lane = threadIdx.x % G, group = threadIdx.x / G;
-    const uint32_t mates = G == 32 ? 0xffffffffu : ((1u << (G & 31)) - 1u) << (threadIdx.x & 31 & ~(G - 1));
     const float c = inv_t * LOG2E;
     const int64_t step = (int64_t)gridDim.x * GROUPS;
     for (int64_t base = (int64_t)blockIdx.x * GROUPS; base < rows; base += step) {  // all lanes of a warp stay together
@@ -498,7 +855,6 @@ __global__ void __launch_bounds__(THREADS)
         }
         Acc a{-CUDART_INF_F, 0.f, 0.f};
         take(a, pairs, largest, c);
-        const float seen = a.m;
         a = group_join<G>(a, c);
         int64_t token = -1;
         float tv = -CUDART_INF_F;
@@ -509,52 +865,21 @@ __global__ void __launch_bounds__(THREADS)
         const float log_sum = a.m == -CUDART_INF_F ? -CUDART_INF_F : a.m < CUDART_INF_F ? logf(a.s) : CUDART_NAN_F;
         if (live && lane == 0) write_row(out, r, vocab, a, token, tv, inv_t);
         if (!out.top) continue;
-        uint32_t bound = 1u;
-        if (G * NV > LIST) {  // else every token fits the list
-            const uint32_t key = order_key(seen);
-            if (__popc(__ballot_sync(0xffffffffu, key >= 1u) & mates) >= out.top) {
-                bound = 0u;
-                for (int bit = 31; bit >= Wide<T>::LOW_BIT; bit--) {
-                    const uint32_t next = bound | 1u << bit;
-                    if (__popc(__ballot_sync(0xffffffffu, key >= next) & mates) >= out.top) bound = next;
-                }
-                bound = max(bound, 1u);
-            }
-        }
         if (lane == 0) counts[group] = 0;
         for (int q = lane; q < out.top; q += G) bests[group][q] = 0u;
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < NV; i++) {
             const uint32_t k = order_key(x[i]);
-            if (k >= bound) {
-                const int at = atomicAdd(&counts[group], 1);
-                if (at < LIST) lists[group][at] = candidate(k, lane + G * i);
-            }
+            if (k) lists[group][atomicAdd(&counts[group], 1)] = candidate(k, lane + G * i);
         }
         __syncwarp();
         const int n = counts[group];
-        if (__any_sync(0xffffffffu, n > LIST)) {  // only where G is a warp: k rounds of a search in registers
-            uint64_t last = ~0ull;
-            for (int q = 0; q < out.top; q++) {
-                uint64_t b = 0u;
-#pragma unroll
-                for (int i = 0; i < NV; i++) {
-                    const uint64_t d = candidate(order_key(x[i]), lane + G * i);
-                    if (d < last && d > b) b = d;
-                }
-#pragma unroll
-                for (int o = G / 2; o; o >>= 1) b = max(b, (uint64_t)__shfl_xor_sync(0xffffffffu, b, o));
-                if (lane == 0) bests[group][q] = b;
-                last = b;
-            }
-        } else {
-            for (int i = lane; i < n; i += G) {
-                const uint64_t d = lists[group][i];
-                int place = 0;
-                for (int q = 0; q < n; q++) place += lists[group][q] > d;
-                if (place < out.top) bests[group][place] = d;
-            }
+        for (int i = lane; i < n; i += G) {
+            const uint64_t d = lists[group][i];
+            int place = 0;
+            for (int q = 0; q < n; q++) place += lists[group][q] > d;
+            if (place < out.top) bests[group][place] = d;
         }
         __syncwarp();
         if (live)
@@ -607,33 +932,38 @@ template <class T> __device__ __forceinline__ T grad_one(const RowGrad &k, float
     return from_f32<T>(k.zero ? 0.f : grad_of(k, make_float2(x, x), c).x + (j == k.token ? k.hit : 0.f));
 }
 
-// Long rows: a block takes rows (or, where they are few, shares of them). The
+// A warp or (long rows) a block takes rows or, where they are few, shares of them. The
 // vectors are the logits' aligned ones; the gradient is stored as vectors where
 // its rows are aligned alike, else element by element.
-template <class T, bool MASK>
-__global__ void __launch_bounds__(THREADS, 6)
+template <class T, bool MASK, int TEAM>
+__global__ void __launch_bounds__(THREADS, TEAM == 32 ? 5 : 6)
     long_backward_kernel(const T *__restrict__ logits, int64_t ld, int64_t rows, int vocab,
                          const uint8_t *__restrict__ legal, int64_t ldlegal, float inv_t, Grads g,
                          T *__restrict__ dlogits, int64_t ldd) {
     constexpr int N = Wide<T>::N;
     const float c = inv_t * LOG2E;
-    for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
+    const int t = threadIdx.x % TEAM;
+    for (int64_t r = blockIdx.y * (THREADS / TEAM) + threadIdx.x / TEAM; r < rows; r += gridDim.y * (THREADS / TEAM)) {
         const Row<T> row(logits + r * ld, MASK ? legal + r * ldlegal : nullptr, vocab);
         T *d = dlogits + r * ldd;
         const bool alike = ((reinterpret_cast<uintptr_t>(d) ^ reinterpret_cast<uintptr_t>(row.x)) & 15) == 0;
         const int lo = (int)((int64_t)row.vectors * blockIdx.x / gridDim.x), hi = (int)((int64_t)row.vectors * (blockIdx.x + 1) / gridDim.x);
         const RowGrad k = row_grad(g, row.x, row.legal, r, vocab, inv_t);
-        for (int i0 = lo + threadIdx.x; i0 < hi; i0 += UNROLL * THREADS) {
+        for (int i0 = lo + t; i0 < hi; i0 += UNROLL * TEAM) {
             uint4 v[UNROLL];
+            uint32_t bits[UNROLL];
 #pragma unroll
             for (int u = 0; u < UNROLL; u++)
-                if (i0 + u * THREADS < hi) v[u] = row.load(i0 + u * THREADS);
+                if (i0 + u * TEAM < hi) {
+                    v[u] = row.load(i0 + u * TEAM);
+                    if (MASK) bits[u] = row.bits(i0 + u * TEAM);
+                }
 #pragma unroll
             for (int u = 0; u < UNROLL; u++) {
-                const int i = i0 + u * THREADS, j = row.first(i);
+                const int i = i0 + u * TEAM, j = row.first(i);
                 if (i >= hi) break;
                 float2 x[N / 2];
-                if (MASK) v[u] = Wide<T>::mask(v[u], row.bits(i));
+                if (MASK) v[u] = Wide<T>::mask(v[u], bits[u]);
                 Wide<T>::unpack(v[u], x);
 #pragma unroll
                 for (int e = 0; e < N / 2; e++) x[e] = grad_of(k, x[e], c);
@@ -651,27 +981,26 @@ __global__ void __launch_bounds__(THREADS, 6)
                     for (int e = 0; e < N; e++) d[j + e] = reinterpret_cast<const T *>(&o)[e];
             }
         }
-        if (blockIdx.x == 0 && threadIdx.x < row.loose) {
-            const int j = row.loose_index(threadIdx.x);
+        if (blockIdx.x == 0 && t < row.loose) {
+            const int j = row.loose_index(t);
             d[j] = grad_one<T>(k, logit_at(row.x, row.legal, j), j, c);
         }
     }
 }
 
-// Short rows: G lanes a row.
-template <class T, int G>
+// Short rows: eight lanes a row.
+template <class T>
 __global__ void __launch_bounds__(THREADS)
     short_backward_kernel(const T *__restrict__ logits, int64_t ld, int64_t rows, int vocab,
                           const uint8_t *__restrict__ legal, int64_t ldlegal, float inv_t, Grads g,
                           T *__restrict__ dlogits, int64_t ldd) {
-    constexpr int GROUPS = THREADS / G;
+    constexpr int G = 8, GROUPS = THREADS / G;
     const float c = inv_t * LOG2E;
     const int lane = threadIdx.x % G;
     for (int64_t r = (int64_t)blockIdx.x * GROUPS + threadIdx.x / G; r < rows; r += (int64_t)gridDim.x * GROUPS) {
         const T *row = logits + r * ld;
         const uint8_t *bits = legal ? legal + r * ldlegal : nullptr;
         const RowGrad k = row_grad(g, row, bits, r, vocab, inv_t);
-#pragma unroll 4
         for (int j = lane; j < vocab; j += G) {
             dlogits[r * ldd + j] = grad_one<T>(k, logit_at(row, bits, j), j, c);
         }
@@ -690,18 +1019,27 @@ static int forward(const void *logits, int64_t ld, int64_t rows, int vocab, cons
                    float inv_t, const Out &out, cudaStream_t s) {
     const T *x = (const T *)logits;
     if (vocab <= SHORT_VOCAB) {
-        if (vocab <= 64)
-            short_forward_kernel<T, 8, 8><<<blocks_of(rows, 32), THREADS, 0, s>>>(x, ld, rows, vocab, legal, ldlegal, inv_t, out);
-        else if (vocab <= 256)
-            short_forward_kernel<T, 32, 8><<<blocks_of(rows, 8), THREADS, 0, s>>>(x, ld, rows, vocab, legal, ldlegal, inv_t, out);
-        else
-            short_forward_kernel<T, 32, 32><<<blocks_of(rows, 8), THREADS, 0, s>>>(x, ld, rows, vocab, legal, ldlegal, inv_t, out);
+        short_forward_kernel<T><<<blocks_of(rows, THREADS / 8), THREADS, 0, s>>>(x, ld, rows, vocab, legal, ldlegal, inv_t, out);
         return (int)cudaGetLastError();
     }
     // a row is split over a cluster while there are too few rows for the 148 SMs (two blocks each) and a
     // block's share stays above two vectors a thread
     int cluster = 1;
     while (cluster < MAX_CLUSTER && rows * cluster < 2 * SMS && vocab / (2 * cluster) >= 2 * THREADS * Wide<T>::N) cluster *= 2;
+    if (cluster == 1) {
+        if (vocab <= MIDDLE_VOCAB) {
+            if (legal)
+                warp_forward_kernel<T, true><<<blocks_of(rows, WARPS), THREADS, 0, s>>>(x, ld, rows, vocab, legal, ldlegal, inv_t, out);
+            else
+                warp_forward_kernel<T, false><<<blocks_of(rows, WARPS), THREADS, 0, s>>>(x, ld, rows, vocab, legal, ldlegal, inv_t, out);
+        } else {
+            const int grid = (int)(rows < SMS * 4 ? rows : SMS * 4);
+            const auto kernel = legal ? long_forward_kernel<T, true> : long_forward_kernel<T, false>;
+            if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(LongShared))) return (int)e;
+            kernel<<<grid, THREADS + 64, sizeof(LongShared), s>>>(x, ld, rows, vocab, legal, ldlegal, inv_t, out);
+        }
+        return (int)cudaGetLastError();
+    }
     const int64_t most = (1 << 20) / cluster;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
@@ -713,8 +1051,8 @@ static int forward(const void *logits, int64_t ld, int64_t rows, int vocab, cons
     cfg.stream = s;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    return (int)(legal ? cudaLaunchKernelEx(&cfg, long_forward_kernel<T, true>, x, ld, rows, vocab, legal, ldlegal, inv_t, cluster, out)
-                       : cudaLaunchKernelEx(&cfg, long_forward_kernel<T, false>, x, ld, rows, vocab, legal, ldlegal, inv_t, cluster, out));
+    return (int)(legal ? cudaLaunchKernelEx(&cfg, cluster_forward_kernel<T, true>, x, ld, rows, vocab, legal, ldlegal, inv_t, cluster, out)
+                       : cudaLaunchKernelEx(&cfg, cluster_forward_kernel<T, false>, x, ld, rows, vocab, legal, ldlegal, inv_t, cluster, out));
 }
 
 template <class T>
@@ -723,10 +1061,15 @@ static int backward(const void *logits, int64_t ld, int64_t rows, int vocab, con
     const T *x = (const T *)logits;
     T *d = (T *)dlogits;
     if (vocab <= SHORT_VOCAB) {
-        if (vocab <= 64)
-            short_backward_kernel<T, 8><<<blocks_of(rows, 32), THREADS, 0, s>>>(x, ld, rows, vocab, legal, ldlegal, inv_t, g, d, ldd);
+        short_backward_kernel<T><<<blocks_of(rows, THREADS / 8), THREADS, 0, s>>>(x, ld, rows, vocab, legal, ldlegal, inv_t, g, d, ldd);
+        return (int)cudaGetLastError();
+    }
+    if (vocab / Wide<T>::N <= 32 * UNROLL * 2) {
+        const dim3 grid(1, (unsigned)(rows < 65535 * WARPS ? (rows + WARPS - 1) / WARPS : 65535));
+        if (legal)
+            long_backward_kernel<T, true, 32><<<grid, THREADS, 0, s>>>(x, ld, rows, vocab, legal, ldlegal, inv_t, g, d, ldd);
         else
-            short_backward_kernel<T, 32><<<blocks_of(rows, 8), THREADS, 0, s>>>(x, ld, rows, vocab, legal, ldlegal, inv_t, g, d, ldd);
+            long_backward_kernel<T, false, 32><<<grid, THREADS, 0, s>>>(x, ld, rows, vocab, legal, ldlegal, inv_t, g, d, ldd);
         return (int)cudaGetLastError();
     }
     // blocks for each row: one, or enough of them for the 148 SMs where rows are few
@@ -734,9 +1077,9 @@ static int backward(const void *logits, int64_t ld, int64_t rows, int vocab, con
     const int64_t want = (SMS * 6 + rows - 1) / rows;
     const dim3 grid((unsigned)(want < tiles ? want : tiles), (unsigned)(rows < 65535 ? rows : 65535));
     if (legal)
-        long_backward_kernel<T, true><<<grid, THREADS, 0, s>>>(x, ld, rows, vocab, legal, ldlegal, inv_t, g, d, ldd);
+        long_backward_kernel<T, true, THREADS><<<grid, THREADS, 0, s>>>(x, ld, rows, vocab, legal, ldlegal, inv_t, g, d, ldd);
     else
-        long_backward_kernel<T, false><<<grid, THREADS, 0, s>>>(x, ld, rows, vocab, legal, ldlegal, inv_t, g, d, ldd);
+        long_backward_kernel<T, false, THREADS><<<grid, THREADS, 0, s>>>(x, ld, rows, vocab, legal, ldlegal, inv_t, g, d, ldd);
     return (int)cudaGetLastError();
 }
 

@@ -49,12 +49,13 @@ def like(t, of, name):
 _F32 = {}
 
 
-def empty_f32(device, shape):
-    """torch.empty of float32 on `device`, by the cheapest route (new_empty of a kept tensor)."""
+def empty_f32(device, *shape):
+    """torch.empty of float32 on `device`, by the cheapest route: new_empty of a kept
+    tensor, with the sizes as numbers (half the cost of torch.empty with a shape)."""
     kept = _F32.get(device)
     if kept is None:
         kept = _F32[device] = torch.empty(0, device=device)
-    return kept.new_empty(shape)
+    return kept.new_empty(*shape) if shape else kept.new_empty(())
 
 
 def empty_like(t):

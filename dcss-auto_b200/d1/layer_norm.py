@@ -29,7 +29,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, out=None):
     else:
         y = like(out, x, 'out')
         ldy = y.stride(0)
-    lead = x.shape[:-1]
+    lead = rows if x.dim() == 2 else x.shape[:-1]
     mean, rstd = empty_f32(dev, lead), empty_f32(dev, lead)
     check(library().d1_layer_norm(m.data_ptr(), m.stride(0), kind, rows, n, w, b, eps, y.data_ptr(), ldy,
                                   mean.data_ptr(), rstd.data_ptr(), stream_of(x)), 'd1_layer_norm')

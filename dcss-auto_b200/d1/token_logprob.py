@@ -30,18 +30,21 @@ class TokenLogprob(NamedTuple):
     top_logp: torch.Tensor = None      # float32 [..., top]
 
 
+_BITS = {torch.uint8: 1, torch.int8: 1, torch.int16: 2, torch.int32: 4, torch.int64: 8}  # bytes of a mask's words
+
+
 def _legal(legal, lead, vocab, device):
     """(address, row pitch in bytes) of the mask."""
     if legal is None:
         return None, 0
-    if legal.is_floating_point() or legal.is_complex() or legal.dtype == torch.bool:
-        raise ValueError('legal must be an integer tensor of bits')
+    size = _BITS.get(legal.dtype)
+    if size is None:
+        raise ValueError(f'legal must be an integer tensor of bits, not {legal.dtype}')
     if legal.shape == lead:
         legal = legal.unsqueeze(-1)
     if legal.shape[:-1] != lead or legal.device != device:
         raise ValueError(f'legal {tuple(legal.shape)} on {legal.device} does not match rows {tuple(lead)} on {device}')
     m = matrix(legal, 'legal')
-    size = m.element_size()
     if m.shape[1] * size * 8 < vocab:
         raise ValueError(f'legal has {m.shape[1] * size * 8} bits a row for {vocab} tokens')
     return m.data_ptr(), m.stride(0) * size
@@ -63,11 +66,11 @@ def token_logprob(logits, tokens, legal=None, temperature=1.0, top=0):
     dev, kind, m, lead, rows, vocab, t, (bits, pitch) = _common(logits, tokens, legal, temperature)
     if not 0 <= top <= MAX_TOP:
         raise ValueError(f'top must be between 0 and {MAX_TOP}')
-    logp, entropy, stats = empty_f32(dev, lead), empty_f32(dev, lead), empty_f32(dev, lead + (2,))
+    shape = (rows,) if len(lead) == 1 else lead
+    logp, entropy, stats = empty_f32(dev, *shape), empty_f32(dev, *shape), empty_f32(dev, *shape, 2)
     top_tokens = top_logp = None
     if top:
-        top_tokens = tokens.new_empty(lead + (top,))
-        top_logp = empty_f32(dev, lead + (top,))
+        top_tokens, top_logp = tokens.new_empty(*shape, top), empty_f32(dev, *shape, top)
     check(library().d1_token_logprob(m.data_ptr(), m.stride(0), kind, rows, vocab, t, bits, pitch, temperature, top,
                                      logp.data_ptr(), entropy.data_ptr(), stats.data_ptr(),
                                      top_tokens.data_ptr() if top else None, top_logp.data_ptr() if top else None,
