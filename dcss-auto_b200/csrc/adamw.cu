@@ -45,8 +45,9 @@ struct Args {
     int tile;  // blocks that a warp takes at a time: 8, handed out, or 2 at fixed places
     void *m, *v;
     float *m_scale, *v_scale;
-    double lr, beta1, beta2, log2_beta1, log2_beta2;
-    float b1, c1, b2, c2, eps, max_norm;
+    double lr, log2_beta1, log2_beta2;
+    double max_norm;
+    float b1, c1, b2, c2, eps;
     int64_t *step;
     uint64_t seed;
     double *partials;            // the norm's sums, one for each of its blocks
@@ -135,7 +136,7 @@ __global__ void __launch_bounds__(THREADS) norm_kernel(Args a) {
     __shared__ double part[WARPS];
     pdl_launch();
     const int lane = threadIdx.x & 31;
-    float s = 0.f;
+    double s = 0.;
     // a fixed share of the blocks, for a fixed order of the sum
     const int lo = (int)((int64_t)a.nblocks * blockIdx.x / gridDim.x), hi = (int)((int64_t)a.nblocks * (blockIdx.x + 1) / gridDim.x);
     Place t;
@@ -151,8 +152,10 @@ __global__ void __launch_bounds__(THREADS) norm_kernel(Args a) {
                 if (c >= t.end) t = locate(a, c);
                 load_grad<false>(t, (int64_t)c * BLOCK + 4 * lane, left_at(t, c), g[c - b]);
             }
+        float q = 0.f;
 #pragma unroll
-        for (int k = 0; k < 2; k++) s += (g[k][0] * g[k][0] + g[k][1] * g[k][1]) + (g[k][2] * g[k][2] + g[k][3] * g[k][3]);
+        for (int k = 0; k < 2; k++) q += (g[k][0] * g[k][0] + g[k][1] * g[k][1]) + (g[k][2] * g[k][2] + g[k][3] * g[k][3]);
+        s += q;
     }
     double d = s;
 #pragma unroll
@@ -228,6 +231,16 @@ template <int BITS> struct Held {
 
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 
+// a b + c d in two columns. For 8-bit moments each operation is rounded by
+// itself, so that a code is that of the formula wherever it is computed: the
+// assembler joins a two-wide product and sum to a fused operation, whatever is
+// asked for, so the sums are single ones.
+template <int BITS> __device__ __forceinline__ float2 blend(float2 a, float b, float2 c, float d) {
+    if constexpr (BITS == 32) return __ffma2_rn(a, both(b), __fmul2_rn(c, both(d)));
+    const float2 p = __fmul2_rn(a, both(b)), q = __fmul2_rn(c, both(d));
+    return make_float2(__fadd_rn(p.x, q.x), __fadd_rn(p.y, q.y));
+}
+
 // The step of one block, stored where its elements belong. at: the lane's first element.
 template <int BITS, bool WIDE>
 __device__ __forceinline__ void step_block(const Args &a, const Step &s, const Place &t, int b, const Held<BITS> &h) {
@@ -257,8 +270,8 @@ __device__ __forceinline__ void step_block(const Args &a, const Step &s, const P
 #pragma unroll
     for (int k = 0; k < 2; k++) {
         const float2 g = __fmul2_rn(g2[k], both(s.clip)), kept = __fmul2_rn(p2[k], both(t.keep));
-        m[k] = __fadd2_rn(__fmul2_rn(m[k], both(s.b1)), __fmul2_rn(g, both(s.c1)));
-        v[k] = __fadd2_rn(__fmul2_rn(v[k], both(s.b2)), __fmul2_rn(__fmul2_rn(g, g), both(s.c2)));
+        m[k] = blend<BITS>(m[k], s.b1, g, s.c1);
+        v[k] = blend<BITS>(v[k], s.b2, __fmul2_rn(g, g), s.c2);
         const float2 d = __ffma2_rn(make_float2(sqrt_approx(v[k].x), sqrt_approx(v[k].y)), both(s.inv_bc2), both(s.eps));
         const float2 ratio = __fmul2_rn(m[k], make_float2(rcp_approx(d.x), rcp_approx(d.y)));
         const float2 new_p = __ffma2_rn(both(-s.rate), ratio, kept);
@@ -385,7 +398,7 @@ template <int BITS> __global__ void __launch_bounds__(THREADS, per_sm(BITS)) ste
     t.end = 0;
     if (tiles.block < a.nblocks) t = locate(a, tiles.block);
     Step s{1.f, 0.f, 0.f, a.eps, a.b1, a.c1, a.b2, a.c2, 0u};
-    if (a.max_norm > 0.f) {
+    if (a.max_norm > 0.) {
         pdl_wait();  // for the norm's partial sums
         double d = 0.;
         for (int i = threadIdx.x; i < a.norm_parts; i += THREADS) d += a.partials[i];
@@ -395,9 +408,10 @@ template <int BITS> __global__ void __launch_bounds__(THREADS, per_sm(BITS)) ste
         __syncthreads();
         d = 0.;
         for (int i = 0; i < WARPS; i++) d += part[i];
-        const float norm = (float)sqrt(d);
-        s.clip = norm == norm ? fminf(1.f, __fdiv_rn(a.max_norm, norm + 1e-6f)) : norm;
-        if (blockIdx.x == 0 && threadIdx.x == 0 && a.grad_norm) *a.grad_norm = norm;
+        // rounded once: with another last bit of the factor, 8-bit codes would be others
+        const double norm = sqrt(d), factor = a.max_norm / (norm + 1e-6);
+        s.clip = factor < 1. ? (float)factor : norm == norm ? 1.f : (float)norm;
+        if (blockIdx.x == 0 && threadIdx.x == 0 && a.grad_norm) *a.grad_norm = (float)norm;
     } else
         __syncthreads();
     s.rate = coef[0];
@@ -467,16 +481,17 @@ extern "C" int d1_adamw(const D1AdamWTensor *tensors, int ntensors, int64_t nblo
         (reinterpret_cast<uintptr_t>(v) & 15) || (reinterpret_cast<uintptr_t>(work) & 15))
         return D1_ERR_BAD_ARGUMENT;
     const int tile = nblocks >= SMS * 32 * 4 * 8 ? 8 : 2;  // 8 where that makes four tiles for each warp
-    Args a{tensors, ntensors, (int)nblocks, tile, m, v, m_scale, v_scale, lr, beta1, beta2, log2(beta1), log2(beta2),
-           (float)beta1, (float)(1. - beta1), (float)beta2, (float)(1. - beta2), (float)(eps > EPS_FLOOR ? eps : EPS_FLOOR), (float)max_norm, step,
-           seed, (double *)work, (unsigned *)((double *)work + NORM_GRID), (unsigned *)((double *)work + NORM_GRID) + 1,
-           0, grad_norm};
+    double *const partials = (double *)work;
+    unsigned *const counts = (unsigned *)(partials + NORM_GRID);
+    Args a{tensors, ntensors, (int)nblocks, tile, m, v, m_scale, v_scale, lr, log2(beta1), log2(beta2), max_norm,
+           (float)beta1, (float)(1. - beta1), (float)beta2, (float)(1. - beta2), (float)(eps > EPS_FLOOR ? eps : EPS_FLOOR),
+           step, seed, partials, counts, counts + 1, 0, grad_norm};
     const cudaStream_t s = (cudaStream_t)stream;
     const int64_t norm_want = (nblocks + 2 * WARPS - 1) / (2 * WARPS), want = (nblocks + tile * WARPS - 1) / (tile * WARPS);
     const int most = SMS * per_sm(state_bits);
     cudaLaunchAttribute attr;
     cudaLaunchConfig_t cfg = d1::pdl_config(dim3((unsigned)(want < most ? want : most)), dim3(THREADS), 0, s, &attr);
-    if (a.max_norm > 0.f) {
+    if (a.max_norm > 0.) {
         a.norm_parts = (int)(norm_want < NORM_GRID ? norm_want : NORM_GRID);
         norm_kernel<<<a.norm_parts, THREADS, 0, s>>>(a);
         if (cudaError_t e = cudaGetLastError()) return (int)e;

@@ -90,6 +90,38 @@ def test_steps(bits, grad_type, offset):
                 g.mul_(-0.5)
 
 
+def mix(z):
+    """The splitmix64 output function of int64 tensors (products wrap, shifts are logical)."""
+    z = z + -7046029254386353131
+    z = (z ^ ((z >> 30) & 0x3ffffffff)) * -4658895280553007687
+    z = (z ^ ((z >> 27) & 0x1fffffffff)) * -7723592293110705685
+    return z ^ ((z >> 31) & 0x1ffffffff)
+
+
+def test_codes_are_the_formulas_with_every_operation_rounded():
+    """m, v, scales and codes bit for bit: products and sums rounded to fp32 one by one, 16 random bits an element."""
+    from d1.adamw import AdamW
+    n = 1 << 24  # a last bit moves one code in a million
+    g = torch.Generator(device='cuda').manual_seed(33)
+    p = [torch.randn(n, device='cuda', generator=g)]
+    grad = [torch.randn(n, device='cuda', generator=g) * torch.exp(3 * torch.randn(n // 128, 1, device='cuda', generator=g)).expand(-1, 128).reshape(-1)]
+    opt = AdamW(p, grad, state_bits=8, seed=5)
+    for step in range(1, 4):
+        m, v = opt.moments(0)
+        m, v = m * 0.9 + grad[0] * (1 - 0.9), v * 0.999 + (grad[0] * grad[0]) * (1 - 0.999)
+        opt.step()
+        word = mix(mix(mix(torch.tensor(5, device='cuda')) + step) + torch.arange(n // 4, device='cuda'))
+        bits = torch.stack([(word >> k) & 0xffff for k in (0, 16, 32, 48)], 1).reshape(-1, 128).to(torch.int32)
+        for x, got, scale, field, bias, drop in ((m, opt.m, opt.m_scale, 7, 7, 20), (v, opt.v, opt.v_scale, 14, 15, 21)):
+            size = x.abs().view(-1, 128)
+            e = ((size.amax(1).view(torch.int32) >> 23) - 127).clamp(min=-100)
+            assert torch.equal(scale, ((e - field + 127) << 23).view(torch.float32))
+            y = size * ((field - e + 127) << 23).view(torch.float32)[:, None] * 2.0 ** (bias - 127)
+            code = (y.view(torch.int32) + (bits << (drop - 16)) + (1 << (drop - 17))) >> drop
+            code = torch.maximum(code, (size > 0).to(torch.int32)) if drop == 21 else code | (x.view(-1, 128) < 0).to(torch.int32) << 7
+            assert torch.equal(got.view(torch.uint8).view(-1, 128).to(torch.int32), code)
+
+
 def test_many_tensors_and_large_ones():
     from d1.adamw import AdamW
     for bits in (32, 8):
