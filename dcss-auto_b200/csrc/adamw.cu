@@ -399,7 +399,9 @@ template <int BITS> __global__ void __launch_bounds__(THREADS, per_sm(BITS)) ste
     if (tiles.block < a.nblocks) t = locate(a, tiles.block);
     Step s{1.f, 0.f, 0.f, a.eps, a.b1, a.c1, a.b2, a.c2, 0u};
     if (a.max_norm > 0.) {
-        pdl_wait();  // for the norm's partial sums
+        // For the norm's partial sums. What came before touches the list, the step and the counter, none of
+        // which the norm's kernel writes, and which was complete before that plain launch began.
+        pdl_wait();
         double d = 0.;
         for (int i = threadIdx.x; i < a.norm_parts; i += THREADS) d += a.partials[i];
 #pragma unroll

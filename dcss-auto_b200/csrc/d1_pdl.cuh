@@ -5,7 +5,8 @@
 // pdl_wait() then blocks until the previous kernel has completed and its memory
 // writes are visible. Every kernel launched this way calls it in every block
 // before its first global-memory read or write (only shared memory, barriers,
-// tensor memory and parameters are touched before it). For a kernel launched
+// tensor memory and parameters are touched before it), but where its comment says
+// that the launch before it was a plain one and left what it touches alone. For a kernel launched
 // without the attribute it returns at once.
 #pragma once
 #include <cuda_runtime.h>

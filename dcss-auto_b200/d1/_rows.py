@@ -1,18 +1,24 @@
-"""What the row operators (layer norm, token log-probabilities) ask of their tensors."""
+"""What the row operators (layer norm, token log-probabilities) ask of their tensors.
+
+They are called on batches of a few microseconds of GPU work, so that the checks
+are written for few Python and torch calls."""
 import torch
 
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # D1_TYPE_* of d1.h
 
 
 def type_of(t, name):
+    """D1_TYPE_* of a tensor on a GPU."""
     code = TYPES.get(t.dtype)
     if code is None:
         raise ValueError(f'{name} must be float32, bfloat16 or float16, not {t.dtype}')
+    if not t.is_cuda:
+        raise ValueError(f'{name} must be on a CUDA device (there is no CPU path)')
     return code
 
 
 def matrix(t, name):
-    """t as [rows, n] with one row pitch and contiguous rows (a view: nothing is copied)."""
+    """(address, rows, n, row pitch) of t as [rows, n] with contiguous rows; nothing is copied."""
     if t.dim() != 2:
         if t.dim() == 0:
             raise ValueError(f'{name} needs at least one dimension')
@@ -21,18 +27,20 @@ def matrix(t, name):
         except RuntimeError:
             raise ValueError(f'{name}: the leading dimensions of shape {tuple(t.shape)} with strides {t.stride()} '
                              'have no single row pitch') from None
-    if t.shape[1] < 1:
+    rows, n = t.shape
+    pitch, step = t.stride()
+    if n < 1:
         raise ValueError(f'{name}: rows are empty')
-    if t.stride(1) != 1 and t.shape[1] > 1:
+    if step != 1 and n > 1:
         raise ValueError(f'{name}: the last dimension must be contiguous')
-    return t
+    return t.data_ptr(), rows, n, pitch
 
 
 def vector(t, count, dtype, device, name):
-    """A contiguous tensor of `count` elements, or None; its address."""
+    """The address of a contiguous tensor of `count` elements, or None."""
     if t is None:
         return None
-    if t.dtype != dtype or t.numel() != count or t.device != device or not t.is_contiguous():
+    if t.dtype is not dtype or t.numel() != count or t.device != device or not t.is_contiguous():
         raise ValueError(f'{name} must be a contiguous {dtype} tensor of {count} elements on {device}, not '
                          f'{t.dtype} {tuple(t.shape)} on {t.device}')
     return t.data_ptr()
@@ -40,7 +48,7 @@ def vector(t, count, dtype, device, name):
 
 def like(t, of, name):
     """An output (or second input) of the shape, type and device of `of`, as a matrix."""
-    if t.shape != of.shape or t.dtype != of.dtype or t.device != of.device:
+    if t.shape != of.shape or t.dtype is not of.dtype or t.device != of.device:
         raise ValueError(f'{name} must be {of.dtype} {tuple(of.shape)} on {of.device}, not {t.dtype} '
                          f'{tuple(t.shape)} on {t.device}')
     return matrix(t, name)
@@ -63,17 +71,8 @@ def empty_like(t):
     return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
-def on_gpu(t, name):
-    if not t.is_cuda:
-        raise ValueError(f'{name} must be on a CUDA device (there is no CPU path)')
-    return t.device
-
-
-def apart(a, b, name, other):
-    """Refuses two matrices whose spans of memory overlap."""
-    ends = []
-    for t in (a, b):
-        span = ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size() if t.shape[0] else 0
-        ends.append((t.data_ptr(), t.data_ptr() + span))
-    if ends[0][0] < ends[1][1] and ends[1][0] < ends[0][1]:
+def apart(a, b, size, name, other):
+    """Refuses two matrices of elements of `size` bytes whose spans of memory overlap."""
+    (p, rows, n, pitch), (q, _, _, step) = a, b
+    if rows and p < q + ((rows - 1) * step + n) * size and q < p + ((rows - 1) * pitch + n) * size:
         raise ValueError(f'{name} overlaps {other}')

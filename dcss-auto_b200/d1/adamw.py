@@ -21,7 +21,6 @@ import ctypes as C
 import torch
 
 from ._lib import check, library, stream_of
-from ._rows import on_gpu
 
 BLOCK = 128
 
@@ -45,7 +44,9 @@ class AdamW:
         decay = list(weight_decay) if isinstance(weight_decay, (list, tuple)) else [weight_decay] * len(params)
         if len(copies) != len(params) or len(decay) != len(params):
             raise ValueError('copies and weight_decay must have one entry for each parameter')
-        self.device = on_gpu(params[0], 'params[0]')
+        self.device = params[0].device
+        if self.device.type != 'cuda':
+            raise ValueError('params[0] must be on a CUDA device (there is no CPU path)')
         for i, (p, c) in enumerate(zip(params, copies)):
             if p.dtype != torch.float32 or p.device != self.device or not p.is_contiguous():
                 raise ValueError(f'params[{i}] must be a contiguous float32 tensor on {self.device}')
@@ -90,16 +91,15 @@ class AdamW:
                                self._first[i], self.decay[i], 0 if g.dtype == torch.float32 else 1, 0)
         self.grads = grads
         self._table = torch.frombuffer(bytearray(table), dtype=torch.uint8).to(self.device)
+        at = lambda t: None if t is None else t.data_ptr()
+        self._state_args = (self._table.data_ptr(), len(grads), self.nblocks, self.state_bits, at(self.m), at(self.v),
+                            at(self.m_scale), at(self.v_scale))
+        self._step_args = (self.step_dev.data_ptr(), self.seed, self._work.data_ptr(), self.grad_norm.data_ptr())
 
     def step(self, lr=None):
         """One step, in place. lr: this step's learning rate (default: self.lr)."""
-        check(self.lib.d1_adamw(self._table.data_ptr(), len(self.params), self.nblocks, self.state_bits,
-                                self.m.data_ptr(), self.v.data_ptr(),
-                                None if self.m_scale is None else self.m_scale.data_ptr(),
-                                None if self.v_scale is None else self.v_scale.data_ptr(),
-                                self.lr if lr is None else lr, self.betas[0], self.betas[1], self.eps, self.max_norm,
-                                self.step_dev.data_ptr(), self.seed, self._work.data_ptr(), self.grad_norm.data_ptr(),
-                                stream_of(self.m)), 'd1_adamw')
+        check(self.lib.d1_adamw(*self._state_args, self.lr if lr is None else lr, self.betas[0], self.betas[1], self.eps,
+                                self.max_norm, *self._step_args, stream_of(self.m)), 'd1_adamw')
 
     def moments(self, i):
         """(m, v) of parameter i as float32 in its shape (decoded copies where the state is in 8 bits)."""

@@ -17,7 +17,7 @@ from typing import NamedTuple
 import torch
 
 from ._lib import check, library, stream_of
-from ._rows import apart, empty_f32, empty_like, like, matrix, on_gpu, type_of, vector
+from ._rows import apart, empty_f32, empty_like, like, matrix, type_of, vector
 
 MAX_TOP = 32
 
@@ -44,37 +44,37 @@ def _legal(legal, lead, vocab, device):
         legal = legal.unsqueeze(-1)
     if legal.shape[:-1] != lead or legal.device != device:
         raise ValueError(f'legal {tuple(legal.shape)} on {legal.device} does not match rows {tuple(lead)} on {device}')
-    m = matrix(legal, 'legal')
-    if m.shape[1] * size * 8 < vocab:
-        raise ValueError(f'legal has {m.shape[1] * size * 8} bits a row for {vocab} tokens')
-    return m.data_ptr(), m.stride(0) * size
+    p, _, words, pitch = matrix(legal, 'legal')
+    if words * size * 8 < vocab:
+        raise ValueError(f'legal has {words * size * 8} bits a row for {vocab} tokens')
+    return p, pitch * size
 
 
 def _common(logits, tokens, legal, temperature):
-    dev, kind, m = on_gpu(logits, 'logits'), type_of(logits, 'logits'), matrix(logits, 'logits')
+    kind, dev, m = type_of(logits, 'logits'), logits.device, matrix(logits, 'logits')
     if not temperature > 0:
         raise ValueError('temperature must be positive')
-    lead, (rows, vocab) = logits.shape[:-1], m.shape
+    lead = logits.shape[:-1]
     if tokens.shape != lead:
         raise ValueError(f'tokens {tuple(tokens.shape)} do not match rows {tuple(lead)}')
-    t = vector(tokens, rows, torch.int64, dev, 'tokens')
-    return dev, kind, m, lead, rows, vocab, t, _legal(legal, lead, vocab, dev)
+    t = vector(tokens, m[1], torch.int64, dev, 'tokens')
+    return dev, kind, m, lead, t, _legal(legal, lead, m[2], dev)
 
 
 def token_logprob(logits, tokens, legal=None, temperature=1.0, top=0):
     """TokenLogprob of softmax(logits / temperature) over the legal tokens."""
-    dev, kind, m, lead, rows, vocab, t, (bits, pitch) = _common(logits, tokens, legal, temperature)
+    dev, kind, (px, rows, vocab, ld), lead, t, (bits, pitch) = _common(logits, tokens, legal, temperature)
     if not 0 <= top <= MAX_TOP:
         raise ValueError(f'top must be between 0 and {MAX_TOP}')
     shape = (rows,) if len(lead) == 1 else lead
     logp, entropy, stats = empty_f32(dev, *shape), empty_f32(dev, *shape), empty_f32(dev, *shape, 2)
-    top_tokens = top_logp = None
+    top_tokens = top_logp = tt = tl = None
     if top:
-        top_tokens, top_logp = tokens.new_empty(*shape, top), empty_f32(dev, *shape, top)
-    check(library().d1_token_logprob(m.data_ptr(), m.stride(0), kind, rows, vocab, t, bits, pitch, temperature, top,
-                                     logp.data_ptr(), entropy.data_ptr(), stats.data_ptr(),
-                                     top_tokens.data_ptr() if top else None, top_logp.data_ptr() if top else None,
-                                     stream_of(logits)), 'd1_token_logprob')
+        top_tokens, top_logp = tokens.new_empty((*shape, top)), empty_f32(dev, *shape, top)
+        tt, tl = top_tokens.data_ptr(), top_logp.data_ptr()
+    check(library().d1_token_logprob(px, ld, kind, rows, vocab, t, bits, pitch, temperature, top, logp.data_ptr(),
+                                     entropy.data_ptr(), stats.data_ptr(), tt, tl, stream_of(logits)),
+          'd1_token_logprob')
     return TokenLogprob(logp, entropy, stats, top_tokens, top_logp)
 
 
@@ -83,7 +83,8 @@ def token_logprob_backward(logits, tokens, stats, entropy, dlogp, dentropy=None,
     """dlogits (the logits' shape and type) from the gradients of logp and of the
     entropy (float32 of the rows' shape; None: zero), written to `out` when given,
     which overlaps no input."""
-    dev, kind, m, lead, rows, vocab, t, (bits, pitch) = _common(logits, tokens, legal, temperature)
+    dev, kind, m, _, t, (bits, pitch) = _common(logits, tokens, legal, temperature)
+    px, rows, vocab, ld = m
     f32 = torch.float32
     s = vector(stats, 2 * rows, f32, dev, 'stats')
     if dentropy is not None and entropy is None:
@@ -91,13 +92,11 @@ def token_logprob_backward(logits, tokens, stats, entropy, dlogp, dentropy=None,
     h, dl = vector(entropy, rows, f32, dev, 'entropy'), vector(dlogp, rows, f32, dev, 'dlogp')
     dh = vector(dentropy, rows, f32, dev, 'dentropy')
     if out is None:
-        d = out = empty_like(logits)
-        ldd = vocab
+        out = empty_like(logits)
+        po, ldo = out.data_ptr(), vocab
     else:
-        d = like(out, logits, 'out')
-        ldd = d.stride(0)
-        apart(d, m, 'out', 'logits')
-    check(library().d1_token_logprob_backward(m.data_ptr(), m.stride(0), kind, rows, vocab, t, bits, pitch,
-                                              temperature, s, h, dl, dh, d.data_ptr(), ldd, stream_of(logits)),
-          'd1_token_logprob_backward')
+        po, _, _, ldo = d = like(out, logits, 'out')
+        apart(d, m, logits.element_size(), 'out', 'logits')
+    check(library().d1_token_logprob_backward(px, ld, kind, rows, vocab, t, bits, pitch, temperature, s, h, dl, dh, po,
+                                              ldo, stream_of(logits)), 'd1_token_logprob_backward')
     return out
