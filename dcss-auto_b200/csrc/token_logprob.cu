@@ -279,41 +279,53 @@ template <class T, int U> __device__ __forceinline__ float take_vectors(Acc &a, 
     a.t = t.x + t.y;
     return top;
 }
-// The thread's vectors first, first + step, ... below `hi`. cell (or not): the
-// largest logit of each `group` batches of U vectors, a place every `step` floats.
-template <class T, bool MASK, int U>
-__device__ __forceinline__ void take_range(Acc &a, const Row<T> &row, int first, int step, int hi, float c, float *cell = nullptr, int group = 1) {
-    int i = first, batch = 0;
-    float largest = -CUDART_INF_F;
-    auto seen = [&](float top, bool end) {
+// The largest logit of each `group` batches of a thread's vectors, a place every
+// THREADS floats (or nowhere).
+struct Cells {
+    float *cell;
+    int group, batch;
+    float largest;
+    __device__ __forceinline__ Cells(float *c, int g) : cell(c), group(g), batch(0) { largest = -CUDART_INF_F; }
+    __device__ __forceinline__ void seen(float top, bool end) {
         if (!cell) return;
         largest = max_nan(largest, top);
         if (end && ++batch == group) {
             *cell = largest;
-            cell += step;
+            cell += THREADS;
             largest = -CUDART_INF_F;
             batch = 0;
         }
-    };
-    for (; i + (U - 1) * step < hi; i += U * step) {
+    }
+    __device__ __forceinline__ void finish() {
+        if (cell) *cell = largest;
+    }
+};
+// The thread's vectors first, first + STEP, ... below `hi`.
+template <class T, bool MASK, int STEP> __device__ __forceinline__ void take_range(Acc &a, const Row<T> &row, int first, int hi, float c, Cells &cells) {
+    constexpr int U = UNROLL;
+    int i = first;
+    for (; i + (U - 1) * STEP < hi; i += U * STEP) {
         uint4 v[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) v[u] = row.load(i + u * step);
+        for (int u = 0; u < U; u++) v[u] = row.load(i + u * STEP);
         if (MASK) {
-            uint32_t bits[U];
+            uint32_t b[U];
 #pragma unroll
-            for (int u = 0; u < U; u++) bits[u] = row.bits(i + u * step);
+            for (int u = 0; u < U; u++) b[u] = row.bits(i + u * STEP);
 #pragma unroll
-            for (int u = 0; u < U; u++) v[u] = Wide<T>::mask(v[u], bits[u]);
+            for (int u = 0; u < U; u++) v[u] = Wide<T>::mask(v[u], b[u]);
         }
-        seen(take_vectors<T>(a, v, c), true);
+        cells.seen(take_vectors<T>(a, v, c), true);
     }
-    for (; i < hi; i += step) {
+    for (; i < hi; i += STEP) {
         uint4 v[1] = {row.load(i)};
         if (MASK) v[0] = Wide<T>::mask(v[0], row.bits(i));
-        seen(take_vectors<T>(a, v, c), false);
+        cells.seen(take_vectors<T>(a, v, c), false);
     }
-    if (cell) *cell = largest;
+}
+template <class T, bool MASK, int STEP> __device__ __forceinline__ void take_range(Acc &a, const Row<T> &row, int first, int hi, float c) {
+    Cells none(nullptr, 1);
+    take_range<T, MASK, STEP>(a, row, first, hi, c, none);
 }
 
 // ---------------------------------------------------------------- one warp's share of the work on a row
@@ -572,7 +584,7 @@ __global__ void __launch_bounds__(THREADS, 5)
         float tv;
         token_of(out, row, r, token, tv);
         Acc a[1] = {{-CUDART_INF_F, 0.f, 0.f}};
-        take_range<T, MASK, UNROLL>(a[0], row, lane, 32, row.vectors, c);
+        take_range<T, MASK, 32>(a[0], row, lane, row.vectors, c);
         const float seen[1] = {a[0].m};
         if (lane < row.loose) take_one(a[0], logit_at(row.x, row.legal, row.loose_index(lane)), c);
         warp_finish<T, MASK, 1>(w, row, a, seen, out, r, token, tv, inv_t);
@@ -608,7 +620,9 @@ __global__ void __launch_bounds__(THREADS + 64, 4)
             const Row<T> row(logits + r * ld, MASK ? legal + r * ldlegal : nullptr, vocab);
             Acc a{-CUDART_INF_F, 0.f, 0.f};
             if (r >= blockIdx.x + 2 * (int64_t)gridDim.x) bar_sync(3 + turn);  // the row before the last is done with
-            take_range<T, MASK, UNROLL>(a, row, tid, THREADS, row.vectors, c, out.top ? &sh.cell[turn][0][tid] : nullptr, group);
+            Cells cells(out.top ? &sh.cell[turn][0][tid] : nullptr, group);
+            take_range<T, MASK, THREADS>(a, row, tid, row.vectors, c, cells);
+            cells.finish();
             const float seen = a.m;
             if (tid < row.loose) take_one(a, logit_at(row.x, row.legal, row.loose_index(tid)), c);
             sh.m[turn][tid] = a.m;
@@ -792,7 +806,7 @@ __global__ void __launch_bounds__(THREADS, 4)
             if (token >= 0 && token < vocab) tv = logit_at(row.x, row.legal, (int)token);
         }
         Acc a{-CUDART_INF_F, 0.f, 0.f};
-        take_range<T, MASK, UNROLL>(a, row, lo + tid, THREADS, hi, c);
+        take_range<T, MASK, THREADS>(a, row, lo + tid, hi, c);
         const float seen = a.m;  // of the vectors alone
         if (rank == 0 && tid < row.loose) {
             take_one(a, logit_at(row.x, row.legal, row.loose_index(tid)), c);
@@ -932,6 +946,46 @@ template <class T> __device__ __forceinline__ T grad_one(const RowGrad &k, float
     return from_f32<T>(k.zero ? 0.f : grad_of(k, make_float2(x, x), c).x + (j == k.token ? k.hit : 0.f));
 }
 
+// The legal bytes of a long row in shared memory: read there, two byte loads a
+// vector cost next to nothing; from global memory they took an eighth of the
+// gradient's time (4,096 rows of 50,021 bf16: 166 us, 147 so, 140 with no mask to
+// read). The forward pass, whose issue slots are its bound, gains nothing by it.
+constexpr int MASK_BYTES = 8192;
+struct alignas(16) MaskShared {
+    uint8_t bytes[MASK_BYTES + 32];
+};
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+template <class T> struct StagedMask {
+    static constexpr int VECTORS = MASK_BYTES * 8 / Wide<T>::N;  // that one copy can serve
+    uint32_t at;  // where byte 0 of the row would be
+    // Copies the bytes of vectors [lo, hi) by THREADS threads, whole 16-byte pieces asynchronously.
+    __device__ __forceinline__ void fetch(MaskShared &to, const Row<T> &row, int lo, int hi, int t) {
+        const int first = row.first(lo) >> 3, last = (row.first(hi) - 1) >> 3;
+        const uint8_t *const p = row.legal + first;
+        const int from = (int)(reinterpret_cast<uintptr_t>(p) & 15), end = from + last - first + 1, tail = end & ~15;
+        const uint32_t base = (uint32_t)__cvta_generic_to_shared(to.bytes);
+        at = base + from - first;
+        if (lo >= hi) return;
+        for (int q = 16 * t; q < end; q += 16 * THREADS)
+            if (q >= from && q + 16 <= end)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(base + q), "l"(p - from + q) : "memory");
+        if (t < 16 && t >= from && t < end && (from || end < 16)) to.bytes[t] = p[t - from];
+        if (t >= 16 && t < 32 && tail && tail + t - 16 < end) to.bytes[tail + t - 16] = p[tail + t - 16 - from];
+    }
+    __device__ __forceinline__ uint32_t bits(const Row<T> &row, int i) const {
+        const int j = row.first(i), k = j >> 3;
+        uint32_t b = byte(k);
+        if (row.head % Wide<T>::N) b |= byte((j + Wide<T>::N - 1) >> 3) << 8;
+        return b >> (j & 7);
+    }
+    __device__ __forceinline__ uint32_t byte(int k) const {
+        uint32_t b;
+        asm volatile("ld.shared.u8 %0, [%1];" : "=r"(b) : "r"(at + k) : "memory");
+        return b;
+    }
+};
+
 // A warp or (long rows) a block takes rows or, where they are few, shares of them. The
 // vectors are the logits' aligned ones; the gradient is stored as vectors where
 // its rows are aligned alike, else element by element.
@@ -942,6 +996,8 @@ __global__ void __launch_bounds__(THREADS, TEAM == 32 ? 5 : 6)
                          T *__restrict__ dlogits, int64_t ldd) {
     constexpr int N = Wide<T>::N;
     const float c = inv_t * LOG2E;
+    constexpr bool STAGED = MASK && TEAM == THREADS;
+    __shared__ MaskShared shared[1];
     const int t = threadIdx.x % TEAM;
     for (int64_t r = blockIdx.y * (THREADS / TEAM) + threadIdx.x / TEAM; r < rows; r += gridDim.y * (THREADS / TEAM)) {
         const Row<T> row(logits + r * ld, MASK ? legal + r * ldlegal : nullptr, vocab);
@@ -949,37 +1005,49 @@ __global__ void __launch_bounds__(THREADS, TEAM == 32 ? 5 : 6)
         const bool alike = ((reinterpret_cast<uintptr_t>(d) ^ reinterpret_cast<uintptr_t>(row.x)) & 15) == 0;
         const int lo = (int)((int64_t)row.vectors * blockIdx.x / gridDim.x), hi = (int)((int64_t)row.vectors * (blockIdx.x + 1) / gridDim.x);
         const RowGrad k = row_grad(g, row.x, row.legal, r, vocab, inv_t);
-        for (int i0 = lo + t; i0 < hi; i0 += UNROLL * TEAM) {
-            uint4 v[UNROLL];
-            uint32_t bits[UNROLL];
-#pragma unroll
-            for (int u = 0; u < UNROLL; u++)
-                if (i0 + u * TEAM < hi) {
-                    v[u] = row.load(i0 + u * TEAM);
-                    if (MASK) bits[u] = row.bits(i0 + u * TEAM);
-                }
-#pragma unroll
-            for (int u = 0; u < UNROLL; u++) {
-                const int i = i0 + u * TEAM, j = row.first(i);
-                if (i >= hi) break;
-                float2 x[N / 2];
-                if (MASK) v[u] = Wide<T>::mask(v[u], bits[u]);
-                Wide<T>::unpack(v[u], x);
-#pragma unroll
-                for (int e = 0; e < N / 2; e++) x[e] = grad_of(k, x[e], c);
-                if ((unsigned)(k.token - j) < (unsigned)N) {
-#pragma unroll
-                    for (int e = 0; e < N; e++)
-                        if (k.token - j == e) (e & 1 ? x[e / 2].y : x[e / 2].x) += k.hit;
-                }
-                uint4 o = Wide<T>::pack(x);
-                if (k.zero) o = make_uint4(0u, 0u, 0u, 0u);
-                if (alike)
-                    *reinterpret_cast<uint4 *>(d + j) = o;
-                else
-#pragma unroll
-                    for (int e = 0; e < N; e++) d[j + e] = reinterpret_cast<const T *>(&o)[e];
+        for (int from = lo; from < hi;) {  // at once, or a share of the legal bytes at a time
+            const int to = STAGED && from + StagedMask<T>::VECTORS < hi ? from + StagedMask<T>::VECTORS : hi;
+            StagedMask<T> mask;
+            if (STAGED) {
+                __syncthreads();  // the share before this one has been read
+                mask.fetch(shared[0], row, from, to, t);
+                commit_copies();
+                wait_copies<0>();
+                __syncthreads();
             }
+            for (int i0 = from + t; i0 < to; i0 += UNROLL * TEAM) {
+                uint4 v[UNROLL];
+                uint32_t bits[UNROLL];
+    #pragma unroll
+                for (int u = 0; u < UNROLL; u++)
+                    if (i0 + u * TEAM < to) {
+                        v[u] = row.load(i0 + u * TEAM);
+                        if (MASK) bits[u] = STAGED ? mask.bits(row, i0 + u * TEAM) : row.bits(i0 + u * TEAM);
+                    }
+    #pragma unroll
+                for (int u = 0; u < UNROLL; u++) {
+                    const int i = i0 + u * TEAM, j = row.first(i);
+                    if (i >= to) break;
+                    float2 x[N / 2];
+                    if (MASK) v[u] = Wide<T>::mask(v[u], bits[u]);
+                    Wide<T>::unpack(v[u], x);
+    #pragma unroll
+                    for (int e = 0; e < N / 2; e++) x[e] = grad_of(k, x[e], c);
+                    if ((unsigned)(k.token - j) < (unsigned)N) {
+    #pragma unroll
+                        for (int e = 0; e < N; e++)
+                            if (k.token - j == e) (e & 1 ? x[e / 2].y : x[e / 2].x) += k.hit;
+                    }
+                    uint4 o = Wide<T>::pack(x);
+                    if (k.zero) o = make_uint4(0u, 0u, 0u, 0u);
+                    if (alike)
+                        *reinterpret_cast<uint4 *>(d + j) = o;
+                    else
+    #pragma unroll
+                        for (int e = 0; e < N; e++) d[j + e] = reinterpret_cast<const T *>(&o)[e];
+                }
+            }
+            from = to;
         }
         if (blockIdx.x == 0 && t < row.loose) {
             const int j = row.loose_index(t);

@@ -126,6 +126,22 @@ def test_few_long_rows_are_split_and_joined(rows):
             check_forward(logits, tokens, legal, 1.0, 32, token_logprob(logits, tokens, legal, top=32))
 
 
+@pytest.mark.parametrize('vocab', [65536, 65544, 70001, 150003])
+def test_gradient_of_long_masked_rows(vocab):
+    from d1.token_logprob import token_logprob, token_logprob_backward
+    for rows, dtype in ((3, torch.bfloat16), (2, torch.float32), (700, torch.bfloat16)):
+        if rows == 700 and vocab != 70001:
+            continue
+        logits, tokens, legal, g = case(rows, vocab, dtype, True, vocab)
+        got = token_logprob(logits, tokens, legal)
+        dlogp, dentropy = torch.randn(rows, device='cuda', generator=g), torch.randn(rows, device='cuda', generator=g)
+        d = token_logprob_backward(logits, tokens, got.stats, got.entropy, dlogp, dentropy, legal)
+        for lo in range(0, rows, 50):
+            part = slice(lo, lo + 50)
+            want, tol = gradient(logits[part], tokens[part], legal[part], 1.0, dlogp[part], dentropy[part])
+            assert ((d[part].double() - want).abs() <= tol + EPS[dtype] * (want.abs() + tol) + TINY[dtype]).all()
+
+
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize('vocab', [28, 300, 3001, 70000])
 def test_rows_at_the_edges(vocab, dtype):
