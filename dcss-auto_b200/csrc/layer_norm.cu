@@ -279,8 +279,8 @@ template <class T, int VEC, int P, int G> __device__ __forceinline__ float plain
 // many and small, so that others load while one adds.
 template <class T, int VEC, int P, int G, int R>
 __global__ void __launch_bounds__(G ? 256 : 1024, G == 32 && P == 16 ? 4 : 1)
-    forward_kernel(const T *__restrict__ x, int64_t ldx, int64_t rows, int n, const float *__restrict__ w,
-                   const float *__restrict__ b, float eps, T *__restrict__ y, int64_t ldy, float *__restrict__ mean,
+    forward_kernel(const T *x, int64_t ldx, int64_t rows, int n, const float *__restrict__ w,
+                   const float *__restrict__ b, float eps, T *y, int64_t ldy, float *__restrict__ mean,
                    float *__restrict__ rstd) {
     __shared__ __align__(16) float part[2][R][32];
     const Columns<VEC, P, G> c(n);
@@ -422,8 +422,8 @@ template <class T, int VEC, int P, int G> struct Rows {
 // Forward of long rows: a block takes row after row.
 template <class T, int VEC, int DEPTH>
 __global__ void __launch_bounds__(1024, 1)
-    long_forward_kernel(const T *__restrict__ x, int64_t ldx, int64_t rows, int n, const float *__restrict__ w,
-                        const float *__restrict__ b, float eps, T *__restrict__ y, int64_t ldy,
+    long_forward_kernel(const T *x, int64_t ldx, int64_t rows, int n, const float *__restrict__ w,
+                        const float *__restrict__ b, float eps, T *y, int64_t ldy,
                         float *__restrict__ mean, float *__restrict__ rstd) {
     constexpr int P = 16;
     using R = Rows<T, VEC, P, 0>;
@@ -636,8 +636,8 @@ constexpr int WIDE = 1024;
 
 template <class T>
 __global__ void __launch_bounds__(WIDE)
-    wide_forward_kernel(const T *__restrict__ x, int64_t ldx, int64_t rows, int n, const float *__restrict__ w,
-                        const float *__restrict__ b, float eps, T *__restrict__ y, int64_t ldy,
+    wide_forward_kernel(const T *x, int64_t ldx, int64_t rows, int n, const float *__restrict__ w,
+                        const float *__restrict__ b, float eps, T *y, int64_t ldy,
                         float *__restrict__ mean, float *__restrict__ rstd) {
     __shared__ __align__(16) float part[2][32];
     for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {

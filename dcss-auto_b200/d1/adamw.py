@@ -74,10 +74,11 @@ class AdamW:
         self.step_dev = torch.zeros(1, dtype=torch.int64, device=dev)
         self.grad_norm = torch.zeros(1, device=dev)  # the last step's, when it clips
         self._work = torch.zeros(self.lib.d1_adamw_work_bytes(), dtype=torch.uint8, device=dev)
+        self._table = torch.empty(len(params) * C.sizeof(_Tensor), dtype=torch.uint8, device=dev)
         self.set_grads(grads)
 
     def set_grads(self, grads):
-        """Read the gradients from other tensors from now on."""
+        """Read the gradients from other tensors from now on (a captured step too)."""
         grads = list(grads)
         if len(grads) != len(self.params):
             raise ValueError(f'{len(self.params)} parameters and {len(grads)} gradients')
@@ -90,7 +91,7 @@ class AdamW:
             table[i] = _Tensor(p.data_ptr(), g.data_ptr(), None if c is None else c.data_ptr(), p.numel(),
                                self._first[i], self.decay[i], 0 if g.dtype == torch.float32 else 1, 0)
         self.grads = grads
-        self._table = torch.frombuffer(bytearray(table), dtype=torch.uint8).to(self.device)
+        self._table.copy_(torch.frombuffer(bytearray(table), dtype=torch.uint8))
         at = lambda t: None if t is None else t.data_ptr()
         self._state_args = (self._table.data_ptr(), len(grads), self.nblocks, self.state_bits, at(self.m), at(self.v),
                             at(self.m_scale), at(self.v_scale))

@@ -194,9 +194,16 @@ def test_resume_graph_and_streams(bits):
         c.step()
     for _ in range(6):
         graph.replay()
+    assert all(torch.equal(p, q) for p, q in zip(a.params, c.params))
+    c.set_grads([torch.zeros_like(g) for g in c.grads])   # the captured step reads them
+    a.set_grads([torch.zeros_like(g) for g in a.grads])
+    d.set_grads(a.grads)
+    graph.replay()
+    a.step()
+    d.step()
     for other in (d, c):
         assert all(torch.equal(p, q) for p, q in zip(a.params, other.params))
-        assert torch.equal(a.m.view(torch.uint8), other.m.view(torch.uint8)) and int(other.step_dev) == 6
+        assert torch.equal(a.m.view(torch.uint8), other.m.view(torch.uint8)) and int(other.step_dev) == 7
 
 
 def test_other_gradients_and_non_finite_ones():
