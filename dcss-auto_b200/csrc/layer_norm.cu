@@ -185,7 +185,8 @@ __device__ __forceinline__ void load_weights(const float *w, const Columns<VEC, 
 }
 
 // Weights in shared memory, zeros past the row: padded, and for vectors of eight
-// with the halves apart, so that a warp's loads of four have no bank conflicts.
+// with the halves apart, so that a warp's loads of four have no bank conflicts
+// (eight in a row had eightfold ones).
 template <int VEC, int P> struct SharedWeights {
     static __host__ __device__ constexpr int floats(int warps) { return warps * 32 * P; }
     static __device__ __forceinline__ int place(int j, int total) {
@@ -194,15 +195,22 @@ template <int VEC, int P> struct SharedWeights {
     static __device__ __forceinline__ void fill(float *s, const float *w, float other, int n, int total) {
         for (int j = threadIdx.x; j < total; j += blockDim.x) s[place(j, total)] = j < n ? w ? __ldg(w + j) : other : 0.f;
     }
-    // Elements 2k and 2k + 1 of the thread's P.
-    static __device__ __forceinline__ float2 pair(const float *s, int start, int k, int total) {
+    // Elements 4q .. 4q + 3 of the thread's P.
+    static __device__ __forceinline__ float4 four(const float *s, int start, int q, int total) {
         constexpr int STEP = 32 * VEC;
         if constexpr (VEC == 8)
-            return *reinterpret_cast<const float2 *>(s + (k & 2 ? total / 2 : 0) + start / 2 + 2 * k / VEC * (STEP / 2) + 2 * (k & 1));
-        else if constexpr (VEC == 1)
-            return make_float2(s[start + 2 * k * STEP], s[start + (2 * k + 1) * STEP]);
-        else
-            return *reinterpret_cast<const float2 *>(s + start + 2 * k / VEC * STEP + 2 * k % VEC);
+            return *reinterpret_cast<const float4 *>(s + (q & 1 ? total / 2 : 0) + start / 2 + q / 2 * (STEP / 2));
+        else if constexpr (VEC == 4)
+            return *reinterpret_cast<const float4 *>(s + start + q * STEP);
+        else if constexpr (VEC == 2) {
+            const float2 a = *reinterpret_cast<const float2 *>(s + start + 2 * q * STEP), b = *reinterpret_cast<const float2 *>(s + start + (2 * q + 1) * STEP);
+            return make_float4(a.x, a.y, b.x, b.y);
+        } else
+            return make_float4(s[start + 4 * q * STEP], s[start + (4 * q + 1) * STEP], s[start + (4 * q + 2) * STEP], s[start + (4 * q + 3) * STEP]);
+    }
+    static __device__ __forceinline__ float2 pair(const float *s, int start, int k, int total) {
+        const float4 f = four(s, start, k / 2, total);
+        return k & 1 ? make_float2(f.z, f.w) : make_float2(f.x, f.y);
     }
 };
 
@@ -469,8 +477,11 @@ __global__ void __launch_bounds__(1024, 1)
         turn ^= 2;
         float2 o[P / 2];
 #pragma unroll
-        for (int k = 0; k < P / 2; k++)
-            o[k] = __ffma2_rn(__fmul2_rn(__fadd2_rn(h.pair(k), both(-mu)), both(rs)), W::pair(sw, c.start, k, total), W::pair(sb, c.start, k, total));
+        for (int q = 0; q < P / 4; q++) {
+            const float4 w4 = W::four(sw, c.start, q, total), b4 = W::four(sb, c.start, q, total);
+            o[2 * q] = __ffma2_rn(__fmul2_rn(__fadd2_rn(h.pair(2 * q), both(-mu)), both(rs)), make_float2(w4.x, w4.y), make_float2(b4.x, b4.y));
+            o[2 * q + 1] = __ffma2_rn(__fmul2_rn(__fadd2_rn(h.pair(2 * q + 1), both(-mu)), both(rs)), make_float2(w4.z, w4.w), make_float2(b4.z, b4.w));
+        }
         store_row<T, VEC, P, 0>(out, c, o);
         if (threadIdx.x == 0) {
             if (mean) mean[r] = mu;
@@ -736,10 +747,13 @@ static int forward(const T *x, int64_t ldx, int64_t rows, int n, const float *w,
     if (n <= 256) D1_LN_FORWARD(8, 32, 2, 256);
     if (n <= 512) D1_LN_FORWARD(16, 32, 2, 256);
     if (n <= 1024) D1_LN_FORWARD(32, 32, 1, 256);
-    const int threads = block_threads(n, 16), warps = threads / 32, depth = n <= 8192 ? 4 : 3;
+    const int threads = block_threads(n, 16), warps = threads / 32;
+    // rows in shared memory: three, or two where that lets an SM hold a second block (8,192 in bf16: 76 us with four,
+    // 64 with two, for 8,192 rows)
+    const int depth = VEC > 2 && n > 4096 && n <= 8192 ? 2 : 3;
     const size_t smem = (size_t)depth * Rows<T, VEC, 16, 0>::bytes(warps) + 8 * (size_t)SharedWeights<VEC, 16>::floats(warps);
     if (threads > 1024 || smem + 2048 > SPACE) D1_LN_FORWARD(32, 0, 1, block_threads(n, 32));
-    const auto kernel = depth == 4 ? long_forward_kernel<T, VEC, 4> : long_forward_kernel<T, VEC, 3>;
+    const auto kernel = depth == 2 ? long_forward_kernel<T, VEC, 2> : long_forward_kernel<T, VEC, 3>;
     if (const int e = allow_space(kernel, smem)) return e;
     const int by_threads = 1024 / threads, by_space = (int)(SPACE / (smem + 2048));
     const int64_t full = (int64_t)SMS * (by_threads < by_space ? by_threads : by_space);
