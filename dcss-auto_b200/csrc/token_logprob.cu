@@ -263,13 +263,14 @@ template <class T> struct Row {
     }
 };
 
-template <class T, int U> __device__ __forceinline__ float take_vectors(Acc &a, const uint4 (&v)[U], float c) {
+template <class T, int U> __device__ __forceinline__ float take_vectors(Acc &a, const uint4 (&v)[U], float c, int count = U) {
     constexpr int N = Wide<T>::N;
     const float top = Wide<T>::top(v);
     rescale(a, max_nan(top, a.m), c);
     float2 s = make_float2(a.s, 0.f), t = make_float2(a.t, 0.f);
 #pragma unroll
     for (int u = 0; u < U; u++) {
+        if (u >= count) break;
         float2 x[N / 2];
         Wide<T>::unpack(v[u], x);
 #pragma unroll
@@ -304,7 +305,8 @@ struct Cells {
 template <class T, bool MASK, int STEP> __device__ __forceinline__ void take_range(Acc &a, const Row<T> &row, int first, int hi, float c, Cells &cells) {
     constexpr int U = UNROLL;
     int i = first;
-    for (; i + (U - 1) * STEP < hi; i += U * STEP) {
+    // whole batches of the warp's last lane
+    for (const int last = 31 - (int)(threadIdx.x & 31); i + last + (U - 1) * STEP < hi; i += U * STEP) {
         uint4 v[U];
 #pragma unroll
         for (int u = 0; u < U; u++) v[u] = row.load(i + u * STEP);
@@ -317,10 +319,21 @@ template <class T, bool MASK, int STEP> __device__ __forceinline__ void take_ran
         }
         cells.seen(take_vectors<T>(a, v, c), true);
     }
-    for (; i < hi; i += STEP) {
-        uint4 v[1] = {row.load(i)};
-        if (MASK) v[0] = Wide<T>::mask(v[0], row.bits(i));
-        cells.seen(take_vectors<T>(a, v, c), false);
+    if (const int w = i - (int)(threadIdx.x & 31); w < hi) {  // what is left for any lane of the warp: a batch with gaps
+        uint4 v[U];
+        uint32_t b[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            v[u] = make_uint4(0u, 0u, 0u, 0u);
+            b[u] = 0u;
+            if (i + u * STEP < hi) {
+                v[u] = row.load(i + u * STEP);
+                b[u] = MASK ? row.bits(i + u * STEP) : ~0u;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) v[u] = Wide<T>::mask(v[u], b[u]);
+        cells.seen(take_vectors<T>(a, v, c, (hi - w + STEP - 1) / STEP), false);
     }
 }
 template <class T, bool MASK, int STEP> __device__ __forceinline__ void take_range(Acc &a, const Row<T> &row, int first, int hi, float c) {
@@ -433,10 +446,11 @@ __device__ __forceinline__ void warp_select(WarpShared &w, const Row<T> &row, co
         float2 x[N / 2];
         Wide<T>::unpack(v, x);
 #pragma unroll
-        for (int k = 0; k < N; k++) {
-            const uint32_t e = element(x, k);
-            if (e >= bound) put(e, row.first(i) + k);
-        }
+        for (int k = 0; k < N; k++)
+            if (!((k & 1 ? x[k / 2].y : x[k / 2].x) < least)) {
+                const uint32_t e = element(x, k);
+                if (e >= bound) put(e, row.first(i) + k);
+            }
     };
     bool many = false;
     int deep = (row.vectors + STEP - 1) / STEP, cells = columns;
@@ -462,8 +476,9 @@ __device__ __forceinline__ void warp_select(WarpShared &w, const Row<T> &row, co
             int i[2];
 #pragma unroll
             for (int u = 0; u < 2; u++) {
-                const int it = it0 + 32 * u + lane, k = it / deep, q = it - k * deep;
                 i[u] = row.vectors;
+                if (it0 + 32 * u >= cells * deep) continue;
+                const int it = it0 + 32 * u + lane, k = it / deep, q = it - k * deep;
                 if (it < cells * deep) {
                     if (EACH > 1) {
                         const int id = cs->cell[k];
