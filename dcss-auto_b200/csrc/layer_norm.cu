@@ -506,10 +506,12 @@ __global__ void __launch_bounds__(MOST, P == 8 && G ? 3 : P == 8 || MOST == 256 
     using C = Columns<VEC, P, G>;
     using R = Rows<T, VEC, P, G>;
     using W = SharedWeights<VEC, P>;
-    constexpr bool KEEP = P <= 16, EARLY = R::VECTOR && DEPTH > 2;
+    // with two places a row is waited for at its beginning, and its mean and rstd come with the row before it
+    constexpr bool KEEP = P <= 16, LATE = DEPTH == 2, EARLY = R::VECTOR || LATE;
+    constexpr int STATS = LATE ? 3 : DEPTH;
     extern __shared__ __align__(16) unsigned char space[];
     __shared__ __align__(16) float part[2][64];
-    __shared__ float stats[TEAMS][DEPTH][2];  // mean and rstd of the rows in their places
+    __shared__ float stats[TEAMS][STATS][2];  // mean and rstd of the rows on their way
     pdl_launch();
     const C c(n);
     const int warps = blockDim.x >> 5, team = G ? threadIdx.x / (G ? G : 1) : 0, bytes = R::bytes(warps), total = W::floats(warps);
@@ -524,17 +526,25 @@ __global__ void __launch_bounds__(MOST, P == 8 && G ? 3 : P == 8 || MOST == 256 
     const int t = G ? threadIdx.x % (G ? G : 1) : threadIdx.x;
     const float *next_stat = (t == 0 ? mean : rstd) + first;
     const uint32_t stat_at = shared_address(&stats[team][0][0]);
-    auto fetch = [&](int slot) {
-        if (t < 2 && next_x.left > 0) {
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(stat_at + 8 * slot + 4 * t), "l"(next_stat) : "memory");
+    int stats_left = next_x.left;
+    auto fetch_stat = [&](int place) {
+        if (t < 2 && stats_left > 0) {
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(stat_at + 8 * place + 4 * t), "l"(next_stat) : "memory");
             next_stat += step;
         }
+        stats_left--;
+    };
+    auto fetch = [&](int slot, int place) {
+        fetch_stat(place);
         next_x.fetch(ring + slot * 2 * bytes, c, n);
         next_dy.fetch(ring + slot * 2 * bytes + bytes, c, n);
         commit_copies();
     };
 #pragma unroll
-    for (int d = 0; d < DEPTH - 1; d++) fetch(d);
+    for (int d = 0; d < DEPTH - 1; d++) {
+        if (LATE) fetch_stat(0);
+        fetch(d, LATE ? 1 : d);
+    }
     float2 wk[P / 2], aw[P / 2], ab[P / 2];
     if (KEEP) load_weights<VEC, P, G>(w, c, 1.f, wk);
 #pragma unroll
@@ -546,7 +556,7 @@ __global__ void __launch_bounds__(MOST, P == 8 && G ? 3 : P == 8 || MOST == 256 
     float2 stat = load_shared<float2>(stat_at);
     const T *xr = x + first * ldx, *dr = dy + first * lddy;
     T *out_row = dx + first * lddx + c.start;
-    int slot = 0, turn = 0;
+    int slot = 0, place = 0, turn = 0;
     const int rounds = (int)((rows - (int64_t)blockIdx.x * TEAMS + step - 1) / step);  // of the block's first team
     int64_t r = first;
     for (int round = 0; round < rounds; round++) {
@@ -554,7 +564,11 @@ __global__ void __launch_bounds__(MOST, P == 8 && G ? 3 : P == 8 || MOST == 256 
         const float mu = stat.x, rs = stat.y;
         // the place of the row before this one takes the next: at once where it was the thread's
         // own, else when the team has done with it
-        if (EARLY) fetch(slot == 0 ? DEPTH - 1 : slot - 1);
+        if (LATE && round > 0) {
+            wait_copies<0>();
+            if (!R::VECTOR) __syncthreads();
+        }
+        if (EARLY) fetch(slot == 0 ? DEPTH - 1 : slot - 1, place == 0 ? STATS - 1 : place - 1);
         const uint32_t stage = ring + slot * 2 * bytes, ds = R::staged(stage + bytes, dr, c);
         float2 xhat[P / 2], g[KEEP ? P / 2 : 1], sum1 = both(0.f), sum2 = both(0.f);
         if (TEAMS == 1 || live) {
@@ -573,12 +587,13 @@ __global__ void __launch_bounds__(MOST, P == 8 && G ? 3 : P == 8 || MOST == 256 
             }
         }
         float s1 = sum1.x + sum1.y, s2 = sum2.x + sum2.y;
-        wait_copies<EARLY ? DEPTH - 2 : DEPTH - 3>();  // for the row after this one
+        if (!LATE) wait_copies<EARLY ? DEPTH - 2 : DEPTH - 3>();  // for the row after this one
         team_sums<G>(s1, s2, part[turn]);
         turn ^= 1;
         if (G) __syncwarp();
-        stat = load_shared<float2>(stat_at + 8 * (slot == DEPTH - 1 ? 0 : slot + 1));
-        if (!EARLY) fetch(slot == 0 ? DEPTH - 1 : slot - 1);
+        if (!EARLY) fetch(slot == 0 ? DEPTH - 1 : slot - 1, place == 0 ? STATS - 1 : place - 1);
+        place = place == STATS - 1 ? 0 : place + 1;
+        stat = load_shared<float2>(stat_at + 8 * place);
         if ((TEAMS == 1 || live) && dx) {
             const float2 c1 = both(-rs * s1 * inv_n), c2 = both(-rs * s2 * inv_n);
             Held<T, VEC, P, G> dv;

@@ -92,6 +92,16 @@ def test_against_the_definition(n, dtype):
 
 
 @pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('n', [1500, 2050, 4096, 5001, 8192, 8200, 12033, 16384])
+def test_many_long_rows(n, dtype):                     # a block's rows follow one another through shared memory
+    from d1.layer_norm import layer_norm, layer_norm_backward
+    x, dy, w, b = data(700, n, dtype, 17 * n)
+    y, mean, rstd = layer_norm(x, w, b)
+    check_forward(x, w, b, 1e-5, (y, mean, rstd))
+    check_backward(dy, x, w, 1e-5, layer_norm_backward(dy, x, mean, rstd, w), (mean, rstd))
+
+
+@pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('n', [8, 500, 512, 1024, 4096, 9000])
 def test_pitches_and_alignments(n, dtype):
     from d1.layer_norm import layer_norm, layer_norm_backward
