@@ -286,7 +286,7 @@ template <class T, int VEC, int P, int G> __device__ __forceinline__ float plain
 // rows' loads are issued together and their sums joined together; blocks are
 // many and small, so that others load while one adds.
 template <class T, int VEC, int P, int G, int R>
-__global__ void __launch_bounds__(G ? 256 : 1024, G == 32 && P == 16 ? 4 : 1)
+__global__ void __launch_bounds__(G ? 256 : P == 64 ? 512 : 1024, G == 32 && P == 16 ? 4 : P == 64 ? 2 : 1)
     forward_kernel(const T *x, int64_t ldx, int64_t rows, int n, const float *__restrict__ w,
                    const float *__restrict__ b, float eps, T *y, int64_t ldy, float *__restrict__ mean,
                    float *__restrict__ rstd) {
@@ -427,13 +427,14 @@ template <class T, int VEC, int P, int G> struct Rows {
     }
 };
 
-// Forward of long rows: a block takes row after row.
-template <class T, int VEC, int DEPTH>
+// Forward of rows over 1,024 where forward_kernel is not faster: a block takes row after row.
+constexpr int LONG_DEPTH = 3;
+template <class T, int VEC>
 __global__ void __launch_bounds__(1024, 1)
     long_forward_kernel(const T *x, int64_t ldx, int64_t rows, int n, const float *__restrict__ w,
                         const float *__restrict__ b, float eps, T *y, int64_t ldy,
                         float *__restrict__ mean, float *__restrict__ rstd) {
-    constexpr int P = 16;
+    constexpr int P = 16, DEPTH = LONG_DEPTH;
     using R = Rows<T, VEC, P, 0>;
     using W = SharedWeights<VEC, P>;
     extern __shared__ __align__(16) unsigned char space[];
@@ -762,18 +763,26 @@ static int forward(const T *x, int64_t ldx, int64_t rows, int n, const float *w,
     if (n <= 256) D1_LN_FORWARD(8, 32, 2, 256);
     if (n <= 512) D1_LN_FORWARD(16, 32, 2, 256);
     if (n <= 1024) D1_LN_FORWARD(32, 32, 1, 256);
-    const int threads = block_threads(n, 16), warps = threads / 32;
-    // rows in shared memory: three, or two where that lets an SM hold a second block (8,192 in bf16: 76 us with four,
-    // 64 with two, for 8,192 rows)
-    const int depth = VEC > 2 && n > 4096 && n <= 8192 ? 2 : 3;
-    const size_t smem = (size_t)depth * Rows<T, VEC, 16, 0>::bytes(warps) + 8 * (size_t)SharedWeights<VEC, 16>::floats(warps);
-    if (threads > 1024 || smem + 2048 > SPACE) D1_LN_FORWARD(32, 0, 1, block_threads(n, 32));
-    const auto kernel = depth == 2 ? long_forward_kernel<T, VEC, 2> : long_forward_kernel<T, VEC, 3>;
-    if (const int e = allow_space(kernel, smem)) return e;
-    const int by_threads = 1024 / threads, by_space = (int)(SPACE / (smem + 2048));
-    const int64_t full = (int64_t)SMS * (by_threads < by_space ? by_threads : by_space);
-    kernel<<<(int)(rows < full ? rows : full), threads, smem, s>>>(x, ldx, rows, n, w, b, eps, y, ldy, mean, rstd);
-    return (int)cudaGetLastError();
+    // Longer rows are a block's. Where the vectors are whole, 32 elements a thread (64 of the longest) need fewer
+    // joins than 16 do, and blocks that come and go keep more rows under way than resident ones with their rows in
+    // shared memory: 16,384 in bf16 63 us against 72 (4,096 rows), 4,096 57 against 59 (16,384 rows, two at a time, for
+    // their weights), 3,156 in fp32 47 against 53 (10,631 rows). Of 1,112 and 1,536 in bf16 it is the other way round:
+    // 74 against 72, 59 against 55, and 1,111 in fp32 (element by element) 92 against 61.
+    if constexpr (VEC == 4)
+        D1_LN_FORWARD(32, 0, 1, block_threads(n, 32));
+    else {
+        if (VEC == 8 && n > 8192) D1_LN_FORWARD((VEC == 8 ? 64 : 32), 0, 1, block_threads(n, 64));
+        if (VEC == 8 ? n >= 2048 : VEC == 2 && n > 4096) D1_LN_FORWARD(32, 0, (VEC > 1 ? 2 : 1), block_threads(n, 32));
+        const int threads = block_threads(n, 16), warps = threads / 32;
+        const size_t smem = (size_t)LONG_DEPTH * Rows<T, VEC, 16, 0>::bytes(warps) + 8 * (size_t)SharedWeights<VEC, 16>::floats(warps);
+        if (threads > 1024 || smem + 2048 > SPACE) D1_LN_FORWARD(32, 0, 1, block_threads(n, 32));
+        const auto kernel = long_forward_kernel<T, VEC>;
+        if (const int e = allow_space(kernel, smem)) return e;
+        const int by_threads = 1024 / threads, by_space = (int)(SPACE / (smem + 2048));
+        const int64_t full = (int64_t)SMS * (by_threads < by_space ? by_threads : by_space);
+        kernel<<<(int)(rows < full ? rows : full), threads, smem, s>>>(x, ldx, rows, n, w, b, eps, y, ldy, mean, rstd);
+        return (int)cudaGetLastError();
+    }
 }
 
 template <class T>
@@ -792,7 +801,9 @@ static int forward_any(const void *x, int64_t ldx, int64_t rows, int n, const fl
 
 // How the backward pass runs: teams of 8 or 32 lanes, or blocks (lanes = 0),
 // with P elements a thread, DEPTH rows in shared memory and as many blocks as
-// the SMs hold at once (more would only write more partial sums).
+// the SMs hold at once (more would only write more partial sums). Eight elements
+// a thread for rows of 513 to 1,024 that are vectors, sixteen for others, whose
+// joins cost more than the idle lanes: 85,707 rows of 783 in fp16, 160 and 123 us.
 struct Backward {
     int lanes, p, depth, threads, grid;
     size_t smem;
@@ -800,7 +811,7 @@ struct Backward {
 static Backward backward_shape(int64_t rows, int n, int size, bool vector) {
     Backward o;
     o.lanes = n <= 64 ? 8 : n <= 512 ? 32 : 0;
-    o.p = n <= 256 || (n > 512 && n <= 1024) ? 8 : n <= 8192 ? 16 : 32;
+    o.p = n <= 256 || (vector && n > 512 && n <= 1024) ? 8 : n <= 8192 ? 16 : 32;
     o.threads = o.lanes ? 256 : block_threads(n, o.p);
     const int teams = o.lanes ? 256 / o.lanes : 1;
     const size_t pair = 2 * (size_t)((o.lanes ? o.lanes : o.threads) * o.p * size + (vector ? 0 : 16));  // a row of x and one of dy
@@ -813,10 +824,10 @@ static Backward backward_shape(int64_t rows, int n, int size, bool vector) {
     o.grid = (int)(want < 1 ? 1 : want < full ? want : full);
     return o;
 }
-// Rows that the backward pass holds: over 8,192 elements only 16-bit vectors are.
-static bool held_backward(int n, int size, bool vector) { return n <= 8192 || (n <= 16384 && size == 2 && vector); }
+// Rows that the backward pass holds: over 8,192 elements only those of 16 bits are.
+static bool held_backward(int n, int size) { return n <= 8192 || (n <= 16384 && size == 2); }
 static int parts_of(int64_t rows, int n, int size, bool vector) {
-    if (!held_backward(n, size, vector)) return (int)(rows < 1 ? 1 : rows < 16 ? rows : 16);
+    if (!held_backward(n, size)) return (int)(rows < 1 ? 1 : rows < 16 ? rows : 16);
     return backward_shape(rows, n, size, vector).grid;
 }
 
@@ -834,7 +845,7 @@ static int backward(const T *dy, int64_t lddy, const T *x, int64_t ldx, int64_t 
         kernel = o.threads <= 256 ? backward_kernel<T, VEC, 16, 0, 4, 256>
                  : o.depth == 4   ? backward_kernel<T, VEC, 16, 0, 4, 512>
                                   : backward_kernel<T, VEC, 16, 0, 3, 512>;
-    if constexpr (VECTOR && sizeof(T) == 2)
+    if constexpr (sizeof(T) == 2)
         if (o.p == 32) kernel = backward_kernel<T, VEC, 32, 0, 2, 512>;
     if (const int e = allow_space(kernel, o.smem)) return e;
     kernel<<<o.grid, o.threads, o.smem, s>>>(dy, lddy, x, ldx, rows, n, w, mean, rstd, dx, lddx, work);
@@ -850,7 +861,7 @@ static int backward_any(const void *dy, int64_t lddy, const void *x, int64_t ldx
                                          (!dx || vectors_of<T>(dx, lddx)) && aligned16(w);
     const int parts = parts_of(rows, n, sizeof(T), vector);
     int e = 0;
-    if (!held_backward(n, sizeof(T), vector)) {
+    if (!held_backward(n, sizeof(T))) {
         if (dx && rows)
             wide_rows_kernel<T><<<(int)(rows < SMS * 2 ? rows : SMS * 2), WIDE, 0, s>>>(
                 (const T *)dy, lddy, (const T *)x, ldx, rows, n, w, mean, rstd, (T *)dx, lddx);
