@@ -132,7 +132,10 @@ __device__ __forceinline__ int left_at(const Place &p, int b) {
 // Whether blocks b and b + 1 are whole and aligned (b or an earlier block lies in the place's tensor).
 __device__ __forceinline__ bool pair_at(const Place &p, int b) { return b + 2 <= p.vectors; }
 
-__global__ void __launch_bounds__(THREADS) norm_kernel(Args a) {
+// The gradients' squares, NB blocks a warp at a time: two where a warp has few (latency
+// is the bound: the clipped step of the conv policy 16.6 us, 17.9 with four), four where
+// it has eight or more (memory is: 64 Mi fp32 gradients, the clipped step 387 and 333 us).
+template <int NB> __global__ void __launch_bounds__(THREADS) norm_kernel(Args a) {
     __shared__ double part[WARPS];
     pdl_launch();
     const int lane = threadIdx.x & 31;
@@ -141,21 +144,26 @@ __global__ void __launch_bounds__(THREADS) norm_kernel(Args a) {
     const int lo = (int)((int64_t)a.nblocks * blockIdx.x / gridDim.x), hi = (int)((int64_t)a.nblocks * (blockIdx.x + 1) / gridDim.x);
     Place t;
     t.end = 0;
-    for (int b = lo + 2 * (threadIdx.x >> 5); b < hi; b += 2 * WARPS) {
-        float g[2][4] = {};
+    for (int b = lo + NB * (threadIdx.x >> 5); b < hi; b += NB * WARPS) {
+        float g[NB][4] = {};
         if (b >= t.end) t = locate(a, b);
-        if (b + 1 < hi && pair_at(t, b)) {
-            load_grad<true>(t, (int64_t)b * BLOCK + 4 * lane, 4, g[0]);
-            load_grad<true>(t, (int64_t)(b + 1) * BLOCK + 4 * lane, 4, g[1]);
-        } else
-            for (int c = b; c < hi && c < b + 2; c++) {
-                if (c >= t.end) t = locate(a, c);
-                load_grad<false>(t, (int64_t)c * BLOCK + 4 * lane, left_at(t, c), g[c - b]);
-            }
-        float q = 0.f;
+        if (b + NB <= hi && b + NB <= t.vectors)
 #pragma unroll
-        for (int k = 0; k < 2; k++) q += (g[k][0] * g[k][0] + g[k][1] * g[k][1]) + (g[k][2] * g[k][2] + g[k][3] * g[k][3]);
-        s += q;
+            for (int k = 0; k < NB; k++) load_grad<true>(t, (int64_t)(b + k) * BLOCK + 4 * lane, 4, g[k]);
+        else
+#pragma unroll
+            for (int k = 0; k < NB; k++) {
+                if (b + k >= hi) break;
+                if (b + k >= t.end) t = locate(a, b + k);
+                load_grad<false>(t, (int64_t)(b + k) * BLOCK + 4 * lane, left_at(t, b + k), g[k]);
+            }
+#pragma unroll
+        for (int p = 0; p < NB; p += 2) {
+            float q = 0.f;
+#pragma unroll
+            for (int k = p; k < p + 2; k++) q += (g[k][0] * g[k][0] + g[k][1] * g[k][1]) + (g[k][2] * g[k][2] + g[k][3] * g[k][3]);
+            s += q;
+        }
     }
     double d = s;
 #pragma unroll
@@ -380,9 +388,13 @@ struct Tiles {
     }
 };
 
-constexpr int per_sm(int) { return 3; }  // blocks of step_kernel
+constexpr int PER_SM = 3;  // blocks of step_kernel
 
-template <int BITS> __global__ void __launch_bounds__(THREADS, per_sm(BITS)) step_kernel(Args a) {
+// The step, in one pass over everything. 128 Mi parameters take 561 us with 32-bit
+// moments (6.7 TB/s, at a copy's rate: memory is the bound) and 403 us with 8-bit ones,
+// bf16 gradients and copies (5.4 TB/s, 82 %: the bound is issue slots, 77 instructions an
+// element, most of them the two codes'). Two Mi and less take 10 to 17 us, latency.
+template <int BITS> __global__ void __launch_bounds__(THREADS, PER_SM) step_kernel(Args a) {
     __shared__ double part[WARPS];
     __shared__ float coef[2];
     __shared__ int64_t now;
@@ -490,12 +502,15 @@ extern "C" int d1_adamw(const D1AdamWTensor *tensors, int ntensors, int64_t nblo
            step, seed, partials, counts, counts + 1, 0, grad_norm};
     const cudaStream_t s = (cudaStream_t)stream;
     const int64_t norm_want = (nblocks + 2 * WARPS - 1) / (2 * WARPS), want = (nblocks + tile * WARPS - 1) / (tile * WARPS);
-    const int most = SMS * per_sm(state_bits);
+    const int most = SMS * PER_SM;
     cudaLaunchAttribute attr;
     cudaLaunchConfig_t cfg = d1::pdl_config(dim3((unsigned)(want < most ? want : most)), dim3(THREADS), 0, s, &attr);
     if (a.max_norm > 0.) {
         a.norm_parts = (int)(norm_want < NORM_GRID ? norm_want : NORM_GRID);
-        norm_kernel<<<a.norm_parts, THREADS, 0, s>>>(a);
+        if (nblocks >= NORM_GRID * WARPS * 8)
+            norm_kernel<4><<<a.norm_parts, THREADS, 0, s>>>(a);
+        else
+            norm_kernel<2><<<a.norm_parts, THREADS, 0, s>>>(a);
         if (cudaError_t e = cudaGetLastError()) return (int)e;
     } else
         cfg.numAttrs = 0;
