@@ -6,7 +6,7 @@
 //   dw_j = sum_r dy xhat       db_j = sum_r dy
 //
 // Both passes are bound by memory. A row is read once and held in registers, P
-// elements a thread, by a team of 8 or 32 lanes (short rows, joined by shuffles)
+// elements a thread, by a team of 4 to 32 lanes (short rows, joined by shuffles)
 // or by a block (joined through shared memory); the variance is the mean square
 // of the held x - mean, not a difference of sums. In the backward pass a thread
 // owns the same columns in every row, so that the weights' gradients are sums in
@@ -500,7 +500,7 @@ __global__ void __launch_bounds__(1024, 1)
     }
 }
 
-// dx of the rows that a team (8 or 32 lanes, or the block) takes, and the
+// dx of the rows that a team (8 to 32 lanes, or the block) takes, and the
 // block's partial sums of dw and db in work[blockIdx.x]. Up to P = 16 the weights
 // and dy w stay in registers; with 32 the weights are in shared memory and dy w
 // is taken again. 16,384 rows of 4,096 in bf16 take 77 us (5.2 TB/s, 80 % of a
@@ -776,9 +776,20 @@ static int forward(const T *x, int64_t ldx, int64_t rows, int n, const float *w,
         forward_kernel<T, VEC, P, G, R><<<(int)blocks, threads, 0, s>>>(x, ldx, rows, n, w, b, eps, y, ldy, mean, rstd); \
         return (int)cudaGetLastError();                                                                               \
     } while (0)
+    // Sixteen elements a lane by as few lanes as hold the row, for a row's joins cost the same whatever they join:
+    // 233,016 rows of 72 in bf16 take 23 us with 8 lanes, 51 with 32; 83,886 of 200 19 us with 16, 23 with 32. Element
+    // by element 8 a lane are as good, and where rows are too few for the SMs, 32 lanes have the shorter way.
+    const bool many = rows >= SMS * 32;
+    if (VEC == 8 && n <= 64 && many) D1_LN_FORWARD(16, 4, 2, 256);
     if (n <= 64) D1_LN_FORWARD(8, 8, 2, 256);
+    if (VEC > 1 && n <= 128 && many) D1_LN_FORWARD(16, 8, 2, 256);
+    if (VEC > 1 && n <= 256 && many) D1_LN_FORWARD(16, 16, 2, 256);
     if (n <= 256) D1_LN_FORWARD(8, 32, 2, 256);
+    // (12 and 24 elements a lane leave fewer idle where the bound is instructions: 120,266 rows of 279 in bf16 49 and
+    // 46 us, 64,403 of 521 in fp16 50 and 44)
+    if (VEC <= 2 && n <= 384) D1_LN_FORWARD((VEC <= 2 ? 12 : 16), 32, 2, 256);
     if (n <= 512) D1_LN_FORWARD(16, 32, 2, 256);
+    if (VEC == 2 && n <= 768) D1_LN_FORWARD((VEC == 2 ? 24 : 32), 32, 1, 256);
     if (n <= 1024) D1_LN_FORWARD(32, 32, 1, 256);
     // Longer rows are a block's. Where the vectors are whole, 32 elements a thread (64 of the longest) need fewer
     // joins than 16 do, and blocks that come and go keep more rows under way than resident ones with their rows in
@@ -816,19 +827,23 @@ static int forward_any(const void *x, int64_t ldx, int64_t rows, int n, const fl
     return forward<T, sizeof(T) == 2 ? 2 : 1>((const T *)x, ldx, rows, n, w, b, eps, (T *)y, ldy, mean, rstd, s);
 }
 
-// How the backward pass runs: teams of 8 or 32 lanes, or blocks (lanes = 0),
+// How the backward pass runs: teams of 8, 16 or 32 lanes, or blocks (lanes = 0),
 // with P elements a thread, DEPTH rows in shared memory and as many blocks as
 // the SMs hold at once (more would only write more partial sums). Eight elements
 // a thread for rows of 513 to 1,024 that are vectors, sixteen for others, whose
 // joins cost more than the idle lanes: 85,707 rows of 783 in fp16, 160 and 123 us.
+// Twelve for those of 257 to 384: 120,266 of 279 in bf16, 91 us with sixteen and 70.
+// Rows of 65 to 256 have sixteen too, in 8 or 16 lanes, but for element by element:
+// 131,072 of 128 in bf16 40 us in 32 lanes, 22 in 8; 83,886 of 200 30 and 25.
 struct Backward {
     int lanes, p, depth, threads, grid;
     size_t smem;
 };
 static Backward backward_shape(int64_t rows, int n, int size, bool vector) {
     Backward o;
-    o.lanes = n <= 64 ? 8 : n <= 512 ? 32 : 0;
-    o.p = n <= 256 || (vector && n > 512 && n <= 1024) ? 8 : n <= 8192 ? 16 : 32;
+    const bool single = size == 4 && !vector;
+    o.lanes = n <= (single ? 64 : 128) ? 8 : n <= 256 && !single ? 16 : n <= 512 ? 32 : 0;
+    o.p = !single && n > 64 && n <= 256 ? 16 : n <= 256 || (vector && n > 512 && n <= 1024) ? 8 : !vector && n <= 384 ? 12 : n <= 8192 ? 16 : 32;
     o.threads = o.lanes ? 256 : block_threads(n, o.p);
     const int teams = o.lanes ? 256 / o.lanes : 1;
     const size_t pair = 2 * (size_t)((o.lanes ? o.lanes : o.threads) * o.p * size + (vector ? 0 : 16));  // a row of x and one of dy
@@ -855,9 +870,13 @@ static int backward(const T *dy, int64_t lddy, const T *x, int64_t ldx, int64_t 
     const Backward o = backward_shape(rows, n, sizeof(T), VECTOR);
     auto kernel = backward_kernel<T, VEC, 8, 0, 4, 512>;
     if (o.lanes == 8)
-        kernel = backward_kernel<T, VEC, 8, 8, 4, 256>;
+        kernel = o.p == 8 ? backward_kernel<T, VEC, 8, 8, 4, 256> : backward_kernel<T, VEC, 16, 8, 4, 256>;
+    else if (o.lanes == 16)
+        kernel = backward_kernel<T, VEC, 16, 16, 4, 256>;
     else if (o.lanes == 32)
-        kernel = o.p == 8 ? backward_kernel<T, VEC, 8, 32, 4, 256> : backward_kernel<T, VEC, 16, 32, 4, 256>;
+        kernel = o.p == 8    ? backward_kernel<T, VEC, 8, 32, 4, 256>
+                 : o.p == 12 ? backward_kernel<T, VEC, VEC <= 2 ? 12 : 16, 32, 4, 256>
+                             : backward_kernel<T, VEC, 16, 32, 4, 256>;
     else if (o.p == 16)
         kernel = o.threads <= 256 ? backward_kernel<T, VEC, 16, 0, 4, 256>
                  : o.depth == 4   ? backward_kernel<T, VEC, 16, 0, 4, 512>

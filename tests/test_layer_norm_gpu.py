@@ -102,6 +102,16 @@ def test_many_long_rows(n, dtype):                     # a block's rows follow o
 
 
 @pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('n', [3, 16, 33, 64, 65, 72, 100, 128, 130, 200, 256, 279, 384, 521, 767])
+def test_thousands_of_short_rows(n, dtype):            # in the teams that many rows have, the last one not full
+    from d1.layer_norm import layer_norm, layer_norm_backward
+    x, dy, w, b = data(5003, n, dtype, 19 * n)
+    y, mean, rstd = layer_norm(x, w, b)
+    check_forward(x, w, b, 1e-5, (y, mean, rstd))
+    check_backward(dy, x, w, 1e-5, layer_norm_backward(dy, x, mean, rstd, w), (mean, rstd))
+
+
+@pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('n', [8, 500, 512, 1024, 4096, 9000])
 def test_pitches_and_alignments(n, dtype):
     from d1.layer_norm import layer_norm, layer_norm_backward
