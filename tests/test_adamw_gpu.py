@@ -134,6 +134,20 @@ def test_many_tensors_and_large_ones():
         check_step(opt, before, grads, [0.01] * len(sizes), min(1.0, 1.0 / (norm + 1e-6)), 1e-3)
 
 
+@pytest.mark.parametrize('bits', [32, 8])
+def test_tiles_that_are_handed_out(bits):              # four and more for each warp; the counter is left as it was found
+    from d1.adamw import AdamW
+    sizes = [17_000_003, 700, 1, 4_000_100, 130]
+    params, grads, copies = tensors(sizes, 6, torch.bfloat16 if bits == 8 else torch.float32, offset=1)
+    opt = AdamW(params, grads, state_bits=bits, copies=copies, max_norm=1.0)
+    norm = math.sqrt(sum(float(g.double().square().sum()) for g in grads))
+    for step in range(3):
+        before = [(p.clone(), *(x.clone() for x in opt.moments(i))) for i, p in enumerate(params)]
+        opt.step()
+        assert abs(float(opt.grad_norm) - norm) <= 1e-6 * norm
+        check_step(opt, before, grads, [0.01] * len(sizes), min(1.0, 1.0 / (norm + 1e-6)), 1e-3)
+
+
 def test_rounding_is_unbiased_and_moments_decay():
     """Elements of one value per block: the decoded mean is the value within five standard errors (at most half a
     code each); and with no gradient v falls as 0.999^t, which rounding to nearest would not let it."""

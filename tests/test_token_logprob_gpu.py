@@ -117,6 +117,20 @@ def test_forward_and_gradient(vocab, dtype):
         assert ((d.double() - want).abs() <= tol + EPS[dtype] * (want.abs() + tol) + TINY[dtype]).all()
 
 
+@pytest.mark.parametrize('rows, vocab, dtype, masked, top', [
+    (1900, 8200, torch.bfloat16, True, 9), (1900, 9001, torch.float32, False, 3), (2500, 12288, torch.float16, True, 0),
+    (80003, 70, torch.float16, True, 5), (310003, 5, torch.bfloat16, True, 2), (310003, 64, torch.float32, False, 0)])
+def test_more_rows_than_a_grid_holds(rows, vocab, dtype, masked, top):
+    from d1.token_logprob import token_logprob, token_logprob_backward
+    logits, tokens, legal, g = case(rows, vocab, dtype, masked, rows + vocab)
+    got = token_logprob(logits, tokens, legal, 0.9, top)
+    check_forward(logits, tokens, legal, 0.9, top, got)
+    dlogp, dentropy = torch.randn(rows, device='cuda', generator=g), torch.randn(rows, device='cuda', generator=g)
+    d = token_logprob_backward(logits, tokens, got.stats, got.entropy, dlogp, dentropy, legal, 0.9)
+    want, tol = gradient(logits, tokens, legal, 0.9, dlogp, dentropy)
+    assert ((d.double() - want).abs() <= tol + EPS[dtype] * (want.abs() + tol) + TINY[dtype]).all()
+
+
 @pytest.mark.parametrize('rows', [1, 2, 9, 40])
 def test_few_long_rows_are_split_and_joined(rows):
     from d1.token_logprob import token_logprob
