@@ -200,8 +200,6 @@ template <int VEC, int P> struct SharedWeights {
         constexpr int STEP = 32 * VEC;
         if constexpr (VEC == 8)
             return *reinterpret_cast<const float4 *>(s + (q & 1 ? total / 2 : 0) + start / 2 + q / 2 * (STEP / 2));
-        else if constexpr (VEC == 4)
-            return *reinterpret_cast<const float4 *>(s + start + q * STEP);
         else if constexpr (VEC == 2) {
             const float2 a = *reinterpret_cast<const float2 *>(s + start + 2 * q * STEP), b = *reinterpret_cast<const float2 *>(s + start + (2 * q + 1) * STEP);
             return make_float4(a.x, a.y, b.x, b.y);
