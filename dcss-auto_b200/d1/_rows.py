@@ -59,10 +59,11 @@ _F32 = {}
 
 def empty_f32(device, *shape):
     """torch.empty of float32 on `device`, by the cheapest route: new_empty of a kept
-    tensor, with the sizes as numbers (half the cost of torch.empty with a shape)."""
+    tensor, with the sizes as numbers (half the cost of torch.empty with a shape).
+    The type is named: the kernels write 4 bytes an element whatever torch's default is."""
     kept = _F32.get(device)
     if kept is None:
-        kept = _F32[device] = torch.empty(0, device=device)
+        kept = _F32[device] = torch.empty(0, dtype=torch.float32, device=device)
     return kept.new_empty(*shape) if shape else kept.new_empty(())
 
 

@@ -63,16 +63,17 @@ class AdamW:
         if not self.nblocks:
             raise ValueError('the parameters hold no elements')
         n, dev = self.nblocks * BLOCK, self.device
+        f32 = dict(dtype=torch.float32, device=dev)
         if state_bits == 32:
-            self.m, self.v = torch.zeros(n, device=dev), torch.zeros(n, device=dev)
+            self.m, self.v = torch.zeros(n, **f32), torch.zeros(n, **f32)
             self.m_scale = self.v_scale = None
         else:
             self.m = torch.zeros(n, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)
             self.v = torch.zeros(n, dtype=torch.uint8, device=dev).view(torch.float8_e5m2)
-            self.m_scale, self.v_scale = torch.ones(self.nblocks, device=dev), torch.ones(self.nblocks, device=dev)
+            self.m_scale, self.v_scale = torch.ones(self.nblocks, **f32), torch.ones(self.nblocks, **f32)
         self.lib = library()
         self.step_dev = torch.zeros(1, dtype=torch.int64, device=dev)
-        self.grad_norm = torch.zeros(1, device=dev)  # the last step's, when it clips
+        self.grad_norm = torch.zeros(1, **f32)  # the last step's, when it clips
         self._work = torch.zeros(self.lib.d1_adamw_work_bytes(), dtype=torch.uint8, device=dev)
         self._table = torch.empty(len(params) * C.sizeof(_Tensor), dtype=torch.uint8, device=dev)
         self.set_grads(grads)

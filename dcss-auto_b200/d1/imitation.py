@@ -26,6 +26,7 @@ from .conv_policy import WIDTH
 from .layer_norm import layer_norm, layer_norm_backward
 from .token_logprob import token_logprob, token_logprob_backward
 
+F32 = torch.float32
 JOINT, PITCH = 28, 32  # joint actions; logits of a row with their padding
 
 
@@ -42,10 +43,11 @@ class JointHead:
     def __init__(self, device='cuda', seed=0, lr=3e-4, weight_decay=0.01, max_grad_norm=0.5, ent_coef=0.0, state_bits=8):
         self.device = dev = resolve_device(device)
         g = torch.Generator(device='cpu').manual_seed(seed)
-        w = torch.zeros(PITCH, WIDTH)
-        w[:JOINT] = torch.randn(JOINT, WIDTH, generator=g) / WIDTH ** 0.5
-        self.params = {'w': w.to(dev), 'b': torch.zeros(PITCH, device=dev), 'norm_w': torch.ones(WIDTH, device=dev),
-                       'norm_b': torch.zeros(WIDTH, device=dev)}
+        w = torch.zeros(PITCH, WIDTH, dtype=F32)
+        w[:JOINT] = torch.randn(JOINT, WIDTH, generator=g, dtype=F32) / WIDTH ** 0.5
+        f32 = dict(dtype=F32, device=dev)
+        self.params = {'w': w.to(dev), 'b': torch.zeros(PITCH, **f32), 'norm_w': torch.ones(WIDTH, **f32),
+                       'norm_b': torch.zeros(WIDTH, **f32)}
         self.grads = {k: torch.zeros_like(p) for k, p in self.params.items()}
         self.w = self.params['w'].to(torch.bfloat16)
         self.ent_coef = ent_coef
@@ -74,11 +76,11 @@ class JointHead:
         n, g = h.shape[0], self.grads
         dl = torch.zeros((n, PITCH), dtype=torch.bfloat16, device=self.device)
         token_logprob_backward(logits, joint, r.stats, r.entropy, dlogp, dentropy, legal=bits, out=dl[:, :JOINT])
-        slabs = torch.empty((G.splits_for(n, 8), PITCH, WIDTH), device=self.device)
+        slabs = torch.empty((G.splits_for(n, 8), PITCH, WIDTH), dtype=F32, device=self.device)
         G.gemm_ex(dl, y, a_kn=True, b_kn=True, out_f32=slabs, splits=slabs.shape[0])
         check(self.lib.d1_reduce_slabs(slabs.data_ptr(), slabs.shape[0], PITCH * WIDTH, g['w'].data_ptr(),
                                        launch_stream(self.device)), 'd1_reduce_slabs')
-        torch.sum(dl, 0, dtype=torch.float32, out=g['b'])
+        torch.sum(dl, 0, dtype=F32, out=g['b'])
         dh, dw, db = layer_norm_backward(G.gemm_bkn(dl, self.w), h, mean, rstd, self.params['norm_w'])
         g['norm_w'].copy_(dw)
         g['norm_b'].copy_(db)
@@ -90,8 +92,8 @@ class JointHead:
         log-probabilities and entropies before the step, on the device."""
         n = h.shape[0]
         r, saved = self.forward(h, joint, legal)
-        dlogp = torch.full((n,), -1.0 / n, device=self.device)
-        dentropy = torch.full((n,), -self.ent_coef / n, device=self.device) if self.ent_coef else None
+        dlogp = torch.full((n,), -1.0 / n, dtype=F32, device=self.device)
+        dentropy = torch.full((n,), -self.ent_coef / n, dtype=F32, device=self.device) if self.ent_coef else None
         self.backward(r, saved, dlogp, dentropy)
         self.optimizer.step()
         return r.logp, r.entropy
