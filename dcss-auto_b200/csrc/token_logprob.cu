@@ -28,6 +28,7 @@
 #include <math_constants.h>
 
 #include "d1_elem.cuh"
+#include "d1_rows.h"
 
 namespace d1 {
 namespace lp {
@@ -254,6 +255,8 @@ template <class T> struct Row {
     __device__ __forceinline__ int first(int i) const { return head + i * N; }
     __device__ __forceinline__ int loose_index(int k) const { return k < head ? k : k + vectors * N; }
     __device__ __forceinline__ uint4 load(int i) const { return __ldg(reinterpret_cast<const uint4 *>(x + first(i))); }
+    // the same where the kernel may write over the row
+    __device__ __forceinline__ uint4 load_own(int i) const { return *reinterpret_cast<const uint4 *>(x + first(i)); }
     // The legal bits of vector i: its N bits lie in one byte (in all of a row's
     // vectors, where the first starts at a multiple of N) or in two.
     __device__ __forceinline__ uint32_t bits(int i) const {
@@ -1017,17 +1020,32 @@ template <class T> struct StagedMask {
     }
 };
 
+// The gradient may be written over the logits (IN_PLACE): a thread reads the elements
+// that it writes before it writes them, and every thread of a row reads the token's
+// logit besides, for the row's constants. So there a row has one team, which waits for
+// its slowest reader before it stores; the pointers are not __restrict__, nor are the
+// logits read as data that nobody writes. These are kernels of their own, because
+// without the promise of __restrict__ the others would lose 1 to 4 %.
+template <class T, bool IN_PLACE> struct Apart {
+    using In = const T *__restrict__;
+    using Result = T *__restrict__;
+};
+template <class T> struct Apart<T, true> {
+    using In = const T *;
+    using Result = T *;
+};
+
 // A warp or (long rows) a block takes rows or, where they are few, shares of them. The
 // vectors are the logits' aligned ones; the gradient is stored as vectors where
 // its rows are aligned alike, else element by element. Memory is its bound: 4,096
 // rows of 32,768 in bf16 take 88 us (94 % of a copy's rate), 4,096 of 50,021 with
 // a mask 146 us (89 %); with rows of a few vectors a lane the constants of each
 // row show (65,536 of 1,000: 57 us, 70 %).
-template <class T, bool MASK, int TEAM>
+template <class T, bool MASK, int TEAM, bool IN_PLACE>
 __global__ void __launch_bounds__(THREADS, TEAM == 32 ? 5 : 6)
-    long_backward_kernel(const T *__restrict__ logits, int64_t ld, int64_t rows, int vocab,
+    long_backward_kernel(typename Apart<T, IN_PLACE>::In logits, int64_t ld, int64_t rows, int vocab,
                          const uint8_t *__restrict__ legal, int64_t ldlegal, float inv_t, Grads g,
-                         T *__restrict__ dlogits, int64_t ldd) {
+                         typename Apart<T, IN_PLACE>::Result dlogits, int64_t ldd) {
     constexpr int N = Wide<T>::N;
     const float c = inv_t * LOG2E;
     constexpr bool STAGED = MASK && TEAM == THREADS;
@@ -1039,6 +1057,12 @@ __global__ void __launch_bounds__(THREADS, TEAM == 32 ? 5 : 6)
         const bool alike = ((reinterpret_cast<uintptr_t>(d) ^ reinterpret_cast<uintptr_t>(row.x)) & 15) == 0;
         const int lo = (int)((int64_t)row.vectors * blockIdx.x / gridDim.x), hi = (int)((int64_t)row.vectors * (blockIdx.x + 1) / gridDim.x);
         const RowGrad k = row_grad(g, row.x, row.legal, r, vocab, inv_t);
+        if (IN_PLACE) {
+            if (TEAM == THREADS)
+                __syncthreads();
+            else
+                __syncwarp();
+        }
         for (int from = lo; from < hi;) {  // at once, or a share of the legal bytes at a time
             const int to = STAGED && from + StagedMask<T>::VECTORS < hi ? from + StagedMask<T>::VECTORS : hi;
             StagedMask<T> mask;
@@ -1055,7 +1079,7 @@ __global__ void __launch_bounds__(THREADS, TEAM == 32 ? 5 : 6)
     #pragma unroll
                 for (int u = 0; u < UNROLL; u++)
                     if (i0 + u * TEAM < to) {
-                        v[u] = row.load(i0 + u * TEAM);
+                        v[u] = IN_PLACE ? row.load_own(i0 + u * TEAM) : row.load(i0 + u * TEAM);
                         if (MASK) bits[u] = STAGED ? mask.bits(row, i0 + u * TEAM) : row.bits(i0 + u * TEAM);
                     }
     #pragma unroll
@@ -1091,11 +1115,11 @@ __global__ void __launch_bounds__(THREADS, TEAM == 32 ? 5 : 6)
 }
 
 // Short rows: eight lanes a row (65,536 of 28 in fp32, masked: 10 us, latency).
-template <class T>
+template <class T, bool IN_PLACE>
 __global__ void __launch_bounds__(THREADS)
-    short_backward_kernel(const T *__restrict__ logits, int64_t ld, int64_t rows, int vocab,
+    short_backward_kernel(typename Apart<T, IN_PLACE>::In logits, int64_t ld, int64_t rows, int vocab,
                           const uint8_t *__restrict__ legal, int64_t ldlegal, float inv_t, Grads g,
-                          T *__restrict__ dlogits, int64_t ldd) {
+                          typename Apart<T, IN_PLACE>::Result dlogits, int64_t ldd) {
     constexpr int G = 8, GROUPS = THREADS / G;
     const float c = inv_t * LOG2E;
     const int lane = threadIdx.x % G;
@@ -1103,6 +1127,7 @@ __global__ void __launch_bounds__(THREADS)
         const T *row = logits + r * ld;
         const uint8_t *bits = legal ? legal + r * ldlegal : nullptr;
         const RowGrad k = row_grad(g, row, bits, r, vocab, inv_t);
+        if (IN_PLACE) __syncwarp(0xffu << (threadIdx.x & 24));
         for (int j = lane; j < vocab; j += G) {
             dlogits[r * ldd + j] = grad_one<T>(k, logit_at(row, bits, j), j, c);
         }
@@ -1157,32 +1182,37 @@ static int forward(const void *logits, int64_t ld, int64_t rows, int vocab, cons
                        : cudaLaunchKernelEx(&cfg, cluster_forward_kernel<T, false>, x, ld, rows, vocab, legal, ldlegal, inv_t, cluster, out));
 }
 
+// A launch of `kernel`, or of `own` where the gradient goes over the logits.
+#define D1_LP_BACKWARD(kernel, own, grid)                                                                             \
+    do {                                                                                                              \
+        if (d == x)                                                                                                   \
+            own<<<grid, THREADS, 0, s>>>(x, ld, rows, vocab, legal, ldlegal, inv_t, g, d, ldd);                        \
+        else                                                                                                          \
+            kernel<<<grid, THREADS, 0, s>>>(x, ld, rows, vocab, legal, ldlegal, inv_t, g, d, ldd);                     \
+        return (int)cudaGetLastError();                                                                               \
+    } while (0)
+template <class T, bool MASK>
+static int backward_long(const T *x, int64_t ld, int64_t rows, int vocab, const uint8_t *legal, int64_t ldlegal,
+                         float inv_t, const Grads &g, T *d, int64_t ldd, cudaStream_t s) {
+    if (vocab / Wide<T>::N <= 32 * UNROLL * 2) {
+        const dim3 grid(1, (unsigned)(rows < 65535 * WARPS ? (rows + WARPS - 1) / WARPS : 65535));
+        D1_LP_BACKWARD((long_backward_kernel<T, MASK, 32, false>), (long_backward_kernel<T, MASK, 32, true>), grid);
+    }
+    // blocks for each row: one, or enough of them for the 148 SMs where rows are few
+    const int tiles = vocab / (Wide<T>::N * THREADS * UNROLL) + 1;
+    const int64_t want = d == x ? 1 : (SMS * 6 + rows - 1) / rows;
+    const dim3 grid((unsigned)(want < tiles ? want : tiles), (unsigned)(rows < 65535 ? rows : 65535));
+    D1_LP_BACKWARD((long_backward_kernel<T, MASK, THREADS, false>), (long_backward_kernel<T, MASK, THREADS, true>), grid);
+}
 template <class T>
 static int backward(const void *logits, int64_t ld, int64_t rows, int vocab, const uint8_t *legal, int64_t ldlegal,
                     float inv_t, const Grads &g, void *dlogits, int64_t ldd, cudaStream_t s) {
     const T *x = (const T *)logits;
     T *d = (T *)dlogits;
-    if (vocab <= SHORT_VOCAB) {
-        short_backward_kernel<T><<<blocks_of(rows, THREADS / 8), THREADS, 0, s>>>(x, ld, rows, vocab, legal, ldlegal, inv_t, g, d, ldd);
-        return (int)cudaGetLastError();
-    }
-    if (vocab / Wide<T>::N <= 32 * UNROLL * 2) {
-        const dim3 grid(1, (unsigned)(rows < 65535 * WARPS ? (rows + WARPS - 1) / WARPS : 65535));
-        if (legal)
-            long_backward_kernel<T, true, 32><<<grid, THREADS, 0, s>>>(x, ld, rows, vocab, legal, ldlegal, inv_t, g, d, ldd);
-        else
-            long_backward_kernel<T, false, 32><<<grid, THREADS, 0, s>>>(x, ld, rows, vocab, legal, ldlegal, inv_t, g, d, ldd);
-        return (int)cudaGetLastError();
-    }
-    // blocks for each row: one, or enough of them for the 148 SMs where rows are few
-    const int tiles = vocab / (Wide<T>::N * THREADS * UNROLL) + 1;
-    const int64_t want = (SMS * 6 + rows - 1) / rows;
-    const dim3 grid((unsigned)(want < tiles ? want : tiles), (unsigned)(rows < 65535 ? rows : 65535));
-    if (legal)
-        long_backward_kernel<T, true, THREADS><<<grid, THREADS, 0, s>>>(x, ld, rows, vocab, legal, ldlegal, inv_t, g, d, ldd);
-    else
-        long_backward_kernel<T, false, THREADS><<<grid, THREADS, 0, s>>>(x, ld, rows, vocab, legal, ldlegal, inv_t, g, d, ldd);
-    return (int)cudaGetLastError();
+    if (vocab <= SHORT_VOCAB)
+        D1_LP_BACKWARD((short_backward_kernel<T, false>), (short_backward_kernel<T, true>), blocks_of(rows, THREADS / 8));
+    return legal ? backward_long<T, true>(x, ld, rows, vocab, legal, ldlegal, inv_t, g, d, ldd, s)
+                 : backward_long<T, false>(x, ld, rows, vocab, legal, ldlegal, inv_t, g, d, ldd, s);
 }
 
 }  // namespace lp
@@ -1217,6 +1247,10 @@ extern "C" int d1_token_logprob_backward(const void *logits, int64_t ld, int typ
         (rows > 1 && ldd < vocab) || !element_aligned(logits, type) || !element_aligned(dlogits, type))
         return D1_ERR_BAD_ARGUMENT;
     if (rows == 0) return 0;
+    const int64_t size = type == D1_TYPE_F32 ? 4 : 2;
+    if (dlogits == logits ? rows > 1 && ldd != ld
+                          : rows_overlap({(uintptr_t)logits, rows, vocab * size, ld * size}, {(uintptr_t)dlogits, rows, vocab * size, ldd * size}))
+        return D1_ERR_BAD_ARGUMENT;
     const float inv_t = 1.f / temperature;
     const lp::Grads g{tokens, stats, entropy, dlogp, dentropy};
     const uint8_t *bits = (const uint8_t *)legal;

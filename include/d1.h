@@ -694,7 +694,8 @@ int d1_token_logprob(const void *logits, int64_t ld, int type, int64_t rows, int
  *   dlogits_j = ([j == token] dlogp - p_j (dlogp + dentropy (log p_j + entropy))) / temperature
  * A token that is left out gets 0; a row without a token, or whose token is left
  * out, has no dlogp; a row with nothing left gets zeros. dlogits may be logits
- * itself (same pitch) and overlaps nothing else. */
+ * itself (same pitch; few long rows are then not split over blocks) and
+ * overlaps nothing else. */
 int d1_token_logprob_backward(const void *logits, int64_t ld, int type, int64_t rows, int vocab,
                               const int64_t *tokens, const void *legal, int64_t ldlegal, float temperature,
                               const float *stats, const float *entropy, const float *dlogp, const float *dentropy,
