@@ -3,6 +3,12 @@
 #pragma once
 #include <stdint.h>
 
+#ifdef __CUDACC__
+#define D1_ROWS_BOTH __host__ __device__ __forceinline__
+#else
+#define D1_ROWS_BOTH inline
+#endif
+
 namespace d1 {
 
 // `count` rows of `width` bytes, `pitch` bytes apart.
@@ -37,6 +43,20 @@ inline bool rows_overlap(RowSpan a, RowSpan b) {
     int64_t k = (low >= 0 ? low / p : -((-low + p - 1) / p)) + 1;
     if (k < 1 - b.count) k = 1 - b.count;
     return k < a.count && k * p < d + b.width;
+}
+
+// The 16-byte piece at offset p (a multiple of 16) of a row of `size` bytes,
+// counted from the last 16-byte boundary at or before it: where it is copied from and
+// how many of its bytes are read. A piece past the row's end reads nothing, but a
+// copy's source is aligned whatever its size, so there it is that boundary.
+struct RowPiece {
+    uintptr_t from;
+    int bytes;
+};
+D1_ROWS_BOTH RowPiece row_piece(uintptr_t row, int size, int p) {
+    const uintptr_t base = row & ~(uintptr_t)15;
+    const int left = (int)(row & 15) + size - p;
+    return {left > 0 ? base + p : base, left < 0 ? 0 : left < 16 ? left : 16};
 }
 
 }  // namespace d1

@@ -20,6 +20,7 @@
 // last warp has to look where the row ends.
 #include "d1_elem.cuh"
 #include "d1_pdl.cuh"
+#include "d1_rows.h"
 
 namespace d1 {
 namespace ln {
@@ -408,8 +409,10 @@ template <class T, int VEC, int P, int G> struct Rows {
                         using U = typename Word<sizeof(T)>::U;
                         Word<sizeof(T)>::store(stage + e, e < to ? *reinterpret_cast<const U *>(base + e) : U(0));
                     }
-                else
-                    copy_async16(stage + p, p < to ? reinterpret_cast<const void *>(base + p) : at, to - p < 0 ? 0 : to - p < 16 ? to - p : 16);
+                else {
+                    const RowPiece piece = row_piece(reinterpret_cast<uintptr_t>(at), n * (int)sizeof(T), p);
+                    copy_async16(stage + p, reinterpret_cast<const void *>(piece.from), piece.bytes);
+                }
             }
         }
         left--;
