@@ -72,8 +72,32 @@ def empty_like(t):
     return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
+def rows_meet(p, rows, width, pitch, q, rows_q, width_q, pitch_q):
+    """Whether `rows` rows of `width` bytes from p on, `pitch` apart, share a byte with
+    those from q on. Exact: column slices of one buffer lie between one another."""
+    if not pitch:
+        rows = min(rows, 1)
+    if not pitch_q:
+        rows_q = min(rows_q, 1)
+    if not (rows and rows_q and p < q + (rows_q - 1) * pitch_q + width_q and q < p + (rows - 1) * pitch + width):
+        return False
+    if rows == 1:
+        pitch = pitch_q
+    if rows_q == 1:
+        pitch_q = pitch
+    if rows == rows_q == 1:
+        return True
+    if pitch != pitch_q:  # row by row of the one that has fewer
+        if rows <= rows_q:
+            return any(rows_meet(p + i * pitch, 1, width, 0, q, rows_q, width_q, pitch_q) for i in range(rows))
+        return any(rows_meet(p, rows, width, pitch, q + i * pitch_q, 1, width_q, 0) for i in range(rows_q))
+    # rows i and j meet where q - p - width < k pitch < q - p + width_q with k = i - j
+    k = max((q - p - width) // pitch + 1, 1 - rows_q)
+    return k < rows and k * pitch < q - p + width_q
+
+
 def apart(a, b, size, name, other):
-    """Refuses two matrices of elements of `size` bytes whose spans of memory overlap."""
-    (p, rows, n, pitch), (q, _, _, step) = a, b
-    if rows and p < q + ((rows - 1) * step + n) * size and q < p + ((rows - 1) * pitch + n) * size:
+    """Refuses two matrices of elements of `size` bytes that share memory."""
+    (p, rows, n, pitch), (q, rows_q, n_q, step) = a, b
+    if rows_meet(p, rows, n * size, pitch * size, q, rows_q, n_q * size, step * size):
         raise ValueError(f'{name} overlaps {other}')
