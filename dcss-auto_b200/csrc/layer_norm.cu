@@ -929,6 +929,9 @@ extern "C" int d1_layer_norm(const void *x, int64_t ldx, int type, int64_t rows,
         (rows > 1 && ldy < n) || !element_aligned(x, type) || !element_aligned(y, type))
         return D1_ERR_BAD_ARGUMENT;
     if (rows == 0) return 0;
+    const int64_t size = type == D1_TYPE_F32 ? 4 : 2;
+    const RowSpan in{(uintptr_t)x, rows, n * size, ldx * size}, result{(uintptr_t)y, rows, n * size, ldy * size};
+    if (x == y ? rows > 1 && ldx != ldy : rows_overlap(in, result)) return D1_ERR_BAD_ARGUMENT;
     const cudaStream_t s = (cudaStream_t)stream;
     if (type == D1_TYPE_F32) return ln::forward_any<float>(x, ldx, rows, n, weight, bias, eps, y, ldy, mean, rstd, s);
     if (type == D1_TYPE_BF16)
@@ -953,6 +956,10 @@ extern "C" int d1_layer_norm_backward(const void *dy, int64_t lddy, const void *
     if (!type_ok(type) || rows < 0 || n < 1 || (rows && (!dy || !x || !mean || !rstd)) || lddy < 0 || ldx < 0 ||
         lddx < 0 || (dx && rows > 1 && lddx < n) || ((dweight || dbias) && !work) || !element_aligned(x, type) ||
         !element_aligned(dy, type) || !element_aligned(dx, type))
+        return D1_ERR_BAD_ARGUMENT;
+    const int64_t size = type == D1_TYPE_F32 ? 4 : 2;
+    const RowSpan result{(uintptr_t)dx, dx ? rows : 0, n * size, lddx * size};
+    if (rows_overlap(result, {(uintptr_t)x, rows, n * size, ldx * size}) || rows_overlap(result, {(uintptr_t)dy, rows, n * size, lddy * size}))
         return D1_ERR_BAD_ARGUMENT;
     const cudaStream_t s = (cudaStream_t)stream;
     if (type == D1_TYPE_F32)

@@ -18,10 +18,11 @@ F32 = torch.float32
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, out=None):
-    """(y, mean, rstd): y as x (or written to `out`, which may be x), mean and
-    rstd float32 of x's leading shape, which the backward pass takes."""
+    """(y, mean, rstd): y as x (or written to `out`, which may be x but shares no
+    memory with it otherwise), mean and rstd float32 of x's leading shape, which
+    the backward pass takes."""
     kind, dev = type_of(x, 'x'), x.device
-    px, rows, n, ldx = matrix(x, 'x')
+    px, rows, n, ldx = mx = matrix(x, 'x')
     if not eps >= 0:
         raise ValueError('eps must not be negative')
     w, b = vector(weight, n, F32, dev, 'weight'), vector(bias, n, F32, dev, 'bias')
@@ -29,7 +30,9 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, out=None):
         out = empty_like(x)
         py, ldy = out.data_ptr(), n
     else:
-        py, _, _, ldy = like(out, x, 'out')
+        py, _, _, ldy = mo = like(out, x, 'out')
+        if py != px or (ldy != ldx and rows > 1):
+            apart(mo, mx, x.element_size(), 'out', 'x')
     lead = rows if x.dim() == 2 else x.shape[:-1]
     mean, rstd = empty_f32(dev, lead), empty_f32(dev, lead)
     check(library().d1_layer_norm(px, ldx, kind, rows, n, w, b, eps, py, ldy, mean.data_ptr(), rstd.data_ptr(),

@@ -657,7 +657,8 @@ int d1_ppo_gather_x(const void *obs, int F, const int64_t *idx, int n, void *x, 
 /* y[r] = (x[r] - mean_r) rstd_r weight + bias, with rstd_r = 1 / sqrt(var_r + eps)
  * over the n elements of row r. weight and bias are f32 [n] (NULL: 1 and 0);
  * mean and rstd (f32 [rows], NULL: not wanted) are what the backward pass takes.
- * x and y have type `type`; y may be x itself. eps >= 0, n >= 1. */
+ * x and y have type `type`; y may be x itself (same pitch) and shares no memory
+ * with it otherwise. eps >= 0, n >= 1. */
 int d1_layer_norm(const void *x, int64_t ldx, int type, int64_t rows, int n, const float *weight, const float *bias,
                   float eps, void *y, int64_t ldy, float *mean, float *rstd, void *stream);
 /* Number of partial sums d1_layer_norm_backward makes for each weight: its
@@ -667,7 +668,8 @@ int d1_layer_norm_parts(int64_t rows, int n);
  * wanted), dweight and dbias (f32 [n]; NULL: not wanted). work: f32
  * [d1_layer_norm_parts(rows, n) * 2 * n], 16-byte aligned, needed for dweight or
  * dbias. The partial sums are added in a fixed order: the same inputs give the
- * same bits. rows == 0 gives zero dweight and dbias. dx overlaps no input. */
+ * same bits. rows == 0 gives zero dweight and dbias. dx overlaps no input (its
+ * rows may lie between those of x or dy). */
 int d1_layer_norm_backward(const void *dy, int64_t lddy, const void *x, int64_t ldx, int type, int64_t rows, int n,
                            const float *weight, const float *mean, const float *rstd, void *dx, int64_t lddx,
                            float *dweight, float *dbias, float *work, void *stream);

@@ -54,3 +54,15 @@ def test_the_gradient_of_log_probabilities_is_the_logits_or_apart():
     for bad in (dict(d=P + 2), dict(d=P + 80), dict(d=P + 3 * 80 + 78), dict(d=P - 2), dict(ldd=48), dict(ld=60, ldd=60, d=P + 42),
                 dict(ld=80, ldd=100, d=P + 80)):
         assert lib.d1_token_logprob_backward(*dict(good, **bad).values()) == BAD, bad
+
+
+def test_layer_norm_in_place_or_apart():
+    from d1 import _lib
+    lib, P = _lib.library(), 1 << 20
+    good = dict(x=P, ldx=8, type=1, rows=4, n=8, w=P << 4, b=P << 5, eps=1e-5, y=P, ldy=8, mean=P << 6, rstd=P << 7, s=None)
+    for bad in (dict(y=P + 16), dict(y=P - 16), dict(y=P + 2), dict(ldy=16), dict(ldx=20, ldy=20, y=P + 14), dict(ldx=0), dict(ldx=4, ldy=8, y=P + 8)):
+        assert lib.d1_layer_norm(*dict(good, **bad).values()) == BAD, bad
+    good = dict(dy=P, lddy=8, x=P << 1, ldx=8, type=0, rows=4, n=8, w=None, mean=P << 4, rstd=P << 5, dx=P << 2, lddx=8, dw=P << 6,
+                db=P << 7, work=P << 8, s=None)
+    for bad in (dict(dx=P), dict(dx=P << 1), dict(dx=P + 32), dict(dx=(P << 1) - 4), dict(dx=(P << 1) + 100)):
+        assert lib.d1_layer_norm_backward(*dict(good, **bad).values()) == BAD, bad
