@@ -7,6 +7,8 @@ params are contiguous float32 tensors (masters) of any size and alignment,
 grads float32 or bfloat16 of the same shapes; each step reads whatever the
 gradient tensors then hold. copies (bfloat16, or None for a tensor that has
 none) are refreshed by the step. weight_decay and copies may differ by tensor.
+No parameter or copy shares memory with another one or with a gradient, and each
+keeps its storage for the optimizer's life (the step has their addresses).
 
 Moments are held in 32 bits, or in 8: m as float8_e4m3fn and v as float8_e5m2
 codes with a power-of-two scale for each block of 128 elements, 2.06 bytes a
@@ -16,6 +18,7 @@ float32. The step count is on the device, so a captured step stays correct.
 Steps of one optimizer share its work buffer: run them on one stream, or
 ordered.
 """
+import bisect
 import ctypes as C
 
 import torch
@@ -28,6 +31,24 @@ BLOCK = 128
 class _Tensor(C.Structure):
     _fields_ = [('param', C.c_void_p), ('grad', C.c_void_p), ('copy', C.c_void_p), ('count', C.c_int64),
                 ('first_block', C.c_int64), ('decay', C.c_double), ('grad_type', C.c_int), ('reserved', C.c_int)]
+
+
+def _spans(named):
+    """(first addresses, ends, names) in order of the (name, tensor) pairs that a step
+    writes, which may share no memory: two warps would write the same elements."""
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), name) for name, t in named if t.numel())
+    for (_, end, name), (at, _, other) in zip(spans, spans[1:]):
+        if at < end:
+            raise ValueError(f'{name} and {other} share memory')
+    return tuple(zip(*spans)) or ((), (), ())
+
+
+def _outside(t, name, spans):
+    """Refuses a tensor that a step reads while it writes one of the spans over it."""
+    starts, ends, names = spans
+    i = bisect.bisect_left(starts, t.data_ptr() + t.numel() * t.element_size()) - 1
+    if t.numel() and i >= 0 and ends[i] > t.data_ptr():
+        raise ValueError(f'{name} shares memory with {names[i]}')
 
 
 class AdamW:
@@ -53,6 +74,8 @@ class AdamW:
             if c is not None and (c.dtype != torch.bfloat16 or c.shape != p.shape or c.device != self.device or
                                   not c.is_contiguous()):
                 raise ValueError(f'copies[{i}] must be a contiguous bfloat16 tensor of shape {tuple(p.shape)}')
+        self._written = _spans([(f'params[{i}]', p) for i, p in enumerate(params)] +
+                               [(f'copies[{i}]', c) for i, c in enumerate(copies) if c is not None])
         self.params, self.copies, self.decay = params, copies, decay
         self.lr, self.betas, self.eps, self.max_norm = lr, betas, eps, max_norm
         self.state_bits, self.seed = state_bits, seed
@@ -89,6 +112,7 @@ class AdamW:
                     not g.is_contiguous()):
                 raise ValueError(f'grads[{i}] must be a contiguous float32 or bfloat16 tensor of shape '
                                  f'{tuple(p.shape)} on {self.device}')
+            _outside(g, f'grads[{i}]', self._written)
             table[i] = _Tensor(p.data_ptr(), g.data_ptr(), None if c is None else c.data_ptr(), p.numel(),
                                self._first[i], self.decay[i], 0 if g.dtype == torch.float32 else 1, 0)
         self.grads = grads
