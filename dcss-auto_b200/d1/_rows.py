@@ -7,6 +7,12 @@ import torch
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # D1_TYPE_* of d1.h
 
 
+def recorded(x, weight=None, bias=None):
+    """Whether torch records gradients of one of them."""
+    return torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
+                                        (bias is not None and bias.requires_grad))
+
+
 def type_of(t, name):
     """D1_TYPE_* of a tensor on a GPU."""
     code = TYPES.get(t.dtype)

@@ -77,6 +77,7 @@ class AdamW:
         self._written = _spans([(f'params[{i}]', p) for i, p in enumerate(params)] +
                                [(f'copies[{i}]', c) for i, c in enumerate(copies) if c is not None])
         self.params, self.copies, self.decay = params, copies, decay
+        self._leaves = [p for p in params if p.requires_grad]
         self.lr, self.betas, self.eps, self.max_norm = lr, betas, eps, max_norm
         self.state_bits, self.seed = state_bits, seed
         blocks = [(p.numel() + BLOCK - 1) // BLOCK for p in params]
@@ -126,6 +127,8 @@ class AdamW:
         """One step, in place. lr: this step's learning rate (default: self.lr)."""
         check(self.lib.d1_adamw(*self._state_args, self.lr if lr is None else lr, self.betas[0], self.betas[1], self.eps,
                                 self.max_norm, *self._step_args, stream_of(self.m)), 'd1_adamw')
+        if self._leaves:  # torch then refuses a backward pass through what the step has overwritten
+            torch.autograd.graph.increment_version(self._leaves)
 
     def moments(self, i):
         """(m, v) of parameter i as float32 in its shape (decoded copies where the state is in 8 bits)."""

@@ -10,14 +10,16 @@ the environments' legal masks do: an integer tensor [...] or [..., words], bit
 j of a row (counted from its lowest byte) for token j; a mask shared by all
 rows may be expanded. A token whose bit is clear counts for nothing, whatever
 its logit holds. The calls launch on the current stream of the logits' device
-and can be captured in a CUDA graph.
+and can be captured in a CUDA graph. Where torch records gradients of the
+logits, logp and entropy have their (first) gradient; the others have none.
 """
 from typing import NamedTuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from ._lib import check, library, stream_of
-from ._rows import apart, empty_f32, empty_like, like, matrix, type_of, vector
+from ._rows import apart, empty_f32, empty_like, like, matrix, recorded, type_of, vector
 
 MAX_TOP = 32
 
@@ -61,8 +63,34 @@ def _common(logits, tokens, legal, temperature):
     return dev, kind, m, lead, t, _legal(legal, lead, m[2], dev)
 
 
+class _TokenLogprob(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, legal, temperature, top):
+        r = _token_logprob(logits, tokens, legal, temperature, top)
+        ctx.save_for_backward(logits, tokens, legal, r.stats, r.entropy)
+        ctx.temperature = temperature
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(*(t for t in r[2:] if t is not None))
+        return tuple(r)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dlogp, dentropy, *others):
+        if dlogp is None and dentropy is None:
+            return (None,) * 5
+        logits, tokens, legal, stats, entropy = ctx.saved_tensors
+        dlogp, dentropy = (None if g is None else g.contiguous() for g in (dlogp, dentropy))
+        return token_logprob_backward(logits, tokens, stats, entropy, dlogp, dentropy, legal, ctx.temperature), None, None, None, None
+
+
 def token_logprob(logits, tokens, legal=None, temperature=1.0, top=0):
     """TokenLogprob of softmax(logits / temperature) over the legal tokens."""
+    if recorded(logits):
+        return TokenLogprob(*_TokenLogprob.apply(logits, tokens, legal, temperature, top))
+    return _token_logprob(logits, tokens, legal, temperature, top)
+
+
+def _token_logprob(logits, tokens, legal, temperature, top):
     dev, kind, (px, rows, vocab, ld), lead, t, (bits, pitch) = _common(logits, tokens, legal, temperature)
     if not 0 <= top <= MAX_TOP:
         raise ValueError(f'top must be between 0 and {MAX_TOP}')
@@ -81,7 +109,7 @@ def token_logprob(logits, tokens, legal=None, temperature=1.0, top=0):
 def token_logprob_backward(logits, tokens, stats, entropy, dlogp, dentropy=None, legal=None, temperature=1.0,
                            out=None):
     """dlogits (the logits' shape and type) from the gradients of logp and of the
-    entropy (float32 of the rows' shape; None: zero), written to `out` when given,
+    entropy (float32 of the rows' shape; either may be None: zero), written to `out` when given,
     which overlaps no input."""
     dev, kind, m, _, t, (bits, pitch) = _common(logits, tokens, legal, temperature)
     px, rows, vocab, ld = m
