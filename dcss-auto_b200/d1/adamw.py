@@ -121,12 +121,12 @@ class AdamW:
         at = lambda t: None if t is None else t.data_ptr()
         self._state_args = (self._table.data_ptr(), len(grads), self.nblocks, self.state_bits, at(self.m), at(self.v),
                             at(self.m_scale), at(self.v_scale))
-        self._step_args = (self.step_dev.data_ptr(), self.seed, self._work.data_ptr(), self.grad_norm.data_ptr())
+        self._step_dev, self._step_args = self.step_dev.data_ptr(), (self._work.data_ptr(), self.grad_norm.data_ptr())
 
     def step(self, lr=None):
         """One step, in place. lr: this step's learning rate (default: self.lr)."""
         check(self.lib.d1_adamw(*self._state_args, self.lr if lr is None else lr, self.betas[0], self.betas[1], self.eps,
-                                self.max_norm, *self._step_args, stream_of(self.m)), 'd1_adamw')
+                                self.max_norm, self._step_dev, self.seed, *self._step_args, stream_of(self.m)), 'd1_adamw')
         if self._leaves:  # torch then refuses a backward pass through what the step has overwritten
             torch.autograd.graph.increment_version(self._leaves)
 
@@ -146,12 +146,14 @@ class AdamW:
         return {k: getattr(self, k) for k in ('m', 'v', 'm_scale', 'v_scale') if getattr(self, k) is not None}
 
     def state_dict(self):
-        """Copies of the moments and the step count; a run that loads them goes on bit for bit."""
-        return dict({k: t.clone() for k, t in self._state().items()}, step=int(self.step_dev.item()))
+        """Copies of the moments, the step count and the seed of the 8-bit rounding: a run that
+        loads them, with the same parameters, rates and gradients, goes on bit for bit."""
+        return dict({k: t.clone() for k, t in self._state().items()}, step=int(self.step_dev.item()), seed=self.seed)
 
     def load_state_dict(self, state):
+        """Takes over a state_dict() (one without a seed leaves the seed as it is)."""
         own = self._state()
-        if set(state) != set(own) | {'step'}:
+        if set(state) - {'seed'} != set(own) | {'step'}:
             raise ValueError(f'the state has {sorted(state)}, not {sorted(own) + ["step"]}')
         for k, t in own.items():
             if state[k].dtype != t.dtype or state[k].shape != t.shape:
@@ -159,3 +161,4 @@ class AdamW:
         for k, t in own.items():
             t.copy_(state[k])
         self.step_dev.fill_(state['step'])
+        self.seed = state.get('seed', self.seed)
