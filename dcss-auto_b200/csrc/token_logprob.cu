@@ -8,7 +8,8 @@
 //   d log p_t / d x_j = (1[j = t] - p_j) / T        d H / d x_j = -p_j (log p_j + H) / T
 //
 // A row with nothing left has log p = -inf, H = 0, no alternatives and a zero
-// gradient. A NaN or +inf that is not left out makes S, log p and H NaN.
+// gradient. A NaN or +inf that is not left out makes S, log p, H and the gradient of
+// what is not left out NaN.
 //
 // One pass over the logits: each thread keeps a running maximum m, the sum s of
 // 2^{(x - m) c} and the sum t of (x - m) c 2^{(x - m) c}, with c = log2(e) / T,
@@ -952,8 +953,12 @@ struct RowGrad {
 template <class T>
 __device__ __forceinline__ RowGrad row_grad(const Grads &g, const T *x, const uint8_t *legal, int64_t r, int vocab, float inv_t) {
     RowGrad k;
-    k.m = g.stats[2 * r];
-    k.l2 = g.stats[2 * r + 1] * LOG2E;
+    // With a NaN or +inf in the row all is NaN where p is not 0: from the lowest number on, x - m is not
+    // negative for any finite x, so that p is 1 or more, while -inf still gives 0.
+    const float log_sum = g.stats[2 * r + 1];
+    const bool undefined = log_sum != log_sum;
+    k.m = undefined ? -3.402823466e38f : g.stats[2 * r];
+    k.l2 = undefined ? 0.f : log_sum * LOG2E;
     k.zero = k.m == -CUDART_INF_F;
     const int64_t token = g.dlogp ? g.tokens[r] : -1;
     const float b = g.dentropy ? g.dentropy[r] : 0.f, h = g.dentropy ? g.entropy[r] : 0.f;
@@ -965,6 +970,7 @@ __device__ __forceinline__ RowGrad row_grad(const Grads &g, const T *x, const ui
         a = g.dlogp[r];
         k.token = (int)token;
     }
+    if (undefined) a = CUDART_NAN_F;
     k.hit = a * inv_t;
     k.w0 = -(a + b * h) * inv_t;
     k.w1 = -b * inv_t * LN2;
