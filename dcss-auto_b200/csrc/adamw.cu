@@ -491,8 +491,8 @@ extern "C" int d1_adamw(const D1AdamWTensor *tensors, int ntensors, int64_t nblo
     if (nblocks > INT32_MAX - 8) return D1_ERR_TOO_LARGE;
     if (!tensors || ntensors < 1 || nblocks < 1 || (state_bits != 32 && state_bits != 8) || !m || !v || !step ||
         !work || (state_bits == 8 && (!m_scale || !v_scale)) || !(beta1 >= 0. && beta1 < 1.) ||
-        !(beta2 >= 0. && beta2 < 1.) || !(eps >= 0.) || (reinterpret_cast<uintptr_t>(m) & 15) ||
-        (reinterpret_cast<uintptr_t>(v) & 15) || (reinterpret_cast<uintptr_t>(work) & 15))
+        !(beta2 >= 0. && beta2 < 1.) || !(eps >= 0.) || !d1::aligned_to(16, m, v, work) ||
+        !d1::aligned_to(8, tensors, step) || !d1::aligned_to(4, m_scale, v_scale, grad_norm))
         return D1_ERR_BAD_ARGUMENT;
     const int tile = nblocks >= SMS * 32 * 4 * 8 ? 8 : 2;  // 8 where that makes four tiles for each warp
     double *const partials = (double *)work;

@@ -27,9 +27,11 @@ __device__ __forceinline__ float warp_sum(float x) {
     return x;
 }
 
-inline bool element_aligned(const void *p, int type) {
-    return (reinterpret_cast<uintptr_t>(p) & (type == D1_TYPE_F32 ? 3 : 1)) == 0;
+// Whether every pointer is a multiple of `bytes` (NULL is).
+template <class... P> inline bool aligned_to(int bytes, const P *...p) {
+    return ((reinterpret_cast<uintptr_t>(p) | ...) & (uintptr_t)(bytes - 1)) == 0;
 }
+inline bool element_aligned(const void *p, int type) { return aligned_to(type == D1_TYPE_F32 ? 4 : 2, p); }
 inline bool type_ok(int type) { return type == D1_TYPE_F32 || type == D1_TYPE_BF16 || type == D1_TYPE_F16; }
 
 }  // namespace d1

@@ -926,7 +926,8 @@ extern "C" int d1_layer_norm(const void *x, int64_t ldx, int type, int64_t rows,
                              void *stream) {
     using namespace d1;
     if (!type_ok(type) || rows < 0 || n < 1 || (rows && (!x || !y)) || !(eps >= 0.f) || ldx < 0 || ldy < 0 ||
-        (rows > 1 && ldy < n) || !element_aligned(x, type) || !element_aligned(y, type))
+        (rows > 1 && ldy < n) || !element_aligned(x, type) || !element_aligned(y, type) ||
+        !aligned_to(4, weight, bias, mean, rstd))
         return D1_ERR_BAD_ARGUMENT;
     if (rows == 0) return 0;
     const int64_t size = type == D1_TYPE_F32 ? 4 : 2;
@@ -955,7 +956,8 @@ extern "C" int d1_layer_norm_backward(const void *dy, int64_t lddy, const void *
     using namespace d1;
     if (!type_ok(type) || rows < 0 || n < 1 || (rows && (!dy || !x || !mean || !rstd)) || lddy < 0 || ldx < 0 ||
         lddx < 0 || (dx && rows > 1 && lddx < n) || ((dweight || dbias) && !work) || !element_aligned(x, type) ||
-        !element_aligned(dy, type) || !element_aligned(dx, type))
+        !element_aligned(dy, type) || !element_aligned(dx, type) ||
+        !aligned_to(4, weight, mean, rstd, dweight, dbias) || !aligned_to(16, work))
         return D1_ERR_BAD_ARGUMENT;
     const int64_t size = type == D1_TYPE_F32 ? 4 : 2;
     const RowSpan result{(uintptr_t)dx, dx ? rows : 0, n * size, lddx * size};

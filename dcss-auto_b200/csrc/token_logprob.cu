@@ -1230,7 +1230,8 @@ extern "C" int d1_token_logprob(const void *logits, int64_t ld, int type, int64_
                                 void *stream) {
     using namespace d1;
     if (!type_ok(type) || rows < 0 || vocab < 1 || ld < 0 || ldlegal < 0 || !(temperature > 0.f) || top < 0 ||
-        (rows && (!logits || (logp && !tokens) || (top > 0 && (!top_tokens || !top_logp)))) || !element_aligned(logits, type))
+        (rows && (!logits || (logp && !tokens) || (top > 0 && (!top_tokens || !top_logp)))) || !element_aligned(logits, type) ||
+        !aligned_to(8, tokens, top_tokens) || !aligned_to(4, logp, entropy, stats, top_logp))
         return D1_ERR_BAD_ARGUMENT;
     if (top > lp::MAX_TOP) return D1_ERR_TOO_LARGE;
     if (rows == 0) return 0;
@@ -1250,7 +1251,8 @@ extern "C" int d1_token_logprob_backward(const void *logits, int64_t ld, int typ
     using namespace d1;
     if (!type_ok(type) || rows < 0 || vocab < 1 || ld < 0 || ldlegal < 0 || !(temperature > 0.f) ||
         (rows && (!logits || !stats || !dlogits || (dlogp && !tokens) || (dentropy && !entropy))) || ldd < 0 ||
-        (rows > 1 && ldd < vocab) || !element_aligned(logits, type) || !element_aligned(dlogits, type))
+        (rows > 1 && ldd < vocab) || !element_aligned(logits, type) || !element_aligned(dlogits, type) ||
+        !aligned_to(8, tokens) || !aligned_to(4, stats, entropy, dlogp, dentropy))
         return D1_ERR_BAD_ARGUMENT;
     if (rows == 0) return 0;
     const int64_t size = type == D1_TYPE_F32 ? 4 : 2;
