@@ -654,18 +654,19 @@ __global__ void __launch_bounds__(1024)
     reduce_kernel(const float *__restrict__ work, int parts, int n, float *__restrict__ dw, float *__restrict__ db) {
     __shared__ float sums[32][33];
     pdl_wait();
-    const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, j = blockIdx.x * 32 + lane;
+    const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
+    const unsigned j = blockIdx.x * 32 + lane, columns = 2u * n;  // twice the longest row passes 31 bits
     float s = 0.f;
-    if (j < 2 * n) {
+    if (j < columns) {
 #pragma unroll 8
         for (int p = slice; p < parts; p += 32) s += work[(int64_t)p * 2 * n + j];
     }
     sums[slice][lane] = s;
     __syncthreads();
     s = warp_sum(sums[lane][slice]);  // warp `slice` adds the slices of its column
-    const int c = blockIdx.x * 32 + slice;
-    if (lane || c >= 2 * n) return;
-    if (c < n) {
+    const unsigned c = blockIdx.x * 32 + slice;
+    if (lane || c >= columns) return;
+    if (c < (unsigned)n) {
         if (dw) dw[c] = s;
     } else if (db)
         db[c - n] = s;
@@ -674,7 +675,8 @@ __global__ void __launch_bounds__(1024)
 // ---------------------------------------------------------------- rows too long for registers
 
 // Plain passes over the row, element by element, the second and third from L2: for
-// completeness more than for speed. 1,024 rows of 65,536 in fp32 take 212 us forward
+// completeness more than for speed. Columns are counted without a sign: the step past
+// the end of the longest rows passes 31 bits. 1,024 rows of 65,536 in fp32 take 212 us forward
 // (39 % of a copy's rate) and 348 us backward (35 %).
 
 constexpr int WIDE = 1024;
@@ -688,15 +690,15 @@ __global__ void __launch_bounds__(WIDE)
     for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
         const T *xr = x + r * ldx;
         float s = 0.f;
-        for (int j = threadIdx.x; j < n; j += WIDE) s += to_f32(xr[j]);
+        for (unsigned j = threadIdx.x; j < (unsigned)n; j += WIDE) s += to_f32(xr[j]);
         const float mu = team_sum<0>(s, part[0]) / n;
         s = 0.f;
-        for (int j = threadIdx.x; j < n; j += WIDE) {
+        for (unsigned j = threadIdx.x; j < (unsigned)n; j += WIDE) {
             const float c = to_f32(xr[j]) - mu;
             s += c * c;
         }
         const float rs = 1.f / sqrtf(team_sum<0>(s, part[1]) / n + eps);
-        for (int j = threadIdx.x; j < n; j += WIDE)
+        for (unsigned j = threadIdx.x; j < (unsigned)n; j += WIDE)
             y[r * ldy + j] = from_f32<T>((to_f32(xr[j]) - mu) * rs * (w ? w[j] : 1.f) + (b ? b[j] : 0.f));
         if (threadIdx.x == 0) {
             if (mean) mean[r] = mu;
@@ -715,7 +717,7 @@ __global__ void __launch_bounds__(WIDE)
     for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
         const float mu = mean[r], rs = rstd[r];
         float s1 = 0.f, s2 = 0.f;
-        for (int j = threadIdx.x; j < n; j += WIDE) {
+        for (unsigned j = threadIdx.x; j < (unsigned)n; j += WIDE) {
             const float g = to_f32(dy[r * lddy + j]) * (w ? w[j] : 1.f);
             s1 += g;
             s2 += g * ((to_f32(x[r * ldx + j]) - mu) * rs);
@@ -724,7 +726,7 @@ __global__ void __launch_bounds__(WIDE)
         turn ^= 1;
         s1 /= n;
         s2 /= n;
-        for (int j = threadIdx.x; j < n; j += WIDE) {
+        for (unsigned j = threadIdx.x; j < (unsigned)n; j += WIDE) {
             const float g = to_f32(dy[r * lddy + j]) * (w ? w[j] : 1.f);
             dx[r * lddx + j] = from_f32<T>(rs * (g - s1 - (to_f32(x[r * ldx + j]) - mu) * rs * s2));
         }
@@ -737,8 +739,8 @@ __global__ void __launch_bounds__(256)
     wide_columns_kernel(const T *__restrict__ dy, int64_t lddy, const T *__restrict__ x, int64_t ldx, int64_t rows,
                         int n, const float *__restrict__ mean, const float *__restrict__ rstd,
                         float *__restrict__ work) {
-    const int j = blockIdx.x * 256 + threadIdx.x;
-    if (j >= n) return;
+    const unsigned j = blockIdx.x * 256 + threadIdx.x;
+    if (j >= (unsigned)n) return;
     const int64_t lo = rows * blockIdx.y / gridDim.y, hi = rows * (blockIdx.y + 1) / gridDim.y;
     float sw = 0.f, sb = 0.f;
 #pragma unroll 4
@@ -904,7 +906,7 @@ static int backward_any(const void *dy, int64_t lddy, const void *x, int64_t ldx
                 (const T *)dy, lddy, (const T *)x, ldx, rows, n, w, mean, rstd, (T *)dx, lddx);
         if ((e = (int)cudaGetLastError())) return e;
         if (sums)
-            wide_columns_kernel<T><<<dim3((n + 255) / 256, parts), 256, 0, s>>>((const T *)dy, lddy, (const T *)x, ldx,
+            wide_columns_kernel<T><<<dim3(((unsigned)n + 255) / 256, parts), 256, 0, s>>>((const T *)dy, lddy, (const T *)x, ldx,
                                                                                 rows, n, mean, rstd, work);
         e = (int)cudaGetLastError();
     } else if (vector)
@@ -914,7 +916,7 @@ static int backward_any(const void *dy, int64_t lddy, const void *x, int64_t ldx
                                                 sums ? work : nullptr, s);
     if (e || !sums) return e;
     cudaLaunchAttribute attr;
-    const cudaLaunchConfig_t cfg = pdl_config(dim3((2 * n + 31) / 32), dim3(1024), 0, s, &attr);
+    const cudaLaunchConfig_t cfg = pdl_config(dim3((2u * n + 31) / 32), dim3(1024), 0, s, &attr);
     return (int)cudaLaunchKernelEx(&cfg, reduce_kernel, (const float *)work, parts, n, dw, db);
 }
 

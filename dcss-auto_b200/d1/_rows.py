@@ -5,6 +5,7 @@ are written for few Python and torch calls."""
 import torch
 
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # D1_TYPE_* of d1.h
+MAX_COLUMNS = 2 ** 31 - 1
 
 
 def recorded(x, weight=None, bias=None):
@@ -28,6 +29,8 @@ def matrix(t, name):
     if t.dim() != 2:
         if t.dim() == 0:
             raise ValueError(f'{name} needs at least one dimension')
+        if t.shape[-1] == 0:
+            raise ValueError(f'{name}: rows are empty')
         try:
             t = t.view(-1, t.shape[-1]) if t.numel() else t.reshape(-1, t.shape[-1])
         except RuntimeError:
@@ -37,6 +40,8 @@ def matrix(t, name):
     pitch, step = t.stride()
     if n < 1:
         raise ValueError(f'{name}: rows are empty')
+    if n > MAX_COLUMNS:  # the C entries take it as an int, and ctypes would cut it off without a word
+        raise ValueError(f'{name}: rows of {n} elements are longer than {MAX_COLUMNS}')
     if step != 1 and n > 1:
         raise ValueError(f'{name}: the last dimension must be contiguous')
     return t.data_ptr(), rows, n, pitch
