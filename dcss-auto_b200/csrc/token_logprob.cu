@@ -26,6 +26,7 @@
 // (about k of them, unless logits are equal in great numbers) are ordered by
 // counting, for each, how many are better. Where more of them reach the bound
 // than the list holds, a search in k rounds replaces it.
+#include <float.h>
 #include <math_constants.h>
 
 #include "d1_elem.cuh"
@@ -1224,12 +1225,15 @@ static int backward(const void *logits, int64_t ld, int64_t rows, int vocab, con
 }  // namespace lp
 }  // namespace d1
 
+// Of a smaller temperature the reciprocal would not be finite, of an infinite one -inf times it NaN.
+static bool temperature_ok(float t) { return t >= FLT_MIN && t <= FLT_MAX; }
+
 extern "C" int d1_token_logprob(const void *logits, int64_t ld, int type, int64_t rows, int vocab,
                                 const int64_t *tokens, const void *legal, int64_t ldlegal, float temperature, int top,
                                 float *logp, float *entropy, float *stats, int64_t *top_tokens, float *top_logp,
                                 void *stream) {
     using namespace d1;
-    if (!type_ok(type) || rows < 0 || vocab < 1 || ld < 0 || ldlegal < 0 || !(temperature > 0.f) || top < 0 ||
+    if (!type_ok(type) || rows < 0 || vocab < 1 || ld < 0 || ldlegal < 0 || !temperature_ok(temperature) || top < 0 ||
         (rows && (!logits || (logp && !tokens) || (top > 0 && (!top_tokens || !top_logp)))) || !element_aligned(logits, type) ||
         !aligned_to(8, tokens, top_tokens) || !aligned_to(4, logp, entropy, stats, top_logp))
         return D1_ERR_BAD_ARGUMENT;
@@ -1249,7 +1253,7 @@ extern "C" int d1_token_logprob_backward(const void *logits, int64_t ld, int typ
                                          const float *stats, const float *entropy, const float *dlogp,
                                          const float *dentropy, void *dlogits, int64_t ldd, void *stream) {
     using namespace d1;
-    if (!type_ok(type) || rows < 0 || vocab < 1 || ld < 0 || ldlegal < 0 || !(temperature > 0.f) ||
+    if (!type_ok(type) || rows < 0 || vocab < 1 || ld < 0 || ldlegal < 0 || !temperature_ok(temperature) ||
         (rows && (!logits || !stats || !dlogits || (dlogp && !tokens) || (dentropy && !entropy))) || ldd < 0 ||
         (rows > 1 && ldd < vocab) || !element_aligned(logits, type) || !element_aligned(dlogits, type) ||
         !aligned_to(8, tokens) || !aligned_to(4, stats, entropy, dlogp, dentropy))

@@ -22,6 +22,7 @@ from ._lib import check, library, stream_of
 from ._rows import apart, empty_f32, empty_like, like, matrix, recorded, type_of, vector
 
 MAX_TOP = 32
+LEAST, MOST = 2.0 ** -126, 3.4028234663852886e38  # temperatures: fp32 numbers with a finite reciprocal
 
 
 class TokenLogprob(NamedTuple):
@@ -54,8 +55,8 @@ def _legal(legal, lead, vocab, device):
 
 def _common(logits, tokens, legal, temperature):
     kind, dev, m = type_of(logits, 'logits'), logits.device, matrix(logits, 'logits')
-    if not temperature > 0:
-        raise ValueError('temperature must be positive')
+    if not LEAST <= temperature <= MOST:
+        raise ValueError(f'temperature must be between {LEAST} and {MOST}')
     lead = logits.shape[:-1]
     if tokens.shape != lead:
         raise ValueError(f'tokens {tuple(tokens.shape)} do not match rows {tuple(lead)}')

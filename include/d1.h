@@ -686,7 +686,7 @@ int d1_layer_norm_backward(const void *dy, int64_t lddy, const void *x, int64_t 
  * stats (-inf, -inf). top (0..32) > 0: top_tokens[r][k] and top_logp[r][k] are
  * the k-th likeliest token (the lower one first where logits are equal) and its
  * log-probability, -1 and -inf where no token is left. Any of logp, entropy and
- * stats may be NULL. */
+ * stats may be NULL. temperature is a positive, finite and not subnormal number. */
 int d1_token_logprob(const void *logits, int64_t ld, int type, int64_t rows, int vocab, const int64_t *tokens,
                      const void *legal, int64_t ldlegal, float temperature, int top, float *logp, float *entropy,
                      float *stats, int64_t *top_tokens, float *top_logp, void *stream);
