@@ -162,7 +162,11 @@ template <int NB> __global__ void __launch_bounds__(THREADS) norm_kernel(Args a)
             float q = 0.f;
 #pragma unroll
             for (int k = p; k < p + 2; k++) q += (g[k][0] * g[k][0] + g[k][1] * g[k][1]) + (g[k][2] * g[k][2] + g[k][3] * g[k][3]);
-            s += q;
+            if (!(q <= 3.402823466e38f)) {  // past fp32, from 1.8e19 on (or not finite): in 64 bits
+#pragma unroll
+                for (int i = 0; i < 8; i++) s += (double)g[p + i / 4][i % 4] * g[p + i / 4][i % 4];
+            } else
+                s += q;
         }
     }
     double d = s;
