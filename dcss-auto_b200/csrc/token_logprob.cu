@@ -378,6 +378,12 @@ template <int EACH> __device__ __forceinline__ Acc warp_join(const Acc (&a)[EACH
     return Acc{m, warp_sum(s), warp_sum(t)};
 }
 
+// A bound found down to bit LOW_BIT, as a key: the bits below are those of every key of
+// its sign (16-bit numbers fill only the upper ones, and a negative one's key is its
+// complement), so that equal logits compare equal to it; at least 1.
+template <int LOW_BIT> __device__ __forceinline__ uint32_t whole_bound(uint32_t bound) {
+    return bound == 0u ? 1u : bound & 0x80000000u ? bound : bound | ((1u << LOW_BIT) - 1u);
+}
 // A bound that at least `top` of the warp's keys reach, and seldom many more (or
 // 1, which every token reaches): bisection, by ballots where a lane has one key,
 // else two bits at a time with three counts (below 1,024) in one sum.
@@ -407,7 +413,7 @@ template <int EACH, int LOW_BIT> __device__ __forceinline__ uint32_t bound_of(co
             if ((n3 >= top ? n3 : n2 >= top ? n2 : n1) <= top + top / 4) break;
         }
     }
-    return max(bound, 1u);
+    return whole_bound<LOW_BIT>(bound);
 }
 
 // The row's best `top` candidates, into w.best, by one warp. seen[i]: the largest
@@ -747,7 +753,7 @@ __device__ __forceinline__ void select_top(Shared &sh, const Row<T> &row, int lo
                     if (n <= top + top / 4) break;
                 }
             }
-        bound = max(bound, 1u);
+        bound = whole_bound<Wide<T>::LOW_BIT>(bound);
         int columns = 0;
 #pragma unroll
         for (int i = 0; i < EACH; i++) {
