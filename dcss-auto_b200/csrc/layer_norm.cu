@@ -783,16 +783,21 @@ static int forward(const T *x, int64_t ldx, int64_t rows, int n, const float *w,
     // 233,016 rows of 72 in bf16 take 23 us with 8 lanes, 51 with 32; 83,886 of 200 19 us with 16, 23 with 32. Element
     // by element 8 a lane are as good, and where rows are too few for the SMs, 32 lanes have the shorter way.
     const bool many = rows >= SMS * 32;
-    if (VEC == 8 && n <= 64 && many) D1_LN_FORWARD(16, 4, 2, 256);
+    if constexpr (VEC == 8)
+        if (n <= 64 && many) D1_LN_FORWARD(16, 4, 2, 256);
     if (n <= 64) D1_LN_FORWARD(8, 8, 2, 256);
-    if (VEC > 1 && n <= 128 && many) D1_LN_FORWARD(16, 8, 2, 256);
-    if (VEC > 1 && n <= 256 && many) D1_LN_FORWARD(16, 16, 2, 256);
+    if constexpr (VEC > 1) {
+        if (n <= 128 && many) D1_LN_FORWARD(16, 8, 2, 256);
+        if (n <= 256 && many) D1_LN_FORWARD(16, 16, 2, 256);
+    }
     if (n <= 256) D1_LN_FORWARD(8, 32, 2, 256);
     // (12 and 24 elements a lane leave fewer idle where the bound is instructions: 120,266 rows of 279 in bf16 49 and
     // 46 us, 64,403 of 521 in fp16 50 and 44)
-    if (VEC <= 2 && n <= 384) D1_LN_FORWARD((VEC <= 2 ? 12 : 16), 32, 2, 256);
+    if constexpr (VEC <= 2)
+        if (n <= 384) D1_LN_FORWARD(12, 32, 2, 256);
     if (n <= 512) D1_LN_FORWARD(16, 32, 2, 256);
-    if (VEC == 2 && n <= 768) D1_LN_FORWARD((VEC == 2 ? 24 : 32), 32, 1, 256);
+    if constexpr (VEC == 2)
+        if (n <= 768) D1_LN_FORWARD(24, 32, 1, 256);
     if (n <= 1024) D1_LN_FORWARD(32, 32, 1, 256);
     // Longer rows are a block's. Where the vectors are whole, 32 elements a thread (64 of the longest) need fewer
     // joins than 16 do, and blocks that come and go keep more rows under way than resident ones with their rows in
@@ -802,11 +807,14 @@ static int forward(const T *x, int64_t ldx, int64_t rows, int n, const float *w,
     if constexpr (VEC == 4)
         D1_LN_FORWARD(32, 0, 1, block_threads(n, 32));
     else {
-        if (VEC == 8 && n > 8192) D1_LN_FORWARD((VEC == 8 ? 64 : 32), 0, 1, block_threads(n, 64));
-        if (VEC == 8 ? n >= 2048 : VEC == 2 && n > 4096) D1_LN_FORWARD(32, 0, (VEC > 1 ? 2 : 1), block_threads(n, 32));
+        if constexpr (VEC == 8)
+            if (n > 8192) D1_LN_FORWARD(64, 0, 1, block_threads(n, 64));
+        if constexpr (VEC > 1)
+            if (n >= (VEC == 8 ? 2048 : 4097)) D1_LN_FORWARD(32, 0, 2, block_threads(n, 32));
         const int threads = block_threads(n, 16), warps = threads / 32;
         const size_t smem = (size_t)LONG_DEPTH * Rows<T, VEC, 16, 0>::bytes(warps) + 8 * (size_t)SharedWeights<VEC, 16>::floats(warps);
-        if (threads > 1024 || smem + 2048 > SPACE) D1_LN_FORWARD(32, 0, 1, block_threads(n, 32));
+        if constexpr (VEC == 1)  // the others have at most 256 threads here
+            if (threads > 1024 || smem + 2048 > SPACE) D1_LN_FORWARD(32, 0, 1, block_threads(n, 32));
         const auto kernel = long_forward_kernel<T, VEC>;
         if (const int e = allow_space(kernel, smem)) return e;
         const int by_threads = 1024 / threads, by_space = (int)(SPACE / (smem + 2048));
@@ -871,21 +879,25 @@ static int backward(const T *dy, int64_t lddy, const T *x, int64_t ldx, int64_t 
                     const float *mean, const float *rstd, T *dx, int64_t lddx, float *work, cudaStream_t s) {
     constexpr bool VECTOR = VEC * sizeof(T) == 16;
     const Backward o = backward_shape(rows, n, sizeof(T), VECTOR);
-    auto kernel = backward_kernel<T, VEC, 8, 0, 4, 512>;
-    if (o.lanes == 8)
-        kernel = o.p == 8 ? backward_kernel<T, VEC, 8, 8, 4, 256> : backward_kernel<T, VEC, 16, 8, 4, 256>;
-    else if (o.lanes == 16)
-        kernel = backward_kernel<T, VEC, 16, 16, 4, 256>;
-    else if (o.lanes == 32)
-        kernel = o.p == 8    ? backward_kernel<T, VEC, 8, 32, 4, 256>
-                 : o.p == 12 ? backward_kernel<T, VEC, VEC <= 2 ? 12 : 16, 32, 4, 256>
-                             : backward_kernel<T, VEC, 16, 32, 4, 256>;
-    else if (o.p == 16)
-        kernel = o.threads <= 256 ? backward_kernel<T, VEC, 16, 0, 4, 256>
-                 : o.depth == 4   ? backward_kernel<T, VEC, 16, 0, 4, 512>
-                                  : backward_kernel<T, VEC, 16, 0, 3, 512>;
-    if constexpr (sizeof(T) == 2)
+    auto kernel = backward_kernel<T, VEC, 8, 8, 4, 256>;  // lanes and p are 8
+    if (o.lanes == 32)
+        kernel = backward_kernel<T, VEC, 16, 32, 4, 256>;
+    else if (o.lanes == 0)
+        kernel = o.threads <= 256 ? backward_kernel<T, VEC, 16, 0, 4, 256> : backward_kernel<T, VEC, 16, 0, 4, 512>;
+    if constexpr (VEC == 1) {
+        if (o.lanes == 32 && o.p == 8) kernel = backward_kernel<T, VEC, 8, 32, 4, 256>;
+    } else {
+        if (o.lanes == 8 && o.p == 16) kernel = backward_kernel<T, VEC, 16, 8, 4, 256>;
+        if (o.lanes == 16) kernel = backward_kernel<T, VEC, 16, 16, 4, 256>;
+    }
+    if constexpr (VECTOR) {
+        if (o.lanes == 0 && o.p == 8) kernel = backward_kernel<T, VEC, 8, 0, 4, 512>;
+    } else if (o.p == 12)
+        kernel = backward_kernel<T, VEC, 12, 32, 4, 256>;
+    if constexpr (sizeof(T) == 2) {
         if (o.p == 32) kernel = backward_kernel<T, VEC, 32, 0, 2, 512>;
+    } else if (o.depth == 3)
+        kernel = backward_kernel<T, VEC, 16, 0, 3, 512>;
     if (const int e = allow_space(kernel, o.smem)) return e;
     kernel<<<o.grid, o.threads, o.smem, s>>>(dy, lddy, x, ldx, rows, n, w, mean, rstd, dx, lddx, work);
     return (int)cudaGetLastError();
