@@ -26,6 +26,7 @@ import torch
 from ._lib import check, library, stream_of
 
 BLOCK = 128
+GRAD_TYPES = {torch.float32: 0, torch.bfloat16: 1}  # D1_TYPE_* of d1.h
 
 
 class _Tensor(C.Structure):
@@ -43,12 +44,14 @@ def _spans(named):
     return tuple(zip(*spans)) or ((), (), ())
 
 
-def _outside(t, name, spans):
-    """Refuses a tensor that a step reads while it writes one of the spans over it."""
+def _outside(t, i, spans):
+    """Refuses gradient i, which a step reads, if it writes one of the spans over it."""
     starts, ends, names = spans
-    i = bisect.bisect_left(starts, t.data_ptr() + t.numel() * t.element_size()) - 1
-    if t.numel() and i >= 0 and ends[i] > t.data_ptr():
-        raise ValueError(f'{name} shares memory with {names[i]}')
+    at = t.data_ptr()
+    end = at + t.nbytes
+    near = bisect.bisect_left(starts, end) - 1  # the last span that begins before its end
+    if near >= 0 and ends[near] > at < end:
+        raise ValueError(f'grads[{i}] shares memory with {names[near]}')
 
 
 class AdamW:
@@ -100,28 +103,29 @@ class AdamW:
         self.grad_norm = torch.zeros(1, **f32)  # the last step's, when it clips
         self._work = torch.zeros(self.lib.d1_adamw_work_bytes(), dtype=torch.uint8, device=dev)
         self._table = torch.empty(len(params) * C.sizeof(_Tensor), dtype=torch.uint8, device=dev)
+        at = lambda t: None if t is None else t.data_ptr()
+        self._state_args = (self._table.data_ptr(), len(params), self.nblocks, state_bits, at(self.m), at(self.v),
+                            at(self.m_scale), at(self.v_scale))
+        self._step_dev, self._step_args = self.step_dev.data_ptr(), (self._work.data_ptr(), self.grad_norm.data_ptr())
         self.set_grads(grads)
 
     def set_grads(self, grads):
-        """Read the gradients from other tensors from now on (a captured step too)."""
+        """Read the gradients from other tensors from now on (a captured step too). The tensors'
+        list is copied on the current stream: the steps', or one that is ordered with it."""
         grads = list(grads)
         if len(grads) != len(self.params):
             raise ValueError(f'{len(self.params)} parameters and {len(grads)} gradients')
         table = (_Tensor * len(grads))()
         for i, (p, g, c) in enumerate(zip(self.params, grads, self.copies)):
-            if (g.dtype not in (torch.float32, torch.bfloat16) or g.shape != p.shape or g.device != self.device or
-                    not g.is_contiguous()):
+            kind = GRAD_TYPES.get(g.dtype)
+            if kind is None or g.shape != p.shape or g.device != self.device or not g.is_contiguous():
                 raise ValueError(f'grads[{i}] must be a contiguous float32 or bfloat16 tensor of shape '
                                  f'{tuple(p.shape)} on {self.device}')
-            _outside(g, f'grads[{i}]', self._written)
+            _outside(g, i, self._written)
             table[i] = _Tensor(p.data_ptr(), g.data_ptr(), None if c is None else c.data_ptr(), p.numel(),
-                               self._first[i], self.decay[i], 0 if g.dtype == torch.float32 else 1, 0)
+                               self._first[i], self.decay[i], kind, 0)
         self.grads = grads
         self._table.copy_(torch.frombuffer(bytearray(table), dtype=torch.uint8))
-        at = lambda t: None if t is None else t.data_ptr()
-        self._state_args = (self._table.data_ptr(), len(grads), self.nblocks, self.state_bits, at(self.m), at(self.v),
-                            at(self.m_scale), at(self.v_scale))
-        self._step_dev, self._step_args = self.step_dev.data_ptr(), (self._work.data_ptr(), self.grad_norm.data_ptr())
 
     def step(self, lr=None):
         """One step, in place. lr: this step's learning rate (default: self.lr)."""
