@@ -24,8 +24,11 @@
 // a candidate: about k columns of vectors are read again, from L2 (of long
 // rows, only the cells of them whose own maximum reaches it). The candidates
 // (about k of them, unless logits are equal in great numbers) are ordered by
-// counting, for each, how many are better. Where more of them reach the bound
-// than the list holds, a search in k rounds replaces it.
+// counting, for each, how many are better. Where more of them reach the bound than
+// the list holds, one more pass takes what is above the bound and the first that equal
+// it (600 rows of 131,072 equal logits in bf16, k = 20: 570 us in place of 53), and only
+// where hundreds are above it, or where few long rows are split over SMs, a search in
+// k rounds (4 such rows: 98 us in place of 13).
 #include <float.h>
 #include <math_constants.h>
 
@@ -599,7 +602,7 @@ template <class T> __device__ __forceinline__ void token_of(const Out &out, cons
 // Middling rows: a warp each, so that nothing waits for a barrier. With few vectors
 // a lane, the joins and the alternatives are what it costs: 16,384 rows of 4,099
 // in fp16 with 5 of them take 45 us (46 % of a copy's rate), 65,536 of 1,000 in
-// bf16 81 us (26 %). (A block a row: 218 and 517 us.)
+// bf16 81 us (26 %; 91 with 8, 78 % of the issue slots). (A block a row: 218 and 517 us.)
 template <class T, bool MASK>
 __global__ void __launch_bounds__(THREADS, 5)
     warp_forward_kernel(const T *__restrict__ logits, int64_t ld, int64_t rows, int vocab,
@@ -626,8 +629,8 @@ __global__ void __launch_bounds__(THREADS, 5)
 // the eight read on. Each of the two has a place for one row's sums, and a pair
 // of barriers that hand it over and back. (Without them the blocks' reading
 // stopped for each row's alternatives: 4,096 rows of 32,768 in bf16 took 87 us.)
-// They take 66 us with 8 alternatives (4.0 TB/s, 62 % of a copy's rate), 56 without
-// and 78 with a mask. Its bounds lie close together: the exponentials alone take
+// They take 66 us with 8 alternatives (4.0 TB/s, 62 % of a copy's rate), 56 without,
+// 78 with a mask and 91 with both. Its bounds lie close together: the exponentials alone take
 // 30 us at 16 a clock and SM, half of the issue slots are used, and more bytes on
 // their way (copies into shared memory two batches ahead) cost the L1 that the
 // alternatives and masks are read through: 69 to 100 us.
@@ -882,8 +885,12 @@ __global__ void __launch_bounds__(THREADS, 4)
 
 // ---------------------------------------------------------------- short rows: eight lanes each, in registers
 
-// One read of the row, joins of three steps. 65,536 rows of 28 in bf16, masked, take
-// 11 us; 4,096 in fp32 with 4 alternatives 6.3 us, most of it latency.
+// One read of the row, joins of three steps. 4,096 rows of 28 in fp32, masked, with 4
+// alternatives take 6.3 us, which is latency. 65,536 in bf16 take 10.8 us (8 % of a
+// copy's rate), 25.8 with 4 alternatives; of 12 tokens 9.7. There the bound is
+// instructions, 129 of a warp for each row: a load, a mask byte and an exponential for
+// each of 64 tokens whatever the vocabulary, and the waits for a second read of the
+// token's logit (65 % of the issue slots).
 
 template <class T>
 __global__ void __launch_bounds__(THREADS)
@@ -1127,7 +1134,9 @@ __global__ void __launch_bounds__(THREADS, TEAM == 32 ? 5 : 6)
     }
 }
 
-// Short rows: eight lanes a row (65,536 of 28 in fp32, masked: 10 us, latency).
+// Short rows: eight lanes a row. 65,536 of 28, masked, take 10.3 us in fp32 (25 % of a
+// copy's rate) and 9.1 in bf16 (16 %), of 12 in bf16 5.8: each lane waits for the row's
+// constants, then for one logit and one mask byte at a time (52 % of the issue slots).
 template <class T, bool IN_PLACE>
 __global__ void __launch_bounds__(THREADS)
     short_backward_kernel(typename Apart<T, IN_PLACE>::In logits, int64_t ld, int64_t rows, int vocab,
