@@ -9,6 +9,7 @@ gradient tensors then hold. copies (bfloat16, or None for a tensor that has
 none) are refreshed by the step. weight_decay and copies may differ by tensor.
 No parameter or copy shares memory with another one or with a gradient, and each
 keeps its storage for the optimizer's life (the step has their addresses).
+An eps below 2^-63 counts as 2^-63.
 
 Moments are held in 32 bits, or in 8: m as float8_e4m3fn and v as float8_e5m2
 codes with a power-of-two scale for each block of 128 elements, 2.06 bytes a

@@ -706,7 +706,8 @@ int d1_token_logprob_backward(const void *logits, int64_t ld, int type, int64_t 
 /* One parameter tensor of d1_adamw: `count` fp32 elements at param, its gradient
  * (fp32 or bf16), the bf16 compute copy that each step refreshes (or NULL),
  * decay = its weight decay. first_block = number of 128-element blocks of the
- * tensors before it (each has (count + 127) / 128). */
+ * tensors before it (each has (count + 127) / 128). param and copy overlap no
+ * other param, copy or gradient. */
 typedef struct {
     float *param;
     const void *grad;
