@@ -1,0 +1,337 @@
+// Gated linear recurrence over time and its gradient (sm_100a).
+//
+//   average:  a = sigmoid(g)   h_t = a_t k_t h_{t-1} + (1 - a_t) x_t
+//   sum:      a = e^g          h_t = a_t k_t h_{t-1} + x_t
+//
+// with k_t = 0 where an episode begins at t (reset), else 1; every channel of
+// every sequence has its own state. Backward, with E_t = a_t k_t D_t what flows
+// from step t to the one before it:
+//
+//   D_t = dy_t + E_{t+1}    dx_t = (1 - a_t) D_t  or  D_t
+//   dg_t = D_t (k_t h_{t-1} - x_t) a_t (1 - a_t)  or  D_t k_t h_{t-1} a_t
+//
+// States, products of decays and gradients of states are fp32; a 16-bit result
+// is rounded once. The gradient reads h_{t-1} as the forward pass stored it
+// (rounded to y's type): recomputing it would cost the forward pass again for
+// half a rounding step of dg.
+//
+// Both directions are the map s -> a s + b, whose composition over a chunk of
+// steps is again such a map (P, Q). With enough channels one thread walks each
+// of them through the whole time, a few steps' loads ahead of the arithmetic.
+// With few channels the time is cut into chunks: one launch reduces each chunk
+// to its (P, Q), a second runs over the chunks, a third walks all of them side
+// by side from their true states. The order of all sums is fixed.
+//
+// 1 - sigmoid(g) is e / (1 + e) with e = e^-|g| or its counterpart, never a
+// difference from 1, and a reset replaces the state (a product with 0 would
+// keep an infinity).
+#include "d1_common.cuh"
+#include "d1_elem.cuh"
+#include "d1_pdl.cuh"
+
+namespace d1 {
+namespace gs {
+
+constexpr int SMS = 148, THREADS = 128, CARRY_WARPS = 32;
+// P of a chunk with a reset in it: the state before it does not reach its end (decays
+// are not negative, and one that has underflowed to 0 still lets an infinity through).
+constexpr float CUT = -1.f;
+
+// A [T, B, D] operand with contiguous channels: strides in elements.
+template <class T> struct Span {
+    T *p;
+    int64_t st, sb;
+};
+
+template <class T> struct Args {
+    Span<const T> x, gate, y, dy;  // y, dy: backward
+    T *out, *dgate;                // y forward; dx backward (contiguous)
+    const uint8_t *reset;          // NULL: none
+    int64_t reset_t, reset_b;
+    const float *start;            // h0 forward, dlast backward (NULL: zeros)
+    const float *h0;               // backward: the first step's state (NULL: zeros)
+    float *last;                   // last forward, dh0 backward (may be NULL)
+    float2 *carry;                 // [chunks][B * D]: (P, Q), then (state before the chunk, -)
+    int64_t T_, B, D, lanes;       // lanes = B * D / V
+    int64_t size;                  // steps of a chunk
+    int chunks;
+};
+
+// (a, 1 - a) of the average form.
+__device__ __forceinline__ float2 gates(float g) {
+    const float e = expf(-fabsf(g)), r = __fdividef(1.f, 1.f + e), s = e * r;
+    return g < 0.f ? make_float2(s, r) : make_float2(r, s);
+}
+
+template <class T, int V> struct Step {  // one step's operands of V channels
+    Elems<T, V> x, gate, y, dy;
+    bool keep;
+};
+
+// PART 0: reduce a chunk; 1: walk it. Loads step t into s.
+template <class T, int V, bool SUM, bool BACK, int PART>
+__device__ __forceinline__ void load(const Args<T> &a, int64_t t, const T *x, const T *gate, const T *y, const T *dy,
+                                     const uint8_t *reset, Step<T, V> &s) {
+    using E = Elems<T, V>;
+    s.gate = *reinterpret_cast<const E *>(gate + t * a.gate.st);
+    if constexpr (!BACK || (PART == 1 && !SUM)) s.x = *reinterpret_cast<const E *>(x + t * a.x.st);
+    if constexpr (BACK) s.dy = *reinterpret_cast<const E *>(dy + t * a.dy.st);
+    if constexpr (BACK && PART == 1)
+        if (t > 0) s.y = *reinterpret_cast<const E *>(y + (t - 1) * a.y.st);
+    s.keep = !reset || !reset[t * a.reset_t];
+}
+
+template <class T, int V, bool SUM, bool BACK, int PART, int U>
+__global__ void __launch_bounds__(THREADS) scan_kernel(Args<T> a) {
+    pdl_wait();
+    const int64_t lane = (int64_t)blockIdx.x * THREADS + threadIdx.x;
+    // the walk goes over the chunks from the side that the reduction read last
+    const int chunk = PART == 1 ? a.chunks - 1 - (int)blockIdx.y : (int)blockIdx.y;
+    if (lane >= a.lanes) return;
+    const int64_t per = a.D / V, b = lane / per, d = (lane - b * per) * V, c = b * a.D + d, C = a.B * a.D;
+    const T *const x = a.x.p + b * a.x.sb + d, *const gate = a.gate.p + b * a.gate.sb + d;
+    const T *const y = BACK ? a.y.p + b * a.y.sb + d : nullptr, *const dy = BACK ? a.dy.p + b * a.dy.sb + d : nullptr;
+    const uint8_t *const reset = a.reset ? a.reset + b * a.reset_b : nullptr;
+    // step i of the chunk in the direction of the recurrence is time first + i or first - i
+    const int64_t from = chunk * a.size, n = min(a.T_ - from, a.size);
+    const int64_t first = BACK ? a.T_ - 1 - from : from;
+    float s[V], prod[V];
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+        prod[v] = 1.f;
+        s[v] = 0.f;
+        if constexpr (PART == 1) s[v] = chunk ? a.carry[chunk * C + c + v].x : a.start ? a.start[c + v] : 0.f;
+    }
+    Step<T, V> now[U], next[U];
+    const auto at = [&](int64_t i) { return BACK ? first - i : first + i; };
+    const auto fetch = [&](int64_t i, Step<T, V>(&to)[U]) {
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (i + u < n) load<T, V, SUM, BACK, PART>(a, at(i + u), x, gate, y, dy, reset, to[u]);
+    };
+    fetch(0, now);
+    for (int64_t i = 0; i < n; i += U) {
+        fetch(i + U, next);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (i + u >= n) break;
+            const Step<T, V> &o = now[u];
+            const int64_t t = at(i + u);
+            Elems<T, V> r, dg;
+#pragma unroll
+            for (int v = 0; v < V; v++) {
+                const float g = to_f32(o.gate.v[v]);
+                float2 w;
+                if constexpr (SUM)
+                    w = make_float2(expf(g), 1.f);
+                else
+                    w = gates(g);
+                if constexpr (!BACK) {
+                    const float in = SUM ? to_f32(o.x.v[v]) : w.y * to_f32(o.x.v[v]);
+                    s[v] = o.keep ? fmaf(w.x, s[v], in) : in;
+                    r.v[v] = from_f32<T>(s[v]);
+                } else {
+                    const float D = to_f32(o.dy.v[v]) + s[v];
+                    if constexpr (PART == 1) {
+                        float h = t > 0 ? to_f32(o.y.v[v]) : a.h0 ? a.h0[c + v] : 0.f;
+                        if (!o.keep) h = 0.f;
+                        r.v[v] = from_f32<T>(SUM ? D : D * w.y);
+                        dg.v[v] = from_f32<T>(SUM ? D * h * w.x : D * (h - to_f32(o.x.v[v])) * w.x * w.y);
+                    }
+                    s[v] = o.keep ? w.x * D : 0.f;
+                }
+                if constexpr (PART == 0) prod[v] = !o.keep || prod[v] < 0.f ? CUT : prod[v] * w.x;
+            }
+            if constexpr (PART == 1) {
+                *reinterpret_cast<Elems<T, V> *>(a.out + t * C + c) = r;
+                if constexpr (BACK) *reinterpret_cast<Elems<T, V> *>(a.dgate + t * C + c) = dg;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) now[u] = next[u];
+    }
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+        if constexpr (PART == 0)
+            a.carry[chunk * C + c + v] = make_float2(prod[v], s[v]);
+        else if (a.last && chunk == a.chunks - 1)
+            a.last[c + v] = s[v];
+    }
+}
+
+__device__ __forceinline__ float through(float2 map, float s) { return map.x < 0.f ? map.y : fmaf(map.x, s, map.y); }
+
+// The state before every chunk, in place of its (P, Q): a lane for each channel,
+// the chunks divided between the block's warps.
+__global__ void __launch_bounds__(32 * CARRY_WARPS) carry_kernel(float2 *carry, const float *start, int64_t C, int chunks) {
+    pdl_wait();
+    __shared__ float2 sums[CARRY_WARPS][32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+    const int each = (chunks + CARRY_WARPS - 1) / CARRY_WARPS, lo = min(chunks, warp * each), hi = min(chunks, lo + each);
+    float p = 1.f, q = 0.f;
+    if (c < C)
+#pragma unroll 8
+        for (int k = lo; k < hi; k++) {
+            const float2 m = carry[k * C + c];
+            q = through(m, q);
+            p = m.x < 0.f || p < 0.f ? CUT : p * m.x;
+        }
+    sums[warp][lane] = make_float2(p, q);
+    __syncthreads();
+    if (c >= C) return;
+    float s = start ? start[c] : 0.f;
+    for (int w = 0; w < warp; w++) s = through(sums[w][lane], s);
+#pragma unroll 8
+    for (int k = lo; k < hi; k++) {
+        const float2 m = carry[k * C + c];
+        carry[k * C + c].x = s;
+        s = through(m, s);
+    }
+}
+
+// Chunks that the time is cut into: 1 where a thread for each channel is enough.
+// By the number of channels alone, whatever the vectors' width is.
+static int chunks_of(int64_t T, int64_t C) {
+    const int64_t want = (int64_t)SMS * 2048 / (C < 1 ? 1 : C), most = (T + 31) / 32;
+    int64_t n = want < 4 ? 1 : want < most ? want : most;
+    if (n > 4096) n = 4096;
+    return (int)(n < 1 ? 1 : n);
+}
+
+template <class T, int V, bool SUM, bool BACK> static int run(Args<T> &a, cudaStream_t s) {
+    constexpr int U = V * sizeof(T) >= 8 ? 4 : 8;
+    a.lanes = a.B * a.D / V;
+    const int64_t blocks = (a.lanes + THREADS - 1) / THREADS;
+    if (blocks > INT32_MAX) return D1_ERR_TOO_LARGE;
+    cudaLaunchAttribute attr;
+    cudaLaunchConfig_t cfg = pdl_config(dim3((unsigned)blocks, (unsigned)a.chunks), dim3(THREADS), 0, s, &attr);
+    cfg.numAttrs = 0;
+    if (a.chunks > 1) {
+        if (cudaError_t e = cudaLaunchKernelEx(&cfg, scan_kernel<T, V, SUM, BACK, 0, U>, a)) return (int)e;
+        cfg.numAttrs = 1;
+        cudaLaunchConfig_t mid = cfg;
+        const int64_t C = a.B * a.D;
+        mid.gridDim = dim3((unsigned)((C + 31) / 32));
+        mid.blockDim = dim3(32 * CARRY_WARPS);
+        if (cudaError_t e = cudaLaunchKernelEx(&mid, carry_kernel, a.carry, a.start, C, a.chunks)) return (int)e;
+    }
+    return (int)cudaLaunchKernelEx(&cfg, scan_kernel<T, V, SUM, BACK, 1, U>, a);
+}
+
+template <class T> static bool pairs(const Span<const T> &s) {
+    return aligned_to(2 * sizeof(T), s.p) && s.st % 2 == 0 && s.sb % 2 == 0;
+}
+
+template <class T, bool BACK> static int any(Args<T> a, int form, void *work, cudaStream_t s) {
+    a.chunks = chunks_of(a.T_, a.B * a.D);
+    a.size = (a.T_ + a.chunks - 1) / a.chunks;
+    a.chunks = (int)((a.T_ + a.size - 1) / a.size);
+    a.carry = (float2 *)work;
+    if (a.chunks > 1 && (!work || !aligned_to(8, work))) return D1_ERR_BAD_ARGUMENT;
+    const bool two = a.D % 2 == 0 && pairs(a.gate) && pairs(a.x) && aligned_to(2 * sizeof(T), a.out) &&
+                     (!BACK || (pairs(a.dy) && pairs(a.y) && aligned_to(2 * sizeof(T), a.dgate)));
+    if (form == D1_SCAN_SUM) return two ? run<T, 2, true, BACK>(a, s) : run<T, 1, true, BACK>(a, s);
+    return two ? run<T, 2, false, BACK>(a, s) : run<T, 1, false, BACK>(a, s);
+}
+
+// Whether sizes and strides are in range: D, B, T >= 0 and all offsets within 62 bits.
+static bool shape_ok(int64_t T, int64_t B, int64_t D) {
+    return T >= 0 && B >= 0 && D >= 1 && T <= ((int64_t)1 << 40) && B <= ((int64_t)1 << 40) && D <= INT32_MAX &&
+           (B == 0 || D <= ((int64_t)1 << 42) / B) && (T == 0 || B * D <= ((int64_t)1 << 58) / T);
+}
+
+// Whether the contiguous result at q meets the range of a [T, B, D] operand.
+static bool meets(const void *q, const void *p, int64_t st, int64_t sb, int64_t T, int64_t B, int64_t D, int size) {
+    if (!q || !p || T < 1 || B < 1) return false;
+    const uintptr_t a = (uintptr_t)q, b = (uintptr_t)p;
+    return a < b + (uintptr_t)(((T - 1) * st + (B - 1) * sb + D) * size) && b < a + (uintptr_t)(T * B * D * size);
+}
+static bool stride_ok(int64_t s) { return s >= 0 && s <= ((int64_t)1 << 42); }
+
+}  // namespace gs
+}  // namespace d1
+
+extern "C" int64_t d1_gated_scan_work_bytes(int64_t T, int64_t B, int64_t D) {
+    using namespace d1::gs;
+    if (!shape_ok(T, B, D)) return -1;
+    const int chunks = chunks_of(T, B * D);
+    return chunks > 1 ? 8 * chunks * B * D : 0;
+}
+
+extern "C" int d1_gated_scan(const void *x, int64_t x_t, int64_t x_b, const void *gate, int64_t gate_t, int64_t gate_b,
+                             int type, int form, int64_t T, int64_t B, int64_t D, const float *h0, const uint8_t *reset,
+                             int64_t reset_t, int64_t reset_b, void *y, float *last, void *work, void *stream) {
+    using namespace d1;
+    if (!type_ok(type) || (form != D1_SCAN_AVERAGE && form != D1_SCAN_SUM) || !gs::shape_ok(T, B, D) ||
+        (T && B && (!x || !gate || !y)) || !gs::stride_ok(x_t) || !gs::stride_ok(x_b) || !gs::stride_ok(gate_t) ||
+        !gs::stride_ok(gate_b) || !gs::stride_ok(reset_t) || !gs::stride_ok(reset_b) || !element_aligned(x, type) ||
+        !element_aligned(gate, type) || !element_aligned(y, type) || !aligned_to(4, h0, last))
+        return D1_ERR_BAD_ARGUMENT;
+    const int size = type == D1_TYPE_F32 ? 4 : 2;
+    if (gs::meets(y, x, x_t, x_b, T, B, D, size) || gs::meets(y, gate, gate_t, gate_b, T, B, D, size))
+        return D1_ERR_BAD_ARGUMENT;
+    const cudaStream_t s = (cudaStream_t)stream;
+    if (B == 0) return 0;
+    if (T == 0) {  // the state is what it was
+        if (!last) return 0;
+        return (int)(h0 ? cudaMemcpyAsync(last, h0, (size_t)(B * D) * 4, cudaMemcpyDeviceToDevice, s)
+                        : cudaMemsetAsync(last, 0, (size_t)(B * D) * 4, s));
+    }
+    const auto go = [&](auto one) {
+        using E = decltype(one);
+        gs::Args<E> a{};
+        a.x = {(const E *)x, x_t, x_b};
+        a.gate = {(const E *)gate, gate_t, gate_b};
+        a.out = (E *)y;
+        a.reset = reset, a.reset_t = reset_t, a.reset_b = reset_b;
+        a.start = h0, a.last = last;
+        a.T_ = T, a.B = B, a.D = D;
+        return gs::any<E, false>(a, form, work, s);
+    };
+    return type == D1_TYPE_F32 ? go(float{}) : type == D1_TYPE_BF16 ? go(__nv_bfloat16{}) : go(__half{});
+}
+
+extern "C" int d1_gated_scan_backward(const void *dy, int64_t dy_t, int64_t dy_b, const void *x, int64_t x_t, int64_t x_b,
+                                      const void *gate, int64_t gate_t, int64_t gate_b, const void *y, int64_t y_t,
+                                      int64_t y_b, int type, int form, int64_t T, int64_t B, int64_t D, const float *h0,
+                                      const float *dlast, const uint8_t *reset, int64_t reset_t, int64_t reset_b, void *dx,
+                                      void *dgate, float *dh0, void *work, void *stream) {
+    using namespace d1;
+    if (!type_ok(type) || (form != D1_SCAN_AVERAGE && form != D1_SCAN_SUM) || !gs::shape_ok(T, B, D) ||
+        (T && B && (!dy || !x || !gate || !y || !dx || !dgate)) || !gs::stride_ok(x_t) || !gs::stride_ok(x_b) ||
+        !gs::stride_ok(gate_t) || !gs::stride_ok(gate_b) || !gs::stride_ok(y_t) || !gs::stride_ok(y_b) ||
+        !gs::stride_ok(dy_t) || !gs::stride_ok(dy_b) || !gs::stride_ok(reset_t) || !gs::stride_ok(reset_b) ||
+        !element_aligned(x, type) || !element_aligned(gate, type) || !element_aligned(y, type) ||
+        !element_aligned(dy, type) || !element_aligned(dx, type) || !element_aligned(dgate, type) ||
+        !aligned_to(4, h0, dlast, dh0))
+        return D1_ERR_BAD_ARGUMENT;
+    const int size = type == D1_TYPE_F32 ? 4 : 2;
+    void *const results[2] = {dx, dgate};
+    for (void *q : results)
+        if (gs::meets(q, x, x_t, x_b, T, B, D, size) || gs::meets(q, gate, gate_t, gate_b, T, B, D, size) ||
+            gs::meets(q, y, y_t, y_b, T, B, D, size) || gs::meets(q, dy, dy_t, dy_b, T, B, D, size))
+            return D1_ERR_BAD_ARGUMENT;
+    if (gs::meets(dx, dgate, B * D, D, T, B, D, size)) return D1_ERR_BAD_ARGUMENT;
+    const cudaStream_t s = (cudaStream_t)stream;
+    if (B == 0) return 0;
+    if (T == 0) {
+        if (!dh0) return 0;
+        return (int)(dlast ? cudaMemcpyAsync(dh0, dlast, (size_t)(B * D) * 4, cudaMemcpyDeviceToDevice, s)
+                           : cudaMemsetAsync(dh0, 0, (size_t)(B * D) * 4, s));
+    }
+    const auto go = [&](auto one) {
+        using E = decltype(one);
+        gs::Args<E> a{};
+        a.x = {(const E *)x, x_t, x_b};
+        a.gate = {(const E *)gate, gate_t, gate_b};
+        a.y = {(const E *)y, y_t, y_b};
+        a.dy = {(const E *)dy, dy_t, dy_b};
+        a.out = (E *)dx, a.dgate = (E *)dgate;
+        a.reset = reset, a.reset_t = reset_t, a.reset_b = reset_b;
+        a.start = dlast, a.h0 = h0, a.last = dh0;
+        a.T_ = T, a.B = B, a.D = D;
+        return gs::any<E, true>(a, form, work, s);
+    };
+    return type == D1_TYPE_F32 ? go(float{}) : type == D1_TYPE_BF16 ? go(__nv_bfloat16{}) : go(__half{});
+}

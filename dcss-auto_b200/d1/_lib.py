@@ -9,7 +9,7 @@ ERR_TOO_LARGE = 9003
 
 _P, _I, _U64, _F = C.c_void_p, C.c_int, C.c_uint64, C.c_float
 _I64, _D = C.c_int64, C.c_double
-# name -> argtypes; every export returns int.
+# name -> argtypes; every export returns int (those of RETURNS a 64-bit one).
 SIGNATURES = {
     'learn_state_bytes': [], 'learn_obs_size': [], 'learn_action_size': [], 'learn_out_size': [],
     'learn_config_bytes': [],
@@ -101,9 +101,14 @@ SIGNATURES = {
     'd1_layer_norm_backward': [_P, _I64, _P, _I64, _I, _I64, _I, _P, _P, _P, _P, _I64, _P, _P, _P, _P],
     'd1_token_logprob': [_P, _I64, _I, _I64, _I, _P, _P, _I64, _F, _I, _P, _P, _P, _P, _P, _P],
     'd1_token_logprob_backward': [_P, _I64, _I, _I64, _I, _P, _P, _I64, _F, _P, _P, _P, _P, _P, _I64, _P],
+    'd1_gated_scan_work_bytes': [_I64, _I64, _I64],
+    'd1_gated_scan': [_P, _I64, _I64, _P, _I64, _I64, _I, _I, _I64, _I64, _I64, _P, _P, _I64, _I64, _P, _P, _P, _P],
+    'd1_gated_scan_backward': [_P, _I64, _I64] * 4 + [_I, _I, _I64, _I64, _I64, _P, _P, _P, _I64, _I64, _P, _P, _P, _P, _P],
     'd1_adamw_work_bytes': [],
     'd1_adamw': [_P, _I, _I64, _I, _P, _P, _P, _P, _D, _D, _D, _D, _D, _P, _U64, _P, _P, _P],
 }
+
+RETURNS = {'d1_gated_scan_work_bytes': _I64}
 
 _LIB = None
 
@@ -123,7 +128,7 @@ def library():
         for name, argtypes in SIGNATURES.items():
             fn = getattr(lib, name)
             fn.argtypes = argtypes
-            fn.restype = C.c_int
+            fn.restype = RETURNS.get(name, C.c_int)
         _LIB = lib
     return _LIB
 

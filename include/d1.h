@@ -734,6 +734,38 @@ int d1_adamw(const D1AdamWTensor *tensors, int ntensors, int64_t nblocks, int st
              float *m_scale, float *v_scale, double lr, double beta1, double beta2, double eps, double max_norm,
              int64_t *step, uint64_t seed, void *work, float *grad_norm, void *stream);
 
+/* ======================================================================
+ * Operators for training a policy with a memory by reinforcement: a gated
+ * linear recurrence, the clipped policy loss and the Muon step. No counterpart
+ * in the reference.
+ * ====================================================================== */
+#define D1_SCAN_AVERAGE 0 /* a = sigmoid(gate), h_t = a_t h_{t-1} + (1 - a_t) x_t */
+#define D1_SCAN_SUM 1     /* a = e^gate,        h_t = a_t h_{t-1} + x_t */
+
+/* Bytes of the work buffer of d1_gated_scan and its backward pass (0: none
+ * needed); -1 for sizes out of range. */
+int64_t d1_gated_scan_work_bytes(int64_t T, int64_t B, int64_t D);
+/* y[t, b, d] = h_t of channel d of sequence b, over T steps from h0 (f32 [B, D];
+ * NULL: zeros). x and gate are [T, B, D] of type `type` with contiguous
+ * channels; step t and sequence b lie t * x_t + b * x_b elements on. Where
+ * reset[t * reset_t + b * reset_b] (bytes; NULL: nowhere) is not 0, an episode begins
+ * at t: the state before it counts for nothing. States are f32; y (contiguous
+ * [T, B, D], type `type`) is rounded once and shares no memory with the range
+ * of x or gate; last (f32 [B, D]; NULL: not wanted) is the state after step
+ * T - 1, h0 when T is 0. work: 8-byte aligned, of the size above. */
+int d1_gated_scan(const void *x, int64_t x_t, int64_t x_b, const void *gate, int64_t gate_t, int64_t gate_b, int type,
+                  int form, int64_t T, int64_t B, int64_t D, const float *h0, const uint8_t *reset, int64_t reset_t,
+                  int64_t reset_b, void *y, float *last, void *work, void *stream);
+/* The gradients of d1_gated_scan from dy (type `type`) and dlast (f32 [B, D];
+ * NULL: zeros): dx and dgate (contiguous, type `type`), dh0 (f32 [B, D]; NULL: not
+ * wanted). y is what the forward pass gave. dx and dgate share no memory with
+ * the range of an input. */
+int d1_gated_scan_backward(const void *dy, int64_t dy_t, int64_t dy_b, const void *x, int64_t x_t, int64_t x_b,
+                           const void *gate, int64_t gate_t, int64_t gate_b, const void *y, int64_t y_t, int64_t y_b,
+                           int type, int form, int64_t T, int64_t B, int64_t D, const float *h0, const float *dlast,
+                           const uint8_t *reset, int64_t reset_t, int64_t reset_b, void *dx, void *dgate, float *dh0,
+                           void *work, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
