@@ -104,11 +104,14 @@ SIGNATURES = {
     'd1_gated_scan_work_bytes': [_I64, _I64, _I64],
     'd1_gated_scan': [_P, _I64, _I64, _P, _I64, _I64, _I, _I, _I64, _I64, _I64, _P, _P, _I64, _I64, _P, _P, _P, _P],
     'd1_gated_scan_backward': [_P, _I64, _I64] * 4 + [_I, _I, _I64, _I64, _I64, _P, _P, _P, _I64, _I64, _P, _P, _P, _P, _P],
+    'd1_policy_loss_work_bytes': [_I64, _I64],
+    'd1_policy_loss': [_P, _I64, _P, _I64, _P, _I64, _I, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _D, _D, _D, _D, _I, _P, _P, _P,
+                       _P, _P, _P],
     'd1_adamw_work_bytes': [],
     'd1_adamw': [_P, _I, _I64, _I, _P, _P, _P, _P, _D, _D, _D, _D, _D, _P, _U64, _P, _P, _P],
 }
 
-RETURNS = {'d1_gated_scan_work_bytes': _I64}
+RETURNS = {'d1_gated_scan_work_bytes': _I64, 'd1_policy_loss_work_bytes': _I64}
 
 _LIB = None
 

@@ -766,6 +766,28 @@ int d1_gated_scan_backward(const void *dy, int64_t dy_t, int64_t dy_b, const voi
                            const uint8_t *reset, int64_t reset_t, int64_t reset_b, void *dx, void *dgate, float *dh0,
                            void *work, void *stream);
 
+/* Bytes of the work buffer of d1_policy_loss (0: none needed); -1 for sizes out
+ * of range. */
+int64_t d1_policy_loss_work_bytes(int64_t rows, int64_t length);
+/* The clipped policy loss over the tokens of `rows` rows of `length`, and its gradient:
+ *   loss = mean( -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (e^d - d - 1) - ent_coef H )
+ * with r = e^(logp - old_logp), d = ref_logp - logp. Operands are f32 with a
+ * pitch in elements between rows; per_row: advantage is one number a row, at
+ * advantage[row * ld_advantage]. ref_logp, entropy and mask (bytes) may be NULL: no KL
+ * term, no entropy term, every token counts; what the mask leaves out is not looked
+ * at. by_row 0: the mean is over all tokens; 1: over the rows that have any, of
+ * the row's mean. Without a token that counts everything is 0. stats = the
+ * means (of the same kind) of the clipped term, of e^d - d - 1, of H, of the
+ * tokens that were clipped, and of r - 1 - log r. dlogp and dentropy (contiguous f32;
+ * NULL: not wanted) are the loss's gradients, 0 where the mask is, and share no
+ * memory with the operands; so may loss and stats be NULL. Without a mask length is at
+ * most 2^31 - 1, with one rows * length is. work: 8-byte aligned, of the size above. */
+int d1_policy_loss(const float *logp, int64_t ld_logp, const float *old_logp, int64_t ld_old, const float *advantage,
+                   int64_t ld_advantage, int per_row, const float *ref_logp, int64_t ld_ref, const float *entropy,
+                   int64_t ld_entropy, const uint8_t *mask, int64_t ld_mask, int64_t rows, int64_t length,
+                   double clip_low, double clip_high, double kl_coef, double ent_coef, int by_row, float *loss,
+                   float *stats, float *dlogp, float *dentropy, void *work, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
