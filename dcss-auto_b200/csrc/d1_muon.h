@@ -1,0 +1,121 @@
+// How the Newton-Schulz products lay out and divide their work, by plain
+// arithmetic (no CUDA type or call, so that it is checked on the host).
+//
+// All 16-bit operands live in one buffer of blocks: 64 x 64 elements in 64 rows
+// of 128 bytes, so that one tensor map of 64-element rows serves every matrix
+// and a block is an operand of the tensor cores in either orientation. A matrix
+// of r x c elements has ceil(r / 64) x ceil(c / 64) blocks, row of blocks after
+// row of blocks, zero past its edges; products of zeros keep them zero.
+#pragma once
+#include <stdint.h>
+
+#include "../../include/d1.h"
+
+#ifdef __CUDACC__
+#define D1_MUON_BOTH __host__ __device__ __forceinline__
+#else
+#define D1_MUON_BOTH inline
+#endif
+
+namespace d1 {
+namespace muon {
+
+constexpr int SIDE = 64, BLOCK_BYTES = SIDE * SIDE * 2;
+constexpr int MOST_PARTS = 256;  // partial sums of one matrix's norm
+constexpr int64_t MOST_BLOCKS = (int64_t)1 << 24;  // rows of the tensor map stay below 2^30
+
+// One matrix. X is held as hi + lo, hi twice (a product reads one and writes the other).
+struct Matrix {
+    float *param;         // Muon: the master (NULL: orthogonalize)
+    const void *grad;     // the gradient, or the matrix to orthogonalize
+    void *out;            // Muon: the bf16 copy or NULL; orthogonalize: the result
+    float *momentum;      // Muon
+    int64_t pitch;        // elements between rows of grad (param, out and momentum are contiguous)
+    int rows, cols;       // of the matrix
+    int rb, cb;           // of its blocks
+    int sb;               // blocks along the smaller side
+    int tall;             // rows > cols: the Gram matrix is X^T X
+    int hi[2], lo, gram, quad;  // first blocks
+    int fine;             // small: A and B are pairs too (the second one a block after the first), and products take all three terms
+    int part0, parts;     // partial sums of the norm
+    int grad_type, out_type;
+    float rate, keep_decay;  // 0.2 sqrt(max(rows, cols)); the weight decay
+};
+
+// A tile of a product: row and column of tiles.
+struct Tile {
+    int matrix;
+    uint16_t i, j;
+};
+// The blocks k, k + parts, ... of a matrix, k < parts.
+struct Part {
+    int matrix, k;
+};
+
+D1_MUON_BOTH int blocks_of(int64_t n) { return (int)((n + SIDE - 1) / SIDE); }
+D1_MUON_BOTH int tiles_of(int blocks, int side) { return (blocks + side - 1) / side; }
+
+// Blocks of A, or of B. With one block along the smaller side it is a pair.
+D1_MUON_BOTH int64_t gram_blocks(int64_t sb) { return sb == 1 ? 2 : sb * sb; }
+
+// Sizes, blocks (from `block` on) and parts (from `part` on) of a matrix; moves both on.
+inline void place(Matrix &m, int64_t rows, int64_t cols, int64_t &block, int64_t &part) {
+    m.rows = (int)rows, m.cols = (int)cols;
+    m.rb = blocks_of(rows), m.cb = blocks_of(cols);
+    m.tall = rows > cols;
+    m.sb = m.tall ? m.cb : m.rb;
+    m.fine = m.sb == 1;
+    const int64_t n = (int64_t)m.rb * m.cb, s = gram_blocks(m.sb);
+    m.hi[0] = (int)block;
+    m.hi[1] = (int)(block + n);
+    m.lo = (int)(block + 2 * n);
+    m.gram = (int)(block + 3 * n);
+    m.quad = (int)(block + 3 * n + s);
+    block += 3 * n + 2 * s;
+    m.part0 = (int)part;
+    m.parts = (int)(n < MOST_PARTS ? n : MOST_PARTS);
+    part += m.parts;
+}
+// Blocks that place() takes; -1 for a matrix that is out of range.
+inline int64_t blocks_needed(int64_t rows, int64_t cols) {
+    if (rows < 1 || cols < 1 || rows > ((int64_t)1 << 21) || cols > ((int64_t)1 << 21)) return -1;
+    const int64_t rb = blocks_of(rows), cb = blocks_of(cols), sb = rows > cols ? cb : rb;
+    return 3 * rb * cb + 2 * gram_blocks(sb);
+}
+
+// Tile t of a symmetric matrix of tiles: row i >= column j, row after row.
+D1_MUON_BOTH void symmetric_tile(int64_t t, int &i, int &j) {
+    int64_t r = 0, step = (int64_t)1 << 30;  // the largest r with r (r + 1) / 2 <= t
+    while (step >>= 1)
+        if ((r + step) * (r + step + 1) / 2 <= t) r += step;
+    i = (int)r;
+    j = (int)(t - r * (r + 1) / 2);
+}
+// Tile t of tm x tn: eight rows of tiles at a time, column after column, so that tiles that
+// run together share operands in L2.
+D1_MUON_BOTH void grouped_tile(int64_t t, int tm, int tn, int &i, int &j) {
+    const int64_t per = (int64_t)8 * tn, g = t / per, r = t - g * per;
+    const int64_t high = tm - 8 * g < 8 ? tm - 8 * g : 8;
+    i = (int)(8 * g + r % high);
+    j = (int)(r / high);
+}
+
+D1_MUON_BOTH int64_t symmetric_tiles(const Matrix &m, int side) {
+    const int64_t n = tiles_of(m.sb, side);
+    return n * (n + 1) / 2;
+}
+D1_MUON_BOTH int64_t full_tiles(const Matrix &m, int side) { return (int64_t)tiles_of(m.rb, side) * tiles_of(m.cb, side); }
+
+// What a plan begins with: sizes of its lists and where they start (bytes).
+struct Plan {
+    int64_t bytes, matrices, parts, symmetric, full;
+    int64_t at_matrices, at_parts, at_symmetric, at_full;
+    int64_t blocks;  // of the work buffer
+    int side;        // blocks along a tile's side: 2 or 4
+    int reserved;
+};
+
+D1_MUON_BOTH int64_t work_blocks_bytes(int64_t blocks) { return blocks * BLOCK_BYTES; }
+
+}  // namespace muon
+}  // namespace d1

@@ -1,0 +1,829 @@
+// Muon: momentum, orthogonalisation of the update by Newton-Schulz products, and
+// the step, over many weight matrices at a time (sm_100a, tcgen05 + TMA).
+//
+//   m' = mu m + g        u = g + mu m' (Nesterov) or m'
+//   X = u / |u|_F, then `steps` times:  A = X X^T (or X^T X)   B = b A + c A^2   X' = a X + B X (or X B)
+//   p' = p (1 - lr decay) - lr 0.2 sqrt(max(rows, cols)) X
+//
+// with the published coefficients (a, b, c) = (3.4445, -4.7750, 2.0315), which bring
+// every singular value of X between about 0.7 and 1.2.
+//
+// Rounding. The products run on the tensor cores in fp16 with fp32 sums: |X| <= 1.3
+// and its products are bounded too, so that a scale of 2^12 keeps all of them inside fp16's range, and fp16
+// has eight times bf16's precision at the same rate. Singular directions that the update hardly has are
+// amplified by a = 3.4 a step, 485 in five, and with them whatever rounding puts there: of a gradient of low
+// rank the result would be noise to a large part (simulated, rank 32 of 512: 3 % of its norm in fp16, 22 %
+// in bf16). So X is held as a pair hi + lo of fp16, 22 bits, and a X is taken from the pair; the products read hi
+// alone, and the error that they make lies in directions that X has (0.06 % there, 0.2 % of a full-rank one). In a
+// matrix with a side of at most 64, where few roundings average out (up to 1 % in some), A and B are pairs too and a product takes all three
+// terms: it is as good as one in fp32, and its time is the launches' all the same.
+//
+// The three products of all matrices are one launch each. A and B are symmetric: only the tiles on and below the
+// diagonal are computed, and each is stored a second time transposed. The epilogues hold the rest of the
+// formulas, the last one the step itself. All operands are blocks of 64 x 64 elements (d1_muon.h) that the TMA
+// swizzles on its way to shared memory, as K-major operands or as MN-major ones: X is never transposed.
+#include <cuda.h>
+#include <math.h>
+
+#include <algorithm>
+#include <new>
+
+#include "d1_common.cuh"
+#include "d1_elem.cuh"
+#include "d1_muon.h"
+#include "d1_pdl.cuh"
+#include "d1_rows.h"
+#include "tc_ptx.cuh"
+
+namespace d1 {
+namespace muon {
+
+using namespace tcx;
+
+constexpr int SMS = 148, STAGES = 6, HALF_BYTES = 2 * BLOCK_BYTES, STAGE_BYTES = 2 * HALF_BYTES, EPI_WARPS = 8;
+constexpr int THREADS = 64 + 32 * EPI_WARPS, SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256, PREP = 256;
+constexpr uint32_t WAIT_LIMIT = 1u << 22;
+constexpr float SCALE = 4096.f, UNSCALE = 1.f / 4096.f;  // of X, A and B in fp16
+constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
+
+__device__ int g_error;
+
+struct Job {
+    const Matrix *matrices;  // NULL: a stack of `one`
+    const Tile *symmetric, *full;
+    const Part *parts;
+    Matrix one;
+    int64_t grad_step, out_step;  // bytes from one matrix of the stack to the next
+    int block_step;
+    int count_symmetric, count_full, per_symmetric, per_full, tm, tn;
+    uint8_t *work;
+    double *partials;
+    float mu;
+    int nesterov;
+    double lr;
+    int from;  // which hi is read
+};
+
+__device__ __forceinline__ Matrix matrix_of(const Job &o, int m) {
+    if (o.matrices) return o.matrices[m];
+    Matrix x = o.one;
+    x.grad = (const char *)x.grad + m * o.grad_step;
+    x.out = (char *)x.out + m * o.out_step;
+    const int b = m * o.block_step;
+    x.hi[0] += b, x.hi[1] += b, x.lo += b, x.gram += b, x.quad += b;
+    x.part0 += m * x.parts;
+    return x;
+}
+__device__ __forceinline__ Tile tile_of(const Job &o, bool symmetric, int t) {
+    if (o.matrices) return symmetric ? o.symmetric[t] : o.full[t];
+    const int per = symmetric ? o.per_symmetric : o.per_full;
+    Tile r;
+    r.matrix = t / per;
+    int i, j;
+    if (symmetric)
+        symmetric_tile(t - r.matrix * per, i, j);
+    else
+        grouped_tile(t - r.matrix * per, o.tm, o.tn, i, j);
+    r.i = (uint16_t)i, r.j = (uint16_t)j;
+    return r;
+}
+
+// ---------------------------------------------------------------- momentum, norm, X
+
+// n of 8 consecutive elements (the others 0).
+template <class T> __device__ __forceinline__ void load8(const T *p, int n, bool wide, float (&v)[8]) {
+    if (wide) {
+        constexpr int N = 16 / sizeof(T);
+#pragma unroll
+        for (int k = 0; k < 8; k += N) {
+            const Elems<T, N> e = *reinterpret_cast<const Elems<T, N> *>(p + k);
+#pragma unroll
+            for (int i = 0; i < N; i++) v[k + i] = to_f32(e.v[i]);
+        }
+    } else
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] = k < n ? to_f32(p[k]) : 0.f;
+}
+__device__ __forceinline__ void load8(const void *base, int type, int64_t at, int n, float (&v)[8]) {
+    if (type == D1_TYPE_F32) {
+        const float *p = (const float *)base + at;
+        load8(p, n, n == 8 && ((uintptr_t)p & 15) == 0, v);
+    } else if (type == D1_TYPE_BF16) {
+        const __nv_bfloat16 *p = (const __nv_bfloat16 *)base + at;
+        load8(p, n, n == 8 && ((uintptr_t)p & 15) == 0, v);
+    } else {
+        const __half *p = (const __half *)base + at;
+        load8(p, n, n == 8 && ((uintptr_t)p & 15) == 0, v);
+    }
+}
+
+// Sum over the block in a fixed order, in every thread.
+__device__ __forceinline__ double block_sum(double s, double *shared) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = s;
+    __syncthreads();
+    s = 0.;
+#pragma unroll
+    for (int w = 0; w < PREP / 32; w++) s += shared[w];
+    return s;
+}
+
+// FIRST: the new momentum and the sum of the squares of u (in fp64: squares of fp32 numbers neither overflow
+// nor vanish there). Else X = u / |u|, as hi + lo.
+template <bool FIRST> __global__ void __launch_bounds__(PREP) prepare_kernel(Job o) {
+    __shared__ double shared[PREP / 32];
+    pdl_wait();
+    Part part;
+    if (o.matrices)
+        part = o.parts[blockIdx.x];
+    else
+        part.matrix = blockIdx.x / o.one.parts, part.k = blockIdx.x % o.one.parts;
+    const Matrix m = matrix_of(o, part.matrix);
+    double sum = 0., inverse = 0.;
+    if (!FIRST) {
+        if ((int)threadIdx.x < m.parts) sum = o.partials[m.part0 + threadIdx.x];
+        const double norm = sqrt(block_sum(sum, shared));
+        inverse = norm == 0. ? 0. : (double)SCALE / norm;
+    }
+    for (int b = part.k; b < m.rb * m.cb; b += m.parts) {
+        const int ib = b / m.cb, jb = b - ib * m.cb;
+#pragma unroll
+        for (int q = 0; q < 2; q++) {
+            const int e = threadIdx.x + PREP * q, row = e >> 3, col = (e & 7) * 8;
+            const int i = ib * SIDE + row, j = jb * SIDE + col, n = i < m.rows ? min(8, max(0, m.cols - j)) : 0;
+            float u[8] = {};
+            if (n) {
+                load8(m.grad, m.grad_type, i * m.pitch + j, n, u);
+                if (m.momentum) {
+                    float *p = m.momentum + (int64_t)i * m.cols + j, v[8];
+                    const bool wide = n == 8 && ((uintptr_t)p & 15) == 0;
+                    load8(p, n, wide, v);
+                    if (FIRST) {
+#pragma unroll
+                        for (int k = 0; k < 8; k++) v[k] = fmaf(o.mu, v[k], u[k]);
+                        if (wide) {
+                            *(float4 *)p = make_float4(v[0], v[1], v[2], v[3]);
+                            *(float4 *)(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+                        } else
+#pragma unroll
+                            for (int k = 0; k < 8; k++)
+                                if (k < n) p[k] = v[k];
+                    }
+#pragma unroll
+                    for (int k = 0; k < 8; k++) u[k] = o.nesterov ? fmaf(o.mu, v[k], u[k]) : v[k];
+                }
+            }
+            if (FIRST) {
+#pragma unroll
+                for (int k = 0; k < 8; k++) sum = fma((double)u[k], (double)u[k], sum);
+            } else {
+                Elems<__half, 8> hi, lo;
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const float x = (float)((double)u[k] * inverse);
+                    hi.v[k] = __float2half_rn(x);
+                    lo.v[k] = __float2half_rn(x - __half2float(hi.v[k]));
+                }
+                const int at = row * 128 + col * 2;
+                *reinterpret_cast<Elems<__half, 8> *>(o.work + (int64_t)(m.hi[0] + b) * BLOCK_BYTES + at) = hi;
+                *reinterpret_cast<Elems<__half, 8> *>(o.work + (int64_t)(m.lo + b) * BLOCK_BYTES + at) = lo;
+            }
+        }
+    }
+    if (FIRST) {
+        sum = block_sum(sum, shared);
+        if (threadIdx.x == 0) o.partials[m.part0 + part.k] = sum;
+    }
+}
+
+// ---------------------------------------------------------------- products
+
+enum Phase { GRAM, QUAD, APPLY, STEP };  // A; B; X'; the step with the last X' (or the result itself)
+
+// Where the operands of a phase lie: block (i, k) of the first at a + i * ai + k * ak, of the second at
+// b + j * bj + k * bk; their blocks along i, j and k.
+struct Operands {
+    int a, ai, ak, b, bj, bk, ni, nj, nk;
+    bool a_mn, b_mn;
+    int terms;         // 1; 3 where operands are pairs: hi hi, lo hi, hi lo (lo lo is below fp32's last bit)
+    int a_lo, b_lo;    // from a hi block to its lo block
+};
+__device__ __forceinline__ Operands operands(const Matrix &m, int phase, int from) {
+    const int hi = from ? m.hi[1] : m.hi[0], x_lo = m.lo - hi, terms = m.fine ? 3 : 1;
+    if (phase == GRAM)
+        return m.tall ? Operands{hi, 1, m.cb, hi, 1, m.cb, m.sb, m.sb, m.rb, true, true, terms, x_lo, x_lo}
+                      : Operands{hi, m.cb, 1, hi, m.cb, 1, m.sb, m.sb, m.cb, false, false, terms, x_lo, x_lo};
+    if (phase == QUAD) return Operands{m.gram, m.sb, 1, m.gram, m.sb, 1, m.sb, m.sb, m.sb, false, false, terms, 1, 1};
+    return m.tall ? Operands{hi, m.cb, 1, m.quad, m.sb, 1, m.rb, m.cb, m.sb, false, false, terms, x_lo, 1}
+                  : Operands{m.quad, m.sb, 1, hi, 1, m.cb, m.rb, m.cb, m.sb, false, true, terms, 1, x_lo};
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// A TMA load into this CTA's shared memory that completes on a barrier of either CTA of the pair.
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void mma_pair(uint32_t tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void commit_pair(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+// 32 elements of a block's row in fp16.
+struct alignas(16) Halves {
+    __half v[32];
+};
+__device__ __forceinline__ Halves load_row(const uint8_t *p) {
+    Halves r;
+#pragma unroll
+    for (int k = 0; k < 4; k++) reinterpret_cast<uint4 *>(&r)[k] = reinterpret_cast<const uint4 *>(p)[k];
+    return r;
+}
+__device__ __forceinline__ void store_row(uint8_t *p, const Halves &r) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) reinterpret_cast<uint4 *>(p)[k] = reinterpret_cast<const uint4 *>(&r)[k];
+}
+
+__device__ __forceinline__ void split(const float (&x)[32], Halves &hi, Halves &lo) {
+#pragma unroll
+    for (int k = 0; k < 32; k++) {
+        hi.v[k] = __float2half_rn(x[k]);
+        lo.v[k] = __float2half_rn(x[k] - __half2float(hi.v[k]));
+    }
+}
+
+// The step on 32 elements of a row (n of them exist), or the result itself.
+__device__ __forceinline__ void finish(const Job &o, const Matrix &m, int64_t at, int n, const float (&x)[32]) {
+    if (!m.param) {
+        if (m.out_type == D1_TYPE_BF16) {
+            __nv_bfloat16 *p = (__nv_bfloat16 *)m.out + at;
+            if (n == 32 && ((uintptr_t)p & 15) == 0) {
+#pragma unroll
+                for (int k = 0; k < 32; k += 8) {
+                    Elems<__nv_bfloat16, 8> e;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) e.v[i] = __float2bfloat16_rn(x[k + i] * UNSCALE);
+                    *reinterpret_cast<Elems<__nv_bfloat16, 8> *>(p + k) = e;
+                }
+            } else
+#pragma unroll
+                for (int k = 0; k < 32; k++)
+                    if (k < n) p[k] = __float2bfloat16_rn(x[k] * UNSCALE);
+        } else {
+            __half *p = (__half *)m.out + at;
+            if (n == 32 && ((uintptr_t)p & 15) == 0) {
+#pragma unroll
+                for (int k = 0; k < 32; k += 8) {
+                    Elems<__half, 8> e;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) e.v[i] = __float2half_rn(x[k + i] * UNSCALE);
+                    *reinterpret_cast<Elems<__half, 8> *>(p + k) = e;
+                }
+            } else
+#pragma unroll
+                for (int k = 0; k < 32; k++)
+                    if (k < n) p[k] = __float2half_rn(x[k] * UNSCALE);
+        }
+        return;
+    }
+    const float keep = (float)(1. - o.lr * (double)m.keep_decay), rate = (float)(-o.lr * (double)m.rate) * UNSCALE;
+    float *p = m.param + at;
+    __nv_bfloat16 *c = m.out ? (__nv_bfloat16 *)m.out + at : nullptr;
+    if (n == 32 && ((uintptr_t)p & 15) == 0 && ((uintptr_t)c & 7) == 0) {
+#pragma unroll
+        for (int k = 0; k < 32; k += 4) {
+            float4 v = *reinterpret_cast<const float4 *>(p + k);
+            v.x = fmaf(rate, x[k], v.x * keep);
+            v.y = fmaf(rate, x[k + 1], v.y * keep);
+            v.z = fmaf(rate, x[k + 2], v.z * keep);
+            v.w = fmaf(rate, x[k + 3], v.w * keep);
+            *reinterpret_cast<float4 *>(p + k) = v;
+            if (c) {
+                const Elems<__nv_bfloat16, 4> e = {__float2bfloat16_rn(v.x), __float2bfloat16_rn(v.y), __float2bfloat16_rn(v.z),
+                                                   __float2bfloat16_rn(v.w)};
+                *reinterpret_cast<Elems<__nv_bfloat16, 4> *>(c + k) = e;
+            }
+        }
+    } else
+#pragma unroll
+        for (int k = 0; k < 32; k++)
+            if (k < n) {
+                const float v = fmaf(rate, x[k], p[k] * keep);
+                p[k] = v;
+                if (c) c[k] = __float2bfloat16_rn(v);
+            }
+}
+
+// One product of all matrices: a persistent kernel whose CTAs (PAIR: pairs of CTAs) take tiles of 128 x 128
+// (256 x 256) elements. Warp 0 loads blocks of 64 x 64 elements, 128 rows of each operand a stage, through a ring of
+// six; one thread of warp 1 (of the pair's first CTA) issues the products into one of two accumulators; eight
+// warps read the other one, 128 rows of the tile in each CTA.
+template <int PHASE, bool PAIR>
+__global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ Job o) {
+    constexpr int SIDES = PAIR ? 4 : 2, COLS = SIDES * SIDE;  // blocks along a tile; columns of an accumulator
+    constexpr bool SYMMETRIC = PHASE == GRAM || PHASE == QUAD;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + STAGES * STAGE_BYTES);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * STAGES + 4);
+    const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES);
+    const uint32_t accf0 = smem_u32(bars + 2 * STAGES), acce0 = smem_u32(bars + 2 * STAGES + 2);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = PAIR ? (int)cluster_rank() : 0;
+    const int first = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x;
+    const int tiles = SYMMETRIC ? o.count_symmetric : o.count_full;
+
+    if (warp == 0 && lane == 0) {
+        for (int s = 0; s < STAGES; s++) {
+            mbar_init(full0 + 8 * s, 1);
+            mbar_init(empty0 + 8 * s, 1);
+        }
+        for (int b = 0; b < 2; b++) {
+            mbar_init(accf0 + 8 * b, 1);
+            mbar_init(acce0 + 8 * b, (PAIR ? 2 : 1) * EPI_WARPS);
+        }
+        mbar_init_fence();
+    }
+    if (warp == 1) {
+        if (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(2 * COLS) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(2 * COLS) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (PAIR) cluster_sync();  // both CTAs' barriers exist before any signal between them
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_wait();
+
+    if (warp == 0 && lane == 0) {
+        // ---- loads: this CTA's 128 rows of the first operand and 128 of the second
+        int it = 0, in_flight = 0;
+        bool ok = true;
+        for (int t = first; t < tiles && ok; t += step) {
+            const Tile tile = tile_of(o, SYMMETRIC, t);
+            const Operands p = operands(matrix_of(o, tile.matrix), PHASE, o.from);
+            const int i0 = tile.i * SIDES + 2 * rank, j0 = tile.j * SIDES + 2 * rank;
+            // blocks that exist, of the tile (whose bytes the barrier expects) and of this CTA
+            const int all = min(SIDES, p.ni - tile.i * SIDES) + min(SIDES, p.nj - tile.j * SIDES);
+            const int na = min(2, p.ni - i0), nb = min(2, p.nj - j0);
+            const int a0 = p.a + i0 * p.ai, b0 = p.b + j0 * p.bj;
+            for (int n = 0, k = 0, term = 0; n < p.nk * p.terms; n++, it++) {
+                const int s = it % STAGES;
+                const int a_at = (a0 + k * p.ak + (term == 1 ? p.a_lo : 0)) * SIDE, b_at = (b0 + k * p.bk + (term == 2 ? p.b_lo : 0)) * SIDE;
+                if (++k == p.nk) k = 0, term++;
+                if (it >= STAGES && !mbar_wait(empty0 + 8 * s, ((uint32_t)(it / STAGES) & 1u) ^ 1u, WAIT_LIMIT)) {
+                    ok = false;
+                    break;
+                }
+                if (it >= STAGES) in_flight = it - STAGES + 1;
+                const uint32_t a_dst = smem_u32(smem + s * STAGE_BYTES), b_dst = a_dst + HALF_BYTES;
+                const uint32_t full = PAIR ? mapa(full0 + 8 * s, 0) : full0 + 8 * s;
+                if (rank == 0) mbar_expect_tx(full0 + 8 * s, all * BLOCK_BYTES);
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    if (PAIR) {
+                        if (h < na) tma_load_2d_pair(a_dst + h * BLOCK_BYTES, &map, full, 0, a_at + h * p.ai * SIDE);
+                        if (h < nb) tma_load_2d_pair(b_dst + h * BLOCK_BYTES, &map, full, 0, b_at + h * p.bj * SIDE);
+                    } else {
+                        if (h < na) tma_load_2d(a_dst + h * BLOCK_BYTES, &map, full, 0, a_at + h * p.ai * SIDE);
+                        if (h < nb) tma_load_2d(b_dst + h * BLOCK_BYTES, &map, full, 0, b_at + h * p.bj * SIDE);
+                    }
+                }
+            }
+        }
+        if (!ok) {
+            atomicExch(&g_error, 1);
+            if (rank == 0)  // copies under way land before the block leaves
+                for (int i = in_flight; i < it; i++) mbar_wait(full0 + 8 * (i % STAGES), (uint32_t)(i / STAGES) & 1u, WAIT_LIMIT);
+        } else  // and so do the last signals that a stage is free
+            for (int i = it > STAGES ? it - STAGES : 0; i < it; i++)
+                mbar_wait(empty0 + 8 * (i % STAGES), (uint32_t)(i / STAGES) & 1u, WAIT_LIMIT);
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+        // ---- products
+        int it = 0, local = 0;
+        bool ok = true;
+        for (int t = first; t < tiles && ok; t += step, local++) {
+            const Tile tile = tile_of(o, SYMMETRIC, t);
+            const Operands p = operands(matrix_of(o, tile.matrix), PHASE, o.from);
+            constexpr uint32_t BASE = (1u << 4) | ((uint32_t)(COLS >> 3) << 17) | ((uint32_t)(COLS >> 4) << 24);  // fp16, fp32 sums
+            const uint32_t idesc = BASE | (p.a_mn ? 1u << 15 : 0u) | (p.b_mn ? 1u << 16 : 0u);
+            const int b = local & 1;
+            const uint32_t acc = tmem + (uint32_t)(b * COLS);
+            if (local >= 2 && !mbar_wait(acce0 + 8 * b, ((uint32_t)(local >> 1) & 1u) ^ 1u, WAIT_LIMIT)) {
+                atomicExch(&g_error, 2);
+                break;
+            }
+            tc_fence_after();
+            for (int k = 0; k < p.nk * p.terms; k++, it++) {
+                const int s = it % STAGES;
+                if (!mbar_wait(full0 + 8 * s, (uint32_t)(it / STAGES) & 1u, WAIT_LIMIT)) {
+                    atomicExch(&g_error, 3);
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t a = smem_u32(smem + s * STAGE_BYTES), c = a + HALF_BYTES;
+#pragma unroll
+                for (int kk = 0; kk < SIDE / 16; kk++) {
+                    const uint64_t da = p.a_mn ? desc_sw128_mn(a + kk * 2048, BLOCK_BYTES) : desc_sw128_k(a + kk * 32);
+                    const uint64_t db = p.b_mn ? desc_sw128_mn(c + kk * 2048, BLOCK_BYTES) : desc_sw128_k(c + kk * 32);
+                    if (PAIR)
+                        mma_pair(acc, da, db, idesc, k || kk);
+                    else
+                        mma_bf16(acc, da, db, idesc, k || kk);
+                }
+                if (PAIR) {
+                    commit_pair(empty0 + 8 * s);
+                    commit_pair(mapa(empty0 + 8 * s, 1));
+                } else
+                    mma_commit(empty0 + 8 * s);
+            }
+            if (!ok) break;
+            if (PAIR) {
+                commit_pair(accf0 + 8 * b);
+                commit_pair(mapa(accf0 + 8 * b, 1));
+            } else
+                mma_commit(accf0 + 8 * b);
+        }
+    } else if (warp >= 2) {
+        // ---- epilogue: warp w holds rows 32 (w % 4) .. + 31 of this CTA's 128, in one half of the columns
+        const int q = warp & 3, half = (warp - 2) >> 2;
+        int local = 0;
+        for (int t = first; t < tiles; t += step, local++) {
+            const Tile tile = tile_of(o, SYMMETRIC, t);
+            const Matrix m = matrix_of(o, tile.matrix);
+            const Operands p = operands(m, PHASE, o.from);
+            const int b = local & 1;
+            if (!mbar_wait(accf0 + 8 * b, (uint32_t)(local >> 1) & 1u, WAIT_LIMIT)) {
+                atomicExch(&g_error, 4);
+                break;
+            }
+            tc_fence_after();
+            const int row = 32 * q + lane, ib = tile.i * SIDES + 2 * rank + (q >> 1), r = row & (SIDE - 1);
+#pragma unroll 1
+            for (int c = 0; c < COLS / 2; c += 32) {
+                const int col = half * (COLS / 2) + c, jb = tile.j * SIDES + col / SIDE, cc = col & (SIDE - 1);
+                if (ib >= p.ni || jb >= p.nj) continue;  // the same for the whole warp
+                uint32_t v[32];
+                D1X_TMEM_LD32(tmem + (uint32_t)(b * COLS + col) + ((uint32_t)(32 * q) << 16), v);
+                tmem_wait_ld();
+                Halves h, l;
+                if constexpr (SYMMETRIC) {
+                    const int64_t at = (int64_t)(ib * m.sb + jb) * BLOCK_BYTES + r * 128 + cc * 2;
+                    uint8_t *const out = o.work + (int64_t)(PHASE == GRAM ? m.gram : m.quad) * BLOCK_BYTES;
+                    float x[32];
+                    if constexpr (PHASE == GRAM) {
+#pragma unroll
+                        for (int k = 0; k < 32; k++) x[k] = __uint_as_float(v[k]) * UNSCALE;
+                    } else {
+                        const uint8_t *const g = o.work + (int64_t)m.gram * BLOCK_BYTES + at;
+                        h = load_row(g);
+#pragma unroll
+                        for (int k = 0; k < 32; k++) x[k] = fmaf(NS_C * UNSCALE, __uint_as_float(v[k]), NS_B * __half2float(h.v[k]));
+                        if (m.fine) {
+                            l = load_row(g + BLOCK_BYTES);
+#pragma unroll
+                            for (int k = 0; k < 32; k++) x[k] = fmaf(NS_B, __half2float(l.v[k]), x[k]);
+                        }
+                    }
+                    split(x, h, l);
+                    store_row(out + at, h);
+                    if (m.fine) store_row(out + BLOCK_BYTES + at, l);  // one block: no mirror
+                    if (tile.i != tile.j) {
+                        __half *mirror = reinterpret_cast<__half *>(out + (int64_t)(jb * m.sb + ib) * BLOCK_BYTES) + cc * SIDE + r;
+#pragma unroll
+                        for (int k = 0; k < 32; k++) mirror[k * SIDE] = h.v[k];
+                    }
+                } else {
+                    const int64_t at = (int64_t)(ib * m.cb + jb) * BLOCK_BYTES + r * 128 + cc * 2;
+                    uint8_t *const lo = o.work + (int64_t)m.lo * BLOCK_BYTES + at;
+                    const Halves xh = load_row(o.work + (int64_t)(o.from ? m.hi[1] : m.hi[0]) * BLOCK_BYTES + at), xl = load_row(lo);
+                    float x[32];
+#pragma unroll
+                    for (int k = 0; k < 32; k++)
+                        x[k] = fmaf(UNSCALE, __uint_as_float(v[k]), NS_A * (__half2float(xh.v[k]) + __half2float(xl.v[k])));
+                    if constexpr (PHASE == APPLY) {
+                        split(x, h, l);
+                        store_row(o.work + (int64_t)(o.from ? m.hi[0] : m.hi[1]) * BLOCK_BYTES + at, h);
+                        store_row(lo, l);
+                    } else {
+                        const int i = ib * SIDE + r, j = jb * SIDE + cc;
+                        if (i < m.rows && j < m.cols) finish(o, m, (int64_t)i * m.cols + j, min(32, m.cols - j), x);
+                    }
+                }
+                __syncwarp();
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if (PAIR)
+                    arrive_cluster(mapa(acce0 + 8 * b, 0));
+                else
+                    mbar_arrive(acce0 + 8 * b);
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (PAIR) cluster_sync();  // no signal between the CTAs is outstanding past this point
+    if (warp == 1) {
+        tc_fence_after();
+        if (PAIR)
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * COLS) : "memory");
+        else
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * COLS) : "memory");
+    }
+}
+
+// ---------------------------------------------------------------- host side
+
+typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                                const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                                CUtensorMapFloatOOBfill);
+
+// The work buffer's blocks as rows of 64 fp16 elements.
+static int make_map(CUtensorMap *map, void *work, int64_t blocks) {
+    static EncodeTiled encode = nullptr;
+    if (!encode) {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q)) return (int)e;
+        if (q != cudaDriverEntryPointSuccess) return (int)cudaErrorNotSupported;
+        encode = reinterpret_cast<EncodeTiled>(p);
+    }
+    const cuuint64_t dims[2] = {SIDE, (cuuint64_t)blocks * SIDE}, strides[1] = {128};
+    const cuuint32_t box[2] = {SIDE, SIDE}, one[2] = {1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, work, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? 0
+               : D1_ERR_BAD_ARGUMENT;
+}
+
+typedef void (*Product)(const CUtensorMap, const Job);
+static Product product_of(int phase, bool pair) {
+    static const Product all[2][4] = {
+        {product_kernel<GRAM, false>, product_kernel<QUAD, false>, product_kernel<APPLY, false>, product_kernel<STEP, false>},
+        {product_kernel<GRAM, true>, product_kernel<QUAD, true>, product_kernel<APPLY, true>, product_kernel<STEP, true>}};
+    return all[pair][phase];
+}
+static int allow_space() {
+    static uint64_t ready = 0;
+    int dev = 0;
+    if (cudaError_t e = cudaGetDevice(&dev)) return (int)e;
+    if (dev < 64 && ((ready >> dev) & 1)) return 0;
+    for (int k = 0; k < 8; k++)
+        if (cudaError_t e = cudaFuncSetAttribute(product_of(k & 3, k >> 2), cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES)) return (int)e;
+    if (dev < 64) ready |= 1ull << dev;
+    return 0;
+}
+
+// Blocks along a tile's side: 256 x 256 tiles of CTA pairs where every pair has one.
+static int side_for(int64_t symmetric_of_pairs) { return symmetric_of_pairs >= SMS / 2 ? 4 : 2; }
+
+static int launch(Job &o, int64_t parts, int64_t blocks, int side, int steps, cudaStream_t s) {
+    if (parts > INT32_MAX) return D1_ERR_TOO_LARGE;
+    CUtensorMap map;
+    if (const int e = make_map(&map, o.work, blocks)) return e;
+    if (const int e = allow_space()) return e;
+    cudaLaunchAttribute attr[2];
+    cudaLaunchConfig_t cfg = pdl_config(dim3((unsigned)parts), dim3(PREP), 0, s, attr);
+    cfg.numAttrs = 0;
+    if (cudaError_t e = cudaLaunchKernelEx(&cfg, prepare_kernel<true>, o)) return (int)e;
+    cfg.numAttrs = 1;
+    if (cudaError_t e = cudaLaunchKernelEx(&cfg, prepare_kernel<false>, o)) return (int)e;
+    const bool pair = side == 4;
+    if (pair) {
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = 2;
+        attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+        cfg.numAttrs = 2;
+    }
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = SMEM_BYTES;
+    for (int k = 0; k < steps; k++, o.from ^= 1)
+        for (int phase = 0; phase < 3; phase++) {
+            const int tiles = phase < 2 ? o.count_symmetric : o.count_full;
+            const int most = pair ? SMS / 2 : SMS, n = tiles < most ? tiles : most;
+            cfg.gridDim = dim3((unsigned)(pair ? 2 * n : n));
+            if (cudaError_t e = cudaLaunchKernelEx(&cfg, product_of(phase == 2 && k == steps - 1 ? STEP : phase, pair), map, o)) return (int)e;
+        }
+    return 0;
+}
+
+}  // namespace muon
+}  // namespace d1
+
+using namespace d1::muon;
+
+// Sizes of a plan, and the plan itself when `out` is not NULL.
+static int plan(const D1MuonTensor *tensors, int n, float *momentum, Plan &head, uint8_t *out) {
+    if (!tensors || n < 1) return D1_ERR_BAD_ARGUMENT;
+    head = Plan{};
+    for (int pass = 0; pass < 2; pass++) {  // sizes, then (with the tile's side known) the number of tiles
+        int64_t block = 0, part = 0;
+        head.matrices = head.symmetric = head.full = 0;
+        for (int t = 0; t < n; t++) {
+            const D1MuonTensor &d = tensors[t];
+            const int64_t need = blocks_needed(d.rows, d.cols);
+            if (need < 0 || d.count < 0 || d.count > MOST_BLOCKS) return D1_ERR_BAD_ARGUMENT;
+            if (need * d.count + block > MOST_BLOCKS) return D1_ERR_TOO_LARGE;
+            for (int64_t k = 0; k < d.count; k++) {
+                Matrix m;
+                place(m, d.rows, d.cols, block, part);
+                head.matrices++;
+                head.symmetric += symmetric_tiles(m, pass ? head.side : 4);
+                head.full += full_tiles(m, pass ? head.side : 4);
+            }
+        }
+        head.parts = part;
+        head.blocks = block;
+        if (!pass) head.side = side_for(head.symmetric);
+    }
+    if (!head.matrices) return D1_ERR_BAD_ARGUMENT;
+    if (head.symmetric > INT32_MAX || head.full > INT32_MAX || head.parts > INT32_MAX) return D1_ERR_TOO_LARGE;
+    head.at_matrices = (sizeof(Plan) + 15) / 16 * 16;
+    head.at_parts = head.at_matrices + head.matrices * (int64_t)sizeof(Matrix);
+    head.at_symmetric = head.at_parts + head.parts * (int64_t)sizeof(Part);
+    head.at_full = head.at_symmetric + head.symmetric * (int64_t)sizeof(Tile);
+    head.bytes = head.at_full + head.full * (int64_t)sizeof(Tile);
+    if (!out) return 0;
+    *(Plan *)out = head;
+    Matrix *const matrices = (Matrix *)(out + head.at_matrices);
+    Part *parts = (Part *)(out + head.at_parts);
+    int64_t block = 0, part = 0, momentum_at = 0;
+    int k = 0;
+    for (int t = 0; t < n; t++) {
+        const D1MuonTensor &d = tensors[t];
+        const int64_t size = d.rows * d.cols, grad_size = d.grad_type == D1_TYPE_F32 ? 4 : 2;
+        for (int64_t c = 0; c < d.count; c++, k++) {
+            Matrix m{};
+            place(m, d.rows, d.cols, block, part);
+            m.param = d.param + c * size;
+            m.grad = (const char *)d.grad + c * size * grad_size;
+            m.out = d.copy ? (char *)d.copy + c * size * 2 : nullptr;
+            m.momentum = momentum + momentum_at + c * size;
+            m.pitch = d.cols;
+            m.grad_type = d.grad_type;
+            m.out_type = D1_TYPE_BF16;
+            m.rate = (float)(0.2 * sqrt((double)(d.rows > d.cols ? d.rows : d.cols)));
+            m.keep_decay = (float)d.decay;
+            matrices[k] = m;
+            for (int p = 0; p < m.parts; p++) *parts++ = Part{k, p};
+        }
+        momentum_at += (size * d.count + 127) / 128 * 128;
+    }
+    // the longest sums first, so that the last tiles to be taken are short ones
+    int *const order = new (std::nothrow) int[head.matrices];
+    if (!order) return D1_ERR_TOO_LARGE;
+    for (int i = 0; i < k; i++) order[i] = i;
+    const auto list = [&](Tile *to, bool symmetric) {
+        std::stable_sort(order, order + k, [&](int a, int b) {
+            const auto depth = [&](const Matrix &m) { return symmetric ? (m.tall ? m.rb : m.cb) : m.sb; };
+            return depth(matrices[a]) > depth(matrices[b]);
+        });
+        for (int q = 0; q < k; q++) {
+            const Matrix &m = matrices[order[q]];
+            const int64_t count = symmetric ? symmetric_tiles(m, head.side) : full_tiles(m, head.side);
+            for (int64_t t = 0; t < count; t++) {
+                int i, j;
+                if (symmetric)
+                    symmetric_tile(t, i, j);
+                else
+                    grouped_tile(t, tiles_of(m.rb, head.side), tiles_of(m.cb, head.side), i, j);
+                *to++ = Tile{order[q], (uint16_t)i, (uint16_t)j};
+            }
+        }
+    };
+    list((Tile *)(out + head.at_symmetric), true);
+    list((Tile *)(out + head.at_full), false);
+    delete[] order;
+    return 0;
+}
+
+static int64_t bytes_of(int64_t blocks, int64_t parts) { return work_blocks_bytes(blocks) + parts * 8; }
+
+extern "C" int64_t d1_muon_plan_bytes(const D1MuonTensor *tensors, int ntensors) {
+    Plan head;
+    return plan(tensors, ntensors, nullptr, head, nullptr) ? -1 : head.bytes;
+}
+extern "C" int64_t d1_muon_work_bytes(const D1MuonTensor *tensors, int ntensors) {
+    Plan head;
+    return plan(tensors, ntensors, nullptr, head, nullptr) ? -1 : bytes_of(head.blocks, head.parts);
+}
+
+extern "C" int d1_muon_plan(const D1MuonTensor *tensors, int ntensors, float *momentum, void *host_plan, int64_t bytes) {
+    Plan head;
+    if (const int e = plan(tensors, ntensors, momentum, head, nullptr)) return e;
+    if (!momentum || !host_plan || bytes < head.bytes || !d1::aligned_to(8, host_plan) || !d1::aligned_to(16, momentum)) return D1_ERR_BAD_ARGUMENT;
+    for (int i = 0; i < ntensors; i++) {
+        const D1MuonTensor &t = tensors[i];
+        if (t.count && (!t.param || !t.grad || (t.grad_type != D1_TYPE_F32 && t.grad_type != D1_TYPE_BF16) || !(t.decay == t.decay) ||
+                        !d1::aligned_to(4, t.param) || !d1::element_aligned(t.grad, t.grad_type) || !d1::aligned_to(2, t.copy)))
+            return D1_ERR_BAD_ARGUMENT;
+    }
+    return plan(tensors, ntensors, momentum, head, (uint8_t *)host_plan);
+}
+
+extern "C" int d1_muon(const void *host_plan, const void *device_plan, double lr, double momentum, int nesterov, int steps, void *work,
+                       void *stream) {
+    if (!host_plan || !device_plan || !work || steps < 1 || steps > 64 || !(momentum >= 0. && momentum < 1.) || !(lr == lr) ||
+        !d1::aligned_to(8, host_plan, device_plan) || !d1::aligned_to(128, work))
+        return D1_ERR_BAD_ARGUMENT;
+    const Plan &head = *(const Plan *)host_plan;
+    const uint8_t *const at = (const uint8_t *)device_plan;
+    Job o{};
+    o.matrices = (const Matrix *)(at + head.at_matrices);
+    o.parts = (const Part *)(at + head.at_parts);
+    o.symmetric = (const Tile *)(at + head.at_symmetric);
+    o.full = (const Tile *)(at + head.at_full);
+    o.count_symmetric = (int)head.symmetric, o.count_full = (int)head.full;
+    o.work = (uint8_t *)work;
+    o.partials = (double *)(o.work + work_blocks_bytes(head.blocks));
+    o.mu = (float)momentum, o.nesterov = nesterov != 0, o.lr = lr;
+    return launch(o, head.parts, head.blocks, head.side, steps, (cudaStream_t)stream);
+}
+
+// The stack's one matrix, its blocks and parts; false when it is out of range.
+static bool stack(int64_t count, int64_t rows, int64_t cols, Matrix &m, int64_t &blocks, int64_t &parts) {
+    const int64_t need = blocks_needed(rows, cols);
+    if (need < 0 || count < 0 || count > MOST_BLOCKS || need * count > MOST_BLOCKS) return false;
+    m = Matrix{};
+    blocks = parts = 0;
+    place(m, rows, cols, blocks, parts);
+    return true;
+}
+
+extern "C" int64_t d1_orthogonalize_work_bytes(int64_t count, int64_t rows, int64_t cols) {
+    Matrix m;
+    int64_t blocks, parts;
+    return stack(count, rows, cols, m, blocks, parts) ? bytes_of(count * blocks, count * parts) : -1;
+}
+
+extern "C" int d1_orthogonalize(const void *x, int64_t ldx, int64_t x_step, int type, int64_t count, int64_t rows, int64_t cols, void *y, int y_type,
+                                int steps, void *work, void *stream) {
+    Matrix m;
+    int64_t blocks, parts;
+    if (!d1::type_ok(type) || (y_type != D1_TYPE_BF16 && y_type != D1_TYPE_F16) || !stack(count, rows, cols, m, blocks, parts) || steps < 1 ||
+        steps > 64 || (count && (!x || !y || !work)) || ldx < 0 || x_step < 0 || ldx > ((int64_t)1 << 42) || x_step > ((int64_t)1 << 42) ||
+        !d1::element_aligned(x, type) || !d1::aligned_to(2, y) || !d1::aligned_to(128, work))
+        return D1_ERR_BAD_ARGUMENT;
+    if (count == 0) return 0;
+    const int64_t size = type == D1_TYPE_F32 ? 4 : 2;
+    // the result shares no memory with the range of x
+    const uintptr_t a = (uintptr_t)x, b = (uintptr_t)y;
+    if (a < b + (uintptr_t)(count * rows * cols * 2) && b < a + (uintptr_t)(((count - 1) * x_step + (rows - 1) * ldx + cols) * size))
+        return D1_ERR_BAD_ARGUMENT;
+    m.grad = x, m.grad_type = type, m.pitch = ldx;
+    m.out = y, m.out_type = y_type;
+    Job o{};
+    o.one = m;
+    o.grad_step = x_step * size, o.out_step = rows * cols * 2;
+    o.block_step = (int)blocks;
+    const int side = side_for(count * symmetric_tiles(m, 4));
+    const int64_t symmetric = symmetric_tiles(m, side), full = full_tiles(m, side);
+    if (symmetric * count > INT32_MAX || full * count > INT32_MAX) return D1_ERR_TOO_LARGE;
+    o.per_symmetric = (int)symmetric, o.per_full = (int)full;
+    o.count_symmetric = (int)(symmetric * count), o.count_full = (int)(full * count);
+    o.tm = tiles_of(m.rb, side), o.tn = tiles_of(m.cb, side);
+    o.work = (uint8_t *)work;
+    o.partials = (double *)(o.work + work_blocks_bytes(count * blocks));
+    return launch(o, count * parts, count * blocks, side, steps, (cudaStream_t)stream);
+}
+
+// Last error recorded by a wait that ran out (0 = none); clears it.
+extern "C" int d1_muon_error(void) {
+    int h = 0, z = 0;
+    if (cudaMemcpyFromSymbol(&h, g_error, sizeof(int)) != cudaSuccess) return -1;
+    if (h) cudaMemcpyToSymbol(g_error, &z, sizeof(int));
+    return h;
+}

@@ -788,6 +788,44 @@ int d1_policy_loss(const float *logp, int64_t ld_logp, const float *old_logp, in
                    double clip_low, double clip_high, double kl_coef, double ent_coef, int by_row, float *loss,
                    float *stats, float *dlogp, float *dentropy, void *work, void *stream);
 
+/* One parameter tensor of d1_muon: `count` matrices of rows x cols (at most 2^21 each)
+ * fp32 elements behind one another at param, their gradients (fp32 or bf16), the bf16
+ * compute copy that each step refreshes (or NULL), decay = the weight decay. param
+ * and copy overlap no other param, copy or gradient. */
+typedef struct {
+    float *param;
+    const void *grad;
+    void *copy;
+    int64_t count, rows, cols;
+    double decay;
+    int grad_type, reserved;
+} D1MuonTensor;
+/* Bytes of the plan and of the work buffer for these tensors (a HOST array); -1 when
+ * they are out of range or hold no matrix. Both are worked out on the host. */
+int64_t d1_muon_plan_bytes(const D1MuonTensor *tensors, int ntensors);
+int64_t d1_muon_work_bytes(const D1MuonTensor *tensors, int ntensors);
+/* Writes the plan to host memory (8-byte aligned); the caller copies it to the
+ * device as it is. momentum: f32, 16-byte aligned, zero at the start, one number for each
+ * element, every tensor's at the next multiple of 128 elements. */
+int d1_muon_plan(const D1MuonTensor *tensors, int ntensors, float *momentum, void *host_plan, int64_t bytes);
+/* One Muon step over the plan's tensors:
+ *   m = momentum * m + grad,   u = grad + momentum * m (nesterov) or m
+ *   X = u / |u|_F, and `steps` (1 to 64) times X = 3.4445 X - 4.7750 (X X^T) X + 2.0315 (X X^T)^2 X
+ *   p = p (1 - lr decay) - lr 0.2 sqrt(max(rows, cols)) X
+ * An update of zeros leaves X zero. Products are fp16 with fp32 sums, X is held
+ * to 22 bits. host_plan and device_plan are the two copies of the plan; work is
+ * 128-byte aligned. Calls that share work or state must not overlap. */
+int d1_muon(const void *host_plan, const void *device_plan, double lr, double momentum, int nesterov, int steps, void *work, void *stream);
+/* The orthogonalisation by itself: y[k] = X after `steps` steps from u = x[k], for
+ * `count` matrices of type `type` with row pitch ldx, x_step elements from one to the
+ * next. y is contiguous, of type y_type (bf16 or fp16), and shares no memory with the
+ * range of x. work: 128-byte aligned, of d1_orthogonalize_work_bytes (-1: out of range). */
+int64_t d1_orthogonalize_work_bytes(int64_t count, int64_t rows, int64_t cols);
+int d1_orthogonalize(const void *x, int64_t ldx, int64_t x_step, int type, int64_t count, int64_t rows, int64_t cols, void *y, int y_type,
+                     int steps, void *work, void *stream);
+/* Last error recorded by a wait of the products that ran out (0: none); clears it. */
+int d1_muon_error(void);
+
 #ifdef __cplusplus
 }
 #endif
