@@ -22,9 +22,9 @@
 // to its (P, Q), a second runs over the chunks, a third walks all of them side
 // by side from their true states. The order of all sums is fixed.
 //
-// 1 - sigmoid(g) is e / (1 + e) with e = e^-|g| or its counterpart, never a
-// difference from 1, and a reset replaces the state (a product with 0 would
-// keep an infinity).
+// A reset replaces the state: a product with 0 would keep an infinity.
+#include <type_traits>
+
 #include "d1_common.cuh"
 #include "d1_elem.cuh"
 #include "d1_pdl.cuh"
@@ -57,44 +57,108 @@ template <class T> struct Args {
     int chunks;
 };
 
-// (a, 1 - a) of the average form.
+// (a, 1 - a) of the average form from E = e^g, as E / (1 + E) and 1 / (1 + E): both are right to a few
+// roundings at every g, neither is a difference from 1. E is capped where 1 / E would vanish (a NaN passes).
 __device__ __forceinline__ float2 gates(float g) {
-    const float e = expf(-fabsf(g)), r = __fdividef(1.f, 1.f + e), s = e * r;
-    return g < 0.f ? make_float2(s, r) : make_float2(r, s);
+    float x = g * 1.4426950408889634f, e, w;
+    asm("min.NaN.f32 %0, %1, 0f42FC0000;" : "=f"(x) : "f"(x));  // 126
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(1.f + e));
+    return make_float2(e * w, w);
 }
 
-template <class T, int V> struct Step {  // one step's operands of V channels
-    Elems<T, V> x, gate, y, dy;
-    bool keep;
+// V elements as they lie in memory: words, so that a step under way takes no more registers than its bytes.
+template <class T, int V> struct Raw {
+    using Word = std::conditional_t<sizeof(T) * V == 2, uint16_t, uint32_t>;
+    static constexpr int N = sizeof(T) * V / sizeof(Word);
+    struct alignas(sizeof(T) * V) Words {
+        Word w[N];
+    } r;
+
+    __device__ __forceinline__ void load(const T *p) { r = *reinterpret_cast<const Words *>(p); }
+    __device__ __forceinline__ float get(int v) const {
+        if constexpr (sizeof(T) == 4)
+            return __uint_as_float(r.w[v]);
+        else if constexpr (std::is_same_v<T, __nv_bfloat16>)
+            return __uint_as_float(V > 1 && v & 1 ? r.w[v / 2] & 0xffff0000u : (uint32_t)r.w[v / 2] << 16);
+        else
+            return __half2float(__ushort_as_half((unsigned short)(V > 1 && v & 1 ? r.w[v / 2] >> 16 : r.w[v / 2])));
+    }
+    static __device__ __forceinline__ void store(T *p, const float (&x)[V]) {
+        Words o;
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int v = 0; v < V; v++) o.w[v] = __float_as_uint(x[v]);
+        } else if constexpr (V == 1) {
+            const T e = from_f32<T>(x[0]);
+            o.w[0] = *reinterpret_cast<const uint16_t *>(&e);
+        } else {
+#pragma unroll
+            for (int v = 0; v < V; v += 2) {
+                if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+                    const __nv_bfloat162 e = __floats2bfloat162_rn(x[v], x[v + 1]);
+                    o.w[v / 2] = *reinterpret_cast<const uint32_t *>(&e);
+                } else {
+                    const __half2 e = __floats2half2_rn(x[v], x[v + 1]);
+                    o.w[v / 2] = *reinterpret_cast<const uint32_t *>(&e);
+                }
+            }
+        }
+        *reinterpret_cast<Words *>(p) = o;
+    }
 };
 
-// PART 0: reduce a chunk; 1: walk it. Loads step t into s.
-template <class T, int V, bool SUM, bool BACK, int PART>
-__device__ __forceinline__ void load(const Args<T> &a, int64_t t, const T *x, const T *gate, const T *y, const T *dy,
-                                     const uint8_t *reset, Step<T, V> &s) {
-    using E = Elems<T, V>;
-    s.gate = *reinterpret_cast<const E *>(gate + t * a.gate.st);
-    if constexpr (!BACK || (PART == 1 && !SUM)) s.x = *reinterpret_cast<const E *>(x + t * a.x.st);
-    if constexpr (BACK) s.dy = *reinterpret_cast<const E *>(dy + t * a.dy.st);
-    if constexpr (BACK && PART == 1)
-        if (t > 0) s.y = *reinterpret_cast<const E *>(y + (t - 1) * a.y.st);
-    s.keep = !reset || !reset[t * a.reset_t];
-}
+template <class T, int V> struct Step {  // one step's operands of V channels
+    Raw<T, V> x, gate, y, dy;
+};
 
+// Where a thread reads and writes: its channels' addresses at its next step, and how far a step moves them.
+template <class T, int V, bool SUM, bool BACK, int PART> struct Walk {
+    const T *x, *gate, *y, *dy;
+    T *out, *dgate;
+    int64_t sx, sgate, sy, sdy, sout;
+
+    __device__ __forceinline__ void load(Step<T, V> &s) {
+        s.gate.load(gate);
+        gate += sgate;
+        if constexpr (!BACK || (PART == 1 && !SUM)) {
+            s.x.load(x);
+            x += sx;
+        }
+        if constexpr (BACK) {
+            s.dy.load(dy);
+            dy += sdy;
+        }
+    }
+    __device__ __forceinline__ void load_before(Step<T, V> &s) {  // y of the step before (backward)
+        s.y.load(y);
+        y += sy;
+    }
+};
+
+// PART 0: reduce a chunk; 1: walk it. A thread has V channels of one sequence in one chunk of the time.
 template <class T, int V, bool SUM, bool BACK, int PART, int U>
-__global__ void __launch_bounds__(THREADS) scan_kernel(Args<T> a) {
+__global__ void __launch_bounds__(THREADS, V == 1 ? (BACK && PART == 1 ? 5 : 6) : BACK && PART == 1 ? 3 : 5) scan_kernel(Args<T> a) {
     pdl_wait();
-    const int64_t lane = (int64_t)blockIdx.x * THREADS + threadIdx.x;
+    const int64_t index = (int64_t)blockIdx.x * THREADS + threadIdx.x;
+    const int order = (int)(index / a.lanes);
+    if (order >= a.chunks) return;
     // the walk goes over the chunks from the side that the reduction read last
-    const int chunk = PART == 1 ? a.chunks - 1 - (int)blockIdx.y : (int)blockIdx.y;
-    if (lane >= a.lanes) return;
-    const int64_t per = a.D / V, b = lane / per, d = (lane - b * per) * V, c = b * a.D + d, C = a.B * a.D;
-    const T *const x = a.x.p + b * a.x.sb + d, *const gate = a.gate.p + b * a.gate.sb + d;
-    const T *const y = BACK ? a.y.p + b * a.y.sb + d : nullptr, *const dy = BACK ? a.dy.p + b * a.dy.sb + d : nullptr;
-    const uint8_t *const reset = a.reset ? a.reset + b * a.reset_b : nullptr;
+    const int chunk = PART == 1 ? a.chunks - 1 - order : order;
+    const int64_t lane = index - order * a.lanes, per = a.D / V, b = lane / per, d = (lane - b * per) * V, c = b * a.D + d, C = a.B * a.D;
     // step i of the chunk in the direction of the recurrence is time first + i or first - i
-    const int64_t from = chunk * a.size, n = min(a.T_ - from, a.size);
-    const int64_t first = BACK ? a.T_ - 1 - from : from;
+    const int64_t from = chunk * a.size, first = BACK ? a.T_ - 1 - from : from;
+    const int n = (int)min(a.T_ - from, a.size);
+    constexpr int SIGN = BACK ? -1 : 1;
+    Walk<T, V, SUM, BACK, PART> w;
+    w.x = a.x.p + first * a.x.st + b * a.x.sb + d, w.sx = SIGN * a.x.st;
+    w.gate = a.gate.p + first * a.gate.st + b * a.gate.sb + d, w.sgate = SIGN * a.gate.st;
+    if constexpr (BACK) {
+        w.dy = a.dy.p + first * a.dy.st + b * a.dy.sb + d, w.sdy = -a.dy.st;
+        w.y = a.y.p + (first - 1) * a.y.st + b * a.y.sb + d, w.sy = -a.y.st;
+        w.dgate = a.dgate + first * C + c;
+    }
+    w.out = a.out + first * C + c, w.sout = SIGN * C;
     float s[V], prod[V];
 #pragma unroll
     for (int v = 0; v < V; v++) {
@@ -102,53 +166,106 @@ __global__ void __launch_bounds__(THREADS) scan_kernel(Args<T> a) {
         s[v] = 0.f;
         if constexpr (PART == 1) s[v] = chunk ? a.carry[chunk * C + c + v].x : a.start ? a.start[c + v] : 0.f;
     }
-    Step<T, V> now[U], next[U];
-    const auto at = [&](int64_t i) { return BACK ? first - i : first + i; };
-    const auto fetch = [&](int64_t i, Step<T, V>(&to)[U]) {
-#pragma unroll
-        for (int u = 0; u < U; u++)
-            if (i + u < n) load<T, V, SUM, BACK, PART>(a, at(i + u), x, gate, y, dy, reset, to[u]);
+    // Resets: where a warp has one sequence and one chunk its lanes look at 32 steps at a time.
+    const bool shared = a.reset && a.lanes % 32 == 0 && per % 32 == 0;
+    const uint8_t *reset = a.reset ? a.reset + b * a.reset_b + (first + (shared ? SIGN * (int)(threadIdx.x & 31) : 0)) * a.reset_t : nullptr;
+    const int64_t sreset = SIGN * (shared ? 32 : 1) * a.reset_t;
+    int looked = 0;  // steps whose flags have been asked for
+    uint32_t window = 0;
+    uint8_t ahead = 0;
+    const auto look = [&] {
+        ahead = looked + (int)(threadIdx.x & 31) < n ? *reset : 0;
+        reset += sreset;
+        looked += 32;
     };
-    fetch(0, now);
-    for (int64_t i = 0; i < n; i += U) {
-        fetch(i + U, next);
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            if (i + u >= n) break;
-            const Step<T, V> &o = now[u];
-            const int64_t t = at(i + u);
-            Elems<T, V> r, dg;
-#pragma unroll
-            for (int v = 0; v < V; v++) {
-                const float g = to_f32(o.gate.v[v]);
-                float2 w;
-                if constexpr (SUM)
-                    w = make_float2(expf(g), 1.f);
-                else
-                    w = gates(g);
-                if constexpr (!BACK) {
-                    const float in = SUM ? to_f32(o.x.v[v]) : w.y * to_f32(o.x.v[v]);
-                    s[v] = o.keep ? fmaf(w.x, s[v], in) : in;
-                    r.v[v] = from_f32<T>(s[v]);
-                } else {
-                    const float D = to_f32(o.dy.v[v]) + s[v];
-                    if constexpr (PART == 1) {
-                        float h = t > 0 ? to_f32(o.y.v[v]) : a.h0 ? a.h0[c + v] : 0.f;
-                        if (!o.keep) h = 0.f;
-                        r.v[v] = from_f32<T>(SUM ? D : D * w.y);
-                        dg.v[v] = from_f32<T>(SUM ? D * h * w.x : D * (h - to_f32(o.x.v[v])) * w.x * w.y);
-                    }
-                    s[v] = o.keep ? w.x * D : 0.f;
-                }
-                if constexpr (PART == 0) prod[v] = !o.keep || prod[v] < 0.f ? CUT : prod[v] * w.x;
+    if (shared) look();
+    const auto cuts_of = [&](int i, int count) -> uint32_t {  // bit u: a reset at step i + u
+        if (!a.reset) return 0;
+        uint32_t bits = 0;
+        if (shared) {
+            if (i % 32 == 0) {
+                window = __ballot_sync(0xffffffffu, ahead);
+                if (looked < n) look();
             }
-            if constexpr (PART == 1) {
-                *reinterpret_cast<Elems<T, V> *>(a.out + t * C + c) = r;
-                if constexpr (BACK) *reinterpret_cast<Elems<T, V> *>(a.dgate + t * C + c) = dg;
-            }
+            return window >> (i % 32);
         }
 #pragma unroll
-        for (int u = 0; u < U; u++) now[u] = next[u];
+        for (int u = 0; u < U; u++)
+            if (u < count) {
+                bits |= *reset ? 1u << u : 0u;
+                reset += sreset;
+            }
+        return bits;
+    };
+    const auto advance = [&](const Step<T, V> &o, bool cut, bool earliest) {
+        float r[V], dg[V];
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+            const float g = o.gate.get(v);
+            float2 f;
+            if constexpr (SUM)
+                f = make_float2(expf(g), 1.f);
+            else
+                f = gates(g);
+            if constexpr (!BACK) {
+                const float in = SUM ? o.x.get(v) : f.y * o.x.get(v);
+                s[v] = cut ? in : fmaf(f.x, s[v], in);
+                r[v] = s[v];
+            } else {
+                const float D = o.dy.get(v) + s[v];
+                if constexpr (PART == 1) {
+                    float h = earliest ? (a.h0 ? a.h0[c + v] : 0.f) : o.y.get(v);
+                    if (cut) h = 0.f;
+                    const float into = SUM ? D : D * f.y;
+                    r[v] = into;
+                    dg[v] = SUM ? into * h * f.x : into * (h - o.x.get(v)) * f.x;
+                }
+                s[v] = cut ? 0.f : f.x * D;
+            }
+            if constexpr (PART == 0) prod[v] = cut || prod[v] < 0.f ? CUT : prod[v] * f.x;
+        }
+        if constexpr (PART == 1) {
+            Raw<T, V>::store(w.out, r);
+            w.out += w.sout;
+            if constexpr (BACK) {
+                Raw<T, V>::store(w.dgate, dg);
+                w.dgate += w.sout;
+            }
+        }
+    };
+    // Groups of U steps, the next one's loads under way during a group's arithmetic. The earliest step of the
+    // time has no y before it: backward it is left to the single steps that follow.
+    constexpr bool BEFORE = BACK && PART == 1;
+    const int groups = (n - (BEFORE && first - (n - 1) == 0 ? 1 : 0)) / U;
+    Step<T, V> p[U], q[U];
+    uint32_t cp, cq;
+    const auto fetch = [&](Step<T, V>(&to)[U], int group) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            w.load(to[u]);
+            if constexpr (BEFORE) w.load_before(to[u]);
+        }
+        return cuts_of(group * U, U);
+    };
+    const auto compute = [&](const Step<T, V>(&of)[U], uint32_t cuts) {
+#pragma unroll
+        for (int u = 0; u < U; u++) advance(of[u], cuts >> u & 1, false);
+    };
+    if (groups) cp = fetch(p, 0);
+    for (int k = 0; k < groups; k += 2) {
+        if (k + 1 < groups) cq = fetch(q, k + 1);
+        compute(p, cp);
+        if (k + 1 < groups) {
+            if (k + 2 < groups) cp = fetch(p, k + 2);
+            compute(q, cq);
+        }
+    }
+#pragma unroll 1
+    for (int i = groups * U; i < n; i++) {
+        w.load(p[0]);
+        const bool earliest = BEFORE && i == n - 1 && first == n - 1;
+        if (BEFORE && !earliest) w.load_before(p[0]);
+        advance(p[0], cuts_of(i, 1) & 1, earliest);
     }
 #pragma unroll
     for (int v = 0; v < V; v++) {
@@ -190,22 +307,22 @@ __global__ void __launch_bounds__(32 * CARRY_WARPS) carry_kernel(float2 *carry, 
     }
 }
 
-// Chunks that the time is cut into: 1 where a thread for each channel is enough.
+// Chunks that the time is cut into: 1 where the channels alone give an SM some hundred threads of four.
 // By the number of channels alone, whatever the vectors' width is.
 static int chunks_of(int64_t T, int64_t C) {
-    const int64_t want = (int64_t)SMS * 2048 / (C < 1 ? 1 : C), most = (T + 31) / 32;
+    const int64_t want = (int64_t)SMS * 4096 / (C < 1 ? 1 : C), most = (T + 31) / 32;
     int64_t n = want < 4 ? 1 : want < most ? want : most;
-    if (n > 4096) n = 4096;
+    if (n > 2048) n = 2048;
     return (int)(n < 1 ? 1 : n);
 }
 
 template <class T, int V, bool SUM, bool BACK> static int run(Args<T> &a, cudaStream_t s) {
-    constexpr int U = V * sizeof(T) >= 8 ? 4 : 8;
+    constexpr int U = 4;
     a.lanes = a.B * a.D / V;
-    const int64_t blocks = (a.lanes + THREADS - 1) / THREADS;
+    const int64_t blocks = (a.lanes * a.chunks + THREADS - 1) / THREADS;
     if (blocks > INT32_MAX) return D1_ERR_TOO_LARGE;
     cudaLaunchAttribute attr;
-    cudaLaunchConfig_t cfg = pdl_config(dim3((unsigned)blocks, (unsigned)a.chunks), dim3(THREADS), 0, s, &attr);
+    cudaLaunchConfig_t cfg = pdl_config(dim3((unsigned)blocks), dim3(THREADS), 0, s, &attr);
     cfg.numAttrs = 0;
     if (a.chunks > 1) {
         if (cudaError_t e = cudaLaunchKernelEx(&cfg, scan_kernel<T, V, SUM, BACK, 0, U>, a)) return (int)e;
@@ -219,20 +336,22 @@ template <class T, int V, bool SUM, bool BACK> static int run(Args<T> &a, cudaSt
     return (int)cudaLaunchKernelEx(&cfg, scan_kernel<T, V, SUM, BACK, 1, U>, a);
 }
 
-template <class T> static bool pairs(const Span<const T> &s) {
-    return aligned_to(2 * sizeof(T), s.p) && s.st % 2 == 0 && s.sb % 2 == 0;
+template <class T> static bool vectors(const Span<const T> &s) {
+    return aligned_to(8, s.p) && s.st % (8 / (int)sizeof(T)) == 0 && s.sb % (8 / (int)sizeof(T)) == 0;
 }
 
 template <class T, bool BACK> static int any(Args<T> a, int form, void *work, cudaStream_t s) {
+    constexpr int V = 8 / sizeof(T);
     a.chunks = chunks_of(a.T_, a.B * a.D);
     a.size = (a.T_ + a.chunks - 1) / a.chunks;
     a.chunks = (int)((a.T_ + a.size - 1) / a.size);
+    if (a.size > INT32_MAX) return D1_ERR_TOO_LARGE;
     a.carry = (float2 *)work;
     if (a.chunks > 1 && (!work || !aligned_to(8, work))) return D1_ERR_BAD_ARGUMENT;
-    const bool two = a.D % 2 == 0 && pairs(a.gate) && pairs(a.x) && aligned_to(2 * sizeof(T), a.out) &&
-                     (!BACK || (pairs(a.dy) && pairs(a.y) && aligned_to(2 * sizeof(T), a.dgate)));
-    if (form == D1_SCAN_SUM) return two ? run<T, 2, true, BACK>(a, s) : run<T, 1, true, BACK>(a, s);
-    return two ? run<T, 2, false, BACK>(a, s) : run<T, 1, false, BACK>(a, s);
+    const bool wide = a.D % V == 0 && vectors(a.gate) && vectors(a.x) && aligned_to(8, a.out) &&
+                      (!BACK || (vectors(a.dy) && vectors(a.y) && aligned_to(8, a.dgate)));
+    if (form == D1_SCAN_SUM) return wide ? run<T, V, true, BACK>(a, s) : run<T, 1, true, BACK>(a, s);
+    return wide ? run<T, V, false, BACK>(a, s) : run<T, 1, false, BACK>(a, s);
 }
 
 // Whether sizes and strides are in range: D, B, T >= 0 and all offsets within 62 bits.
