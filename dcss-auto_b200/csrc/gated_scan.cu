@@ -32,7 +32,8 @@
 namespace d1 {
 namespace gs {
 
-constexpr int SMS = 148, THREADS = 128, CARRY_WARPS = 32;
+constexpr int SMS = 148, THREADS = 128, CARRY_CHANNELS = 8, CARRY_RUNS = 128, CARRY_EACH = 16;
+constexpr int MOST_CHUNKS = CARRY_RUNS * CARRY_EACH;
 // P of a chunk with a reset in it: the state before it does not reach its end (decays
 // are not negative, and one that has underflowed to 0 still lets an infinity through).
 constexpr float CUT = -1.f;
@@ -276,35 +277,45 @@ __global__ void __launch_bounds__(THREADS, V == 1 ? (BACK && PART == 1 ? 5 : 6) 
     }
 }
 
+// The map of one piece and then another.
+__device__ __forceinline__ float2 after(float2 first, float2 then) {
+    return make_float2(first.x < 0.f || then.x < 0.f ? CUT : first.x * then.x, then.x < 0.f ? then.y : fmaf(then.x, first.y, then.y));
+}
 __device__ __forceinline__ float through(float2 map, float s) { return map.x < 0.f ? map.y : fmaf(map.x, s, map.y); }
 
-// The state before every chunk, in place of its (P, Q): a lane for each channel,
-// the chunks divided between the block's warps.
-__global__ void __launch_bounds__(32 * CARRY_WARPS) carry_kernel(float2 *carry, const float *start, int64_t C, int chunks) {
+// The state before every chunk, in place of its (P, Q): eight channels a block, the chunks divided between 128
+// threads for each, which hold theirs and join them by doubling. (A warp for each of 32 runs of chunks, reading
+// them twice, took 26 us for 2,048 chunks of 256 channels: the latency of its loads.)
+__global__ void __launch_bounds__(CARRY_RUNS * CARRY_CHANNELS) carry_kernel(float2 *carry, const float *start, int64_t C, int chunks) {
     pdl_wait();
-    __shared__ float2 sums[CARRY_WARPS][32];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t c = (int64_t)blockIdx.x * 32 + lane;
-    const int each = (chunks + CARRY_WARPS - 1) / CARRY_WARPS, lo = min(chunks, warp * each), hi = min(chunks, lo + each);
-    float p = 1.f, q = 0.f;
-    if (c < C)
-#pragma unroll 8
-        for (int k = lo; k < hi; k++) {
-            const float2 m = carry[k * C + c];
-            q = through(m, q);
-            p = m.x < 0.f || p < 0.f ? CUT : p * m.x;
-        }
-    sums[warp][lane] = make_float2(p, q);
+    __shared__ float2 sums[CARRY_RUNS][CARRY_CHANNELS];
+    const int run = threadIdx.x / CARRY_CHANNELS, lane = threadIdx.x % CARRY_CHANNELS;
+    const int64_t c = (int64_t)blockIdx.x * CARRY_CHANNELS + lane;
+    const int each = (chunks + CARRY_RUNS - 1) / CARRY_RUNS, lo = run * each;
+    float2 m[CARRY_EACH];
+#pragma unroll
+    for (int k = 0; k < CARRY_EACH; k++)
+        m[k] = k < each && lo + k < chunks && c < C ? carry[(lo + k) * C + c] : make_float2(1.f, 0.f);
+    float2 all = m[0];
+#pragma unroll
+    for (int k = 1; k < CARRY_EACH; k++) all = after(all, m[k]);
+    sums[run][lane] = all;
     __syncthreads();
-    if (c >= C) return;
-    float s = start ? start[c] : 0.f;
-    for (int w = 0; w < warp; w++) s = through(sums[w][lane], s);
-#pragma unroll 8
-    for (int k = lo; k < hi; k++) {
-        const float2 m = carry[k * C + c];
-        carry[k * C + c].x = s;
-        s = through(m, s);
+#pragma unroll
+    for (int d = 1; d < CARRY_RUNS; d *= 2) {
+        const float2 before = run >= d ? sums[run - d][lane] : make_float2(1.f, 0.f);
+        __syncthreads();
+        sums[run][lane] = all = after(before, all);
+        __syncthreads();
     }
+    float s = start && c < C ? start[c] : 0.f;
+    if (run) s = through(sums[run - 1][lane], s);
+#pragma unroll
+    for (int k = 0; k < CARRY_EACH; k++)
+        if (k < each && lo + k < chunks && c < C) {
+            carry[(lo + k) * C + c].x = s;
+            s = through(m[k], s);
+        }
 }
 
 // Chunks that the time is cut into: 1 where the channels alone give an SM some hundred threads of four.
@@ -312,7 +323,7 @@ __global__ void __launch_bounds__(32 * CARRY_WARPS) carry_kernel(float2 *carry, 
 static int chunks_of(int64_t T, int64_t C) {
     const int64_t want = (int64_t)SMS * 4096 / (C < 1 ? 1 : C), most = (T + 31) / 32;
     int64_t n = want < 4 ? 1 : want < most ? want : most;
-    if (n > 2048) n = 2048;
+    if (n > MOST_CHUNKS) n = MOST_CHUNKS;
     return (int)(n < 1 ? 1 : n);
 }
 
@@ -329,8 +340,8 @@ template <class T, int V, bool SUM, bool BACK> static int run(Args<T> &a, cudaSt
         cfg.numAttrs = 1;
         cudaLaunchConfig_t mid = cfg;
         const int64_t C = a.B * a.D;
-        mid.gridDim = dim3((unsigned)((C + 31) / 32));
-        mid.blockDim = dim3(32 * CARRY_WARPS);
+        mid.gridDim = dim3((unsigned)((C + CARRY_CHANNELS - 1) / CARRY_CHANNELS));
+        mid.blockDim = dim3(CARRY_RUNS * CARRY_CHANNELS);
         if (cudaError_t e = cudaLaunchKernelEx(&mid, carry_kernel, a.carry, a.start, C, a.chunks)) return (int)e;
     }
     return (int)cudaLaunchKernelEx(&cfg, scan_kernel<T, V, SUM, BACK, 1, U>, a);
