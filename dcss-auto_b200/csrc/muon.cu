@@ -40,8 +40,10 @@ namespace muon {
 
 using namespace tcx;
 
-constexpr int SMS = 148, STAGES = 6, HALF_BYTES = 2 * BLOCK_BYTES, STAGE_BYTES = 2 * HALF_BYTES, EPI_WARPS = 8;
-constexpr int THREADS = 64 + 32 * EPI_WARPS, SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256, PREP = 256;
+constexpr int SMS = 148, STAGES = 5, HALF_BYTES = 2 * BLOCK_BYTES, STAGE_BYTES = 2 * HALF_BYTES, EPI_WARPS = 8;
+constexpr int THREADS = 64 + 32 * EPI_WARPS, PREP = 256;
+constexpr int ROOM = BLOCK_BYTES;  // of an epilogue warp: 32 rows of two blocks
+constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_WARPS * ROOM + 1024 + 256;
 constexpr uint32_t WAIT_LIMIT = 1u << 22;
 constexpr float SCALE = 4096.f, UNSCALE = 1.f / 4096.f;  // of X, A and B in fp16
 constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
@@ -254,103 +256,103 @@ __device__ __forceinline__ void commit_pair(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
-// 32 elements of a block's row in fp16.
-struct alignas(16) Halves {
-    __half v[32];
+// A warp's share of the epilogue: 32 rows of a block of 64 x 64, a row a lane. Operands and results pass through
+// 8 KB of shared memory of the warp's own, by TMA: a lane that reads or writes its row in memory touches a line of its own
+// with each access, which bounded the epilogues (X' of 1024 x 1024 x 1024 at 0.66 PFLOP/s, the step with it at 0.33).
+struct Halves8 {
+    __half2 v[4];
 };
-__device__ __forceinline__ Halves load_row(const uint8_t *p) {
-    Halves r;
+__device__ __forceinline__ void unpack(uint4 w, float (&x)[8]) {
+    const Halves8 h = *reinterpret_cast<const Halves8 *>(&w);
 #pragma unroll
-    for (int k = 0; k < 4; k++) reinterpret_cast<uint4 *>(&r)[k] = reinterpret_cast<const uint4 *>(p)[k];
-    return r;
-}
-__device__ __forceinline__ void store_row(uint8_t *p, const Halves &r) {
-#pragma unroll
-    for (int k = 0; k < 4; k++) reinterpret_cast<uint4 *>(p)[k] = reinterpret_cast<const uint4 *>(&r)[k];
-}
-
-__device__ __forceinline__ void split(const float (&x)[32], Halves &hi, Halves &lo) {
-#pragma unroll
-    for (int k = 0; k < 32; k++) {
-        hi.v[k] = __float2half_rn(x[k]);
-        lo.v[k] = __float2half_rn(x[k] - __half2float(hi.v[k]));
+    for (int k = 0; k < 4; k++) {
+        const float2 f = __half22float2(h.v[k]);
+        x[2 * k] = f.x, x[2 * k + 1] = f.y;
     }
 }
+// x as hi + lo.
+__device__ __forceinline__ void split(const float (&x)[8], uint4 &hi, uint4 &lo) {
+    Halves8 h, l;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        h.v[k] = __floats2half2_rn(x[2 * k], x[2 * k + 1]);
+        const float2 f = __half22float2(h.v[k]);
+        l.v[k] = __floats2half2_rn(x[2 * k] - f.x, x[2 * k + 1] - f.y);
+    }
+    hi = *reinterpret_cast<const uint4 *>(&h);
+    lo = *reinterpret_cast<const uint4 *>(&l);
+}
 
-// The step on 32 elements of a row (n of them exist), or the result itself.
-__device__ __forceinline__ void finish(const Job &o, const Matrix &m, int64_t at, int n, const float (&x)[32]) {
+// The step on 32 rows of 64 columns (or the result itself): x holds a row a lane, memory is touched a row at a time. `room`
+// turns one into the other: row r's 16-byte pieces at piece ^ (r & 15).
+__device__ __forceinline__ void finish(const Job &o, const Matrix &m, int i0, int j0, const float (&x)[64], float *room) {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < 16; k++)
+        *reinterpret_cast<float4 *>(room + lane * 64 + ((k ^ (lane & 15)) * 4)) = make_float4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
+    __syncwarp();
+    const int rows = min(32, m.rows - i0);
+    const auto at = [&](int r, int c) { return room[r * 64 + ((((c >> 2) ^ (r & 15)) << 2) | (c & 3))]; };
+    const int64_t first = (int64_t)i0 * m.cols + j0 + lane;
+    const bool left = j0 + lane < m.cols, right = j0 + lane + 32 < m.cols;
     if (!m.param) {
-        if (m.out_type == D1_TYPE_BF16) {
-            __nv_bfloat16 *p = (__nv_bfloat16 *)m.out + at;
-            if (n == 32 && ((uintptr_t)p & 15) == 0) {
-#pragma unroll
-                for (int k = 0; k < 32; k += 8) {
-                    Elems<__nv_bfloat16, 8> e;
-#pragma unroll
-                    for (int i = 0; i < 8; i++) e.v[i] = __float2bfloat16_rn(x[k + i] * UNSCALE);
-                    *reinterpret_cast<Elems<__nv_bfloat16, 8> *>(p + k) = e;
-                }
-            } else
-#pragma unroll
-                for (int k = 0; k < 32; k++)
-                    if (k < n) p[k] = __float2bfloat16_rn(x[k] * UNSCALE);
-        } else {
-            __half *p = (__half *)m.out + at;
-            if (n == 32 && ((uintptr_t)p & 15) == 0) {
-#pragma unroll
-                for (int k = 0; k < 32; k += 8) {
-                    Elems<__half, 8> e;
-#pragma unroll
-                    for (int i = 0; i < 8; i++) e.v[i] = __float2half_rn(x[k + i] * UNSCALE);
-                    *reinterpret_cast<Elems<__half, 8> *>(p + k) = e;
-                }
-            } else
-#pragma unroll
-                for (int k = 0; k < 32; k++)
-                    if (k < n) p[k] = __float2half_rn(x[k] * UNSCALE);
+#pragma unroll 8
+        for (int r = 0; r < rows; r++) {
+            const int64_t k = first + (int64_t)r * m.cols;
+            const float a = at(r, lane) * UNSCALE, b = at(r, lane + 32) * UNSCALE;
+            if (m.out_type == D1_TYPE_BF16) {
+                if (left) ((__nv_bfloat16 *)m.out)[k] = __float2bfloat16_rn(a);
+                if (right) ((__nv_bfloat16 *)m.out)[k + 32] = __float2bfloat16_rn(b);
+            } else {
+                if (left) ((__half *)m.out)[k] = __float2half_rn(a);
+                if (right) ((__half *)m.out)[k + 32] = __float2half_rn(b);
+            }
         }
-        return;
+    } else {
+        const float keep = (float)(1. - o.lr * (double)m.keep_decay), rate = (float)(-o.lr * (double)m.rate) * UNSCALE;
+        __nv_bfloat16 *const copy = (__nv_bfloat16 *)m.out;
+#pragma unroll 1
+        for (int r0 = 0; r0 < rows; r0 += 8) {
+            float a[8], b[8];
+#pragma unroll
+            for (int r = 0; r < 8; r++) {
+                const int64_t k = first + (int64_t)(r0 + r) * m.cols;
+                if (r0 + r < rows && left) a[r] = m.param[k];
+                if (r0 + r < rows && right) b[r] = m.param[k + 32];
+            }
+#pragma unroll
+            for (int r = 0; r < 8; r++) {
+                const int64_t k = first + (int64_t)(r0 + r) * m.cols;
+                a[r] = fmaf(rate, at(r0 + r, lane), a[r] * keep);
+                b[r] = fmaf(rate, at(r0 + r, lane + 32), b[r] * keep);
+                if (r0 + r < rows && left) {
+                    m.param[k] = a[r];
+                    if (copy) copy[k] = __float2bfloat16_rn(a[r]);
+                }
+                if (r0 + r < rows && right) {
+                    m.param[k + 32] = b[r];
+                    if (copy) copy[k + 32] = __float2bfloat16_rn(b[r]);
+                }
+            }
+        }
     }
-    const float keep = (float)(1. - o.lr * (double)m.keep_decay), rate = (float)(-o.lr * (double)m.rate) * UNSCALE;
-    float *p = m.param + at;
-    __nv_bfloat16 *c = m.out ? (__nv_bfloat16 *)m.out + at : nullptr;
-    if (n == 32 && ((uintptr_t)p & 15) == 0 && ((uintptr_t)c & 7) == 0) {
-#pragma unroll
-        for (int k = 0; k < 32; k += 4) {
-            float4 v = *reinterpret_cast<const float4 *>(p + k);
-            v.x = fmaf(rate, x[k], v.x * keep);
-            v.y = fmaf(rate, x[k + 1], v.y * keep);
-            v.z = fmaf(rate, x[k + 2], v.z * keep);
-            v.w = fmaf(rate, x[k + 3], v.w * keep);
-            *reinterpret_cast<float4 *>(p + k) = v;
-            if (c) {
-                const Elems<__nv_bfloat16, 4> e = {__float2bfloat16_rn(v.x), __float2bfloat16_rn(v.y), __float2bfloat16_rn(v.z),
-                                                   __float2bfloat16_rn(v.w)};
-                *reinterpret_cast<Elems<__nv_bfloat16, 4> *>(c + k) = e;
-            }
-        }
-    } else
-#pragma unroll
-        for (int k = 0; k < 32; k++)
-            if (k < n) {
-                const float v = fmaf(rate, x[k], p[k] * keep);
-                p[k] = v;
-                if (c) c[k] = __float2bfloat16_rn(v);
-            }
+    __syncwarp();
 }
 
 // One product of all matrices: a persistent kernel whose CTAs (PAIR: pairs of CTAs) take tiles of 128 x 128
 // (256 x 256) elements. Warp 0 loads blocks of 64 x 64 elements, 128 rows of each operand a stage, through a ring of
-// six; one thread of warp 1 (of the pair's first CTA) issues the products into one of two accumulators; eight
+// five; one thread of warp 1 (of the pair's first CTA) issues the products into one of two accumulators; eight
 // warps read the other one, 128 rows of the tile in each CTA.
 template <int PHASE, bool PAIR>
-__global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ Job o) {
+__global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ CUtensorMap map_rows,
+                                                              const __grid_constant__ CUtensorMap map_columns, const __grid_constant__ Job o) {
     constexpr int SIDES = PAIR ? 4 : 2, COLS = SIDES * SIDE;  // blocks along a tile; columns of an accumulator
     constexpr bool SYMMETRIC = PHASE == GRAM || PHASE == QUAD;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + STAGES * STAGE_BYTES);
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * STAGES + 4);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + STAGES * STAGE_BYTES + EPI_WARPS * ROOM), *sides = bars + 2 * STAGES + 4;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sides + EPI_WARPS);
     const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES);
     const uint32_t accf0 = smem_u32(bars + 2 * STAGES), acce0 = smem_u32(bars + 2 * STAGES + 2);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -367,6 +369,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
             mbar_init(accf0 + 8 * b, 1);
             mbar_init(acce0 + 8 * b, (PAIR ? 2 : 1) * EPI_WARPS);
         }
+        for (int w = 0; w < EPI_WARPS; w++) mbar_init(smem_u32(sides + w), 1);
         mbar_init_fence();
     }
     if (warp == 1) {
@@ -478,70 +481,138 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
     } else if (warp >= 2) {
         // ---- epilogue: warp w holds rows 32 (w % 4) .. + 31 of this CTA's 128, in one half of the columns
         const int q = warp & 3, half = (warp - 2) >> 2;
+        uint8_t *const room = smem + STAGES * STAGE_BYTES + (warp - 2) * ROOM;
+        const uint32_t room_at = smem_u32(room), side = smem_u32(sides + (warp - 2));
+        constexpr bool SIDE_LO = PHASE != QUAD;  // what comes through the room: hi and lo of X, or A (a pair where it is fine)
+        uint32_t asked = 0, loads = 0;  // loads into the room, and those that have been waited for
         int local = 0;
-        for (int t = first; t < tiles; t += step, local++) {
+        bool ok = true;
+        for (int t = first; t < tiles && ok; t += step, local++) {
             const Tile tile = tile_of(o, SYMMETRIC, t);
             const Matrix m = matrix_of(o, tile.matrix);
             const Operands p = operands(m, PHASE, o.from);
-            const int b = local & 1;
+            const int b = local & 1, ib = tile.i * SIDES + 2 * rank + (q >> 1), r0 = 32 * (q & 1);
+            const int hi_to = o.from ? m.hi[0] : m.hi[1], hi_from = o.from ? m.hi[1] : m.hi[0];
+            const auto block_of = [&](int u) { return ib * (SYMMETRIC ? m.sb : m.cb) + tile.j * SIDES + half * (SIDES / 2) + u; };
+            const auto exists = [&](int u) { return ib < p.ni && tile.j * SIDES + half * (SIDES / 2) + u < p.nj; };
+            const auto fetch = [&](int u) {  // what the epilogue of block u reads
+                if (PHASE == GRAM || !exists(u)) return;
+                asked++;
+                if (lane) return;
+                bulk_wait_read();
+                const bool two = SIDE_LO || m.fine;
+                mbar_expect_tx(side, two ? ROOM : ROOM / 2);
+                const int y = block_of(u) * SIDE + r0;
+                tma_load_2d(room_at, &map_rows, side, 0, (PHASE == QUAD ? m.gram : hi_from) * SIDE + y);
+                if (two) tma_load_2d(room_at + ROOM / 2, &map_rows, side, 0, (PHASE == QUAD ? m.gram + 1 : m.lo) * SIDE + y);
+            };
+            fetch(0);
             if (!mbar_wait(accf0 + 8 * b, (uint32_t)(local >> 1) & 1u, WAIT_LIMIT)) {
                 atomicExch(&g_error, 4);
                 break;
             }
             tc_fence_after();
-            const int row = 32 * q + lane, ib = tile.i * SIDES + 2 * rank + (q >> 1), r = row & (SIDE - 1);
 #pragma unroll 1
-            for (int c = 0; c < COLS / 2; c += 32) {
-                const int col = half * (COLS / 2) + c, jb = tile.j * SIDES + col / SIDE, cc = col & (SIDE - 1);
-                if (ib >= p.ni || jb >= p.nj) continue;  // the same for the whole warp
-                uint32_t v[32];
-                D1X_TMEM_LD32(tmem + (uint32_t)(b * COLS + col) + ((uint32_t)(32 * q) << 16), v);
+            for (int u = 0; u < SIDES / 2; u++) {
+                if (!exists(u)) break;  // the same for the whole warp, and for the blocks after it
+                uint32_t v[64];
+                const uint32_t at = tmem + (uint32_t)(b * COLS + half * (COLS / 2) + u * SIDE) + ((uint32_t)(32 * q) << 16);
+                D1X_TMEM_LD32(at, v);
+                D1X_TMEM_LD32(at + 32, (v + 32));
                 tmem_wait_ld();
-                Halves h, l;
-                if constexpr (SYMMETRIC) {
-                    const int64_t at = (int64_t)(ib * m.sb + jb) * BLOCK_BYTES + r * 128 + cc * 2;
-                    uint8_t *const out = o.work + (int64_t)(PHASE == GRAM ? m.gram : m.quad) * BLOCK_BYTES;
-                    float x[32];
-                    if constexpr (PHASE == GRAM) {
-#pragma unroll
-                        for (int k = 0; k < 32; k++) x[k] = __uint_as_float(v[k]) * UNSCALE;
-                    } else {
-                        const uint8_t *const g = o.work + (int64_t)m.gram * BLOCK_BYTES + at;
-                        h = load_row(g);
-#pragma unroll
-                        for (int k = 0; k < 32; k++) x[k] = fmaf(NS_C * UNSCALE, __uint_as_float(v[k]), NS_B * __half2float(h.v[k]));
-                        if (m.fine) {
-                            l = load_row(g + BLOCK_BYTES);
-#pragma unroll
-                            for (int k = 0; k < 32; k++) x[k] = fmaf(NS_B, __half2float(l.v[k]), x[k]);
-                        }
-                    }
-                    split(x, h, l);
-                    store_row(out + at, h);
-                    if (m.fine) store_row(out + BLOCK_BYTES + at, l);  // one block: no mirror
-                    if (tile.i != tile.j) {
-                        __half *mirror = reinterpret_cast<__half *>(out + (int64_t)(jb * m.sb + ib) * BLOCK_BYTES) + cc * SIDE + r;
-#pragma unroll
-                        for (int k = 0; k < 32; k++) mirror[k * SIDE] = h.v[k];
+                if (PHASE != GRAM) {
+                    if (!mbar_wait(side, loads++ & 1u, WAIT_LIMIT)) {
+                        atomicExch(&g_error, 5);
+                        ok = false;
+                        break;
                     }
                 } else {
-                    const int64_t at = (int64_t)(ib * m.cb + jb) * BLOCK_BYTES + r * 128 + cc * 2;
-                    uint8_t *const lo = o.work + (int64_t)m.lo * BLOCK_BYTES + at;
-                    const Halves xh = load_row(o.work + (int64_t)(o.from ? m.hi[1] : m.hi[0]) * BLOCK_BYTES + at), xl = load_row(lo);
-                    float x[32];
+                    if (lane == 0) bulk_wait_read();
+                    __syncwarp();
+                }
+                const int y = block_of(u) * SIDE + r0;
+                // this lane's row: its 16-byte piece k lies at k ^ (row & 7), as the TMA's swizzle has it
+                uint8_t *const mine = room + lane * 128;
+                const int turn = lane & 7;
+                const auto piece = [&](int k) { return (k ^ turn) << 4; };
+                if constexpr (SYMMETRIC) {
+                    const bool mirrored = tile.i != tile.j;
+                    __half *const across = reinterpret_cast<__half *>(room + ROOM / 2) + lane;
 #pragma unroll
-                    for (int k = 0; k < 32; k++)
-                        x[k] = fmaf(UNSCALE, __uint_as_float(v[k]), NS_A * (__half2float(xh.v[k]) + __half2float(xl.v[k])));
-                    if constexpr (PHASE == APPLY) {
-                        split(x, h, l);
-                        store_row(o.work + (int64_t)(o.from ? m.hi[0] : m.hi[1]) * BLOCK_BYTES + at, h);
-                        store_row(lo, l);
-                    } else {
-                        const int i = ib * SIDE + r, j = jb * SIDE + cc;
-                        if (i < m.rows && j < m.cols) finish(o, m, (int64_t)i * m.cols + j, min(32, m.cols - j), x);
+                    for (int k = 0; k < 8; k++) {
+                        float x[8];
+                        uint4 hi, lo;
+                        if constexpr (PHASE == GRAM) {
+#pragma unroll
+                            for (int e = 0; e < 8; e++) x[e] = __uint_as_float(v[8 * k + e]) * UNSCALE;
+                        } else {
+                            float g[8];
+                            unpack(*reinterpret_cast<const uint4 *>(mine + piece(k)), g);
+#pragma unroll
+                            for (int e = 0; e < 8; e++) x[e] = fmaf(NS_C * UNSCALE, __uint_as_float(v[8 * k + e]), NS_B * g[e]);
+                            if (m.fine) {
+                                unpack(*reinterpret_cast<const uint4 *>(mine + ROOM / 2 + piece(k)), g);
+#pragma unroll
+                                for (int e = 0; e < 8; e++) x[e] = fmaf(NS_B, g[e], x[e]);
+                            }
+                        }
+                        split(x, hi, lo);
+                        *reinterpret_cast<uint4 *>(mine + piece(k)) = hi;
+                        if (m.fine) *reinterpret_cast<uint4 *>(mine + ROOM / 2 + piece(k)) = lo;  // one tile: none is mirrored
+                        if (mirrored) {
+                            const __half *const h = reinterpret_cast<const __half *>(&hi);
+#pragma unroll
+                            for (int e = 0; e < 8; e++) across[(8 * k + e) * 32] = h[e];
+                        }
                     }
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) {
+                        const int to = PHASE == GRAM ? m.gram : m.quad;
+                        tma_store_2d(&map_rows, room_at, 0, to * SIDE + y);
+                        if (m.fine) tma_store_2d(&map_rows, room_at + ROOM / 2, 0, (to + 1) * SIDE + y);
+                        if (mirrored) {
+                            const int jb = tile.j * SIDES + half * (SIDES / 2) + u;
+                            tma_store_2d(&map_columns, room_at + ROOM / 2, r0, (to + jb * m.sb + ib) * SIDE);
+                        }
+                        bulk_commit();
+                    }
+                } else if constexpr (PHASE == APPLY) {
+#pragma unroll
+                    for (int k = 0; k < 8; k++) {
+                        float h[8], l[8], x[8];
+                        unpack(*reinterpret_cast<const uint4 *>(mine + piece(k)), h);
+                        unpack(*reinterpret_cast<const uint4 *>(mine + ROOM / 2 + piece(k)), l);
+#pragma unroll
+                        for (int e = 0; e < 8; e++) x[e] = fmaf(UNSCALE, __uint_as_float(v[8 * k + e]), NS_A * (h[e] + l[e]));
+                        uint4 hi, lo;
+                        split(x, hi, lo);
+                        *reinterpret_cast<uint4 *>(mine + piece(k)) = hi;
+                        *reinterpret_cast<uint4 *>(mine + ROOM / 2 + piece(k)) = lo;
+                    }
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) {
+                        tma_store_2d(&map_rows, room_at, 0, hi_to * SIDE + y);
+                        tma_store_2d(&map_rows, room_at + ROOM / 2, 0, m.lo * SIDE + y);
+                        bulk_commit();
+                    }
+                } else {
+                    float x[64];
+#pragma unroll
+                    for (int k = 0; k < 8; k++) {
+                        float h[8], l[8];
+                        unpack(*reinterpret_cast<const uint4 *>(mine + piece(k)), h);
+                        unpack(*reinterpret_cast<const uint4 *>(mine + ROOM / 2 + piece(k)), l);
+#pragma unroll
+                        for (int e = 0; e < 8; e++) x[8 * k + e] = fmaf(UNSCALE, __uint_as_float(v[8 * k + e]), NS_A * (h[e] + l[e]));
+                    }
+                    const int i0 = ib * SIDE + r0, j0 = (tile.j * SIDES + half * (SIDES / 2) + u) * SIDE;
+                    finish(o, m, i0, j0, x, reinterpret_cast<float *>(room));
+                    fence_proxy_async();  // the next load into the room comes after these reads
                 }
                 __syncwarp();
+                if (u + 1 < SIDES / 2) fetch(u + 1);
             }
             tc_fence_before();
             __syncwarp();
@@ -552,6 +623,8 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
                     mbar_arrive(acce0 + 8 * b);
             }
         }
+        if (asked != loads) mbar_wait(side, loads & 1u, WAIT_LIMIT);  // after an error: a load under way lands before the block leaves
+        if (lane == 0) bulk_wait();
     }
     tc_fence_before();
     __syncthreads();
@@ -571,8 +644,11 @@ typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, 
                                 const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
                                 CUtensorMapFloatOOBfill);
 
-// The work buffer's blocks as rows of 64 fp16 elements.
-static int make_map(CUtensorMap *map, void *work, int64_t blocks) {
+// The work buffer's blocks as rows of 64 fp16 elements: whole blocks, 32 rows of one, 32 columns of one (not swizzled).
+struct Maps {
+    CUtensorMap blocks, rows, columns;
+};
+static int make_maps(Maps &maps, void *work, int64_t blocks) {
     static EncodeTiled encode = nullptr;
     if (!encode) {
         void *p = nullptr;
@@ -582,14 +658,19 @@ static int make_map(CUtensorMap *map, void *work, int64_t blocks) {
         encode = reinterpret_cast<EncodeTiled>(p);
     }
     const cuuint64_t dims[2] = {SIDE, (cuuint64_t)blocks * SIDE}, strides[1] = {128};
-    const cuuint32_t box[2] = {SIDE, SIDE}, one[2] = {1, 1};
-    return encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, work, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+    const cuuint32_t one[2] = {1, 1};
+    const auto make = [&](CUtensorMap *map, cuuint32_t columns, cuuint32_t rows, CUtensorMapSwizzle swizzle) {
+        const cuuint32_t box[2] = {columns, rows};
+        return encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, work, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    };
+    return make(&maps.blocks, SIDE, SIDE, CU_TENSOR_MAP_SWIZZLE_128B) && make(&maps.rows, SIDE, 32, CU_TENSOR_MAP_SWIZZLE_128B) &&
+                   make(&maps.columns, 32, SIDE, CU_TENSOR_MAP_SWIZZLE_NONE)
                ? 0
                : D1_ERR_BAD_ARGUMENT;
 }
 
-typedef void (*Product)(const CUtensorMap, const Job);
+typedef void (*Product)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const Job);
 static Product product_of(int phase, bool pair) {
     static const Product all[2][4] = {
         {product_kernel<GRAM, false>, product_kernel<QUAD, false>, product_kernel<APPLY, false>, product_kernel<STEP, false>},
@@ -612,8 +693,8 @@ static int side_for(int64_t symmetric_of_pairs) { return symmetric_of_pairs >= S
 
 static int launch(Job &o, int64_t parts, int64_t blocks, int side, int steps, cudaStream_t s) {
     if (parts > INT32_MAX) return D1_ERR_TOO_LARGE;
-    CUtensorMap map;
-    if (const int e = make_map(&map, o.work, blocks)) return e;
+    Maps maps;
+    if (const int e = make_maps(maps, o.work, blocks)) return e;
     if (const int e = allow_space()) return e;
     cudaLaunchAttribute attr[2];
     cudaLaunchConfig_t cfg = pdl_config(dim3((unsigned)parts), dim3(PREP), 0, s, attr);
@@ -635,7 +716,8 @@ static int launch(Job &o, int64_t parts, int64_t blocks, int side, int steps, cu
             const int tiles = phase < 2 ? o.count_symmetric : o.count_full;
             const int most = pair ? SMS / 2 : SMS, n = tiles < most ? tiles : most;
             cfg.gridDim = dim3((unsigned)(pair ? 2 * n : n));
-            if (cudaError_t e = cudaLaunchKernelEx(&cfg, product_of(phase == 2 && k == steps - 1 ? STEP : phase, pair), map, o)) return (int)e;
+            if (cudaError_t e = cudaLaunchKernelEx(&cfg, product_of(phase == 2 && k == steps - 1 ? STEP : phase, pair), maps.blocks, maps.rows, maps.columns, o))
+                return (int)e;
         }
     return 0;
 }
