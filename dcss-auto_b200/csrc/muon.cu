@@ -42,8 +42,8 @@ using namespace tcx;
 
 constexpr int SMS = 148, STAGES = 5, HALF_BYTES = 2 * BLOCK_BYTES, STAGE_BYTES = 2 * HALF_BYTES, EPI_WARPS = 8;
 constexpr int THREADS = 64 + 32 * EPI_WARPS, PREP = 256;
-constexpr int ROOM = BLOCK_BYTES;  // of an epilogue warp: 32 rows of two blocks
-constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_WARPS * ROOM + 1024 + 256;
+constexpr int ROOM = BLOCK_BYTES / 2;  // 32 x 32 elements of two operands; an epilogue warp has two
+constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_WARPS * 2 * ROOM + 1024 + 512;
 constexpr uint32_t WAIT_LIMIT = 1u << 22;
 constexpr float SCALE = 4096.f, UNSCALE = 1.f / 4096.f;  // of X, A and B in fp16
 constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
@@ -252,13 +252,16 @@ __device__ __forceinline__ void mma_pair(uint32_t tmem, uint64_t a, uint64_t b, 
         "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+// All but the last committed bulk store have finished reading shared memory.
+__device__ __forceinline__ void bulk_wait_read_but_one() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
 __device__ __forceinline__ void commit_pair(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
-// A warp's share of the epilogue: 32 rows of a block of 64 x 64, a row a lane. Operands and results pass through
-// 8 KB of shared memory of the warp's own, by TMA: a lane that reads or writes its row in memory touches a line of its own
-// with each access, which bounded the epilogues (X' of 1024 x 1024 x 1024 at 0.66 PFLOP/s, the step with it at 0.33).
+// A warp's share of the epilogue is a row of the tile a lane, taken 32 columns at a time. Operands and results pass
+// through shared memory of the warp's own, by TMA, two rooms in turn: a lane that reads or writes its row in memory
+// touches a line of its own with each access, which bounded the epilogues (X' of 1024 x 1024 x 1024 at 0.66 PFLOP/s, the
+// step with it at 0.33).
 struct Halves8 {
     __half2 v[4];
 };
@@ -283,59 +286,49 @@ __device__ __forceinline__ void split(const float (&x)[8], uint4 &hi, uint4 &lo)
     lo = *reinterpret_cast<const uint4 *>(&l);
 }
 
-// The step on 32 rows of 64 columns (or the result itself): x holds a row a lane, memory is touched a row at a time. `room`
-// turns one into the other: row r's 16-byte pieces at piece ^ (r & 15).
-__device__ __forceinline__ void finish(const Job &o, const Matrix &m, int i0, int j0, const float (&x)[64], float *room) {
+// Column j of row i of 32 in a room of 32 fp32 columns: pieces of 16 bytes at piece ^ (row & 7), so that neither rows nor
+// columns meet in a bank.
+__device__ __forceinline__ int place_of(int r, int c) { return r * 32 + ((((c >> 2) ^ (r & 7)) << 2) | (c & 3)); }
+
+// The parameters of 32 rows and this lane's column, asked for ahead of the step on them.
+__device__ __forceinline__ void load_params(const Matrix &m, int i0, int j0, float (&p)[32]) {
+    const int j = j0 + (threadIdx.x & 31), rows = j < m.cols ? min(32, m.rows - i0) : 0;
+    const float *at = m.param + (int64_t)i0 * m.cols + j;
+#pragma unroll
+    for (int r = 0; r < 32; r++, at += m.cols)
+        if (r < rows) p[r] = *at;
+}
+
+// The step on 32 rows of 32 columns (or the result itself): x holds a row a lane, memory is touched a row at a time, the room turns
+// one into the other.
+__device__ __forceinline__ void finish(const Job &o, const Matrix &m, int i0, int j0, const float (&x)[32], const float (&p)[32], float *room) {
     const int lane = threadIdx.x & 31;
     __syncwarp();
 #pragma unroll
-    for (int k = 0; k < 16; k++)
-        *reinterpret_cast<float4 *>(room + lane * 64 + ((k ^ (lane & 15)) * 4)) = make_float4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
+    for (int k = 0; k < 32; k += 4) *reinterpret_cast<float4 *>(room + place_of(lane, k)) = make_float4(x[k], x[k + 1], x[k + 2], x[k + 3]);
     __syncwarp();
-    const int rows = min(32, m.rows - i0);
-    const auto at = [&](int r, int c) { return room[r * 64 + ((((c >> 2) ^ (r & 15)) << 2) | (c & 3))]; };
-    const int64_t first = (int64_t)i0 * m.cols + j0 + lane;
-    const bool left = j0 + lane < m.cols, right = j0 + lane + 32 < m.cols;
+    const int rows = j0 + lane < m.cols ? min(32, m.rows - i0) : 0;
+    int64_t at = (int64_t)i0 * m.cols + j0 + lane;
     if (!m.param) {
-#pragma unroll 8
-        for (int r = 0; r < rows; r++) {
-            const int64_t k = first + (int64_t)r * m.cols;
-            const float a = at(r, lane) * UNSCALE, b = at(r, lane + 32) * UNSCALE;
-            if (m.out_type == D1_TYPE_BF16) {
-                if (left) ((__nv_bfloat16 *)m.out)[k] = __float2bfloat16_rn(a);
-                if (right) ((__nv_bfloat16 *)m.out)[k + 32] = __float2bfloat16_rn(b);
-            } else {
-                if (left) ((__half *)m.out)[k] = __float2half_rn(a);
-                if (right) ((__half *)m.out)[k + 32] = __float2half_rn(b);
+        const bool bf16 = m.out_type == D1_TYPE_BF16;
+#pragma unroll
+        for (int r = 0; r < 32; r++, at += m.cols)
+            if (r < rows) {
+                const float y = room[place_of(r, lane)] * UNSCALE;
+                if (bf16)
+                    ((__nv_bfloat16 *)m.out)[at] = __float2bfloat16_rn(y);
+                else
+                    ((__half *)m.out)[at] = __float2half_rn(y);
             }
-        }
     } else {
         const float keep = (float)(1. - o.lr * (double)m.keep_decay), rate = (float)(-o.lr * (double)m.rate) * UNSCALE;
-        __nv_bfloat16 *const copy = (__nv_bfloat16 *)m.out;
-#pragma unroll 1
-        for (int r0 = 0; r0 < rows; r0 += 8) {
-            float a[8], b[8];
 #pragma unroll
-            for (int r = 0; r < 8; r++) {
-                const int64_t k = first + (int64_t)(r0 + r) * m.cols;
-                if (r0 + r < rows && left) a[r] = m.param[k];
-                if (r0 + r < rows && right) b[r] = m.param[k + 32];
+        for (int r = 0; r < 32; r++, at += m.cols)
+            if (r < rows) {
+                const float y = fmaf(rate, room[place_of(r, lane)], p[r] * keep);
+                m.param[at] = y;
+                if (m.out) ((__nv_bfloat16 *)m.out)[at] = __float2bfloat16_rn(y);
             }
-#pragma unroll
-            for (int r = 0; r < 8; r++) {
-                const int64_t k = first + (int64_t)(r0 + r) * m.cols;
-                a[r] = fmaf(rate, at(r0 + r, lane), a[r] * keep);
-                b[r] = fmaf(rate, at(r0 + r, lane + 32), b[r] * keep);
-                if (r0 + r < rows && left) {
-                    m.param[k] = a[r];
-                    if (copy) copy[k] = __float2bfloat16_rn(a[r]);
-                }
-                if (r0 + r < rows && right) {
-                    m.param[k + 32] = b[r];
-                    if (copy) copy[k + 32] = __float2bfloat16_rn(b[r]);
-                }
-            }
-        }
     }
     __syncwarp();
 }
@@ -345,14 +338,13 @@ __device__ __forceinline__ void finish(const Job &o, const Matrix &m, int i0, in
 // five; one thread of warp 1 (of the pair's first CTA) issues the products into one of two accumulators; eight
 // warps read the other one, 128 rows of the tile in each CTA.
 template <int PHASE, bool PAIR>
-__global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ CUtensorMap map_rows,
-                                                              const __grid_constant__ CUtensorMap map_columns, const __grid_constant__ Job o) {
+__global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ CUtensorMap map_units, const __grid_constant__ Job o) {
     constexpr int SIDES = PAIR ? 4 : 2, COLS = SIDES * SIDE;  // blocks along a tile; columns of an accumulator
     constexpr bool SYMMETRIC = PHASE == GRAM || PHASE == QUAD;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + STAGES * STAGE_BYTES + EPI_WARPS * ROOM), *sides = bars + 2 * STAGES + 4;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sides + EPI_WARPS);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + STAGES * STAGE_BYTES + EPI_WARPS * 2 * ROOM), *sides = bars + 2 * STAGES + 4;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sides + 2 * EPI_WARPS);
     const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES);
     const uint32_t accf0 = smem_u32(bars + 2 * STAGES), acce0 = smem_u32(bars + 2 * STAGES + 2);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -369,7 +361,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
             mbar_init(accf0 + 8 * b, 1);
             mbar_init(acce0 + 8 * b, (PAIR ? 2 : 1) * EPI_WARPS);
         }
-        for (int w = 0; w < EPI_WARPS; w++) mbar_init(smem_u32(sides + w), 1);
+        for (int w = 0; w < 2 * EPI_WARPS; w++) mbar_init(smem_u32(sides + w), 1);
         mbar_init_fence();
     }
     if (warp == 1) {
@@ -386,15 +378,24 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
     if (PAIR) cluster_sync();  // both CTAs' barriers exist before any signal between them
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    pdl_wait();
+    // A plan does not change between the launches of a step (the first of them waits for all that came before), so
+    // that a tile is looked up ahead of pdl_wait(), and the next one during the products of this.
+    if (!o.matrices) pdl_wait();
 
     if (warp == 0 && lane == 0) {
         // ---- loads: this CTA's 128 rows of the first operand and 128 of the second
         int it = 0, in_flight = 0;
         bool ok = true;
+        Tile next = tile_of(o, SYMMETRIC, first);
+        Operands next_p = operands(matrix_of(o, next.matrix), PHASE, o.from);
+        pdl_wait();
         for (int t = first; t < tiles && ok; t += step) {
-            const Tile tile = tile_of(o, SYMMETRIC, t);
-            const Operands p = operands(matrix_of(o, tile.matrix), PHASE, o.from);
+            const Tile tile = next;
+            const Operands p = next_p;
+            if (t + step < tiles) {
+                next = tile_of(o, SYMMETRIC, t + step);
+                next_p = operands(matrix_of(o, next.matrix), PHASE, o.from);
+            }
             const int i0 = tile.i * SIDES + 2 * rank, j0 = tile.j * SIDES + 2 * rank;
             // blocks that exist, of the tile (whose bytes the barrier expects) and of this CTA
             const int all = min(SIDES, p.ni - tile.i * SIDES) + min(SIDES, p.nj - tile.j * SIDES);
@@ -435,9 +436,11 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
         // ---- products
         int it = 0, local = 0;
         bool ok = true;
+        Operands next_p = operands(matrix_of(o, tile_of(o, SYMMETRIC, first).matrix), PHASE, o.from);
+        pdl_wait();
         for (int t = first; t < tiles && ok; t += step, local++) {
-            const Tile tile = tile_of(o, SYMMETRIC, t);
-            const Operands p = operands(matrix_of(o, tile.matrix), PHASE, o.from);
+            const Operands p = next_p;
+            if (t + step < tiles) next_p = operands(matrix_of(o, tile_of(o, SYMMETRIC, t + step).matrix), PHASE, o.from);
             constexpr uint32_t BASE = (1u << 4) | ((uint32_t)(COLS >> 3) << 17) | ((uint32_t)(COLS >> 4) << 24);  // fp16, fp32 sums
             const uint32_t idesc = BASE | (p.a_mn ? 1u << 15 : 0u) | (p.b_mn ? 1u << 16 : 0u);
             const int b = local & 1;
@@ -481,138 +484,153 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
     } else if (warp >= 2) {
         // ---- epilogue: warp w holds rows 32 (w % 4) .. + 31 of this CTA's 128, in one half of the columns
         const int q = warp & 3, half = (warp - 2) >> 2;
-        uint8_t *const room = smem + STAGES * STAGE_BYTES + (warp - 2) * ROOM;
-        const uint32_t room_at = smem_u32(room), side = smem_u32(sides + (warp - 2));
-        constexpr bool SIDE_LO = PHASE != QUAD;  // what comes through the room: hi and lo of X, or A (a pair where it is fine)
-        uint32_t asked = 0, loads = 0;  // loads into the room, and those that have been waited for
+        uint8_t *const rooms = smem + STAGES * STAGE_BYTES + (warp - 2) * 2 * ROOM;
+        const uint32_t rooms_at = smem_u32(rooms), sides0 = smem_u32(sides + 2 * (warp - 2));
+        constexpr int UNITS = COLS / 2 / 32;
+        uint32_t asked = 0, got = 0;  // loads into the rooms, in turn, and those that have been waited for
         int local = 0;
         bool ok = true;
+        Tile next = tile_of(o, SYMMETRIC, first);
+        Matrix next_m = matrix_of(o, next.matrix);
+        pdl_wait();
         for (int t = first; t < tiles && ok; t += step, local++) {
-            const Tile tile = tile_of(o, SYMMETRIC, t);
-            const Matrix m = matrix_of(o, tile.matrix);
+            const Tile tile = next;
+            const Matrix m = next_m;
+            if (t + step < tiles) {
+                next = tile_of(o, SYMMETRIC, t + step);
+                next_m = matrix_of(o, next.matrix);
+            }
             const Operands p = operands(m, PHASE, o.from);
             const int b = local & 1, ib = tile.i * SIDES + 2 * rank + (q >> 1), r0 = 32 * (q & 1);
             const int hi_to = o.from ? m.hi[0] : m.hi[1], hi_from = o.from ? m.hi[1] : m.hi[0];
-            const auto block_of = [&](int u) { return ib * (SYMMETRIC ? m.sb : m.cb) + tile.j * SIDES + half * (SIDES / 2) + u; };
-            const auto exists = [&](int u) { return ib < p.ni && tile.j * SIDES + half * (SIDES / 2) + u < p.nj; };
-            const auto fetch = [&](int u) {  // what the epilogue of block u reads
-                if (PHASE == GRAM || !exists(u)) return;
-                asked++;
+            const int jb0 = tile.j * SIDES + half * (SIDES / 2);
+            // unit u: columns 32 (u & 1) .. + 31 of block (ib, jb0 + u / 2); all warps' lanes agree on how many there are
+            const int units = ib < p.ni ? max(0, min(UNITS, 2 * (p.nj - jb0))) : 0;
+            const auto row_of = [&](int u) { return (ib * (SYMMETRIC ? m.sb : m.cb) + jb0 + u / 2) * SIDE + r0; };
+            const auto fetch = [&](int u) {  // what the epilogue of unit u reads: hi and lo of X, or A (a pair where it is fine)
+                if (PHASE == GRAM || u >= units) return;
+                const uint32_t k = asked++ & 1u;
                 if (lane) return;
-                bulk_wait_read();
-                const bool two = SIDE_LO || m.fine;
-                mbar_expect_tx(side, two ? ROOM : ROOM / 2);
-                const int y = block_of(u) * SIDE + r0;
-                tma_load_2d(room_at, &map_rows, side, 0, (PHASE == QUAD ? m.gram : hi_from) * SIDE + y);
-                if (two) tma_load_2d(room_at + ROOM / 2, &map_rows, side, 0, (PHASE == QUAD ? m.gram + 1 : m.lo) * SIDE + y);
+                const bool two = PHASE != QUAD || m.fine;
+                mbar_expect_tx(sides0 + 8 * k, two ? ROOM : ROOM / 2);
+                const int x = 32 * (u & 1), y = row_of(u);
+                tma_load_2d(rooms_at + k * ROOM, &map_units, sides0 + 8 * k, x, (PHASE == QUAD ? m.gram : hi_from) * SIDE + y);
+                if (two) tma_load_2d(rooms_at + k * ROOM + ROOM / 2, &map_units, sides0 + 8 * k, x, (PHASE == QUAD ? m.gram + 1 : m.lo) * SIDE + y);
             };
+            if (lane == 0) bulk_wait_read();
+            __syncwarp();  // the rooms are free
             fetch(0);
+            fetch(1);
+            if (PHASE == STEP && m.param) {  // the parameters are read after the products: into L2 meanwhile, a row a lane
+                const int i = ib * SIDE + r0 + lane, j0 = jb0 * SIDE;
+#pragma unroll
+                for (int j = 0; j < COLS / 2; j += 32)
+                    if (i < m.rows && j0 + j < m.cols) asm volatile("prefetch.global.L2 [%0];" ::"l"(m.param + (int64_t)i * m.cols + j0 + j));
+            }
             if (!mbar_wait(accf0 + 8 * b, (uint32_t)(local >> 1) & 1u, WAIT_LIMIT)) {
                 atomicExch(&g_error, 4);
                 break;
             }
             tc_fence_after();
 #pragma unroll 1
-            for (int u = 0; u < SIDES / 2; u++) {
-                if (!exists(u)) break;  // the same for the whole warp, and for the blocks after it
-                uint32_t v[64];
-                const uint32_t at = tmem + (uint32_t)(b * COLS + half * (COLS / 2) + u * SIDE) + ((uint32_t)(32 * q) << 16);
-                D1X_TMEM_LD32(at, v);
-                D1X_TMEM_LD32(at + 32, (v + 32));
+            for (int u = 0; u < units; u++) {
+                float params[32];
+                if (PHASE == STEP && m.param) load_params(m, ib * SIDE + r0, jb0 * SIDE + 32 * u, params);
+                uint32_t v[32];
+                D1X_TMEM_LD32(tmem + (uint32_t)(b * COLS + half * (COLS / 2) + 32 * u) + ((uint32_t)(32 * q) << 16), v);
                 tmem_wait_ld();
+                const uint32_t k = PHASE == GRAM ? (uint32_t)u & 1u : got & 1u;
                 if (PHASE != GRAM) {
-                    if (!mbar_wait(side, loads++ & 1u, WAIT_LIMIT)) {
+                    if (!mbar_wait(sides0 + 8 * k, got++ >> 1 & 1u, WAIT_LIMIT)) {
                         atomicExch(&g_error, 5);
                         ok = false;
                         break;
                     }
-                } else {
-                    if (lane == 0) bulk_wait_read();
+                } else if (u > 1) {  // the room's last contents have been taken away
+                    if (lane == 0) bulk_wait_read_but_one();
                     __syncwarp();
                 }
-                const int y = block_of(u) * SIDE + r0;
-                // this lane's row: its 16-byte piece k lies at k ^ (row & 7), as the TMA's swizzle has it
-                uint8_t *const mine = room + lane * 128;
-                const int turn = lane & 7;
-                const auto piece = [&](int k) { return (k ^ turn) << 4; };
+                uint8_t *const room = rooms + k * ROOM;
+                const uint32_t room_at = rooms_at + k * ROOM;
+                const int x0 = 32 * (u & 1), y = row_of(u);
+                // this lane's row of 64 bytes: its piece e lies at e ^ (row / 2 & 3), as the TMA's swizzle has it
+                uint8_t *const mine = room + lane * 64;
+                const auto piece = [&](int e) { return (e ^ (lane >> 1 & 3)) << 4; };
                 if constexpr (SYMMETRIC) {
                     const bool mirrored = tile.i != tile.j;
-                    __half *const across = reinterpret_cast<__half *>(room + ROOM / 2) + lane;
 #pragma unroll
-                    for (int k = 0; k < 8; k++) {
+                    for (int e = 0; e < 4; e++) {
                         float x[8];
                         uint4 hi, lo;
                         if constexpr (PHASE == GRAM) {
 #pragma unroll
-                            for (int e = 0; e < 8; e++) x[e] = __uint_as_float(v[8 * k + e]) * UNSCALE;
+                            for (int i = 0; i < 8; i++) x[i] = __uint_as_float(v[8 * e + i]) * UNSCALE;
                         } else {
                             float g[8];
-                            unpack(*reinterpret_cast<const uint4 *>(mine + piece(k)), g);
+                            unpack(*reinterpret_cast<const uint4 *>(mine + piece(e)), g);
 #pragma unroll
-                            for (int e = 0; e < 8; e++) x[e] = fmaf(NS_C * UNSCALE, __uint_as_float(v[8 * k + e]), NS_B * g[e]);
+                            for (int i = 0; i < 8; i++) x[i] = fmaf(NS_C * UNSCALE, __uint_as_float(v[8 * e + i]), NS_B * g[i]);
                             if (m.fine) {
-                                unpack(*reinterpret_cast<const uint4 *>(mine + ROOM / 2 + piece(k)), g);
+                                unpack(*reinterpret_cast<const uint4 *>(mine + ROOM / 2 + piece(e)), g);
 #pragma unroll
-                                for (int e = 0; e < 8; e++) x[e] = fmaf(NS_B, g[e], x[e]);
+                                for (int i = 0; i < 8; i++) x[i] = fmaf(NS_B, g[i], x[i]);
                             }
                         }
                         split(x, hi, lo);
-                        *reinterpret_cast<uint4 *>(mine + piece(k)) = hi;
-                        if (m.fine) *reinterpret_cast<uint4 *>(mine + ROOM / 2 + piece(k)) = lo;  // one tile: none is mirrored
+                        *reinterpret_cast<uint4 *>(mine + piece(e)) = hi;
+                        if (m.fine) *reinterpret_cast<uint4 *>(mine + ROOM / 2 + piece(e)) = lo;  // one tile: none is mirrored
                         if (mirrored) {
                             const __half *const h = reinterpret_cast<const __half *>(&hi);
 #pragma unroll
-                            for (int e = 0; e < 8; e++) across[(8 * k + e) * 32] = h[e];
+                            for (int i = 0; i < 8; i++) {
+                                const int c = 8 * e + i;
+                                *reinterpret_cast<__half *>(room + ROOM / 2 + c * 64 + (((lane >> 3) ^ (c >> 1 & 3)) << 4) + (lane & 7) * 2) = h[i];
+                            }
                         }
                     }
                     fence_proxy_async();
                     __syncwarp();
                     if (lane == 0) {
                         const int to = PHASE == GRAM ? m.gram : m.quad;
-                        tma_store_2d(&map_rows, room_at, 0, to * SIDE + y);
-                        if (m.fine) tma_store_2d(&map_rows, room_at + ROOM / 2, 0, (to + 1) * SIDE + y);
-                        if (mirrored) {
-                            const int jb = tile.j * SIDES + half * (SIDES / 2) + u;
-                            tma_store_2d(&map_columns, room_at + ROOM / 2, r0, (to + jb * m.sb + ib) * SIDE);
-                        }
-                        bulk_commit();
-                    }
-                } else if constexpr (PHASE == APPLY) {
-#pragma unroll
-                    for (int k = 0; k < 8; k++) {
-                        float h[8], l[8], x[8];
-                        unpack(*reinterpret_cast<const uint4 *>(mine + piece(k)), h);
-                        unpack(*reinterpret_cast<const uint4 *>(mine + ROOM / 2 + piece(k)), l);
-#pragma unroll
-                        for (int e = 0; e < 8; e++) x[e] = fmaf(UNSCALE, __uint_as_float(v[8 * k + e]), NS_A * (h[e] + l[e]));
-                        uint4 hi, lo;
-                        split(x, hi, lo);
-                        *reinterpret_cast<uint4 *>(mine + piece(k)) = hi;
-                        *reinterpret_cast<uint4 *>(mine + ROOM / 2 + piece(k)) = lo;
-                    }
-                    fence_proxy_async();
-                    __syncwarp();
-                    if (lane == 0) {
-                        tma_store_2d(&map_rows, room_at, 0, hi_to * SIDE + y);
-                        tma_store_2d(&map_rows, room_at + ROOM / 2, 0, m.lo * SIDE + y);
+                        tma_store_2d(&map_units, room_at, x0, to * SIDE + y);
+                        if (m.fine) tma_store_2d(&map_units, room_at + ROOM / 2, x0, (to + 1) * SIDE + y);
+                        if (mirrored) tma_store_2d(&map_units, room_at + ROOM / 2, r0, (to + (jb0 + u / 2) * m.sb + ib) * SIDE + x0);
                         bulk_commit();
                     }
                 } else {
-                    float x[64];
+                    float x[32];
 #pragma unroll
-                    for (int k = 0; k < 8; k++) {
+                    for (int e = 0; e < 4; e++) {
                         float h[8], l[8];
-                        unpack(*reinterpret_cast<const uint4 *>(mine + piece(k)), h);
-                        unpack(*reinterpret_cast<const uint4 *>(mine + ROOM / 2 + piece(k)), l);
+                        unpack(*reinterpret_cast<const uint4 *>(mine + piece(e)), h);
+                        unpack(*reinterpret_cast<const uint4 *>(mine + ROOM / 2 + piece(e)), l);
 #pragma unroll
-                        for (int e = 0; e < 8; e++) x[8 * k + e] = fmaf(UNSCALE, __uint_as_float(v[8 * k + e]), NS_A * (h[e] + l[e]));
+                        for (int i = 0; i < 8; i++) x[8 * e + i] = fmaf(UNSCALE, __uint_as_float(v[8 * e + i]), NS_A * (h[i] + l[i]));
+                        if constexpr (PHASE == APPLY) {
+                            uint4 hi, lo;
+                            split(reinterpret_cast<const float(&)[8]>(x[8 * e]), hi, lo);
+                            *reinterpret_cast<uint4 *>(mine + piece(e)) = hi;
+                            *reinterpret_cast<uint4 *>(mine + ROOM / 2 + piece(e)) = lo;
+                        }
                     }
-                    const int i0 = ib * SIDE + r0, j0 = (tile.j * SIDES + half * (SIDES / 2) + u) * SIDE;
-                    finish(o, m, i0, j0, x, reinterpret_cast<float *>(room));
-                    fence_proxy_async();  // the next load into the room comes after these reads
+                    if constexpr (PHASE == APPLY) {
+                        fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) {
+                            tma_store_2d(&map_units, room_at, x0, hi_to * SIDE + y);
+                            tma_store_2d(&map_units, room_at + ROOM / 2, x0, m.lo * SIDE + y);
+                            bulk_commit();
+                        }
+                    } else {
+                        finish(o, m, ib * SIDE + r0, jb0 * SIDE + 32 * u, x, params, reinterpret_cast<float *>(room));
+                        fence_proxy_async();  // the next load into the room comes after these reads
+                    }
                 }
                 __syncwarp();
-                if (u + 1 < SIDES / 2) fetch(u + 1);
+                if (PHASE != GRAM && u + 2 < units) {
+                    if (lane == 0) bulk_wait_read();
+                    fetch(u + 2);
+                }
             }
             tc_fence_before();
             __syncwarp();
@@ -623,7 +641,8 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
                     mbar_arrive(acce0 + 8 * b);
             }
         }
-        if (asked != loads) mbar_wait(side, loads & 1u, WAIT_LIMIT);  // after an error: a load under way lands before the block leaves
+        // after an error: loads under way land before the block leaves
+        for (; got != asked; got++) mbar_wait(sides0 + 8 * (got & 1u), got >> 1 & 1u, WAIT_LIMIT);
         if (lane == 0) bulk_wait();
     }
     tc_fence_before();
@@ -644,9 +663,9 @@ typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, 
                                 const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
                                 CUtensorMapFloatOOBfill);
 
-// The work buffer's blocks as rows of 64 fp16 elements: whole blocks, 32 rows of one, 32 columns of one (not swizzled).
+// The work buffer's blocks as rows of 64 fp16 elements: whole blocks, and 32 x 32 elements of one.
 struct Maps {
-    CUtensorMap blocks, rows, columns;
+    CUtensorMap blocks, units;
 };
 static int make_maps(Maps &maps, void *work, int64_t blocks) {
     static EncodeTiled encode = nullptr;
@@ -664,13 +683,12 @@ static int make_maps(Maps &maps, void *work, int64_t blocks) {
         return encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, work, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
     };
-    return make(&maps.blocks, SIDE, SIDE, CU_TENSOR_MAP_SWIZZLE_128B) && make(&maps.rows, SIDE, 32, CU_TENSOR_MAP_SWIZZLE_128B) &&
-                   make(&maps.columns, 32, SIDE, CU_TENSOR_MAP_SWIZZLE_NONE)
+    return make(&maps.blocks, SIDE, SIDE, CU_TENSOR_MAP_SWIZZLE_128B) && make(&maps.units, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B)
                ? 0
                : D1_ERR_BAD_ARGUMENT;
 }
 
-typedef void (*Product)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const Job);
+typedef void (*Product)(const CUtensorMap, const CUtensorMap, const Job);
 static Product product_of(int phase, bool pair) {
     static const Product all[2][4] = {
         {product_kernel<GRAM, false>, product_kernel<QUAD, false>, product_kernel<APPLY, false>, product_kernel<STEP, false>},
@@ -716,7 +734,7 @@ static int launch(Job &o, int64_t parts, int64_t blocks, int side, int steps, cu
             const int tiles = phase < 2 ? o.count_symmetric : o.count_full;
             const int most = pair ? SMS / 2 : SMS, n = tiles < most ? tiles : most;
             cfg.gridDim = dim3((unsigned)(pair ? 2 * n : n));
-            if (cudaError_t e = cudaLaunchKernelEx(&cfg, product_of(phase == 2 && k == steps - 1 ? STEP : phase, pair), maps.blocks, maps.rows, maps.columns, o))
+            if (cudaError_t e = cudaLaunchKernelEx(&cfg, product_of(phase == 2 && k == steps - 1 ? STEP : phase, pair), maps.blocks, maps.units, o))
                 return (int)e;
         }
     return 0;
