@@ -2,7 +2,7 @@
 // the step, over many weight matrices at a time (sm_100a, tcgen05 + TMA).
 //
 //   m' = mu m + g        u = g + mu m' (Nesterov) or m'
-//   X = u / |u|_F, then `steps` times:  A = X X^T (or X^T X)   B = b A + c A^2   X' = a X + B X (or X B)
+//   X = u / |u|_F, then `steps` times:  A = X X^T (or X^T X)   F = a I + b A + c A^2   X' = F X (or X F)
 //   p' = p (1 - lr decay) - lr 0.2 sqrt(max(rows, cols)) X
 //
 // with the published coefficients (a, b, c) = (3.4445, -4.7750, 2.0315), which bring
@@ -15,11 +15,11 @@
 // rank the result would be noise to a large part (simulated, rank 32 of 512: 3 % of its norm in fp16, 22 %
 // in bf16). So X is held as a pair hi + lo of fp16, 22 bits, and a X is taken from the pair; the products read hi
 // alone, and the error that they make lies in directions that X has (0.06 % there, 0.2 % of a full-rank one). In a
-// matrix with a side of at most 64, where few roundings average out (up to 1 % in some), A and B are pairs too and a product takes all three
+// matrix with a side of at most 64, where few roundings average out (up to 1 % in some), A and F are pairs too and a product takes all three
 // terms: it is as good as one in fp32, and its time is the launches' all the same.
 //
-// The three products of all matrices are one launch each. A and B are symmetric: only the tiles on and below the
-// diagonal are computed, and each is stored a second time transposed. The epilogues hold the rest of the
+// The three products of all matrices are one launch each. A and F are symmetric: only the tiles on and below the
+// diagonal are computed and stored, and read transposed for those above. The epilogues hold the rest of the
 // formulas, the last one the step itself. All operands are blocks of 64 x 64 elements (d1_muon.h) that the TMA
 // swizzles on its way to shared memory, as K-major operands or as MN-major ones: X is never transposed.
 #include <cuda.h>
@@ -45,7 +45,7 @@ constexpr int THREADS = 64 + 32 * EPI_WARPS, PREP = 256;
 constexpr int ROOM = BLOCK_BYTES / 2;  // 32 x 32 elements of two operands; an epilogue warp has two
 constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_WARPS * 2 * ROOM + 1024 + 512;
 constexpr uint32_t WAIT_LIMIT = 1u << 22;
-constexpr float SCALE = 4096.f, UNSCALE = 1.f / 4096.f;  // of X, A and B in fp16
+constexpr float SCALE = 4096.f, UNSCALE = 1.f / 4096.f;  // of X, A and F in fp16
 constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
 
 __device__ int g_error;
@@ -201,24 +201,25 @@ template <bool FIRST> __global__ void __launch_bounds__(PREP) prepare_kernel(Job
 
 // ---------------------------------------------------------------- products
 
-enum Phase { GRAM, QUAD, APPLY, STEP };  // A; B; X'; the step with the last X' (or the result itself)
+enum Phase { GRAM, QUAD, APPLY, STEP };  // A; F; X'; the step with the last X' (or the result itself)
 
 // Where the operands of a phase lie: block (i, k) of the first at a + i * ai + k * ak, of the second at
-// b + j * bj + k * bk; their blocks along i, j and k.
+// b + j * bj + k * bk; their blocks along i, j and k. A symmetric one (A, F) has the tiles on and below its diagonal: where k is
+// past the tile, block (k, i) is taken, as an MN-major operand.
 struct Operands {
     int a, ai, ak, b, bj, bk, ni, nj, nk;
-    bool a_mn, b_mn;
+    bool a_mn, b_mn, a_half, b_half;
     int terms;         // 1; 3 where operands are pairs: hi hi, lo hi, hi lo (lo lo is below fp32's last bit)
     int a_lo, b_lo;    // from a hi block to its lo block
 };
 __device__ __forceinline__ Operands operands(const Matrix &m, int phase, int from) {
     const int hi = from ? m.hi[1] : m.hi[0], x_lo = m.lo - hi, terms = m.fine ? 3 : 1;
     if (phase == GRAM)
-        return m.tall ? Operands{hi, 1, m.cb, hi, 1, m.cb, m.sb, m.sb, m.rb, true, true, terms, x_lo, x_lo}
-                      : Operands{hi, m.cb, 1, hi, m.cb, 1, m.sb, m.sb, m.cb, false, false, terms, x_lo, x_lo};
-    if (phase == QUAD) return Operands{m.gram, m.sb, 1, m.gram, m.sb, 1, m.sb, m.sb, m.sb, false, false, terms, 1, 1};
-    return m.tall ? Operands{hi, m.cb, 1, m.quad, m.sb, 1, m.rb, m.cb, m.sb, false, false, terms, x_lo, 1}
-                  : Operands{m.quad, m.sb, 1, hi, 1, m.cb, m.rb, m.cb, m.sb, false, true, terms, 1, x_lo};
+        return m.tall ? Operands{hi, 1, m.cb, hi, 1, m.cb, m.sb, m.sb, m.rb, true, true, false, false, terms, x_lo, x_lo}
+                      : Operands{hi, m.cb, 1, hi, m.cb, 1, m.sb, m.sb, m.cb, false, false, false, false, terms, x_lo, x_lo};
+    if (phase == QUAD) return Operands{m.gram, m.sb, 1, m.gram, m.sb, 1, m.sb, m.sb, m.sb, false, false, true, true, terms, 1, 1};
+    return m.tall ? Operands{hi, m.cb, 1, m.quad, m.sb, 1, m.rb, m.cb, m.sb, false, false, false, true, terms, x_lo, 1}
+                  : Operands{m.quad, m.sb, 1, hi, 1, m.cb, m.rb, m.cb, m.sb, false, true, true, false, terms, 1, x_lo};
 }
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -400,10 +401,11 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
             // blocks that exist, of the tile (whose bytes the barrier expects) and of this CTA
             const int all = min(SIDES, p.ni - tile.i * SIDES) + min(SIDES, p.nj - tile.j * SIDES);
             const int na = min(2, p.ni - i0), nb = min(2, p.nj - j0);
-            const int a0 = p.a + i0 * p.ai, b0 = p.b + j0 * p.bj;
             for (int n = 0, k = 0, term = 0; n < p.nk * p.terms; n++, it++) {
                 const int s = it % STAGES;
-                const int a_at = (a0 + k * p.ak + (term == 1 ? p.a_lo : 0)) * SIDE, b_at = (b0 + k * p.bk + (term == 2 ? p.b_lo : 0)) * SIDE;
+                const bool a_turned = p.a_half && k / SIDES > tile.i, b_turned = p.b_half && k / SIDES > tile.j;
+                const int ai = a_turned ? p.ak : p.ai, ak = a_turned ? p.ai : p.ak, bj = b_turned ? p.bk : p.bj, bk = b_turned ? p.bj : p.bk;
+                const int a_at = (p.a + i0 * ai + k * ak + (term == 1 ? p.a_lo : 0)) * SIDE, b_at = (p.b + j0 * bj + k * bk + (term == 2 ? p.b_lo : 0)) * SIDE;
                 if (++k == p.nk) k = 0, term++;
                 if (it >= STAGES && !mbar_wait(empty0 + 8 * s, ((uint32_t)(it / STAGES) & 1u) ^ 1u, WAIT_LIMIT)) {
                     ok = false;
@@ -416,11 +418,11 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
                     if (PAIR) {
-                        if (h < na) tma_load_2d_pair(a_dst + h * BLOCK_BYTES, &map, full, 0, a_at + h * p.ai * SIDE);
-                        if (h < nb) tma_load_2d_pair(b_dst + h * BLOCK_BYTES, &map, full, 0, b_at + h * p.bj * SIDE);
+                        if (h < na) tma_load_2d_pair(a_dst + h * BLOCK_BYTES, &map, full, 0, a_at + h * ai * SIDE);
+                        if (h < nb) tma_load_2d_pair(b_dst + h * BLOCK_BYTES, &map, full, 0, b_at + h * bj * SIDE);
                     } else {
-                        if (h < na) tma_load_2d(a_dst + h * BLOCK_BYTES, &map, full, 0, a_at + h * p.ai * SIDE);
-                        if (h < nb) tma_load_2d(b_dst + h * BLOCK_BYTES, &map, full, 0, b_at + h * p.bj * SIDE);
+                        if (h < na) tma_load_2d(a_dst + h * BLOCK_BYTES, &map, full, 0, a_at + h * ai * SIDE);
+                        if (h < nb) tma_load_2d(b_dst + h * BLOCK_BYTES, &map, full, 0, b_at + h * bj * SIDE);
                     }
                 }
             }
@@ -436,13 +438,17 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
         // ---- products
         int it = 0, local = 0;
         bool ok = true;
-        Operands next_p = operands(matrix_of(o, tile_of(o, SYMMETRIC, first).matrix), PHASE, o.from);
+        Tile next = tile_of(o, SYMMETRIC, first);
+        Operands next_p = operands(matrix_of(o, next.matrix), PHASE, o.from);
         pdl_wait();
         for (int t = first; t < tiles && ok; t += step, local++) {
+            const Tile tile = next;
             const Operands p = next_p;
-            if (t + step < tiles) next_p = operands(matrix_of(o, tile_of(o, SYMMETRIC, t + step).matrix), PHASE, o.from);
+            if (t + step < tiles) {
+                next = tile_of(o, SYMMETRIC, t + step);
+                next_p = operands(matrix_of(o, next.matrix), PHASE, o.from);
+            }
             constexpr uint32_t BASE = (1u << 4) | ((uint32_t)(COLS >> 3) << 17) | ((uint32_t)(COLS >> 4) << 24);  // fp16, fp32 sums
-            const uint32_t idesc = BASE | (p.a_mn ? 1u << 15 : 0u) | (p.b_mn ? 1u << 16 : 0u);
             const int b = local & 1;
             const uint32_t acc = tmem + (uint32_t)(b * COLS);
             if (local >= 2 && !mbar_wait(acce0 + 8 * b, ((uint32_t)(local >> 1) & 1u) ^ 1u, WAIT_LIMIT)) {
@@ -459,10 +465,12 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
                 }
                 tc_fence_after();
                 const uint32_t a = smem_u32(smem + s * STAGE_BYTES), c = a + HALF_BYTES;
+                const bool a_mn = p.a_mn || (p.a_half && k / SIDES > tile.i), b_mn = p.b_mn || (p.b_half && k / SIDES > tile.j);
+                const uint32_t idesc = BASE | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
 #pragma unroll
                 for (int kk = 0; kk < SIDE / 16; kk++) {
-                    const uint64_t da = p.a_mn ? desc_sw128_mn(a + kk * 2048, BLOCK_BYTES) : desc_sw128_k(a + kk * 32);
-                    const uint64_t db = p.b_mn ? desc_sw128_mn(c + kk * 2048, BLOCK_BYTES) : desc_sw128_k(c + kk * 32);
+                    const uint64_t da = a_mn ? desc_sw128_mn(a + kk * 2048, BLOCK_BYTES) : desc_sw128_k(a + kk * 32);
+                    const uint64_t db = b_mn ? desc_sw128_mn(c + kk * 2048, BLOCK_BYTES) : desc_sw128_k(c + kk * 32);
                     if (PAIR)
                         mma_pair(acc, da, db, idesc, k || kk);
                     else
@@ -502,20 +510,22 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
             }
             const Operands p = operands(m, PHASE, o.from);
             const int b = local & 1, ib = tile.i * SIDES + 2 * rank + (q >> 1), r0 = 32 * (q & 1);
-            const int hi_to = o.from ? m.hi[0] : m.hi[1], hi_from = o.from ? m.hi[1] : m.hi[0];
+            const int hi_to = o.from ? m.hi[0] : m.hi[1];
             const int jb0 = tile.j * SIDES + half * (SIDES / 2);
             // unit u: columns 32 (u & 1) .. + 31 of block (ib, jb0 + u / 2); all warps' lanes agree on how many there are
             const int units = ib < p.ni ? max(0, min(UNITS, 2 * (p.nj - jb0))) : 0;
             const auto row_of = [&](int u) { return (ib * (SYMMETRIC ? m.sb : m.cb) + jb0 + u / 2) * SIDE + r0; };
-            const auto fetch = [&](int u) {  // what the epilogue of unit u reads: hi and lo of X, or A (a pair where it is fine)
-                if (PHASE == GRAM || u >= units) return;
+            // what the epilogue of a unit reads: A (a pair where it is fine), or lo of X (where it is fine, F lo was a term)
+            const bool reads = PHASE == QUAD || (PHASE != GRAM && !m.fine);
+            const auto fetch = [&](int u) {
+                if (!reads || u >= units) return;
                 const uint32_t k = asked++ & 1u;
                 if (lane) return;
-                const bool two = PHASE != QUAD || m.fine;
-                mbar_expect_tx(sides0 + 8 * k, two ? ROOM : ROOM / 2);
                 const int x = 32 * (u & 1), y = row_of(u);
-                tma_load_2d(rooms_at + k * ROOM, &map_units, sides0 + 8 * k, x, (PHASE == QUAD ? m.gram : hi_from) * SIDE + y);
-                if (two) tma_load_2d(rooms_at + k * ROOM + ROOM / 2, &map_units, sides0 + 8 * k, x, (PHASE == QUAD ? m.gram + 1 : m.lo) * SIDE + y);
+                mbar_expect_tx(sides0 + 8 * k, PHASE == QUAD && m.fine ? ROOM : ROOM / 2);
+                if (PHASE != QUAD || m.fine)
+                    tma_load_2d(rooms_at + k * ROOM + ROOM / 2, &map_units, sides0 + 8 * k, x, (PHASE == QUAD ? m.gram + 1 : m.lo) * SIDE + y);
+                if (PHASE == QUAD) tma_load_2d(rooms_at + k * ROOM, &map_units, sides0 + 8 * k, x, m.gram * SIDE + y);
             };
             if (lane == 0) bulk_wait_read();
             __syncwarp();  // the rooms are free
@@ -539,8 +549,8 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
                 uint32_t v[32];
                 D1X_TMEM_LD32(tmem + (uint32_t)(b * COLS + half * (COLS / 2) + 32 * u) + ((uint32_t)(32 * q) << 16), v);
                 tmem_wait_ld();
-                const uint32_t k = PHASE == GRAM ? (uint32_t)u & 1u : got & 1u;
-                if (PHASE != GRAM) {
+                const uint32_t k = (uint32_t)u & 1u;
+                if (reads) {
                     if (!mbar_wait(sides0 + 8 * k, got++ >> 1 & 1u, WAIT_LIMIT)) {
                         atomicExch(&g_error, 5);
                         ok = false;
@@ -557,7 +567,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
                 uint8_t *const mine = room + lane * 64;
                 const auto piece = [&](int e) { return (e ^ (lane >> 1 & 3)) << 4; };
                 if constexpr (SYMMETRIC) {
-                    const bool mirrored = tile.i != tile.j;
+                    const bool diagonal = PHASE == QUAD && ib == jb0 + u / 2 && r0 == x0;  // column i is this lane's own where i == lane
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         float x[8];
@@ -575,18 +585,13 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
 #pragma unroll
                                 for (int i = 0; i < 8; i++) x[i] = fmaf(NS_B, g[i], x[i]);
                             }
+                            if (diagonal)
+#pragma unroll
+                                for (int i = 0; i < 8; i++) x[i] += 8 * e + i == lane ? NS_A * SCALE : 0.f;
                         }
                         split(x, hi, lo);
                         *reinterpret_cast<uint4 *>(mine + piece(e)) = hi;
-                        if (m.fine) *reinterpret_cast<uint4 *>(mine + ROOM / 2 + piece(e)) = lo;  // one tile: none is mirrored
-                        if (mirrored) {
-                            const __half *const h = reinterpret_cast<const __half *>(&hi);
-#pragma unroll
-                            for (int i = 0; i < 8; i++) {
-                                const int c = 8 * e + i;
-                                *reinterpret_cast<__half *>(room + ROOM / 2 + c * 64 + (((lane >> 3) ^ (c >> 1 & 3)) << 4) + (lane & 7) * 2) = h[i];
-                            }
-                        }
+                        if (m.fine) *reinterpret_cast<uint4 *>(mine + ROOM / 2 + piece(e)) = lo;
                     }
                     fence_proxy_async();
                     __syncwarp();
@@ -594,18 +599,20 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
                         const int to = PHASE == GRAM ? m.gram : m.quad;
                         tma_store_2d(&map_units, room_at, x0, to * SIDE + y);
                         if (m.fine) tma_store_2d(&map_units, room_at + ROOM / 2, x0, (to + 1) * SIDE + y);
-                        if (mirrored) tma_store_2d(&map_units, room_at + ROOM / 2, r0, (to + (jb0 + u / 2) * m.sb + ib) * SIDE + x0);
                         bulk_commit();
                     }
                 } else {
                     float x[32];
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        float h[8], l[8];
-                        unpack(*reinterpret_cast<const uint4 *>(mine + piece(e)), h);
-                        unpack(*reinterpret_cast<const uint4 *>(mine + ROOM / 2 + piece(e)), l);
 #pragma unroll
-                        for (int i = 0; i < 8; i++) x[8 * e + i] = fmaf(UNSCALE, __uint_as_float(v[8 * e + i]), NS_A * (h[i] + l[i]));
+                        for (int i = 0; i < 8; i++) x[8 * e + i] = UNSCALE * __uint_as_float(v[8 * e + i]);
+                        if (reads) {
+                            float l[8];
+                            unpack(*reinterpret_cast<const uint4 *>(mine + ROOM / 2 + piece(e)), l);
+#pragma unroll
+                            for (int i = 0; i < 8; i++) x[8 * e + i] = fmaf(NS_A, l[i], x[8 * e + i]);
+                        }
                         if constexpr (PHASE == APPLY) {
                             uint4 hi, lo;
                             split(reinterpret_cast<const float(&)[8]>(x[8 * e]), hi, lo);
@@ -627,7 +634,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
                     }
                 }
                 __syncwarp();
-                if (PHASE != GRAM && u + 2 < units) {
+                if (reads && u + 2 < units) {
                     if (lane == 0) bulk_wait_read();
                     fetch(u + 2);
                 }
