@@ -7,6 +7,7 @@
 // of r x c elements has ceil(r / 64) x ceil(c / 64) blocks, row of blocks after
 // row of blocks, zero past its edges; products of zeros keep them zero.
 #pragma once
+#include <math.h>
 #include <stdint.h>
 
 #include "../../include/d1.h"
@@ -83,21 +84,22 @@ inline int64_t blocks_needed(int64_t rows, int64_t cols) {
     return 3 * rb * cb + 2 * gram_blocks(sb);
 }
 
-// Tile t of a symmetric matrix of tiles: row i >= column j, row after row.
-D1_MUON_BOTH void symmetric_tile(int64_t t, int &i, int &j) {
-    int64_t r = 0, step = (int64_t)1 << 30;  // the largest r with r (r + 1) / 2 <= t
-    while (step >>= 1)
-        if ((r + step) * (r + step + 1) / 2 <= t) r += step;
-    i = (int)r;
-    j = (int)(t - r * (r + 1) / 2);
+// Tile t of a symmetric matrix of tiles: row i >= column j, row after row. (In 32 bits and from a root, because the kernels
+// do it for every tile: t < 2^31.)
+D1_MUON_BOTH void symmetric_tile(int t, int &i, int &j) {
+    int r = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);  // off by a little where t has more than 24 bits
+    while ((int64_t)r * (r + 1) / 2 > t) r--;
+    while ((int64_t)(r + 1) * (r + 2) / 2 <= t) r++;
+    i = r;
+    j = (int)(t - (int64_t)r * (r + 1) / 2);
 }
 // Tile t of tm x tn: eight rows of tiles at a time, column after column, so that tiles that
 // run together share operands in L2.
-D1_MUON_BOTH void grouped_tile(int64_t t, int tm, int tn, int &i, int &j) {
-    const int64_t per = (int64_t)8 * tn, g = t / per, r = t - g * per;
-    const int64_t high = tm - 8 * g < 8 ? tm - 8 * g : 8;
-    i = (int)(8 * g + r % high);
-    j = (int)(r / high);
+D1_MUON_BOTH void grouped_tile(int t, int tm, int tn, int &i, int &j) {
+    const int per = 8 * tn, g = t / per, r = t - g * per;
+    const int high = tm - 8 * g < 8 ? tm - 8 * g : 8;
+    i = 8 * g + r % high;
+    j = r / high;
 }
 
 D1_MUON_BOTH int64_t symmetric_tiles(const Matrix &m, int side) {
@@ -106,13 +108,50 @@ D1_MUON_BOTH int64_t symmetric_tiles(const Matrix &m, int side) {
 }
 D1_MUON_BOTH int64_t full_tiles(const Matrix &m, int side) { return (int64_t)tiles_of(m.rb, side) * tiles_of(m.cb, side); }
 
+// CTAs that share the sum of `depth` blocks of each of a few tiles: as many as there is room for, while it saves ten
+// blocks' time (the exchange of the parts costs some five).
+inline int parts_for(int64_t tiles, int depth) {
+    int parts = 1;
+    for (int n = 2; n <= 8; n *= 2)
+        if (tiles * n <= (n == 8 ? 112 : n == 4 ? 128 : 148) && depth - depth / n >= 10) parts = n;  // what clusters find room for at once
+    return parts;
+}
+
+// What a step is made of with tiles of `side` blocks, and about how long it takes.
+struct Load {
+    int side;
+    int64_t symmetric, full;  // tiles
+    int depth[2];             // the longest sums, in blocks, of A and of the other products
+    double work[3];           // blocks of all sums, by product
+
+    void add(const Matrix &m, int64_t count) {
+        const int64_t s = symmetric_tiles(m, side) * count, f = full_tiles(m, side) * count;
+        const int terms = m.fine ? 3 : 1, first = (m.tall ? m.rb : m.cb) * terms, others = m.sb * terms;
+        symmetric += s, full += f;
+        work[0] += (double)s * first, work[1] += (double)s * others, work[2] += (double)f * others;
+        if (first > depth[0]) depth[0] = first;
+        if (others > depth[1]) depth[1] = others;
+    }
+    // A block of 64 of the sum takes a pair of CTAs 0.43 us for a tile of 256 x 256, a CTA 0.5 us for one of 128 x 128 (both measured with the
+    // GPU full: the one is bound by shared memory, the other by what comes from L2); a pair's launches take 8 us more in all.
+    double microseconds() const {
+        double sum = side == 4 ? 8. : 0.;
+        for (int k = 0; k < 3; k++) {
+            const int parts = side == 4 ? 1 : parts_for(k < 2 ? symmetric : full, depth[k > 0]);
+            const double even = work[k] / (side == 4 ? 74 : 148), longest = (double)depth[k > 0] / parts;
+            sum += (side == 4 ? 0.43 : 0.5) * (even > longest ? even : longest);
+        }
+        return sum;
+    }
+};
+inline Load load_of(int side) { return Load{side, 0, 0, {0, 0}, {0., 0., 0.}}; }
+
 // What a plan begins with: sizes of its lists and where they start (bytes).
 struct Plan {
-    int64_t bytes, matrices, parts, symmetric, full;
+    int64_t bytes, matrices, parts;
     int64_t at_matrices, at_parts, at_symmetric, at_full;
     int64_t blocks;  // of the work buffer
-    int side;        // blocks along a tile's side: 2 or 4
-    int reserved;
+    Load load;
 };
 
 D1_MUON_BOTH int64_t work_blocks_bytes(int64_t blocks) { return blocks * BLOCK_BYTES; }

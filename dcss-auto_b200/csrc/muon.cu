@@ -90,6 +90,31 @@ __device__ __forceinline__ Tile tile_of(const Job &o, bool symmetric, int t) {
     return r;
 }
 
+// A role's tiles first, first + step, ..., each looked up while the one before it is worked on: its record two tiles
+// ahead, its matrix one, so that no load is waited for (a lookup in place took a microsecond of each tile's time).
+struct Tiles {
+    const Job &o;
+    const bool symmetric;
+    const int count, step;
+    int at;
+    Tile tile, next, next2;
+    Matrix next_m;
+
+    __device__ __forceinline__ Tiles(const Job &o, bool symmetric, int count, int first, int step) : o(o), symmetric(symmetric), count(count), step(step), at(first) {
+        next = tile_of(o, symmetric, at);
+        next2 = at + step < count ? tile_of(o, symmetric, at + step) : next;
+        next_m = matrix_of(o, next.matrix);
+    }
+    // The tile to work on; its matrix is `m`.
+    __device__ __forceinline__ void take(Matrix &m) {
+        tile = next, m = next_m;
+        next = next2;
+        at += step;
+        if (at < count) next_m = matrix_of(o, next.matrix);
+        if (at + step < count) next2 = tile_of(o, symmetric, at + step);
+    }
+};
+
 // ---------------------------------------------------------------- momentum, norm, X
 
 // n of 8 consecutive elements (the others 0).
@@ -135,6 +160,7 @@ __device__ __forceinline__ double block_sum(double s, double *shared) {
 // nor vanish there). Else X = u / |u|, as hi + lo.
 template <bool FIRST> __global__ void __launch_bounds__(PREP) prepare_kernel(Job o) {
     __shared__ double shared[PREP / 32];
+    pdl_launch();  // the next launch's blocks come in as these leave, and wait for the last of them
     pdl_wait();
     Part part;
     if (o.matrices)
@@ -201,6 +227,7 @@ template <bool FIRST> __global__ void __launch_bounds__(PREP) prepare_kernel(Job
 
 // ---------------------------------------------------------------- products
 
+enum Mode { SINGLES, PAIRS, SPLITS };  // a CTA, a pair of them, or a cluster for a tile
 enum Phase { GRAM, QUAD, APPLY, STEP };  // A; F; X'; the step with the last X' (or the result itself)
 
 // Where the operands of a phase lie: block (i, k) of the first at a + i * ai + k * ak, of the second at
@@ -222,6 +249,9 @@ __device__ __forceinline__ Operands operands(const Matrix &m, int phase, int fro
                   : Operands{m.quad, m.sb, 1, hi, 1, m.cb, m.rb, m.cb, m.sb, false, true, true, false, terms, 1, x_lo};
 }
 
+// Where part r of `parts` of a product's sum begins.
+__device__ __forceinline__ int part_of(const Operands &p, int r, int parts) { return p.nk * p.terms * r / parts; }
+
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -234,6 +264,15 @@ __device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank) {
 }
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The same for threads that come there one by one; all of the cluster's threads do.
+__device__ __forceinline__ void cluster_meet() {
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+    return r;
 }
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -338,8 +377,13 @@ __device__ __forceinline__ void finish(const Job &o, const Matrix &m, int i0, in
 // (256 x 256) elements. Warp 0 loads blocks of 64 x 64 elements, 128 rows of each operand a stage, through a ring of
 // five; one thread of warp 1 (of the pair's first CTA) issues the products into one of two accumulators; eight
 // warps read the other one, 128 rows of the tile in each CTA.
-template <int PHASE, bool PAIR>
+//
+// SPLIT: a cluster of 2, 4 or 8 CTAs takes a tile of 128 x 128 together, each a part of the sum. Each then owns some of the tile's
+// sixteen units of 32 x 32: the others' parts of them come to its shared memory, and it adds them in the order of the
+// parts. It is for products of few tiles with long sums: X X^T of 512 x 3136 has ten, of 49 blocks each.
+template <int PHASE, int MODE>
 __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ CUtensorMap map_units, const __grid_constant__ Job o) {
+    constexpr bool PAIR = MODE == PAIRS, SPLIT = MODE == SPLITS;
     constexpr int SIDES = PAIR ? 4 : 2, COLS = SIDES * SIDE;  // blocks along a tile; columns of an accumulator
     constexpr bool SYMMETRIC = PHASE == GRAM || PHASE == QUAD;
     extern __shared__ uint8_t smem_raw[];
@@ -350,8 +394,10 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
     const uint32_t accf0 = smem_u32(bars + 2 * STAGES), acce0 = smem_u32(bars + 2 * STAGES + 2);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = PAIR ? (int)cluster_rank() : 0;
-    const int first = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x;
+    const int parts = SPLIT ? (int)cluster_size() : 1, part = SPLIT ? (int)cluster_rank() : 0;
+    const int together = PAIR ? 2 : parts, first = blockIdx.x / together, step = gridDim.x / together;
     const int tiles = SYMMETRIC ? o.count_symmetric : o.count_full;
+    pdl_launch();
 
     if (warp == 0 && lane == 0) {
         for (int s = 0; s < STAGES; s++) {
@@ -376,7 +422,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
     }
     tc_fence_before();
     __syncthreads();
-    if (PAIR) cluster_sync();  // both CTAs' barriers exist before any signal between them
+    if (PAIR || SPLIT) cluster_sync();  // the CTAs' barriers exist before any signal between them
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     // A plan does not change between the launches of a step (the first of them waits for all that came before), so
@@ -387,21 +433,19 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
         // ---- loads: this CTA's 128 rows of the first operand and 128 of the second
         int it = 0, in_flight = 0;
         bool ok = true;
-        Tile next = tile_of(o, SYMMETRIC, first);
-        Operands next_p = operands(matrix_of(o, next.matrix), PHASE, o.from);
+        Tiles list(o, SYMMETRIC, tiles, first, step);
         pdl_wait();
         for (int t = first; t < tiles && ok; t += step) {
-            const Tile tile = next;
-            const Operands p = next_p;
-            if (t + step < tiles) {
-                next = tile_of(o, SYMMETRIC, t + step);
-                next_p = operands(matrix_of(o, next.matrix), PHASE, o.from);
-            }
+            Matrix m;
+            list.take(m);
+            const Tile tile = list.tile;
+            const Operands p = operands(m, PHASE, o.from);
             const int i0 = tile.i * SIDES + 2 * rank, j0 = tile.j * SIDES + 2 * rank;
             // blocks that exist, of the tile (whose bytes the barrier expects) and of this CTA
             const int all = min(SIDES, p.ni - tile.i * SIDES) + min(SIDES, p.nj - tile.j * SIDES);
             const int na = min(2, p.ni - i0), nb = min(2, p.nj - j0);
-            for (int n = 0, k = 0, term = 0; n < p.nk * p.terms; n++, it++) {
+            const int end = part_of(p, part + 1, parts);
+            for (int n = part_of(p, part, parts), k = n % p.nk, term = n / p.nk; n < end; n++, it++) {
                 const int s = it % STAGES;
                 const bool a_turned = p.a_half && k / SIDES > tile.i, b_turned = p.b_half && k / SIDES > tile.j;
                 const int ai = a_turned ? p.ak : p.ai, ak = a_turned ? p.ai : p.ak, bj = b_turned ? p.bk : p.bj, bk = b_turned ? p.bj : p.bk;
@@ -438,16 +482,13 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
         // ---- products
         int it = 0, local = 0;
         bool ok = true;
-        Tile next = tile_of(o, SYMMETRIC, first);
-        Operands next_p = operands(matrix_of(o, next.matrix), PHASE, o.from);
+        Tiles list(o, SYMMETRIC, tiles, first, step);
         pdl_wait();
         for (int t = first; t < tiles && ok; t += step, local++) {
-            const Tile tile = next;
-            const Operands p = next_p;
-            if (t + step < tiles) {
-                next = tile_of(o, SYMMETRIC, t + step);
-                next_p = operands(matrix_of(o, next.matrix), PHASE, o.from);
-            }
+            Matrix m;
+            list.take(m);
+            const Tile tile = list.tile;
+            const Operands p = operands(m, PHASE, o.from);
             constexpr uint32_t BASE = (1u << 4) | ((uint32_t)(COLS >> 3) << 17) | ((uint32_t)(COLS >> 4) << 24);  // fp16, fp32 sums
             const int b = local & 1;
             const uint32_t acc = tmem + (uint32_t)(b * COLS);
@@ -456,7 +497,8 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
                 break;
             }
             tc_fence_after();
-            for (int k = 0; k < p.nk * p.terms; k++, it++) {
+            const int begin = part_of(p, part, parts), end = part_of(p, part + 1, parts);
+            for (int n = begin, k = begin % p.nk; n < end; n++, it++) {
                 const int s = it % STAGES;
                 if (!mbar_wait(full0 + 8 * s, (uint32_t)(it / STAGES) & 1u, WAIT_LIMIT)) {
                     atomicExch(&g_error, 3);
@@ -467,14 +509,15 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
                 const uint32_t a = smem_u32(smem + s * STAGE_BYTES), c = a + HALF_BYTES;
                 const bool a_mn = p.a_mn || (p.a_half && k / SIDES > tile.i), b_mn = p.b_mn || (p.b_half && k / SIDES > tile.j);
                 const uint32_t idesc = BASE | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
+                if (++k == p.nk) k = 0;
 #pragma unroll
                 for (int kk = 0; kk < SIDE / 16; kk++) {
                     const uint64_t da = a_mn ? desc_sw128_mn(a + kk * 2048, BLOCK_BYTES) : desc_sw128_k(a + kk * 32);
                     const uint64_t db = b_mn ? desc_sw128_mn(c + kk * 2048, BLOCK_BYTES) : desc_sw128_k(c + kk * 32);
                     if (PAIR)
-                        mma_pair(acc, da, db, idesc, k || kk);
+                        mma_pair(acc, da, db, idesc, n > begin || kk);
                     else
-                        mma_bf16(acc, da, db, idesc, k || kk);
+                        mma_bf16(acc, da, db, idesc, n > begin || kk);
                 }
                 if (PAIR) {
                     commit_pair(empty0 + 8 * s);
@@ -492,22 +535,23 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
     } else if (warp >= 2) {
         // ---- epilogue: warp w holds rows 32 (w % 4) .. + 31 of this CTA's 128, in one half of the columns
         const int q = warp & 3, half = (warp - 2) >> 2;
-        uint8_t *const rooms = smem + STAGES * STAGE_BYTES + (warp - 2) * 2 * ROOM;
-        const uint32_t rooms_at = smem_u32(rooms), sides0 = smem_u32(sides + 2 * (warp - 2));
         constexpr int UNITS = COLS / 2 / 32;
+        // SPLIT: unit `own` of this warp, if any, is this CTA's; `parts` rooms stand behind one another for it, one
+        // for each part, the first of them its own
+        const int index = 4 * q + 2 * half, own = SPLIT ? ((part - index) & (parts - 1)) : 0;
+        uint8_t *const area = smem + STAGES * STAGE_BYTES;
+        uint8_t *const rooms = area + (SPLIT ? (index + own) / parts * parts : (warp - 2) * 2) * ROOM;
+        const uint32_t rooms_at = smem_u32(rooms), sides0 = smem_u32(sides + 2 * (warp - 2));
+        bool met = false;
         uint32_t asked = 0, got = 0;  // loads into the rooms, in turn, and those that have been waited for
         int local = 0;
         bool ok = true;
-        Tile next = tile_of(o, SYMMETRIC, first);
-        Matrix next_m = matrix_of(o, next.matrix);
+        Tiles list(o, SYMMETRIC, tiles, first, step);
         pdl_wait();
         for (int t = first; t < tiles && ok; t += step, local++) {
-            const Tile tile = next;
-            const Matrix m = next_m;
-            if (t + step < tiles) {
-                next = tile_of(o, SYMMETRIC, t + step);
-                next_m = matrix_of(o, next.matrix);
-            }
+            Matrix m;
+            list.take(m);
+            const Tile tile = list.tile;
             const Operands p = operands(m, PHASE, o.from);
             const int b = local & 1, ib = tile.i * SIDES + 2 * rank + (q >> 1), r0 = 32 * (q & 1);
             const int hi_to = o.from ? m.hi[0] : m.hi[1];
@@ -519,7 +563,8 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
             const bool reads = PHASE == QUAD || (PHASE != GRAM && !m.fine);
             const auto fetch = [&](int u) {
                 if (!reads || u >= units) return;
-                const uint32_t k = asked++ & 1u;
+                const uint32_t k = SPLIT ? 0u : asked & 1u;
+                asked++;
                 if (lane) return;
                 const int x = 32 * (u & 1), y = row_of(u);
                 mbar_expect_tx(sides0 + 8 * k, PHASE == QUAD && m.fine ? ROOM : ROOM / 2);
@@ -529,8 +574,12 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
             };
             if (lane == 0) bulk_wait_read();
             __syncwarp();  // the rooms are free
-            fetch(0);
-            fetch(1);
+            if (SPLIT) {
+                fetch(own);
+            } else {
+                fetch(0);
+                fetch(1);
+            }
             if (PHASE == STEP && m.param) {  // the parameters are read after the products: into L2 meanwhile, a row a lane
                 const int i = ib * SIDE + r0 + lane, j0 = jb0 * SIDE;
 #pragma unroll
@@ -542,16 +591,56 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
                 break;
             }
             tc_fence_after();
+            if (SPLIT) {
+                // the others' units go to their owners
+                for (int u = 0; u < units; u++) {
+                    if (u == own || part_of(p, part, parts) == part_of(p, part + 1, parts)) continue;
+                    uint32_t v[32];
+                    D1X_TMEM_LD32(tmem + (uint32_t)(b * COLS + half * (COLS / 2) + 32 * u) + ((uint32_t)(32 * q) << 16), v);
+                    tmem_wait_ld();
+                    const int to = (index + u) & (parts - 1), slot = (index + u) / parts * parts + 1 + (part < to ? part : part - 1);
+                    const uint32_t at = mapa(smem_u32(area + slot * ROOM) + lane * 16, to);
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + e * 512), "r"(v[4 * e]), "r"(v[4 * e + 1]),
+                                     "r"(v[4 * e + 2]), "r"(v[4 * e + 3])
+                                     : "memory");
+                }
+                __syncwarp();
+                cluster_meet();
+                met = true;
+            }
 #pragma unroll 1
-            for (int u = 0; u < units; u++) {
+            for (int u = SPLIT ? own : 0; u < (SPLIT ? min(units, own + 1) : units); u++) {
                 float params[32];
                 if (PHASE == STEP && m.param) load_params(m, ib * SIDE + r0, jb0 * SIDE + 32 * u, params);
                 uint32_t v[32];
                 D1X_TMEM_LD32(tmem + (uint32_t)(b * COLS + half * (COLS / 2) + 32 * u) + ((uint32_t)(32 * q) << 16), v);
                 tmem_wait_ld();
-                const uint32_t k = (uint32_t)u & 1u;
+                if (SPLIT) {  // a part without a block has left nothing
+                    float sum[32] = {};
+                    for (int r = 0; r < parts; r++) {
+                        if (part_of(p, r, parts) == part_of(p, r + 1, parts)) continue;
+                        if (r == part) {
+#pragma unroll
+                            for (int i = 0; i < 32; i++) sum[i] += __uint_as_float(v[i]);
+                            continue;
+                        }
+                        const float4 *const from = reinterpret_cast<const float4 *>(rooms + (1 + (r < part ? r : r - 1)) * ROOM) + lane;
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            const float4 f = from[32 * e];
+                            sum[4 * e] += f.x, sum[4 * e + 1] += f.y, sum[4 * e + 2] += f.z, sum[4 * e + 3] += f.w;
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; i++) v[i] = __float_as_uint(sum[i]);
+                }
+                const uint32_t k = SPLIT ? 0u : (uint32_t)u & 1u;
                 if (reads) {
-                    if (!mbar_wait(sides0 + 8 * k, got++ >> 1 & 1u, WAIT_LIMIT)) {
+                    const uint32_t parity = SPLIT ? got : got >> 1;
+                    got++;
+                    if (!mbar_wait(sides0 + 8 * k, parity & 1u, WAIT_LIMIT)) {
                         atomicExch(&g_error, 5);
                         ok = false;
                         break;
@@ -634,7 +723,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
                     }
                 }
                 __syncwarp();
-                if (reads && u + 2 < units) {
+                if (!SPLIT && reads && u + 2 < units) {
                     if (lane == 0) bulk_wait_read();
                     fetch(u + 2);
                 }
@@ -649,9 +738,11 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
             }
         }
         // after an error: loads under way land before the block leaves
-        for (; got != asked; got++) mbar_wait(sides0 + 8 * (got & 1u), got >> 1 & 1u, WAIT_LIMIT);
+        for (; got != asked; got++) mbar_wait(sides0 + (SPLIT ? 0 : 8 * (got & 1u)), (SPLIT ? got : got >> 1) & 1u, WAIT_LIMIT);
         if (lane == 0) bulk_wait();
+        if (SPLIT && !met) cluster_meet();
     }
+    if (SPLIT && warp < 2) cluster_meet();  // every thread of the cluster comes there once
     tc_fence_before();
     __syncthreads();
     if (PAIR) cluster_sync();  // no signal between the CTAs is outstanding past this point
@@ -696,28 +787,27 @@ static int make_maps(Maps &maps, void *work, int64_t blocks) {
 }
 
 typedef void (*Product)(const CUtensorMap, const CUtensorMap, const Job);
-static Product product_of(int phase, bool pair) {
-    static const Product all[2][4] = {
-        {product_kernel<GRAM, false>, product_kernel<QUAD, false>, product_kernel<APPLY, false>, product_kernel<STEP, false>},
-        {product_kernel<GRAM, true>, product_kernel<QUAD, true>, product_kernel<APPLY, true>, product_kernel<STEP, true>}};
-    return all[pair][phase];
+static Product product_of(int phase, int mode) {
+    static const Product all[3][4] = {
+        {product_kernel<GRAM, SINGLES>, product_kernel<QUAD, SINGLES>, product_kernel<APPLY, SINGLES>, product_kernel<STEP, SINGLES>},
+        {product_kernel<GRAM, PAIRS>, product_kernel<QUAD, PAIRS>, product_kernel<APPLY, PAIRS>, product_kernel<STEP, PAIRS>},
+        {product_kernel<GRAM, SPLITS>, product_kernel<QUAD, SPLITS>, product_kernel<APPLY, SPLITS>, product_kernel<STEP, SPLITS>}};
+    return all[mode][phase];
 }
 static int allow_space() {
     static uint64_t ready = 0;
     int dev = 0;
     if (cudaError_t e = cudaGetDevice(&dev)) return (int)e;
     if (dev < 64 && ((ready >> dev) & 1)) return 0;
-    for (int k = 0; k < 8; k++)
+    for (int k = 0; k < 12; k++)
         if (cudaError_t e = cudaFuncSetAttribute(product_of(k & 3, k >> 2), cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES)) return (int)e;
     if (dev < 64) ready |= 1ull << dev;
     return 0;
 }
 
-// Blocks along a tile's side: 256 x 256 tiles of CTA pairs where every pair has one.
-static int side_for(int64_t symmetric_of_pairs) { return symmetric_of_pairs >= SMS / 2 ? 4 : 2; }
-
-static int launch(Job &o, int64_t parts, int64_t blocks, int side, int steps, cudaStream_t s) {
-    if (parts > INT32_MAX) return D1_ERR_TOO_LARGE;
+static int launch(Job &o, int64_t parts, int64_t blocks, const Load &load, int steps, cudaStream_t s) {
+    if (parts > INT32_MAX || load.symmetric > INT32_MAX || load.full > INT32_MAX) return D1_ERR_TOO_LARGE;
+    o.count_symmetric = (int)load.symmetric, o.count_full = (int)load.full;
     Maps maps;
     if (const int e = make_maps(maps, o.work, blocks)) return e;
     if (const int e = allow_space()) return e;
@@ -727,22 +817,20 @@ static int launch(Job &o, int64_t parts, int64_t blocks, int side, int steps, cu
     if (cudaError_t e = cudaLaunchKernelEx(&cfg, prepare_kernel<true>, o)) return (int)e;
     cfg.numAttrs = 1;
     if (cudaError_t e = cudaLaunchKernelEx(&cfg, prepare_kernel<false>, o)) return (int)e;
-    const bool pair = side == 4;
-    if (pair) {
-        attr[1].id = cudaLaunchAttributeClusterDimension;
-        attr[1].val.clusterDim.x = 2;
-        attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-        cfg.numAttrs = 2;
-    }
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.blockDim = dim3(THREADS);
     cfg.dynamicSmemBytes = SMEM_BYTES;
     for (int k = 0; k < steps; k++, o.from ^= 1)
         for (int phase = 0; phase < 3; phase++) {
             const int tiles = phase < 2 ? o.count_symmetric : o.count_full;
-            const int most = pair ? SMS / 2 : SMS, n = tiles < most ? tiles : most;
-            cfg.gridDim = dim3((unsigned)(pair ? 2 * n : n));
-            if (cudaError_t e = cudaLaunchKernelEx(&cfg, product_of(phase == 2 && k == steps - 1 ? STEP : phase, pair), maps.blocks, maps.units, o))
-                return (int)e;
+            const int split = load.side == 4 ? 1 : parts_for(tiles, load.depth[phase > 0]);
+            const int together = load.side == 4 ? 2 : split, most = SMS / together, n = tiles < most ? tiles : most;
+            cfg.gridDim = dim3((unsigned)(n * together));
+            cfg.numAttrs = together > 1 ? 2 : 1;
+            attr[1].val.clusterDim.x = together;
+            const Product kernel = product_of(phase == 2 && k == steps - 1 ? STEP : phase, load.side == 4 ? PAIRS : split > 1 ? SPLITS : SINGLES);
+            if (cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, maps.blocks, maps.units, o)) return (int)e;
         }
     return 0;
 }
@@ -756,39 +844,39 @@ using namespace d1::muon;
 static int plan(const D1MuonTensor *tensors, int n, float *momentum, Plan &head, uint8_t *out) {
     if (!tensors || n < 1) return D1_ERR_BAD_ARGUMENT;
     head = Plan{};
-    for (int pass = 0; pass < 2; pass++) {  // sizes, then (with the tile's side known) the number of tiles
-        int64_t block = 0, part = 0;
-        head.matrices = head.symmetric = head.full = 0;
-        for (int t = 0; t < n; t++) {
-            const D1MuonTensor &d = tensors[t];
-            const int64_t need = blocks_needed(d.rows, d.cols);
-            if (need < 0 || d.count < 0 || d.count > MOST_BLOCKS) return D1_ERR_BAD_ARGUMENT;
-            if (need * d.count + block > MOST_BLOCKS) return D1_ERR_TOO_LARGE;
-            for (int64_t k = 0; k < d.count; k++) {
-                Matrix m;
-                place(m, d.rows, d.cols, block, part);
-                head.matrices++;
-                head.symmetric += symmetric_tiles(m, pass ? head.side : 4);
-                head.full += full_tiles(m, pass ? head.side : 4);
-            }
-        }
-        head.parts = part;
-        head.blocks = block;
-        if (!pass) head.side = side_for(head.symmetric);
+    Load small = load_of(2), large = load_of(4);
+    int64_t block = 0, part = 0;
+    for (int t = 0; t < n; t++) {
+        const D1MuonTensor &d = tensors[t];
+        const int64_t need = blocks_needed(d.rows, d.cols);
+        if (need < 0 || d.count < 0 || d.count > MOST_BLOCKS) return D1_ERR_BAD_ARGUMENT;
+        if (need * d.count + block > MOST_BLOCKS) return D1_ERR_TOO_LARGE;
+        if (!d.count) continue;
+        Matrix m;
+        int64_t from = block, from_part = part;
+        place(m, d.rows, d.cols, from, from_part);
+        block += (from - block) * d.count, part += (from_part - part) * d.count;
+        head.matrices += d.count;
+        small.add(m, d.count);
+        large.add(m, d.count);
     }
+    head.parts = part;
+    head.blocks = block;
+    head.load = large.microseconds() < small.microseconds() ? large : small;
     if (!head.matrices) return D1_ERR_BAD_ARGUMENT;
-    if (head.symmetric > INT32_MAX || head.full > INT32_MAX || head.parts > INT32_MAX) return D1_ERR_TOO_LARGE;
+    if (head.load.symmetric > INT32_MAX || head.load.full > INT32_MAX || head.parts > INT32_MAX) return D1_ERR_TOO_LARGE;
     head.at_matrices = (sizeof(Plan) + 15) / 16 * 16;
     head.at_parts = head.at_matrices + head.matrices * (int64_t)sizeof(Matrix);
     head.at_symmetric = head.at_parts + head.parts * (int64_t)sizeof(Part);
-    head.at_full = head.at_symmetric + head.symmetric * (int64_t)sizeof(Tile);
-    head.bytes = head.at_full + head.full * (int64_t)sizeof(Tile);
+    head.at_full = head.at_symmetric + head.load.symmetric * (int64_t)sizeof(Tile);
+    head.bytes = head.at_full + head.load.full * (int64_t)sizeof(Tile);
     if (!out) return 0;
     *(Plan *)out = head;
     Matrix *const matrices = (Matrix *)(out + head.at_matrices);
     Part *parts = (Part *)(out + head.at_parts);
-    int64_t block = 0, part = 0, momentum_at = 0;
+    int64_t momentum_at = 0;
     int k = 0;
+    block = part = 0;
     for (int t = 0; t < n; t++) {
         const D1MuonTensor &d = tensors[t];
         const int64_t size = d.rows * d.cols, grad_size = d.grad_type == D1_TYPE_F32 ? 4 : 2;
@@ -820,13 +908,13 @@ static int plan(const D1MuonTensor *tensors, int n, float *momentum, Plan &head,
         });
         for (int q = 0; q < k; q++) {
             const Matrix &m = matrices[order[q]];
-            const int64_t count = symmetric ? symmetric_tiles(m, head.side) : full_tiles(m, head.side);
-            for (int64_t t = 0; t < count; t++) {
+            const int64_t count = symmetric ? symmetric_tiles(m, head.load.side) : full_tiles(m, head.load.side);
+            for (int t = 0; t < (int)count; t++) {
                 int i, j;
                 if (symmetric)
                     symmetric_tile(t, i, j);
                 else
-                    grouped_tile(t, tiles_of(m.rb, head.side), tiles_of(m.cb, head.side), i, j);
+                    grouped_tile(t, tiles_of(m.rb, head.load.side), tiles_of(m.cb, head.load.side), i, j);
                 *to++ = Tile{order[q], (uint16_t)i, (uint16_t)j};
             }
         }
@@ -873,11 +961,10 @@ extern "C" int d1_muon(const void *host_plan, const void *device_plan, double lr
     o.parts = (const Part *)(at + head.at_parts);
     o.symmetric = (const Tile *)(at + head.at_symmetric);
     o.full = (const Tile *)(at + head.at_full);
-    o.count_symmetric = (int)head.symmetric, o.count_full = (int)head.full;
     o.work = (uint8_t *)work;
     o.partials = (double *)(o.work + work_blocks_bytes(head.blocks));
     o.mu = (float)momentum, o.nesterov = nesterov != 0, o.lr = lr;
-    return launch(o, head.parts, head.blocks, head.side, steps, (cudaStream_t)stream);
+    return launch(o, head.parts, head.blocks, head.load, steps, (cudaStream_t)stream);
 }
 
 // The stack's one matrix, its blocks and parts; false when it is out of range.
@@ -916,15 +1003,16 @@ extern "C" int d1_orthogonalize(const void *x, int64_t ldx, int64_t x_step, int 
     o.one = m;
     o.grad_step = x_step * size, o.out_step = rows * cols * 2;
     o.block_step = (int)blocks;
-    const int side = side_for(count * symmetric_tiles(m, 4));
-    const int64_t symmetric = symmetric_tiles(m, side), full = full_tiles(m, side);
-    if (symmetric * count > INT32_MAX || full * count > INT32_MAX) return D1_ERR_TOO_LARGE;
-    o.per_symmetric = (int)symmetric, o.per_full = (int)full;
-    o.count_symmetric = (int)(symmetric * count), o.count_full = (int)(full * count);
-    o.tm = tiles_of(m.rb, side), o.tn = tiles_of(m.cb, side);
+    Load small = load_of(2), large = load_of(4);
+    small.add(m, count);
+    large.add(m, count);
+    const Load &load = large.microseconds() < small.microseconds() ? large : small;
+    if (load.symmetric > INT32_MAX || load.full > INT32_MAX) return D1_ERR_TOO_LARGE;
+    o.per_symmetric = (int)(load.symmetric / count), o.per_full = (int)(load.full / count);
+    o.tm = tiles_of(m.rb, load.side), o.tn = tiles_of(m.cb, load.side);
     o.work = (uint8_t *)work;
     o.partials = (double *)(o.work + work_blocks_bytes(count * blocks));
-    return launch(o, count * parts, count * blocks, side, steps, (cudaStream_t)stream);
+    return launch(o, count * parts, count * blocks, load, steps, (cudaStream_t)stream);
 }
 
 // Last error recorded by a wait that ran out (0 = none); clears it.

@@ -29,7 +29,7 @@ int main() {
             for (int side : {2, 4}) {
                 std::set<std::pair<int, int>> seen;
                 const int t = tiles_of(m.sb, side);
-                for (int64_t k = 0; k < symmetric_tiles(m, side); k++) {
+                for (int k = 0; k < symmetric_tiles(m, side); k++) {
                     int i, j;
                     symmetric_tile(k, i, j);
                     if (j > i || i >= t || j < 0 || !seen.insert({i, j}).second) return 4;
@@ -37,7 +37,7 @@ int main() {
                 if ((int64_t)seen.size() != (int64_t)t * (t + 1) / 2) return 5;
                 seen.clear();
                 const int tm = tiles_of(m.rb, side), tn = tiles_of(m.cb, side);
-                for (int64_t k = 0; k < full_tiles(m, side); k++) {
+                for (int k = 0; k < full_tiles(m, side); k++) {
                     int i, j;
                     grouped_tile(k, tm, tn, i, j);
                     if (i < 0 || i >= tm || j < 0 || j >= tn || !seen.insert({i, j}).second) return 6;
@@ -46,8 +46,29 @@ int main() {
             }
         }
     int i, j;
-    symmetric_tile((int64_t)40000 * 40001 / 2 + 39999, i, j);
-    if (i != 40000 || j != 39999) return 8;
+    for (int r : {0, 1, 4095, 4096, 5000, 20000, 40000, 65534}) {
+        symmetric_tile((int)((int64_t)r * (r + 1) / 2), i, j);
+        if (i != r || j != 0) return 8;
+        symmetric_tile((int)((int64_t)r * (r + 1) / 2 + r), i, j);
+        if (i != r || j != r) return 8;
+    }
+    for (int64_t tiles : {1, 10, 14, 15, 32, 33, 74, 75, 148, 1000})
+        for (int depth : {1, 8, 16, 49, 1000}) {
+            const int n = parts_for(tiles, depth);
+            if (n != 1 && n != 2 && n != 4 && n != 8) return 10;
+            if (n > 1 && (tiles * n > 148 || depth < 10)) return 11;
+        }
+    if (parts_for(10, 49) != 8 || parts_for(24, 49) != 4 || parts_for(74, 49) != 2 || parts_for(75, 1000) != 1 || parts_for(1, 8) != 1) return 12;
+    for (int64_t n : {64, 1000, 8192}) {
+        Load small = load_of(2), large = load_of(4);
+        Matrix m;
+        int64_t block = 0, part = 0;
+        place(m, n, n, block, part);
+        small.add(m, 3), large.add(m, 3);
+        if (small.symmetric != 3 * symmetric_tiles(m, 2) || large.full != 3 * full_tiles(m, 4) || small.depth[0] != (int)(n + 63) / 64 * (m.fine ? 3 : 1)) return 13;
+        if (n == 64 && !(small.microseconds() < large.microseconds())) return 14;
+        if (n == 8192 && !(large.microseconds() < small.microseconds())) return 15;
+    }
     if (blocks_needed(0, 4) != -1 || blocks_needed(4, (1 << 21) + 1) != -1 || blocks_needed(1 << 21, 1) != 3 * 32768 + 4) return 9;
     std::puts("ok");
 }
@@ -85,8 +106,8 @@ def test_plans(lib):
     assert work >= 8192 * blocks and size > 7 * 100
     host = (C.c_uint64 * ((size + 7) // 8))()
     assert lib.d1_muon_plan(t, 5, P, host, C.sizeof(host)) == 0
-    head = list((C.c_int64 * 10).from_buffer(host))
-    assert head[0] == size and head[1] == 7 and head[9] == blocks
+    head = list((C.c_int64 * 8).from_buffer(host))
+    assert head[0] == size and head[1] == 7 and head[7] == blocks
     assert head[2] == sum(c * min(256, -(-r // 64) * -(-k // 64)) for c, r, k in shapes)
     assert lib.d1_muon_plan(t, 5, P, host, size - 1) == BAD
     assert lib.d1_muon_plan(t, 5, None, host, size) == BAD and lib.d1_muon_plan(t, 5, P + 4, host, size) == BAD
