@@ -349,12 +349,15 @@ __device__ __forceinline__ void finish(const Job &o, const Matrix &m, int i0, in
     __syncwarp();
     const int rows = j0 + lane < m.cols ? min(32, m.rows - i0) : 0;
     int64_t at = (int64_t)i0 * m.cols + j0 + lane;
+    float turned[32];  // all of them before the first store: the compiler keeps loads behind stores that might meet them
+#pragma unroll
+    for (int r = 0; r < 32; r++) turned[r] = room[place_of(r, lane)];
     if (!m.param) {
         const bool bf16 = m.out_type == D1_TYPE_BF16;
 #pragma unroll
         for (int r = 0; r < 32; r++, at += m.cols)
             if (r < rows) {
-                const float y = room[place_of(r, lane)] * UNSCALE;
+                const float y = turned[r] * UNSCALE;
                 if (bf16)
                     ((__nv_bfloat16 *)m.out)[at] = __float2bfloat16_rn(y);
                 else
@@ -365,7 +368,7 @@ __device__ __forceinline__ void finish(const Job &o, const Matrix &m, int i0, in
 #pragma unroll
         for (int r = 0; r < 32; r++, at += m.cols)
             if (r < rows) {
-                const float y = fmaf(rate, room[place_of(r, lane)], p[r] * keep);
+                const float y = fmaf(rate, turned[r], p[r] * keep);
                 m.param[at] = y;
                 if (m.out) ((__nv_bfloat16 *)m.out)[at] = __float2bfloat16_rn(y);
             }
