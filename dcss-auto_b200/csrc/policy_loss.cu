@@ -16,10 +16,9 @@
 // series near 0, where the difference would cancel. Sums are fp64 from four
 // tokens on, joined in a fixed order.
 //
-// The weights need the mask's counts before any token can be finished. Small
-// batches count in the one block that does the rest; larger ones clear and fill
-// integer counts in a launch ahead (whole numbers: the order does not matter),
-// which reads a byte a token where the main pass reads 13 and more.
+// The weights need the mask's counts before any token can be finished. Up to 32,768 tokens are a cluster's: each of its blocks
+// counts the whole mask and takes a part of the tokens, the first one adds the blocks' sums. More have a launch ahead
+// that counts (a byte a token, where the main pass reads 13 and more), and one after it that adds.
 #include <math.h>
 
 #include "d1_common.cuh"
@@ -30,7 +29,9 @@
 namespace d1 {
 namespace pl {
 
-constexpr int SMS = 148, THREADS = 256, BLOCKS = SMS * 4, SMALL = 16384, SMALL_THREADS = 1024, SMALL_ROWS = 2048, TERMS = 5;
+constexpr int SMS = 148, THREADS = 256, BLOCKS = SMS * 3, TERMS = 5;
+constexpr int SMALL = 32768, SMALL_THREADS = 512, SMALL_ROWS = 2048, MOST_TOGETHER = 8;  // a cluster's batch
+constexpr int PIECE = 4096, LONG = 16384;  // tokens of a row that a warp counts; of a row that is too long for one block
 
 struct Rows {  // fp32 [rows, length]: element (r, i) at p[r * ld + i * step]
     const float *p;
@@ -49,14 +50,14 @@ struct Args {
     int by_row;                         // mean of the rows' means
     float *loss, *stats, *dlogp, *dentropy;
     double *parts;                      // [blocks][TERMS]
-    int *counts;                        // [0] tokens or rows that have any; [1 + r] tokens of row r
-    int blocks;
+    int *counts;                        // tokens of row r (by_row)
+    int *totals;                        // [count_blocks] tokens, or rows that have any
+    int blocks, count_blocks;
 };
 
-// e^v - 1 - v.
-__device__ __forceinline__ float beyond_linear(float v, float e1) {
-    if (fabsf(v) >= 0.5f) return e1 - v;
-    // v^2 (1/2! + v/3! + ...): the first term left out is below 2^-25 of the sum
+// e^v - 1 - v, given e^v. Near 0 from the series v^2 (1/2! + v/3! + ...), whose first term left out is below
+// 2^-25 of the sum.
+__device__ __forceinline__ float beyond_linear(float v, float grown) {
     float s = 1.f / 362880.f;
     s = fmaf(s, v, 1.f / 40320.f);
     s = fmaf(s, v, 1.f / 5040.f);
@@ -65,7 +66,7 @@ __device__ __forceinline__ float beyond_linear(float v, float e1) {
     s = fmaf(s, v, 1.f / 24.f);
     s = fmaf(s, v, 1.f / 6.f);
     s = fmaf(s, v, 0.5f);
-    return s * v * v;
+    return fabsf(v) < 0.5f ? s * v * v : grown - 1.f - v;
 }
 
 struct Sums {
@@ -81,13 +82,13 @@ __device__ __forceinline__ float token(const Args &a, float logp, float old, flo
     s.t[0] -= w * ((cut ? (over ? a.most : a.least) : r) * adv);
     float g = cut ? 0.f : -adv * r;
     if (a.ref.p) {
-        const float d = ref - logp, e1 = expm1f(d);
-        s.t[1] += w * beyond_linear(d, e1);
-        g = fmaf(-a.kl, e1, g);
+        const float d = ref - logp, k = beyond_linear(d, expf(d));
+        s.t[1] += w * k;
+        g = fmaf(-a.kl, d + k, g);  // e^d - 1
     }
     if (a.entropy.p) s.t[2] += w * h;
     if (cut) s.t[3] += w;
-    s.t[4] += w * beyond_linear(delta, r - 1.f);
+    s.t[4] += w * beyond_linear(delta, r);
     return g * w;
 }
 
@@ -97,52 +98,80 @@ __device__ __forceinline__ float weight_of(const Args &a, const int *row_counts,
     return n ? rows_inv / (float)n : 0.f;
 }
 
-// Everything of the tokens first, first + stride, ..., V at a time along the flat index (V > 1: every
-// operand's rows lie end to end).
-template <int V>
-__device__ __forceinline__ void pass(const Args &a, const int *row_counts, float flat, float rows_inv, int64_t first, int64_t stride, double (&total)[TERMS]) {
-    const bool small = a.count <= INT32_MAX;
-    for (int64_t i = first * V; i < a.count; i += stride * V) {
-        int64_t row = small ? (int64_t)((uint32_t)i / (uint32_t)a.length) : i / a.length, col = i - row * a.length;
-        Sums s = {};
-        Elems<float, V> lp, old, adv, ref = {}, h = {}, g, dh;
-        Elems<uint8_t, V> keep;
-        if constexpr (V > 1) {
-            lp = *reinterpret_cast<const Elems<float, V> *>(a.logp.p + i);
-            old = *reinterpret_cast<const Elems<float, V> *>(a.old.p + i);
-            if (!a.per_row) adv = *reinterpret_cast<const Elems<float, V> *>(a.adv.p + i);
-            if (a.ref.p) ref = *reinterpret_cast<const Elems<float, V> *>(a.ref.p + i);
-            if (a.entropy.p) h = *reinterpret_cast<const Elems<float, V> *>(a.entropy.p + i);
-            if (a.mask) keep = *reinterpret_cast<const Elems<uint8_t, V> *>(a.mask + i);
-        } else {
-            lp.v[0] = a.logp.p[row * a.logp.ld + col];
-            old.v[0] = a.old.p[row * a.old.ld + col];
-            if (!a.per_row) adv.v[0] = a.adv.p[row * a.adv.ld + col];
-            if (a.ref.p) ref.v[0] = a.ref.p[row * a.ref.ld + col];
-            if (a.entropy.p) h.v[0] = a.entropy.p[row * a.entropy.ld + col];
-            if (a.mask) keep.v[0] = a.mask[row * a.ld_mask + col];
-        }
-        float row_adv = a.per_row ? a.adv.p[row * a.adv.ld] : 0.f, w = weight_of(a, row_counts, row, flat, rows_inv);
-#pragma unroll
-        for (int v = 0; v < V; v++) {
-            if (V > 1 && v && ++col == a.length) {  // the next token is the next row's first
-                col = 0;
-                row++;
-                if (a.per_row) row_adv = a.adv.p[row * a.adv.ld];
-                w = weight_of(a, row_counts, row, flat, rows_inv);
-            }
-            g.v[v] = dh.v[v] = 0.f;
-            if (!a.mask || keep.v[v]) {
-                g.v[v] = token(a, lp.v[v], old.v[v], a.per_row ? row_adv : adv.v[v], ref.v[v], h.v[v], w, s);
-                dh.v[v] = -a.ent * w;
-            }
-        }
-        if (a.dlogp) *reinterpret_cast<Elems<float, V> *>(a.dlogp + i) = g;
-        if (a.dentropy) *reinterpret_cast<Elems<float, V> *>(a.dentropy + i) = dh;
-#pragma unroll
-        for (int k = 0; k < TERMS; k++) total[k] += (double)s.t[k];
+// V tokens as they are read.
+template <int V> struct Held {
+    Elems<float, V> logp, old, adv, ref, h;
+    Elems<uint8_t, V> keep;
+};
+template <int V> __device__ __forceinline__ int64_t row_of(const Args &a, int64_t i) {
+    return a.count <= INT32_MAX ? (int64_t)((uint32_t)i / (uint32_t)a.length) : i / a.length;
+}
+template <int V> __device__ __forceinline__ void load(const Args &a, int64_t i, Held<V> &t) {
+    if constexpr (V > 1) {
+        t.logp = *reinterpret_cast<const Elems<float, V> *>(a.logp.p + i);
+        t.old = *reinterpret_cast<const Elems<float, V> *>(a.old.p + i);
+        if (!a.per_row) t.adv = *reinterpret_cast<const Elems<float, V> *>(a.adv.p + i);
+        if (a.ref.p) t.ref = *reinterpret_cast<const Elems<float, V> *>(a.ref.p + i);
+        if (a.entropy.p) t.h = *reinterpret_cast<const Elems<float, V> *>(a.entropy.p + i);
+        if (a.mask) t.keep = *reinterpret_cast<const Elems<uint8_t, V> *>(a.mask + i);
+    } else {
+        const int64_t row = row_of<V>(a, i), col = i - row * a.length;
+        t.logp.v[0] = a.logp.p[row * a.logp.ld + col];
+        t.old.v[0] = a.old.p[row * a.old.ld + col];
+        if (!a.per_row) t.adv.v[0] = a.adv.p[row * a.adv.ld + col];
+        if (a.ref.p) t.ref.v[0] = a.ref.p[row * a.ref.ld + col];
+        if (a.entropy.p) t.h.v[0] = a.entropy.p[row * a.entropy.ld + col];
+        if (a.mask) t.keep.v[0] = a.mask[row * a.ld_mask + col];
     }
 }
+
+// Everything of V tokens from i on.
+template <int V>
+__device__ __forceinline__ void work(const Args &a, const int *row_counts, float flat, float rows_inv, int64_t i, const Held<V> &t, double (&total)[TERMS]) {
+    int64_t row = 0, col = 0;
+    if (a.by_row || a.per_row) row = row_of<V>(a, i), col = i - row * a.length;
+    float row_adv = a.per_row ? a.adv.p[row * a.adv.ld] : 0.f, w = weight_of(a, row_counts, row, flat, rows_inv);
+    Sums s = {};
+    Elems<float, V> g, dh;
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+        if (V > 1 && v && (a.by_row || a.per_row) && ++col == a.length) {  // the next token is the next row's first
+            col = 0;
+            row++;
+            if (a.per_row) row_adv = a.adv.p[row * a.adv.ld];
+            w = weight_of(a, row_counts, row, flat, rows_inv);
+        }
+        g.v[v] = dh.v[v] = 0.f;
+        if (!a.mask || t.keep.v[v]) {
+            g.v[v] = token(a, t.logp.v[v], t.old.v[v], a.per_row ? row_adv : t.adv.v[v], t.ref.v[v], t.h.v[v], w, s);
+            dh.v[v] = -a.ent * w;
+        }
+    }
+    if (a.dlogp) *reinterpret_cast<Elems<float, V> *>(a.dlogp + i) = g;
+    if (a.dentropy) *reinterpret_cast<Elems<float, V> *>(a.dentropy + i) = dh;
+#pragma unroll
+    for (int k = 0; k < TERMS; k++) total[k] += (double)s.t[k];
+}
+
+// The tokens first, first + stride, ..., V at a time along the flat index (V > 1: every operand's rows lie end to
+// end), the next ones' loads under way during the arithmetic of these. `first` is not past the end.
+template <int V> struct Pass {
+    int64_t i, step;
+    Held<V> now;
+
+    __device__ __forceinline__ Pass(const Args &a, int64_t first, int64_t stride) : i(first * V), step(stride * V) {
+        if (i < a.count) load<V>(a, i, now);
+    }
+    __device__ __forceinline__ void run(const Args &a, const int *row_counts, float flat, float rows_inv, double (&total)[TERMS]) {
+        while (i < a.count) {
+            Held<V> next;
+            if (i + step < a.count) load<V>(a, i + step, next);
+            work<V>(a, row_counts, flat, rows_inv, i, now, total);
+            now = next;
+            i += step;
+        }
+    }
+};
 
 // The block's sums in thread 0, added in a fixed order.
 template <int N> __device__ __forceinline__ void join(double (&total)[TERMS], double (*shared)[TERMS]) {
@@ -173,39 +202,80 @@ __device__ __forceinline__ void finish(const Args &a, const double (&t)[TERMS]) 
 // Weight of a token in the mean over tokens, and 1 / rows that have any.
 __device__ __forceinline__ float inverse(int64_t n) { return n > 0 ? (float)(1. / (double)n) : 0.f; }
 
-// The tokens of every row that the mask keeps, and counts[0].
-__global__ void __launch_bounds__(THREADS) count_kernel(Args a) {
-    const int lane = threadIdx.x & 31;
-    const int64_t warps = (int64_t)gridDim.x * (THREADS / 32), at = (int64_t)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5);
-    // a warp takes 1024 tokens of a row at a time
-    const int64_t pieces = (a.length + 1023) / 1024;
+// How many of `n` bytes are not 0, by the threads k, k + stride, ... of those that count them. Whole 16-byte pieces are read
+// as such, wherever the row begins.
+__device__ __forceinline__ int count_bytes(const uint8_t *p, int64_t n, int k, int stride) {
+    const int64_t head = min(n, (int64_t)(-(intptr_t)p & 15)), pieces = (n - head) / 16, tail = head + pieces * 16;
     int sum = 0;
-    for (int64_t p = at; p < a.rows * pieces; p += warps) {
-        const int64_t row = p / pieces, c0 = (p - row * pieces) * 1024;
-        const uint8_t *m = a.mask + row * a.ld_mask + c0;
-        const int n = (int)min((int64_t)1024, a.length - c0);
-        int k = 0;
-#pragma unroll 8
-        for (int i = lane; i < n; i += 32) k += m[i] != 0;
-        if (a.by_row) {
-            k = __reduce_add_sync(0xffffffffu, k);
-            // whoever adds the row's first tokens counts the row
-            if (lane == 0 && k && atomicAdd(a.counts + 1 + row, k) == 0) atomicAdd(a.counts, 1);
-        } else
-            sum += k;
+    for (int64_t i = k; i < head; i += stride) sum += p[i] != 0;
+    const uint4 *const q = reinterpret_cast<const uint4 *>(p + head);
+#pragma unroll 4
+    for (int64_t i = k; i < pieces; i += stride) {
+        const uint4 w = q[i];
+        sum += __popc(__vcmpne4(w.x, 0) & 0x01010101u) + __popc(__vcmpne4(w.y, 0) & 0x01010101u) + __popc(__vcmpne4(w.z, 0) & 0x01010101u) +
+               __popc(__vcmpne4(w.w, 0) & 0x01010101u);
     }
-    if (!a.by_row) {
-        sum = __reduce_add_sync(0xffffffffu, sum);
-        if (lane == 0 && sum) atomicAdd(a.counts, sum);
-    }
+    for (int64_t i = tail + k; i < n; i += stride) sum += p[i] != 0;
+    return sum;
 }
 
-template <int V> __global__ void __launch_bounds__(THREADS) loss_kernel(Args a) {
-    __shared__ double shared[THREADS / 32][TERMS];
+// Sum over the block of whole numbers, in every thread.
+template <int N> __device__ __forceinline__ int block_sum(int x, int *shared) {
+    x = __reduce_add_sync(0xffffffffu, x);
+    if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = x;
+    __syncthreads();
+    x = 0;
+#pragma unroll
+    for (int w = 0; w < N / 32; w++) x += shared[w];
+    __syncthreads();
+    return x;
+}
+
+// The tokens that the mask keeps: of a flat batch, of rows by a warp each, of long ones by the blocks (into counts that are 0
+// then), and what totals[] says of them.
+__global__ void __launch_bounds__(THREADS) count_kernel(Args a) {
+    __shared__ int shared[THREADS / 32];
+    pdl_launch();
     pdl_wait();
-    const float flat = inverse(a.mask ? a.counts[0] : a.count), rows_inv = inverse(a.mask ? a.counts[0] : a.rows);
+    const int lane = threadIdx.x & 31, warps = (int)gridDim.x * (THREADS / 32), at = (int)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5);
+    int sum = 0;
+    if (!a.by_row) {
+        if (a.ld_mask == a.length || a.rows == 1) {
+            sum = count_bytes(a.mask, a.count, (int)blockIdx.x * THREADS + threadIdx.x, (int)gridDim.x * THREADS);
+        } else
+            for (int64_t row = at; row < a.rows; row += warps) sum += count_bytes(a.mask + row * a.ld_mask, a.length, lane, 32);
+    } else if (a.length <= LONG) {
+        for (int64_t row = at; row < a.rows; row += warps) {
+            const int n = __reduce_add_sync(0xffffffffu, count_bytes(a.mask + row * a.ld_mask, a.length, lane, 32));
+            if (lane == 0) a.counts[row] = n;
+            sum += lane == 0 && n;
+        }
+    } else {
+        const int64_t pieces = (a.length + PIECE - 1) / PIECE;
+        for (int64_t p = at; p < a.rows * pieces; p += warps) {
+            const int64_t row = p / pieces, c0 = (p - row * pieces) * PIECE;
+            const int n = __reduce_add_sync(0xffffffffu, count_bytes(a.mask + row * a.ld_mask + c0, min((int64_t)PIECE, a.length - c0), lane, 32));
+            // whoever adds the row's first tokens counts the row
+            if (lane == 0 && n && atomicAdd(a.counts + row, n) == 0) sum++;
+        }
+    }
+    sum = block_sum<THREADS>(sum, shared);
+    if (threadIdx.x == 0) a.totals[blockIdx.x] = sum;
+}
+
+template <int V> __global__ void __launch_bounds__(THREADS, 3) loss_kernel(Args a) {
+    __shared__ double shared[THREADS / 32][TERMS];
+    __shared__ int counted[THREADS / 32];
+    pdl_launch();
+    Pass<V> pass(a, (int64_t)blockIdx.x * THREADS + threadIdx.x, (int64_t)gridDim.x * THREADS);  // not what the launch before this writes
+    pdl_wait();
+    int n = 0;
+    if (a.mask) {
+        for (int b = threadIdx.x; b < a.count_blocks; b += THREADS) n += a.totals[b];
+        n = block_sum<THREADS>(n, counted);
+    }
     double total[TERMS] = {};
-    pass<V>(a, a.counts + 1, flat, rows_inv, (int64_t)blockIdx.x * THREADS + threadIdx.x, (int64_t)gridDim.x * THREADS, total);
+    pass.run(a, a.counts, inverse(a.mask ? n : a.count), inverse(a.mask ? n : a.rows), total);
     join<THREADS>(total, shared);
     if (threadIdx.x == 0)
         for (int k = 0; k < TERMS; k++) a.parts[(int64_t)blockIdx.x * TERMS + k] = total[k];
@@ -221,34 +291,50 @@ __global__ void __launch_bounds__(1024) finish_kernel(Args a) {
     if (threadIdx.x == 0) finish(a, total);
 }
 
-// All of a small batch in one block.
+// All of a small batch by one cluster.
 template <int V> __global__ void __launch_bounds__(SMALL_THREADS) small_kernel(Args a) {
-    __shared__ double shared[SMALL_THREADS / 32][TERMS];
-    __shared__ int counts[1 + SMALL_ROWS];
+    __shared__ double shared[SMALL_THREADS / 32][TERMS], blocks[MOST_TOGETHER][TERMS];
+    __shared__ int counts[SMALL_ROWS], counted[SMALL_THREADS / 32];
+    uint32_t rank, together;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(together));
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // all blocks have begun before one writes to the first
+    Pass<V> pass(a, rank * SMALL_THREADS + threadIdx.x, together * SMALL_THREADS);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int n = 0;
     if (a.mask) {
-        for (int i = threadIdx.x; i < 1 + (a.by_row ? (int)a.rows : 0); i += SMALL_THREADS) counts[i] = 0;
-        __syncthreads();
-        int sum = 0;
-        for (int i = threadIdx.x; i < (int)a.count; i += SMALL_THREADS) {
-            const int row = i / (int)a.length;
-            if (a.mask[row * a.ld_mask + (i - row * (int)a.length)]) {
-                if (!a.by_row)
-                    sum++;
-                else if (atomicAdd(counts + 1 + row, 1) == 0)
-                    atomicAdd(counts, 1);
+        if (!a.by_row && (a.ld_mask == a.length || a.rows == 1)) {
+            n = count_bytes(a.mask, a.count, threadIdx.x, SMALL_THREADS);
+        } else {
+            for (int row = warp; row < (int)a.rows; row += SMALL_THREADS / 32) {
+                const int k = __reduce_add_sync(0xffffffffu, count_bytes(a.mask + row * a.ld_mask, a.length, lane, 32));
+                if (lane == 0) {
+                    counts[row] = k;
+                    n += a.by_row ? k > 0 : k;
+                }
             }
         }
-        if (!a.by_row) {
-            sum = __reduce_add_sync(0xffffffffu, sum);
-            if ((threadIdx.x & 31) == 0 && sum) atomicAdd(counts, sum);
-        }
-        __syncthreads();
+        n = block_sum<SMALL_THREADS>(n, counted);  // and the rows' counts are there
     }
-    const float flat = inverse(a.mask ? counts[0] : a.count), rows_inv = inverse(a.mask ? counts[0] : a.rows);
     double total[TERMS] = {};
-    pass<V>(a, counts + 1, flat, rows_inv, threadIdx.x, SMALL_THREADS, total);
+    pass.run(a, counts, inverse(a.mask ? n : a.count), inverse(a.mask ? n : a.rows), total);
     join<SMALL_THREADS>(total, shared);
-    if (threadIdx.x == 0) finish(a, total);
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (threadIdx.x == 0) {
+        uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(blocks[rank])), to;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"(at));
+        for (int k = 0; k < TERMS; k++) asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(to + 8 * k), "d"(total[k]) : "memory");
+    }
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (rank == 0 && threadIdx.x == 0) {
+        for (int k = 0; k < TERMS; k++) {
+            total[k] = 0.;
+            for (uint32_t b = 0; b < together; b++) total[k] += blocks[b][k];
+        }
+        finish(a, total);
+    }
 }
 
 static bool is_small(int64_t rows, int64_t count) { return count <= SMALL && rows <= SMALL_ROWS; }
@@ -265,7 +351,7 @@ static bool rows_ok(const void *p, int64_t ld, int64_t rows, int64_t length, boo
 extern "C" int64_t d1_policy_loss_work_bytes(int64_t rows, int64_t length) {
     if (rows < 0 || length < 0 || length > INT32_MAX || (length && rows > ((int64_t)1 << 40) / length)) return -1;
     if (d1::pl::is_small(rows, rows * length)) return 0;
-    return d1::pl::PART_BYTES + 4 * (1 + rows);
+    return d1::pl::PART_BYTES + 4 * (d1::pl::BLOCKS + rows);
 }
 
 extern "C" int d1_policy_loss(const float *logp, int64_t ld_logp, const float *old_logp, int64_t ld_old,
@@ -306,28 +392,36 @@ extern "C" int d1_policy_loss(const float *logp, int64_t ld_logp, const float *o
     a.kl = (float)kl_coef, a.ent = (float)ent_coef, a.by_row = by_row != 0;
     a.loss = loss, a.stats = stats, a.dlogp = dlogp, a.dentropy = dentropy;
     a.parts = (double *)work;
-    a.counts = work ? (int *)((char *)work + PART_BYTES) : nullptr;
+    a.totals = work ? (int *)((char *)work + PART_BYTES) : nullptr;
+    a.counts = work ? a.totals + BLOCKS : nullptr;
     const cudaStream_t s = (cudaStream_t)stream;
     const auto flat = [&](const void *p, int64_t ld, int align) { return !p || (ld == length || rows == 1) && aligned_to(align, p); };
     const bool four = count % 4 == 0 && flat(logp, ld_logp, 16) && flat(old_logp, ld_old, 16) &&
                       (per_row || flat(advantage, ld_advantage, 16)) && flat(ref_logp, ld_ref, 16) &&
                       flat(entropy, ld_entropy, 16) && flat(mask, ld_mask, 4) && aligned_to(16, dlogp, dentropy);
+    cudaLaunchAttribute attr;
     if (is_small(rows, count)) {
-        if (four)
-            small_kernel<4><<<1, SMALL_THREADS, 0, s>>>(a);
-        else
-            small_kernel<1><<<1, SMALL_THREADS, 0, s>>>(a);
-        return (int)cudaGetLastError();
+        int together = 1;
+        while (together < MOST_TOGETHER && together * SMALL_THREADS * 4 < count) together *= 2;
+        cudaLaunchConfig_t cfg = pdl_config(dim3(together), dim3(SMALL_THREADS), 0, s, &attr);
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = together;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        return (int)cudaLaunchKernelEx(&cfg, four ? small_kernel<4> : small_kernel<1>, a);
     }
     const int64_t want = (count + THREADS * 4 - 1) / (THREADS * 4);
     a.blocks = (int)(want < BLOCKS ? want : BLOCKS);
-    cudaLaunchAttribute attr;
     cudaLaunchConfig_t cfg = pdl_config(dim3(a.blocks), dim3(THREADS), 0, s, &attr);
     if (mask) {
-        if (cudaError_t e = cudaMemsetAsync(a.counts, 0, (size_t)(4 * (by_row ? 1 + rows : 1)), s)) return (int)e;
-        const int64_t pieces = rows * ((length + 1023) / 1024), blocks = (pieces + 7) / 8;
-        count_kernel<<<(unsigned)(blocks < SMS * 8 ? blocks : SMS * 8), THREADS, 0, s>>>(a);
-        if (cudaError_t e = cudaGetLastError()) return (int)e;
+        if (by_row && length > LONG)
+            if (cudaError_t e = cudaMemsetAsync(a.counts, 0, (size_t)(4 * rows), s)) return (int)e;
+        // a warp for each row, or 16 bytes a thread
+        const int64_t blocks = by_row || !flat(mask, ld_mask, 1) ? (rows * ((length + PIECE - 1) / PIECE) + 7) / 8 : (count + THREADS * 16 - 1) / (THREADS * 16);
+        a.count_blocks = (int)(blocks < BLOCKS ? blocks : BLOCKS);
+        cudaLaunchConfig_t first = cfg;
+        first.gridDim = dim3(a.count_blocks);
+        first.numAttrs = 0;
+        if (cudaError_t e = cudaLaunchKernelEx(&first, count_kernel, a)) return (int)e;
     } else
         cfg.numAttrs = 0;
     if (cudaError_t e = cudaLaunchKernelEx(&cfg, four ? loss_kernel<4> : loss_kernel<1>, a)) return (int)e;
