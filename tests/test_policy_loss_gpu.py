@@ -1,7 +1,7 @@
 """The clipped policy loss (d1.policy_loss) against its formula in 64 bits.
 
 Tolerances. delta and d are differences rounded once (2^-24 of themselves, which e^delta passes on as
-|delta| 2^-24 of itself), expf and expm1f are off by 1 ulp, a weight is 1 / n rounded up to twice, and
+|delta| 2^-24 of itself, once more where e^delta is 2^(delta log2 e)), that power of two is off by 2^-22, a weight is 1 / n rounded up to twice, and
 products and sums round once each: under 8 half steps of each term beside |delta| or |d|. Doubled below. The loss
 adds the terms' errors: 2^-24 (16 + 2 |delta|) of the sum of their magnitudes.
 """
