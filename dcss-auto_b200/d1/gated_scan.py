@@ -36,8 +36,9 @@ _FLAGS = (torch.bool, torch.uint8)
 
 def _steps(t, name):
     """(address, step pitch, sequence pitch) of t as [T, B, D] with contiguous channels; nothing is copied."""
-    if t.dim() == 3:
-        st, sb, sd = t.stride()
+    strides = t.stride()
+    if len(strides) == 3:
+        st, sb, sd = strides
         if sd != 1 and t.shape[2] > 1:
             raise ValueError(f'{name}: the last dimension must be contiguous')
         return t.data_ptr(), st, sb
@@ -91,6 +92,8 @@ def _sizes(x, form):
 
 
 def _work(T, B, D, device):
+    if T <= 32:  # not cut into chunks
+        return None
     size = library().d1_gated_scan_work_bytes(T, B, D)
     if size < 0:
         raise ValueError(f'{T} steps of {B} sequences of {D} channels are out of range')
@@ -130,7 +133,7 @@ def _gated_scan(x, gate, h0, reset, form):
     ag, dev = _same(gate, x, 'gate'), x.device
     start = vector(h0, B * D, F32, dev, 'h0')
     flags = _flags(reset, x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    y = x.new_empty(x.shape)
     last = empty_f32(dev, *x.shape[1:])
     work = _work(T, B, D, dev)
     check(library().d1_gated_scan(*ax, *ag, kind, code, T, B, D, start, *flags, y.data_ptr(), last.data_ptr(),
@@ -145,7 +148,7 @@ def gated_scan_backward(dy, x, gate, y, h0=None, reset=None, dlast=None, form='a
     ag, ay, ad, dev = _same(gate, x, 'gate'), _same(y, x, 'y'), _same(dy, x, 'dy'), x.device
     first, end = vector(h0, B * D, F32, dev, 'h0'), vector(dlast, B * D, F32, dev, 'dlast')
     flags = _flags(reset, x)
-    dx, dgate = (torch.empty(x.shape, dtype=x.dtype, device=dev) for _ in range(2))
+    dx, dgate = x.new_empty(x.shape), x.new_empty(x.shape)
     dh0 = empty_f32(dev, *x.shape[1:])
     work = _work(T, B, D, dev)
     check(library().d1_gated_scan_backward(*ad, *ax, *ag, *ay, kind, code, T, B, D, first, end, *flags, dx.data_ptr(),

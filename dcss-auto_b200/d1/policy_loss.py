@@ -40,20 +40,24 @@ class PolicyLoss(NamedTuple):
     dentropy: torch.Tensor = None  # float32, by entropy
 
 
-def _floats(t, shape, device, name):
+def _floats(t, like, ld, shape, device, name):
+    """(address, row pitch) of t, whose rows lie as those of `like` (ld) more often than not."""
     if t is None:
         return None, 0
-    if t.dtype is not torch.float32 or t.shape != shape or t.device != device:
+    if t.dtype is torch.float32 and t.device == device and t.shape == shape:
+        if t.stride() == like:
+            return t.data_ptr(), ld
+    else:
         raise ValueError(f'{name} must be float32 {tuple(shape)} on {device}, not {t.dtype} {tuple(t.shape)} on {t.device}')
     p, _, _, ld = matrix(t, name)
     return p, ld
 
 
-def _advantage(t, shape, device):
+def _advantage(t, like, ld, shape, device):
     """(address, row pitch, whether it is one number a row)."""
     if t.shape == shape or t.dim() != len(shape) - 1:
-        return *_floats(t, shape, device, 'advantage'), 0
-    p, ld = _floats(t.unsqueeze(-1), (*shape[:-1], 1), device, 'advantage')
+        return *_floats(t, like, ld, shape, device, 'advantage'), 0
+    p, ld = _floats(t.unsqueeze(-1), None, 0, (*shape[:-1], 1), device, 'advantage')
     return p, ld, 1
 
 
@@ -102,10 +106,11 @@ def _policy_loss(logp, entropy, old_logp, advantage, ref_logp, mask, low, high, 
         pm, _, _, ldm = matrix(mask, 'mask')
     else:
         pm, ldm = None, 0
-    old, adv = _floats(old_logp, shape, dev, 'old_logp'), _advantage(advantage, shape, dev)
-    ref, ent = _floats(ref_logp, shape, dev, 'ref_logp'), _floats(entropy, shape, dev, 'entropy')
+    as_logp = logp.stride(), ld, shape, dev
+    old, adv = _floats(old_logp, *as_logp, 'old_logp'), _advantage(advantage, *as_logp)
+    ref, ent = _floats(ref_logp, *as_logp, 'ref_logp'), _floats(entropy, *as_logp, 'entropy')
     lib = library()
-    size = lib.d1_policy_loss_work_bytes(rows, length)
+    size = 0 if rows * length <= 2048 else lib.d1_policy_loss_work_bytes(rows, length)  # (a small batch needs none)
     if size < 0 or (mask is not None and rows * length > 2 ** 31 - 1):
         raise ValueError(f'{rows} rows of {length} tokens are out of range')
     work = empty_f32(dev, (size + 3) // 4) if size else None
