@@ -137,9 +137,12 @@ template <class T, int V, bool SUM, bool BACK, int PART> struct Walk {
     }
 };
 
+// Blocks of a kernel that an SM holds at once (their registers are limited to that).
+constexpr int blocks_of(int V, bool back, int part) { return V == 1 ? (back && part ? 5 : 6) : back && part ? 3 : 5; }
+
 // PART 0: reduce a chunk; 1: walk it. A thread has V channels of one sequence in one chunk of the time.
 template <class T, int V, bool SUM, bool BACK, int PART, int U>
-__global__ void __launch_bounds__(THREADS, V == 1 ? (BACK && PART == 1 ? 5 : 6) : BACK && PART == 1 ? 3 : 5) scan_kernel(Args<T> a) {
+__global__ void __launch_bounds__(THREADS, blocks_of(V, BACK, PART)) scan_kernel(Args<T> a) {
     pdl_wait();
     const int64_t index = (int64_t)blockIdx.x * THREADS + threadIdx.x;
     const int order = (int)(index / a.lanes);
@@ -318,18 +321,22 @@ __global__ void __launch_bounds__(CARRY_RUNS * CARRY_CHANNELS) carry_kernel(floa
         }
 }
 
-// Chunks that the time is cut into: 1 where the channels alone give an SM some hundred threads of four.
-// By the number of channels alone, whatever the vectors' width is.
-static int chunks_of(int64_t T, int64_t C) {
-    const int64_t want = (int64_t)SMS * 4096 / (C < 1 ? 1 : C), most = (T + 31) / 32;
-    int64_t n = want < 4 ? 1 : want < most ? want : most;
-    if (n > MOST_CHUNKS) n = MOST_CHUNKS;
-    return (int)(n < 1 ? 1 : n);
+// Chunks that the time is cut into: as many as make one wave of threads, each with 32 steps at least. 1 where that
+// would be two: a third of a wave that reads once is as fast as a whole one that reads twice.
+static int chunks_of(int64_t T, int64_t lanes, int blocks) {
+    const int64_t want = (int64_t)SMS * THREADS * blocks / (lanes < 1 ? 1 : lanes), most = (T + 31) / 32;
+    const int64_t n = want < 3 ? 1 : want < most ? want : most;
+    return (int)(n < 1 ? 1 : n < MOST_CHUNKS ? n : MOST_CHUNKS);
 }
 
 template <class T, int V, bool SUM, bool BACK> static int run(Args<T> &a, cudaStream_t s) {
     constexpr int U = 4;
     a.lanes = a.B * a.D / V;
+    a.chunks = chunks_of(a.T_, a.lanes, blocks_of(V, BACK, 1));
+    a.size = (a.T_ + a.chunks - 1) / a.chunks;
+    a.chunks = (int)((a.T_ + a.size - 1) / a.size);
+    if (a.size > INT32_MAX) return D1_ERR_TOO_LARGE;
+    if (a.chunks > 1 && !a.carry) return D1_ERR_BAD_ARGUMENT;
     const int64_t blocks = (a.lanes * a.chunks + THREADS - 1) / THREADS;
     if (blocks > INT32_MAX) return D1_ERR_TOO_LARGE;
     cudaLaunchAttribute attr;
@@ -353,12 +360,8 @@ template <class T> static bool vectors(const Span<const T> &s) {
 
 template <class T, bool BACK> static int any(Args<T> a, int form, void *work, cudaStream_t s) {
     constexpr int V = 8 / sizeof(T);
-    a.chunks = chunks_of(a.T_, a.B * a.D);
-    a.size = (a.T_ + a.chunks - 1) / a.chunks;
-    a.chunks = (int)((a.T_ + a.size - 1) / a.size);
-    if (a.size > INT32_MAX) return D1_ERR_TOO_LARGE;
     a.carry = (float2 *)work;
-    if (a.chunks > 1 && (!work || !aligned_to(8, work))) return D1_ERR_BAD_ARGUMENT;
+    if (!aligned_to(8, work)) return D1_ERR_BAD_ARGUMENT;
     const bool wide = a.D % V == 0 && vectors(a.gate) && vectors(a.x) && aligned_to(8, a.out) &&
                       (!BACK || (vectors(a.dy) && vectors(a.y) && aligned_to(8, a.dgate)));
     if (form == D1_SCAN_SUM) return wide ? run<T, V, true, BACK>(a, s) : run<T, 1, true, BACK>(a, s);
@@ -385,8 +388,14 @@ static bool stride_ok(int64_t s) { return s >= 0 && s <= ((int64_t)1 << 42); }
 extern "C" int64_t d1_gated_scan_work_bytes(int64_t T, int64_t B, int64_t D) {
     using namespace d1::gs;
     if (!shape_ok(T, B, D)) return -1;
-    const int chunks = chunks_of(T, B * D);
-    return chunks > 1 ? 8 * chunks * B * D : 0;
+    // of any width, direction and type
+    int64_t most = 0;
+    for (const int V : {1, 2, 4})
+        for (const bool back : {false, true}) {
+            const int chunks = chunks_of(T, B * D / V, blocks_of(V, back, 1));
+            if (chunks > 1 && chunks > most) most = chunks;
+        }
+    return 8 * most * B * D;
 }
 
 extern "C" int d1_gated_scan(const void *x, int64_t x_t, int64_t x_b, const void *gate, int64_t gate_t, int64_t gate_b,
