@@ -18,7 +18,8 @@
 //
 // The weights need the mask's counts before any token can be finished. Up to 32,768 tokens are a cluster's: each of its blocks
 // counts the whole mask and takes a part of the tokens, the first one adds the blocks' sums. More have a launch ahead
-// that counts (a byte a token, where the main pass reads 13 and more), and one after it that adds.
+// that counts (a byte a token, where the main pass reads 13 and more); without a mask it only clears the count of
+// blocks that are done, by which the last one knows that it is to add the blocks' sums.
 #include <math.h>
 
 #include "d1_common.cuh"
@@ -31,7 +32,8 @@ namespace pl {
 
 constexpr int SMS = 148, THREADS = 256, BLOCKS = SMS * 3, TERMS = 5;
 constexpr int SMALL = 32768, SMALL_THREADS = 512, SMALL_ROWS = 2048, MOST_TOGETHER = 8;  // a cluster's batch
-constexpr int PIECE = 4096, LONG = 16384;  // tokens of a row that a warp counts; of a row that is too long for one block
+constexpr int PIECE = 4096, LONG = 16384;  // tokens of a row too long for one warp that a warp counts; of such a row
+constexpr int TEAM = 4;  // warps that count a row of more than 1,024 tokens
 
 struct Rows {  // fp32 [rows, length]: element (r, i) at p[r * ld + i * step]
     const float *p;
@@ -53,6 +55,7 @@ struct Args {
     double *parts;                      // [blocks][TERMS]
     int *counts;                        // tokens of row r (by_row)
     int *totals;                        // [count_blocks] tokens, or rows that have any
+    unsigned *done;                     // blocks of the main pass that are done
     int blocks, count_blocks;
 };
 
@@ -242,17 +245,33 @@ __global__ void __launch_bounds__(THREADS) count_kernel(Args a) {
     pdl_wait();
     const int lane = threadIdx.x & 31, warps = (int)gridDim.x * (THREADS / 32), at = (int)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5);
     int sum = 0;
-    if (!a.by_row) {
+    if (!a.mask) {
+    } else if (!a.by_row) {
         if (a.ld_mask == a.length || a.rows == 1) {
             sum = count_bytes(a.mask, a.count, (int)blockIdx.x * THREADS + threadIdx.x, (int)gridDim.x * THREADS);
         } else
             for (int64_t row = at; row < a.rows; row += warps) sum += count_bytes(a.mask + row * a.ld_mask, a.length, lane, 32);
-    } else if (a.length <= LONG) {
+    } else if (a.length <= 1024) {
         for (int64_t row = at; row < a.rows; row += warps) {
             const int n = __reduce_add_sync(0xffffffffu, count_bytes(a.mask + row * a.ld_mask, a.length, lane, 32));
             if (lane == 0) a.counts[row] = n;
             sum += lane == 0 && n;
         }
+    } else if (a.length <= LONG) {  // TEAM warps a row, two rows a block
+        const int team = threadIdx.x / (32 * TEAM);
+        for (int64_t row = (int64_t)blockIdx.x * 2; row < a.rows; row += (int64_t)gridDim.x * 2) {
+            int n = 0;
+            if (row + team < a.rows) n = __reduce_add_sync(0xffffffffu, count_bytes(a.mask + (row + team) * a.ld_mask, a.length, threadIdx.x % (32 * TEAM), 32 * TEAM));
+            __syncthreads();
+            if (lane == 0) shared[threadIdx.x >> 5] = n;
+            __syncthreads();
+            if (threadIdx.x % (32 * TEAM) == 0 && row + team < a.rows) {
+                n = shared[TEAM * team] + shared[TEAM * team + 1] + shared[TEAM * team + 2] + shared[TEAM * team + 3];
+                a.counts[row + team] = n;
+                sum += n > 0;
+            }
+        }
+        __syncthreads();
     } else {
         const int64_t pieces = (a.length + PIECE - 1) / PIECE;
         for (int64_t p = at; p < a.rows * pieces; p += warps) {
@@ -264,6 +283,7 @@ __global__ void __launch_bounds__(THREADS) count_kernel(Args a) {
     }
     sum = block_sum<THREADS>(sum, shared);
     if (threadIdx.x == 0) a.totals[blockIdx.x] = sum;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.done = 0;
 }
 
 template <int V> __global__ void __launch_bounds__(THREADS, 3) loss_kernel(Args a) {
@@ -280,17 +300,19 @@ template <int V> __global__ void __launch_bounds__(THREADS, 3) loss_kernel(Args 
     double total[TERMS] = {};
     pass.run(a, a.counts, inverse(a.mask ? n : a.count), inverse(a.mask ? n : a.rows), total);
     join<THREADS>(total, shared);
-    if (threadIdx.x == 0)
+    __shared__ bool last;
+    if (threadIdx.x == 0) {
         for (int k = 0; k < TERMS; k++) a.parts[(int64_t)blockIdx.x * TERMS + k] = total[k];
-}
-
-__global__ void __launch_bounds__(1024) finish_kernel(Args a) {
-    __shared__ double shared[32][TERMS];
-    pdl_wait();
-    double total[TERMS] = {};
-    for (int b = threadIdx.x; b < a.blocks; b += 1024)
-        for (int k = 0; k < TERMS; k++) total[k] += a.parts[(int64_t)b * TERMS + k];
-    join<1024>(total, shared);
+        __threadfence();
+        last = atomicAdd(a.done, 1u) == gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    for (int k = 0; k < TERMS; k++) total[k] = 0.;
+    for (int b = threadIdx.x; b < a.blocks; b += THREADS)
+        for (int k = 0; k < TERMS; k++) total[k] += __ldcg(a.parts + (int64_t)b * TERMS + k);
+    join<THREADS>(total, shared);
     if (threadIdx.x == 0) finish(a, total);
 }
 
@@ -354,7 +376,7 @@ static bool rows_ok(const void *p, int64_t ld, int64_t rows, int64_t length, boo
 extern "C" int64_t d1_policy_loss_work_bytes(int64_t rows, int64_t length) {
     if (rows < 0 || length < 0 || length > INT32_MAX || (length && rows > ((int64_t)1 << 40) / length)) return -1;
     if (d1::pl::is_small(rows, rows * length)) return 0;
-    return d1::pl::PART_BYTES + 4 * (d1::pl::BLOCKS + rows);
+    return d1::pl::PART_BYTES + 4 * (1 + d1::pl::BLOCKS + rows);
 }
 
 extern "C" int d1_policy_loss(const float *logp, int64_t ld_logp, const float *old_logp, int64_t ld_old,
@@ -396,7 +418,8 @@ extern "C" int d1_policy_loss(const float *logp, int64_t ld_logp, const float *o
     a.kl = (float)kl_coef, a.ent = (float)ent_coef, a.by_row = by_row != 0;
     a.loss = loss, a.stats = stats, a.dlogp = dlogp, a.dentropy = dentropy;
     a.parts = (double *)work;
-    a.totals = work ? (int *)((char *)work + PART_BYTES) : nullptr;
+    a.done = work ? (unsigned *)((char *)work + PART_BYTES) : nullptr;
+    a.totals = work ? (int *)a.done + 1 : nullptr;
     a.counts = work ? a.totals + BLOCKS : nullptr;
     const cudaStream_t s = (cudaStream_t)stream;
     const auto flat = [&](const void *p, int64_t ld, int align) { return !p || (ld == length || rows == 1) && aligned_to(align, p); };
@@ -416,21 +439,18 @@ extern "C" int d1_policy_loss(const float *logp, int64_t ld_logp, const float *o
     const int64_t want = (count + THREADS * 4 - 1) / (THREADS * 4);
     a.blocks = (int)(want < BLOCKS ? want : BLOCKS);
     cudaLaunchConfig_t cfg = pdl_config(dim3(a.blocks), dim3(THREADS), 0, s, &attr);
-    if (mask) {
-        if (by_row && length > LONG)
-            if (cudaError_t e = cudaMemsetAsync(a.counts, 0, (size_t)(4 * rows), s)) return (int)e;
-        // a warp for each row, or 16 bytes a thread
-        const int64_t blocks = by_row || !flat(mask, ld_mask, 1) ? (rows * ((length + PIECE - 1) / PIECE) + 7) / 8 : (count + THREADS * 16 - 1) / (THREADS * 16);
-        a.count_blocks = (int)(blocks < BLOCKS ? blocks : BLOCKS);
-        cudaLaunchConfig_t first = cfg;
-        first.gridDim = dim3(a.count_blocks);
-        first.numAttrs = 0;
-        if (cudaError_t e = cudaLaunchKernelEx(&first, count_kernel, a)) return (int)e;
-    } else
-        cfg.numAttrs = 0;
-    if (cudaError_t e = cudaLaunchKernelEx(&cfg, four ? loss_kernel<4> : loss_kernel<1>, a)) return (int)e;
-    cfg.gridDim = dim3(1);
-    cfg.blockDim = dim3(1024);
-    cfg.numAttrs = 1;
-    return (int)cudaLaunchKernelEx(&cfg, finish_kernel, a);
+    if (mask && by_row && length > LONG)
+        if (cudaError_t e = cudaMemsetAsync(a.counts, 0, (size_t)(4 * rows), s)) return (int)e;
+    // 16 bytes a thread; a row a warp, or two a block; a piece a warp
+    const int64_t blocks = !mask ? 1
+                           : !by_row ? (flat(mask, ld_mask, 1) ? (count + THREADS * 16 - 1) / (THREADS * 16) : (rows + 7) / 8)
+                           : length <= 1024 ? (rows + 7) / 8
+                           : length <= LONG ? (rows + 1) / 2
+                                            : (rows * ((length + PIECE - 1) / PIECE) + 7) / 8;
+    a.count_blocks = (int)(blocks < BLOCKS ? blocks : BLOCKS);
+    cudaLaunchConfig_t before = cfg;
+    before.gridDim = dim3(a.count_blocks);
+    before.numAttrs = 0;
+    if (cudaError_t e = cudaLaunchKernelEx(&before, count_kernel, a)) return (int)e;
+    return (int)cudaLaunchKernelEx(&cfg, four ? loss_kernel<4> : loss_kernel<1>, a);
 }

@@ -34,8 +34,8 @@ def test_refusals(lib):
 def test_work_bytes(lib):
     size = lib.d1_policy_loss_work_bytes
     assert size(-1, 1) == size(1, -1) == size(1, 1 << 31) == size(1 << 41, 1) == -1
-    assert size(0, 5) == size(1, 16384) == size(2048, 8) == 0
-    assert size(2049, 1) > 4 * 2049 and size(1, 16385) > 0
+    assert size(0, 5) == size(1, 32768) == size(2048, 16) == 0
+    assert size(2049, 1) > 4 * 2049 and size(1, 32769) > 0
 
 
 def test_host_tensors_are_refused():
