@@ -27,7 +27,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from ._lib import check, library, stream_of
-from ._rows import empty_f32, type_of, vector
+from ._rows import empty_f32, empty_like, type_of, vector
 
 F32 = torch.float32
 FORMS = {'average': 0, 'sum': 1}  # D1_SCAN_* of d1.h
@@ -67,6 +67,8 @@ def _flags(reset, x):
     """(address, step pitch, sequence pitch) of the resets."""
     if reset is None:
         return None, 0, 0
+    if x.dim() == 3 and reset.dtype in _FLAGS and reset.shape == (x.shape[0], x.shape[1]) and reset.device == x.device:
+        return reset.data_ptr(), *reset.stride()
     if reset.dtype not in _FLAGS or reset.shape != x.shape[:-1] or reset.device != x.device:
         raise ValueError(f'reset must be a bool or uint8 tensor {tuple(x.shape[:-1])} on {x.device}, not '
                          f'{reset.dtype} {tuple(reset.shape)} on {reset.device}')
@@ -133,8 +135,8 @@ def _gated_scan(x, gate, h0, reset, form):
     ag, dev = _same(gate, x, 'gate'), x.device
     start = vector(h0, B * D, F32, dev, 'h0')
     flags = _flags(reset, x)
-    y = x.new_empty(x.shape)
-    last = empty_f32(dev, *x.shape[1:])
+    y = empty_like(x)
+    last = torch.empty_like(h0) if h0 is not None and h0.shape == x.shape[1:] else empty_f32(dev, *x.shape[1:])
     work = _work(T, B, D, dev)
     check(library().d1_gated_scan(*ax, *ag, kind, code, T, B, D, start, *flags, y.data_ptr(), last.data_ptr(),
                                   None if work is None else work.data_ptr(), stream_of(x)), 'd1_gated_scan')
@@ -148,8 +150,7 @@ def gated_scan_backward(dy, x, gate, y, h0=None, reset=None, dlast=None, form='a
     ag, ay, ad, dev = _same(gate, x, 'gate'), _same(y, x, 'y'), _same(dy, x, 'dy'), x.device
     first, end = vector(h0, B * D, F32, dev, 'h0'), vector(dlast, B * D, F32, dev, 'dlast')
     flags = _flags(reset, x)
-    dx, dgate = x.new_empty(x.shape), x.new_empty(x.shape)
-    dh0 = empty_f32(dev, *x.shape[1:])
+    dx, dgate, dh0 = empty_like(x), empty_like(x), empty_f32(dev, *x.shape[1:])
     work = _work(T, B, D, dev)
     check(library().d1_gated_scan_backward(*ad, *ax, *ag, *ay, kind, code, T, B, D, first, end, *flags, dx.data_ptr(),
                                            dgate.data_ptr(), dh0.data_ptr(), None if work is None else work.data_ptr(),
