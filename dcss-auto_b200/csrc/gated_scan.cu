@@ -143,7 +143,7 @@ constexpr int blocks_of(int V, bool back, int part) { return V == 1 ? (back && p
 // PART 0: reduce a chunk; 1: walk it. A thread has V channels of one sequence in one chunk of the time.
 template <class T, int V, bool SUM, bool BACK, int PART, int U>
 __global__ void __launch_bounds__(THREADS, blocks_of(V, BACK, PART)) scan_kernel(Args<T> a) {
-    pdl_wait();
+    pdl_launch();
     const int64_t index = (int64_t)blockIdx.x * THREADS + threadIdx.x;
     const int order = (int)(index / a.lanes);
     if (order >= a.chunks) return;
@@ -164,12 +164,6 @@ __global__ void __launch_bounds__(THREADS, blocks_of(V, BACK, PART)) scan_kernel
     }
     w.out = a.out + first * C + c, w.sout = SIGN * C;
     float s[V], prod[V];
-#pragma unroll
-    for (int v = 0; v < V; v++) {
-        prod[v] = 1.f;
-        s[v] = 0.f;
-        if constexpr (PART == 1) s[v] = chunk ? a.carry[chunk * C + c + v].x : a.start ? a.start[c + v] : 0.f;
-    }
     // Resets: where a warp has one sequence and one chunk its lanes look at 32 steps at a time.
     const bool shared = a.reset && a.lanes % 32 == 0 && per % 32 == 0;
     const uint8_t *reset = a.reset ? a.reset + b * a.reset_b + (first + (shared ? SIGN * (int)(threadIdx.x & 31) : 0)) * a.reset_t : nullptr;
@@ -256,6 +250,15 @@ __global__ void __launch_bounds__(THREADS, blocks_of(V, BACK, PART)) scan_kernel
         for (int u = 0; u < U; u++) advance(of[u], cuts >> u & 1, false);
     };
     if (groups) cp = fetch(p, 0);
+    // The launches before this one read what it has read so far, and wrote none of it (the first of them began when all
+    // earlier work was done): its first loads are under way before the states are there.
+    pdl_wait();
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+        prod[v] = 1.f;
+        s[v] = 0.f;
+        if constexpr (PART == 1) s[v] = chunk ? a.carry[chunk * C + c + v].x : a.start ? a.start[c + v] : 0.f;
+    }
     for (int k = 0; k < groups; k += 2) {
         if (k + 1 < groups) cq = fetch(q, k + 1);
         compute(p, cp);
@@ -290,6 +293,7 @@ __device__ __forceinline__ float through(float2 map, float s) { return map.x < 0
 // threads for each, which hold theirs and join them by doubling. (A warp for each of 32 runs of chunks, reading
 // them twice, took 26 us for 2,048 chunks of 256 channels: the latency of its loads.)
 __global__ void __launch_bounds__(CARRY_RUNS * CARRY_CHANNELS) carry_kernel(float2 *carry, const float *start, int64_t C, int chunks) {
+    pdl_launch();
     pdl_wait();
     __shared__ float2 sums[CARRY_RUNS][CARRY_CHANNELS];
     const int run = threadIdx.x / CARRY_CHANNELS, lane = threadIdx.x % CARRY_CHANNELS;
