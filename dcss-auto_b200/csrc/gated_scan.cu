@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(THREADS, blocks_of(V, BACK, PART)) scan_kernel
     for (int v = 0; v < V; v++) {
         prod[v] = 1.f;
         s[v] = 0.f;
-        if constexpr (PART == 1) s[v] = chunk ? a.carry[chunk * C + c + v].x : a.start ? a.start[c + v] : 0.f;
+        if constexpr (PART == 1) s[v] = a.chunks > 1 ? a.carry[chunk * C + c + v].x : a.start ? a.start[c + v] : 0.f;
     }
     for (int k = 0; k < groups; k += 2) {
         if (k + 1 < groups) cq = fetch(q, k + 1);

@@ -89,9 +89,9 @@ __device__ __forceinline__ float token(const Args &a, float logp, float old, flo
     s.t[0] -= w * ((cut ? (over ? a.most : a.least) : r) * adv);
     float g = cut ? 0.f : -adv * r;
     if (a.ref.p) {
-        const float d = ref - logp, k = beyond_linear(d, __expf(d));
+        const float d = ref - logp, grown = __expf(d), k = beyond_linear(d, grown);
         s.t[1] += w * k;
-        g = fmaf(-a.kl, d + k, g);  // e^d - 1
+        g = fmaf(-a.kl, fabsf(d) < 0.5f ? d + k : grown - 1.f, g);  // e^d - 1
     }
     if (a.entropy.p) s.t[2] += w * h;
     if (cut) s.t[3] += w;

@@ -265,6 +265,33 @@ def test_graphs_streams_and_the_default_type():
         torch.set_default_dtype(torch.float32)
 
 
+@pytest.mark.parametrize('T', [3, 900])
+def test_the_state_in_place(T):
+    """The C entries with last in place of h0, and dh0 in place of dlast: the same bits."""
+    from d1._lib import check as ok, library, stream_of
+    from d1.gated_scan import gated_scan, gated_scan_backward
+    x, gate, h0, reset, dy, dlast = inputs((T, 2, 48), torch.bfloat16, rate=0.001)
+    y, last = gated_scan(x, gate, h0, reset=reset)
+    want = gated_scan_backward(dy, x, gate, y, h0, reset=reset, dlast=dlast)
+    lib, at = library(), lambda t: t.data_ptr()
+    work = torch.empty(max(8, lib.d1_gated_scan_work_bytes(T, 2, 48)), dtype=torch.uint8, device='cuda')
+    state, grad, out, dx, dg = h0.clone(), dlast.clone(), torch.empty_like(x), torch.empty_like(x), torch.empty_like(x)
+    ok(lib.d1_gated_scan(at(x), 96, 48, at(gate), 96, 48, 1, 0, T, 2, 48, at(state), at(reset), 2, 1, at(out), at(state), at(work), stream_of(x)))
+    assert torch.equal(out, y) and torch.equal(state, last)
+    ok(lib.d1_gated_scan_backward(at(dy), 96, 48, at(x), 96, 48, at(gate), 96, 48, at(y), 96, 48, 1, 0, T, 2, 48, at(h0), at(grad), at(reset), 2, 1,
+                                  at(dx), at(dg), at(grad), at(work), stream_of(x)))
+    assert torch.equal(dx, want[0]) and torch.equal(dg, want[1]) and torch.equal(grad, want[2])
+
+
+def test_nan_gates_show():
+    from d1.gated_scan import gated_scan
+    x, gate, h0, _, _, _ = inputs((40, 2, 16), torch.bfloat16)
+    gate[20, 1, 3] = float('nan')
+    for form in ('average', 'sum'):
+        y, last = gated_scan(x, gate.clamp(max=0) if form == 'sum' else gate, h0, form=form)
+        assert y[20:, 1, 3].isnan().all() and last[1, 3].isnan() and int(y.isnan().sum()) == 20
+
+
 def test_refusals():
     from d1.gated_scan import gated_scan, gated_scan_backward
     x, gate, h0, reset, dy, dlast = inputs((4, 3, 8), torch.float32)

@@ -190,6 +190,19 @@ def test_ratios_beyond_fp32():
     assert r.loss == math.inf and r.dlogp.tolist() == [0.0, math.inf, 0.0, 0.0]
 
 
+@pytest.mark.parametrize('size', [4, 40000])
+def test_a_reference_far_away(size):
+    """Where the reference holds a token for impossible the KL term is infinite and its gradient kl_coef; far below, the gradient
+    does not cancel."""
+    z = torch.full((size,), -1.0, device='cuda')
+    for away in (-math.inf, -1e30, -3e6, -1e3):
+        ref = z.clone()
+        ref[0] = away
+        r = call(dict(logp=z, old_logp=z, advantage=torch.zeros_like(z), ref_logp=ref, entropy=None, mask=None), kl=0.5)
+        assert abs(float(r.dlogp[0]) * size - 0.5) < 1e-6 and (r.dlogp[1:] == 0).all()
+        assert abs(float(r.stats[1]) * size / -away - 1) < 1e-2 if away > -math.inf else r.stats[1] == math.inf
+
+
 def test_gradient_against_differences():
     """Central differences of 2^-9 in 64-bit steps of fp32 inputs: the loss's own rounding of 2^-22 of about 1 over 2^-8
     and a third derivative's 2^-18: 2e-4. Tokens within 2^-8 of a border are passed over."""
