@@ -22,6 +22,11 @@
 // diagonal are computed and stored, and read transposed for those above. The epilogues hold the rest of the
 // formulas, the last one the step itself. All operands are blocks of 64 x 64 elements (d1_muon.h) that the TMA
 // swizzles on its way to shared memory, as K-major operands or as MN-major ones: X is never transposed.
+//
+// Measured (one B200). 8,192 x 8,192 bf16: 9.97 ms, 1.3 PFLOP/s while the products run (a library product sustains 1.38
+// under the power limit). 72 matrices of 12 layers of 1,024, with masters, momentum and copies: 3.89 ms (floor 1.64). The conv policy's six:
+// 147 us, 17 launches. A pair of CTAs takes 0.43 us for a block of 64 of the sum of its 256 x 256 tile: 32 KB into shared memory and 48 KB read
+// for 512 cycles of the tensor pipe, 640 cycles at 128 bytes each, which bound it.
 #include <cuda.h>
 #include <math.h>
 
