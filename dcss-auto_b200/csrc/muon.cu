@@ -8,15 +8,15 @@
 // with the published coefficients (a, b, c) = (3.4445, -4.7750, 2.0315), which bring
 // every singular value of X between about 0.7 and 1.2.
 //
-// Rounding. The products run on the tensor cores in fp16 with fp32 sums: |X| <= 1.3
-// and its products are bounded too, so that a scale of 2^12 keeps all of them inside fp16's range, and fp16
-// has eight times bf16's precision at the same rate. Singular directions that the update hardly has are
-// amplified by a = 3.4 a step, 485 in five, and with them whatever rounding puts there: of a gradient of low
-// rank the result would be noise to a large part (simulated, rank 32 of 512: 3 % of its norm in fp16, 22 %
-// in bf16). So X is held as a pair hi + lo of fp16, 22 bits, and a X is taken from the pair; the products read hi
-// alone, and the error that they make lies in directions that X has (0.06 % there, 0.2 % of a full-rank one). In a
-// matrix with a side of at most 64, where few roundings average out (up to 1 % in some), A and F are pairs too and a product takes all three
-// terms: it is as good as one in fp32, and its time is the launches' all the same.
+// Rounding. The products run on the tensor cores in fp16 with fp32 sums: X, A and F are bounded (by 1.3, 1.7 and 3.5),
+// so that a scale of 2^12 keeps all of them inside fp16's range, and fp16 has eight times bf16's precision at the same
+// rate. Singular directions that the update hardly has are amplified by a = 3.4 a step, 485 in five, and with them
+// whatever rounding puts there: of a gradient of low rank the result would be noise to a large part (simulated, rank 32 of
+// 512: 3 % of its norm in fp16, 22 % in bf16). So X is held as a pair hi + lo of fp16, 22 bits, and X' = F hi + a lo: where X
+// has nothing F is a, and the pair is carried on as one; elsewhere F lo is not a lo, an error of hi's size, but
+// in directions that X has (0.16 % there, 0.2 % of a full-rank one). In a matrix with a side of at most 64, where few
+// roundings average out (up to 1 % in some), A and F are pairs too and a product takes all three terms: it is as good as
+// one in fp32, and its time is the launches' all the same.
 //
 // The three products of all matrices are one launch each. A and F are symmetric: only the tiles on and below the
 // diagonal are computed and stored, and read transposed for those above. The epilogues hold the rest of the
