@@ -110,10 +110,11 @@ D1_MUON_BOTH int64_t full_tiles(const Matrix &m, int side) { return (int64_t)til
 
 // CTAs that share the sum of `depth` blocks of each of a few tiles: as many as there is room for, while it saves ten
 // blocks' time (the exchange of the parts costs some five).
+inline bool saves(int depth, int parts) { return depth - depth / parts >= 10; }
 inline int parts_for(int64_t tiles, int depth) {
     int parts = 1;
     for (int n = 2; n <= 8; n *= 2)
-        if (tiles * n <= (n == 8 ? 112 : n == 4 ? 128 : 148) && depth - depth / n >= 10) parts = n;  // what clusters find room for at once
+        if (tiles * n <= (n == 8 ? 112 : n == 4 ? 128 : 148) && saves(depth, n)) parts = n;  // what clusters find room for at once
     return parts;
 }
 
@@ -123,14 +124,30 @@ struct Load {
     int64_t symmetric, full;  // tiles
     int depth[2];             // the longest sums, in blocks, of A and of the other products
     double work[3];           // blocks of all sums, by product
+    int64_t matrices;
+    int widest, longest;      // the most tiles along a smaller side, and of one X'
 
     void add(const Matrix &m, int64_t count) {
         const int64_t s = symmetric_tiles(m, side) * count, f = full_tiles(m, side) * count;
         const int terms = m.fine ? 3 : 1, first = (m.tall ? m.rb : m.cb) * terms, others = m.sb * terms;
+        const int wide = tiles_of(m.sb, side), most = (int)full_tiles(m, side);
+        matrices += count;
+        if (wide > widest) widest = wide;
+        if (most > longest) longest = most;
         symmetric += s, full += f;
         work[0] += (double)s * first, work[1] += (double)s * others, work[2] += (double)f * others;
         if (first > depth[0]) depth[0] = first;
         if (others > depth[1]) depth[1] = others;
+    }
+    // CTAs of the cluster that takes each matrix through all products in one launch, 0 where that is not done: every
+    // matrix has one tile of A and no more than two of X' a CTA (128 x 4,000, with four, took 138 us in place of the launches'
+    // 121), and all clusters run at once.
+    int small_together() const {
+        if (side != 2 || widest > 1) return 0;
+        int n = 1;
+        while (n < 8 && (n < longest || (!saves(depth[0], n) && saves(depth[0], 2 * n)))) n *= 2;
+        while (n > 1 && matrices * n > (n == 8 ? 112 : n == 4 ? 128 : 148)) n /= 2;
+        return matrices * n <= 148 && longest <= 2 * n ? n : 0;
     }
     // A block of 64 of the sum takes a pair of CTAs 0.43 us for a tile of 256 x 256, a CTA 0.5 us for one of 128 x 128 (both measured with the
     // GPU full: the one is bound by shared memory, the other by what comes from L2); a pair's launches take 8 us more in all.
@@ -144,7 +161,7 @@ struct Load {
         return sum;
     }
 };
-inline Load load_of(int side) { return Load{side, 0, 0, {0, 0}, {0., 0., 0.}}; }
+inline Load load_of(int side) { return Load{side, 0, 0, {0, 0}, {0., 0., 0.}, 0, 0, 0}; }
 
 // What a plan begins with: sizes of its lists and where they start (bytes).
 struct Plan {

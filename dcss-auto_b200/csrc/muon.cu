@@ -32,6 +32,7 @@
 
 #include <algorithm>
 #include <new>
+#include <type_traits>
 
 #include "d1_common.cuh"
 #include "d1_elem.cuh"
@@ -68,7 +69,8 @@ struct Job {
     float mu;
     int nesterov;
     double lr;
-    int from;  // which hi is read
+    int from;   // which hi is read
+    int steps;
 };
 
 __device__ __forceinline__ Matrix matrix_of(const Job &o, int m) {
@@ -102,7 +104,7 @@ struct Tiles {
     const bool symmetric;
     const int count, step;
     int at;
-    Tile tile, next, next2;
+    Tile next, next2;
     Matrix next_m;
 
     __device__ __forceinline__ Tiles(const Job &o, bool symmetric, int count, int first, int step) : o(o), symmetric(symmetric), count(count), step(step), at(first) {
@@ -110,13 +112,38 @@ struct Tiles {
         next2 = at + step < count ? tile_of(o, symmetric, at + step) : next;
         next_m = matrix_of(o, next.matrix);
     }
-    // The tile to work on; its matrix is `m`.
-    __device__ __forceinline__ void take(Matrix &m) {
+    // The next tile to work on and its matrix; false when there is none.
+    __device__ __forceinline__ bool take(Matrix &m, Tile &tile) {
+        if (at >= count) return false;
         tile = next, m = next_m;
         next = next2;
         at += step;
         if (at < count) next_m = matrix_of(o, next.matrix);
         if (at + step < count) next2 = tile_of(o, symmetric, at + step);
+        return true;
+    }
+};
+
+// The tiles first, first + step, ... of one matrix.
+struct MatrixTiles {
+    const Matrix &matrix;
+    const bool symmetric;
+    int at, step, count, tm, tn;
+
+    __device__ __forceinline__ MatrixTiles(const Matrix &m, bool symmetric, int first, int step) : matrix(m), symmetric(symmetric), at(first), step(step) {
+        tm = tiles_of(symmetric ? m.sb : m.rb, 2), tn = tiles_of(symmetric ? m.sb : m.cb, 2);
+        count = symmetric ? tm * (tm + 1) / 2 : tm * tn;
+    }
+    __device__ __forceinline__ bool take(Matrix &m, Tile &tile) {
+        if (at >= count) return false;
+        int i, j;
+        if (symmetric)
+            symmetric_tile(at, i, j);
+        else
+            grouped_tile(at, tm, tn, i, j);
+        m = matrix, tile.matrix = 0, tile.i = (uint16_t)i, tile.j = (uint16_t)j;
+        at += step;
+        return true;
     }
 };
 
@@ -381,79 +408,43 @@ __device__ __forceinline__ void finish(const Job &o, const Matrix &m, int i0, in
     __syncwarp();
 }
 
-// One product of all matrices: a persistent kernel whose CTAs (PAIR: pairs of CTAs) take tiles of 128 x 128
-// (256 x 256) elements. Warp 0 loads blocks of 64 x 64 elements, 128 rows of each operand a stage, through a ring of
-// five; one thread of warp 1 (of the pair's first CTA) issues the products into one of two accumulators; eight
-// warps read the other one, 128 rows of the tile in each CTA.
+// A CTA's part in the products, role by role: warp 0 loads blocks of 64 x 64 elements, 128 rows of each operand a
+// stage, through a ring of five; one thread of warp 1 (of a pair's first CTA) issues the products into one of two
+// accumulators; eight warps read the other one, 128 rows of the tile in each CTA. Every role goes over the same tiles. The
+// ring and the accumulators go on from one product to the next.
 //
-// SPLIT: a cluster of 2, 4 or 8 CTAs takes a tile of 128 x 128 together, each a part of the sum. Each then owns some of the tile's
-// sixteen units of 32 x 32: the others' parts of them come to its shared memory, and it adds them in the order of the
-// parts. It is for products of few tiles with long sums: X X^T of 512 x 3136 has ten, of 49 blocks each.
-template <int PHASE, int MODE>
-__global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ CUtensorMap map_units, const __grid_constant__ Job o) {
-    constexpr bool PAIR = MODE == PAIRS, SPLIT = MODE == SPLITS;
-    constexpr int SIDES = PAIR ? 4 : 2, COLS = SIDES * SIDE;  // blocks along a tile; columns of an accumulator
-    constexpr bool SYMMETRIC = PHASE == GRAM || PHASE == QUAD;
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + STAGES * STAGE_BYTES + EPI_WARPS * 2 * ROOM), *sides = bars + 2 * STAGES + 4;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sides + 2 * EPI_WARPS);
-    const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES);
-    const uint32_t accf0 = smem_u32(bars + 2 * STAGES), acce0 = smem_u32(bars + 2 * STAGES + 2);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rank = PAIR ? (int)cluster_rank() : 0;
-    const int parts = SPLIT ? (int)cluster_size() : 1, part = SPLIT ? (int)cluster_rank() : 0;
-    const int together = PAIR ? 2 : parts, first = blockIdx.x / together, step = gridDim.x / together;
-    const int tiles = SYMMETRIC ? o.count_symmetric : o.count_full;
-    pdl_launch();
+// A tile is 128 x 128 elements, or 256 x 256 of a PAIR. SPLIT: a cluster of 2, 4 or 8 CTAs takes a tile of 128 x 128 together, each
+// a part of the sum. Each then owns some of the tile's sixteen units of 32 x 32: the others' parts of them come to its shared
+// memory, and it adds them in the order of the parts. It is for products of few tiles with long sums: X X^T of 512 x 3136
+// has ten, of 49 blocks each.
+template <bool PAIR> struct Roles {
+    static constexpr int SIDES = PAIR ? 4 : 2, COLS = SIDES * SIDE;  // blocks along a tile; columns of an accumulator
 
-    if (warp == 0 && lane == 0) {
-        for (int s = 0; s < STAGES; s++) {
-            mbar_init(full0 + 8 * s, 1);
-            mbar_init(empty0 + 8 * s, 1);
-        }
-        for (int b = 0; b < 2; b++) {
-            mbar_init(accf0 + 8 * b, 1);
-            mbar_init(acce0 + 8 * b, (PAIR ? 2 : 1) * EPI_WARPS);
-        }
-        for (int w = 0; w < 2 * EPI_WARPS; w++) mbar_init(smem_u32(sides + w), 1);
-        mbar_init_fence();
-    }
-    if (warp == 1) {
-        if (PAIR) {
-            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(2 * COLS) : "memory");
-            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-        } else {
-            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(2 * COLS) : "memory");
-            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-        }
-    }
-    tc_fence_before();
-    __syncthreads();
-    if (PAIR || SPLIT) cluster_sync();  // the CTAs' barriers exist before any signal between them
-    tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
-    // A plan does not change between the launches of a step (the first of them waits for all that came before), so
-    // that a tile is looked up ahead of pdl_wait(), and the next one during the products of this.
-    if (!o.matrices) pdl_wait();
+    const CUtensorMap &map, &map_units;
+    const Job &o;
+    uint8_t *const smem;
+    const uint32_t full0, empty0, accf0, acce0, sides_at;
+    uint32_t tmem;
+    const int warp, lane, rank;
+    int parts, part;          // of a divided sum
+    int it = 0, in_flight = 0;  // stages that the role has gone through
+    int local = 0;            // accumulators
+    uint32_t turns = 0, pending = 0;  // of an epilogue warp's two rooms, a bit each: the parity of the next wait, a load that is under way
+    bool ok = true;
 
-    if (warp == 0 && lane == 0) {
-        // ---- loads: this CTA's 128 rows of the first operand and 128 of the second
-        int it = 0, in_flight = 0;
-        bool ok = true;
-        Tiles list(o, SYMMETRIC, tiles, first, step);
-        pdl_wait();
-        for (int t = first; t < tiles && ok; t += step) {
-            Matrix m;
-            list.take(m);
-            const Tile tile = list.tile;
-            const Operands p = operands(m, PHASE, o.from);
+    static __device__ __forceinline__ constexpr bool symmetric(int phase) { return phase == GRAM || phase == QUAD; }
+
+    template <int PHASE, bool SPLIT, class List> __device__ __forceinline__ void load(List &list, int from) {
+        Matrix m;
+        Tile tile;
+        while (ok && list.take(m, tile)) {
+            const Operands p = operands(m, PHASE, from);
             const int i0 = tile.i * SIDES + 2 * rank, j0 = tile.j * SIDES + 2 * rank;
             // blocks that exist, of the tile (whose bytes the barrier expects) and of this CTA
             const int all = min(SIDES, p.ni - tile.i * SIDES) + min(SIDES, p.nj - tile.j * SIDES);
             const int na = min(2, p.ni - i0), nb = min(2, p.nj - j0);
-            const int end = part_of(p, part + 1, parts);
-            for (int n = part_of(p, part, parts), k = n % p.nk, term = n / p.nk; n < end; n++, it++) {
+            const int end = part_of(p, SPLIT ? part + 1 : 1, SPLIT ? parts : 1);
+            for (int n = part_of(p, SPLIT ? part : 0, SPLIT ? parts : 1), k = n % p.nk, term = n / p.nk; n < end; n++, it++) {
                 const int s = it % STAGES;
                 const bool a_turned = p.a_half && k / SIDES > tile.i, b_turned = p.b_half && k / SIDES > tile.j;
                 const int ai = a_turned ? p.ak : p.ai, ak = a_turned ? p.ai : p.ak, bj = b_turned ? p.bk : p.bj, bk = b_turned ? p.bj : p.bk;
@@ -479,6 +470,9 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
                 }
             }
         }
+    }
+    // After the last product: what is under way lands before the block leaves.
+    __device__ __forceinline__ void loaded() {
         if (!ok) {
             atomicExch(&g_error, 1);
             if (rank == 0)  // copies under way land before the block leaves
@@ -486,26 +480,23 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
         } else  // and so do the last signals that a stage is free
             for (int i = it > STAGES ? it - STAGES : 0; i < it; i++)
                 mbar_wait(empty0 + 8 * (i % STAGES), (uint32_t)(i / STAGES) & 1u, WAIT_LIMIT);
-    } else if (warp == 1 && lane == 0 && rank == 0) {
-        // ---- products
-        int it = 0, local = 0;
-        bool ok = true;
-        Tiles list(o, SYMMETRIC, tiles, first, step);
-        pdl_wait();
-        for (int t = first; t < tiles && ok; t += step, local++) {
-            Matrix m;
-            list.take(m);
-            const Tile tile = list.tile;
-            const Operands p = operands(m, PHASE, o.from);
+    }
+
+    template <int PHASE, bool SPLIT, class List> __device__ __forceinline__ void multiply(List &list, int from) {
+        Matrix m;
+        Tile tile;
+        for (; ok && list.take(m, tile); local++) {
+            const Operands p = operands(m, PHASE, from);
             constexpr uint32_t BASE = (1u << 4) | ((uint32_t)(COLS >> 3) << 17) | ((uint32_t)(COLS >> 4) << 24);  // fp16, fp32 sums
             const int b = local & 1;
             const uint32_t acc = tmem + (uint32_t)(b * COLS);
             if (local >= 2 && !mbar_wait(acce0 + 8 * b, ((uint32_t)(local >> 1) & 1u) ^ 1u, WAIT_LIMIT)) {
                 atomicExch(&g_error, 2);
+                ok = false;
                 break;
             }
             tc_fence_after();
-            const int begin = part_of(p, part, parts), end = part_of(p, part + 1, parts);
+            const int begin = part_of(p, SPLIT ? part : 0, SPLIT ? parts : 1), end = part_of(p, SPLIT ? part + 1 : 1, SPLIT ? parts : 1);
             for (int n = begin, k = begin % p.nk; n < end; n++, it++) {
                 const int s = it % STAGES;
                 if (!mbar_wait(full0 + 8 * s, (uint32_t)(it / STAGES) & 1u, WAIT_LIMIT)) {
@@ -540,8 +531,11 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
             } else
                 mma_commit(accf0 + 8 * b);
         }
-    } else if (warp >= 2) {
-        // ---- epilogue: warp w holds rows 32 (w % 4) .. + 31 of this CTA's 128, in one half of the columns
+    }
+
+    // Warp w holds rows 32 (w % 4) .. + 31 of this CTA's 128, in one half of the columns.
+    template <int PHASE, bool SPLIT, class List> __device__ __forceinline__ void store(List &list, int from) {
+        constexpr bool SYMMETRIC = symmetric(PHASE);
         const int q = warp & 3, half = (warp - 2) >> 2;
         constexpr int UNITS = COLS / 2 / 32;
         // SPLIT: unit `own` of this warp, if any, is this CTA's; `parts` rooms stand behind one another for it, one
@@ -549,20 +543,14 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
         const int index = 4 * q + 2 * half, own = SPLIT ? ((part - index) & (parts - 1)) : 0;
         uint8_t *const area = smem + STAGES * STAGE_BYTES;
         uint8_t *const rooms = area + (SPLIT ? (index + own) / parts * parts : (warp - 2) * 2) * ROOM;
-        const uint32_t rooms_at = smem_u32(rooms), sides0 = smem_u32(sides + 2 * (warp - 2));
+        const uint32_t rooms_at = smem_u32(rooms), sides0 = sides_at + 16 * (warp - 2);
         bool met = false;
-        uint32_t asked = 0, got = 0;  // loads into the rooms, in turn, and those that have been waited for
-        int local = 0;
-        bool ok = true;
-        Tiles list(o, SYMMETRIC, tiles, first, step);
-        pdl_wait();
-        for (int t = first; t < tiles && ok; t += step, local++) {
-            Matrix m;
-            list.take(m);
-            const Tile tile = list.tile;
-            const Operands p = operands(m, PHASE, o.from);
+        Matrix m;
+        Tile tile;
+        for (; ok && list.take(m, tile); local++) {
+            const Operands p = operands(m, PHASE, from);
             const int b = local & 1, ib = tile.i * SIDES + 2 * rank + (q >> 1), r0 = 32 * (q & 1);
-            const int hi_to = o.from ? m.hi[0] : m.hi[1];
+            const int hi_to = from ? m.hi[0] : m.hi[1];
             const int jb0 = tile.j * SIDES + half * (SIDES / 2);
             // unit u: columns 32 (u & 1) .. + 31 of block (ib, jb0 + u / 2); all warps' lanes agree on how many there are
             const int units = ib < p.ni ? max(0, min(UNITS, 2 * (p.nj - jb0))) : 0;
@@ -571,8 +559,8 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
             const bool reads = PHASE == QUAD || (PHASE != GRAM && !m.fine);
             const auto fetch = [&](int u) {
                 if (!reads || u >= units) return;
-                const uint32_t k = SPLIT ? 0u : asked & 1u;
-                asked++;
+                const uint32_t k = SPLIT ? 0u : (uint32_t)u & 1u;
+                pending |= 1u << k;
                 if (lane) return;
                 const int x = 32 * (u & 1), y = row_of(u);
                 mbar_expect_tx(sides0 + 8 * k, PHASE == QUAD && m.fine ? ROOM : ROOM / 2);
@@ -596,13 +584,14 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
             }
             if (!mbar_wait(accf0 + 8 * b, (uint32_t)(local >> 1) & 1u, WAIT_LIMIT)) {
                 atomicExch(&g_error, 4);
+                ok = false;
                 break;
             }
             tc_fence_after();
             if (SPLIT) {
                 // the others' units go to their owners
                 for (int u = 0; u < units; u++) {
-                    if (u == own || part_of(p, part, parts) == part_of(p, part + 1, parts)) continue;
+                    if (u == own || part_of(p, SPLIT ? part : 0, SPLIT ? parts : 1) == part_of(p, SPLIT ? part + 1 : 1, SPLIT ? parts : 1)) continue;
                     uint32_t v[32];
                     D1X_TMEM_LD32(tmem + (uint32_t)(b * COLS + half * (COLS / 2) + 32 * u) + ((uint32_t)(32 * q) << 16), v);
                     tmem_wait_ld();
@@ -646,9 +635,9 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
                 }
                 const uint32_t k = SPLIT ? 0u : (uint32_t)u & 1u;
                 if (reads) {
-                    const uint32_t parity = SPLIT ? got : got >> 1;
-                    got++;
-                    if (!mbar_wait(sides0 + 8 * k, parity & 1u, WAIT_LIMIT)) {
+                    pending &= ~(1u << k);
+                    turns ^= 1u << k;
+                    if (!mbar_wait(sides0 + 8 * k, (turns >> k & 1u) ^ 1u, WAIT_LIMIT)) {
                         atomicExch(&g_error, 5);
                         ok = false;
                         break;
@@ -746,21 +735,137 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
             }
         }
         // after an error: loads under way land before the block leaves
-        for (; got != asked; got++) mbar_wait(sides0 + (SPLIT ? 0 : 8 * (got & 1u)), (SPLIT ? got : got >> 1) & 1u, WAIT_LIMIT);
+        for (uint32_t k = 0; k < 2; k++)
+            if (pending >> k & 1u) mbar_wait(sides0 + 8 * k, turns >> k & 1u, WAIT_LIMIT);
         if (lane == 0) bulk_wait();
         if (SPLIT && !met) cluster_meet();
     }
-    if (SPLIT && warp < 2) cluster_meet();  // every thread of the cluster comes there once
+};
+
+// Barriers and tensor memory; the cluster's CTAs have begun when it returns.
+template <bool PAIR, bool CLUSTER> __device__ __forceinline__ Roles<PAIR> begin(const CUtensorMap &map, const CUtensorMap &map_units, const Job &o) {
+    constexpr int COLS = Roles<PAIR>::COLS;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *const smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t *const bars = reinterpret_cast<uint64_t *>(smem + STAGES * STAGE_BYTES + EPI_WARPS * 2 * ROOM), *const sides = bars + 2 * STAGES + 4;
+    uint32_t *const tmem_slot = reinterpret_cast<uint32_t *>(sides + 2 * EPI_WARPS);
+    const int rank = PAIR ? (int)cluster_rank() : 0, parts = CLUSTER ? (int)cluster_size() : 1, part = CLUSTER ? (int)cluster_rank() : 0;
+    Roles<PAIR> r{map, map_units, o, smem, smem_u32(bars), smem_u32(bars + STAGES), smem_u32(bars + 2 * STAGES), smem_u32(bars + 2 * STAGES + 2),
+                  smem_u32(sides), 0, (int)threadIdx.x >> 5, (int)threadIdx.x & 31, rank, parts, part};
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; s++) {
+            mbar_init(r.full0 + 8 * s, 1);
+            mbar_init(r.empty0 + 8 * s, 1);
+        }
+        for (int b = 0; b < 2; b++) {
+            mbar_init(r.accf0 + 8 * b, 1);
+            mbar_init(r.acce0 + 8 * b, (PAIR ? 2 : 1) * EPI_WARPS);
+        }
+        for (int w = 0; w < 2 * EPI_WARPS; w++) mbar_init(r.sides_at + 8 * w, 1);
+        mbar_init_fence();
+    }
+    if (r.warp == 1) {
+        if (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(2 * COLS) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(2 * COLS) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (PAIR || CLUSTER) cluster_sync();  // the CTAs' barriers exist before any signal between them
+    tc_fence_after();
+    r.tmem = *tmem_slot;
+    return r;
+}
+template <bool PAIR> __device__ __forceinline__ void end(const Roles<PAIR> &r) {
+    constexpr int COLS = Roles<PAIR>::COLS;
     tc_fence_before();
     __syncthreads();
     if (PAIR) cluster_sync();  // no signal between the CTAs is outstanding past this point
-    if (warp == 1) {
+    if (r.warp == 1) {
         tc_fence_after();
         if (PAIR)
-            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * COLS) : "memory");
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(r.tmem), "r"(2 * COLS) : "memory");
         else
-            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * COLS) : "memory");
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(r.tmem), "r"(2 * COLS) : "memory");
     }
+}
+
+// One product of all matrices by a persistent grid: MODE says what a tile belongs to.
+template <int PHASE, int MODE>
+__global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ CUtensorMap map_units, const __grid_constant__ Job o) {
+    constexpr bool PAIR = MODE == PAIRS, SPLIT = MODE == SPLITS, SYMMETRIC = PHASE == GRAM || PHASE == QUAD;
+    pdl_launch();
+    Roles<PAIR> roles = begin<PAIR, SPLIT>(map, map_units, o);
+    const int together = PAIR ? 2 : roles.parts, first = blockIdx.x / together, step = gridDim.x / together;
+    const int tiles = SYMMETRIC ? o.count_symmetric : o.count_full;
+    // A plan does not change between the launches of a step (the first of them waits for all that came before), so
+    // that a tile is looked up ahead of pdl_wait(), and the next one during the products of this.
+    if (!o.matrices) pdl_wait();
+    if (roles.warp == 0 && roles.lane == 0) {
+        Tiles list(o, SYMMETRIC, tiles, first, step);
+        pdl_wait();
+        roles.template load<PHASE, SPLIT>(list, o.from);
+        roles.loaded();
+    } else if (roles.warp == 1 && roles.lane == 0 && roles.rank == 0) {
+        Tiles list(o, SYMMETRIC, tiles, first, step);
+        pdl_wait();
+        roles.template multiply<PHASE, SPLIT>(list, o.from);
+    } else if (roles.warp >= 2) {
+        Tiles list(o, SYMMETRIC, tiles, first, step);
+        pdl_wait();
+        roles.template store<PHASE, SPLIT>(list, o.from);
+    }
+    if (SPLIT && roles.warp < 2) cluster_meet();  // every thread of the cluster comes there once
+    end(roles);
+}
+
+// All products of small matrices (one tile of A each) in one launch: a cluster takes a matrix through all steps, its CTAs share
+// the tiles of X' and, where it is long, the sum of A. A barrier of the cluster stands where the launches' ends stand otherwise:
+// 64 x 64 68 us in place of 87, 8 x 100 x 800 91 in place of 111. (What is left are the first loads of each product, a microsecond,
+// and instructions: every product's code comes from the far instruction cache each time.)
+template <bool DIVIDED>
+__global__ void __launch_bounds__(THREADS, 1) small_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ CUtensorMap map_units, const __grid_constant__ Job o) {
+    Roles<false> roles = begin<false, true>(map, map_units, o);
+    const int together = roles.parts, rank = roles.part;
+    pdl_wait();
+    const Matrix m = matrix_of(o, blockIdx.x / together);
+    int from = 0;
+    for (int k = 0; k < o.steps; k++, from ^= 1) {
+        // a role's share of a product, then the cluster's barrier
+        const auto product = [&](auto phase, auto divided, int first, int step) {
+            constexpr int PHASE = decltype(phase)::value;
+            constexpr bool SPLIT = decltype(divided)::value;
+            MatrixTiles list(m, PHASE == GRAM || PHASE == QUAD, first, step);
+            if (roles.warp == 0) {
+                if (roles.lane == 0) roles.template load<PHASE, SPLIT>(list, from);
+            } else if (roles.warp == 1) {
+                if (roles.lane == 0) roles.template multiply<PHASE, SPLIT>(list, from);
+            } else
+                roles.template store<PHASE, SPLIT>(list, from);
+            if (SPLIT && roles.warp < 2) cluster_meet();
+            // stores by TMA are complete (store() waits for them); loads by TMA come after the barrier, and after what was read
+            // of the rooms
+            fence_proxy_async();
+            cluster_meet();
+            if (roles.lane == 0) asm volatile("fence.proxy.async.global;" ::: "memory");
+        };
+        using One = std::integral_constant<bool, false>;
+        if constexpr (DIVIDED)
+            product(std::integral_constant<int, GRAM>(), std::integral_constant<bool, true>(), 0, 1);
+        else
+            product(std::integral_constant<int, GRAM>(), One(), rank, together);
+        product(std::integral_constant<int, QUAD>(), One(), rank, together);
+        if (k + 1 < o.steps)
+            product(std::integral_constant<int, APPLY>(), One(), rank, together);
+        else
+            product(std::integral_constant<int, STEP>(), One(), rank, together);
+    }
+    if (roles.warp == 0 && roles.lane == 0) roles.loaded();
+    end(roles);
 }
 
 // ---------------------------------------------------------------- host side
@@ -802,6 +907,8 @@ static Product product_of(int phase, int mode) {
         {product_kernel<GRAM, SPLITS>, product_kernel<QUAD, SPLITS>, product_kernel<APPLY, SPLITS>, product_kernel<STEP, SPLITS>}};
     return all[mode][phase];
 }
+typedef Product Small;
+static Small small_of(bool divided) { return divided ? small_kernel<true> : small_kernel<false>; }
 static int allow_space() {
     static uint64_t ready = 0;
     int dev = 0;
@@ -809,6 +916,8 @@ static int allow_space() {
     if (dev < 64 && ((ready >> dev) & 1)) return 0;
     for (int k = 0; k < 12; k++)
         if (cudaError_t e = cudaFuncSetAttribute(product_of(k & 3, k >> 2), cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES)) return (int)e;
+    for (int k = 0; k < 2; k++)
+        if (cudaError_t e = cudaFuncSetAttribute(small_of(k), cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES)) return (int)e;
     if (dev < 64) ready |= 1ull << dev;
     return 0;
 }
@@ -829,6 +938,13 @@ static int launch(Job &o, int64_t parts, int64_t blocks, const Load &load, int s
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.blockDim = dim3(THREADS);
     cfg.dynamicSmemBytes = SMEM_BYTES;
+    o.steps = steps;
+    if (const int together = load.small_together()) {
+        cfg.gridDim = dim3((unsigned)(load.matrices * together));
+        cfg.numAttrs = 2;
+        attr[1].val.clusterDim.x = together;
+        return (int)cudaLaunchKernelEx(&cfg, small_of(together > 1 && saves(load.depth[0], together)), maps.blocks, maps.units, o);
+    }
     for (int k = 0; k < steps; k++, o.from ^= 1)
         for (int phase = 0; phase < 3; phase++) {
             const int tiles = phase < 2 ? o.count_symmetric : o.count_full;

@@ -99,6 +99,19 @@ def test_steps(steps):
     assert y.dtype == torch.bfloat16 and distance(y, emulated(x, steps)) <= SAME.get(steps, 2 * NS) + OUT[y.dtype]
 
 
+@pytest.mark.parametrize('batch, size', [(1, (60, 700)), (13, (60, 700)), (14, (60, 700)), (1, (128, 2000)), (20, (2000, 100)), (148, (20, 30)), (149, (20, 30)),
+                                         (3, (128, 4100)), (40, (128, 500)), (1, (64, 4000))])
+def test_small_ones_together(batch, size):
+    """As many as one launch takes through all products, and more; long ones, whose first sum is divided, and too long ones."""
+    from d1.muon import muon_error, orthogonalize
+    for kind in ('full', 'low'):
+        x = matrix(batch, *size, kind=kind)
+        y = orthogonalize(x)
+        assert distance(y, exact(x)) <= bound(x) + OUT[y.dtype]
+        assert all(torch.equal(orthogonalize(x), y) for _ in range(2))
+    assert muon_error() == 0
+
+
 @pytest.mark.parametrize('size', [(2048, 2500), (2500, 2048), (1300, 5000)])
 def test_large(size):
     """Sizes that pairs of CTAs take together, whole tiles and ragged ones."""
@@ -153,16 +166,20 @@ def optimizer(shapes, grad=torch.float32, copies=True, seed=0, **more):
     return Muon(params, grads, copies=c, **more), params, grads, c
 
 
+SMALL = [(32, 90), (64, 288), (100, 120), (120, 900), (3, 28, 300), (1, 50), (50, 1), (5, 5)]  # one launch for all products
+
+
+@pytest.mark.parametrize('shapes', [SHAPES, SMALL])
 @pytest.mark.parametrize('nesterov', [True, False])
 @pytest.mark.parametrize('grad', [torch.float32, torch.bfloat16])
-def test_step(grad, nesterov):
+def test_step(grad, nesterov, shapes):
     """Three steps; the update is taken from the parameters' change at a rate at which their rounding (2^-24 of 0.05) is far below it."""
-    opt, params, grads, copies = optimizer(SHAPES, grad, lr=0.05, momentum=0.9, nesterov=nesterov, weight_decay=[0.1 * (i % 3) for i in range(len(SHAPES))])
+    opt, params, grads, copies = optimizer(shapes, grad, lr=0.05, momentum=0.9, nesterov=nesterov, weight_decay=[0.1 * (i % 3) for i in range(len(shapes))])
     m = [torch.zeros_like(p, dtype=torch.float64) for p in params]
     for step in range(3):
         before = [p.double() for p in params]
         for i, g in enumerate(grads):
-            g.copy_(1e-3 * matrix(*SHAPES[i], seed=50 * step + i, kind='full' if i % 2 else 'low'))
+            g.copy_(1e-3 * matrix(*shapes[i], seed=50 * step + i, kind='full' if i % 2 else 'low'))
         opt.step()
         for i, (p, g) in enumerate(zip(params, grads)):
             was = m[i]

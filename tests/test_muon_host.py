@@ -59,6 +59,19 @@ int main() {
             if (n > 1 && (tiles * n > 148 || depth < 10)) return 11;
         }
     if (parts_for(10, 49) != 8 || parts_for(24, 49) != 4 || parts_for(74, 49) != 2 || parts_for(75, 1000) != 1 || parts_for(1, 8) != 1) return 12;
+    for (int64_t rows : {1, 64, 128, 129, 700})
+        for (int64_t cols : {1, 128, 600, 2000, 5000})
+            for (int64_t count : {1, 14, 15, 33, 148, 149}) {
+                Load load = load_of(2);
+                Matrix m;
+                int64_t block = 0, part = 0;
+                place(m, rows, cols, block, part);
+                load.add(m, count);
+                const int n = load.small_together();
+                if (n && (symmetric_tiles(m, 2) != 1 || full_tiles(m, 2) > 2 * n || count * n > 148 || (n & (n - 1)) || n > 8)) return 16;
+                if (!n && symmetric_tiles(m, 2) == 1 && full_tiles(m, 2) <= 2 && count <= 148) return 17;
+                if (n && count == 1 && m.cb <= 10 && m.rb <= 2 && n < 8 && n < full_tiles(m, 2)) return 18;
+            }
     for (int64_t n : {64, 1000, 8192}) {
         Load small = load_of(2), large = load_of(4);
         Matrix m;
