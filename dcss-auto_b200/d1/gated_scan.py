@@ -120,7 +120,7 @@ class _GatedScan(torch.autograd.Function):
         dy = torch.zeros_like(y) if dy is None else dy.contiguous()
         dx, dgate, dh0 = gated_scan_backward(dy, x, gate, y, h0, reset, None if dlast is None else dlast.contiguous(), ctx.form)
         need = ctx.needs_input_grad
-        return dx if need[0] else None, dgate if need[1] else None, dh0 if need[2] else None, None, None
+        return dx if need[0] else None, dgate if need[1] else None, dh0.view(h0.shape) if need[2] else None, None, None
 
 
 def gated_scan(x, gate, h0=None, reset=None, form='average'):

@@ -231,6 +231,16 @@ def test_torchs_own_backward():
                                                    dlast=torch.ones_like(h0))[0])
 
 
+def test_a_flat_first_state_has_a_flat_gradient():
+    from d1.gated_scan import gated_scan, gated_scan_backward
+    x, gate, h0, reset, dy, _ = inputs((9, 3, 8), torch.float32)
+    leaf = h0.reshape(-1).clone().requires_grad_()
+    y, _ = gated_scan(x, gate, leaf, reset=reset)
+    (y * dy).sum().backward()
+    assert leaf.grad.shape == leaf.shape
+    assert torch.equal(leaf.grad.view(h0.shape), gated_scan_backward(dy, x, gate, y.detach(), h0, reset=reset)[2])
+
+
 def test_graphs_streams_and_the_default_type():
     """Captured calls of two graphs and an eager one on another stream, with new inputs: none disturbs the others."""
     from d1.gated_scan import gated_scan, gated_scan_backward
