@@ -366,7 +366,7 @@ template <int V> __global__ void __launch_bounds__(SMALL_THREADS) small_kernel(A
     }
 }
 
-static bool is_small(int64_t rows, int64_t count) { return count <= SMALL && rows <= SMALL_ROWS; }
+static bool is_small(int64_t rows, int64_t count) { return count <= SMALL && (rows <= SMALL_ROWS || !count); }
 constexpr int64_t PART_BYTES = (int64_t)BLOCKS * TERMS * 8;
 
 static bool rows_ok(const void *p, int64_t ld, int64_t rows, int64_t length, bool needed) {
@@ -415,7 +415,7 @@ extern "C" int d1_policy_loss(const float *logp, int64_t ld_logp, const float *o
     a.logp = {logp, ld_logp}, a.old = {old_logp, ld_old}, a.adv = {advantage, ld_advantage}, a.ref = {ref_logp, ld_ref};
     a.entropy = {entropy, ld_entropy};
     a.per_row = per_row != 0, a.mask = mask, a.ld_mask = ld_mask;
-    a.rows = rows, a.length = length, a.count = count;
+    a.rows = count ? rows : 0, a.length = length, a.count = count;  // no rows without a token: their counts need no room
     a.over = log1p(clip_high), a.under = clip_low < 1. ? log1p(-clip_low) : -INFINITY;
     a.over32 = (float)a.over, a.under32 = (float)a.under;
     a.most = (float)(1. + clip_high), a.least = (float)(1. - clip_low);

@@ -293,6 +293,19 @@ def test_with_the_log_probabilities_of_a_policy():
     assert torch.equal(own.grad, d)
 
 
+def test_rows_without_tokens_in_the_c_entry():
+    """More rows than a cluster counts, none of which has a token: everything is 0."""
+    from d1._lib import library
+    loss, stats = torch.full((), 7.0, device='cuda'), torch.full((5,), 7.0, device='cuda')
+    mask = torch.ones(8, dtype=torch.uint8, device='cuda')
+    for by_row in (0, 1):
+        for m in (None, mask.data_ptr()):
+            loss.fill_(7.0), stats.fill_(7.0)
+            assert library().d1_policy_loss(None, 0, None, 0, None, 0, 0, None, 0, None, 0, m, 0, 100000, 0, 0.2, 0.2, 0.1, 0.01, by_row,
+                                            loss.data_ptr(), stats.data_ptr(), None, None, None, torch.cuda.current_stream().cuda_stream) == 0
+            assert loss == 0 and (stats == 0).all()
+
+
 def test_refusals():
     from d1.policy_loss import policy_loss
     s = inputs((4, 6), mask=False)

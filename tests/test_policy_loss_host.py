@@ -38,6 +38,10 @@ def test_work_bytes(lib):
     assert size(2049, 1) > 4 * 2049 and size(1, 32769) > 0
 
 
+def test_rows_without_tokens_need_no_work_buffer(lib):
+    assert lib.d1_policy_loss_work_bytes(100000, 0) == 0
+
+
 def test_host_tensors_are_refused():
     from d1.policy_loss import policy_loss
     x = torch.zeros(4, 8)
