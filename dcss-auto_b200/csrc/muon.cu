@@ -176,6 +176,10 @@ __device__ __forceinline__ void load8(const void *base, int type, int64_t at, in
     }
 }
 
+// Where 8 columns of a row stand in a block of lo that is no operand: as the epilogues take them, 32 x 32 elements
+// after 32 x 32, of them 8 columns after 8, row after row (a lane has a row).
+__device__ __forceinline__ int lo_at(int row, int col) { return ((row >> 5) * 2 + (col >> 5)) * ROOM / 2 + (col & 31) / 8 * 512 + (row & 31) * 16; }
+
 // Sum over the block in a fixed order, in every thread.
 __device__ __forceinline__ double block_sum(double s, double *shared) {
 #pragma unroll
@@ -247,7 +251,7 @@ template <bool FIRST> __global__ void __launch_bounds__(PREP) prepare_kernel(Job
                 }
                 const int at = row * 128 + col * 2;
                 *reinterpret_cast<Elems<__half, 8> *>(o.work + (int64_t)(m.hi[0] + b) * BLOCK_BYTES + at) = hi;
-                *reinterpret_cast<Elems<__half, 8> *>(o.work + (int64_t)(m.lo + b) * BLOCK_BYTES + at) = lo;
+                *reinterpret_cast<Elems<__half, 8> *>(o.work + (int64_t)(m.lo + b) * BLOCK_BYTES + (m.fine ? at : lo_at(row, col))) = lo;
             }
         }
     }
@@ -555,21 +559,33 @@ template <bool PAIR> struct Roles {
             // unit u: columns 32 (u & 1) .. + 31 of block (ib, jb0 + u / 2); all warps' lanes agree on how many there are
             const int units = ib < p.ni ? max(0, min(UNITS, 2 * (p.nj - jb0))) : 0;
             const auto row_of = [&](int u) { return (ib * (SYMMETRIC ? m.sb : m.cb) + jb0 + u / 2) * SIDE + r0; };
-            // what the epilogue of a unit reads: A (a pair where it is fine), or lo of X (where it is fine, F lo was a term)
-            const bool reads = PHASE == QUAD || (PHASE != GRAM && !m.fine);
+            // what the epilogue of a unit reads: A by TMA (a pair where it is fine), or lo of X (where it is fine, F lo was a
+            // term), which only this lane reads and writes: straight, the next unit's ahead
+            constexpr bool reads = PHASE == QUAD;
             const auto fetch = [&](int u) {
                 if (!reads || u >= units) return;
                 const uint32_t k = SPLIT ? 0u : (uint32_t)u & 1u;
                 pending |= 1u << k;
                 if (lane) return;
                 const int x = 32 * (u & 1), y = row_of(u);
-                mbar_expect_tx(sides0 + 8 * k, PHASE == QUAD && m.fine ? ROOM : ROOM / 2);
-                if (PHASE != QUAD || m.fine)
-                    tma_load_2d(rooms_at + k * ROOM + ROOM / 2, &map_units, sides0 + 8 * k, x, (PHASE == QUAD ? m.gram + 1 : m.lo) * SIDE + y);
-                if (PHASE == QUAD) tma_load_2d(rooms_at + k * ROOM, &map_units, sides0 + 8 * k, x, m.gram * SIDE + y);
+                mbar_expect_tx(sides0 + 8 * k, m.fine ? ROOM : ROOM / 2);
+                if (m.fine) tma_load_2d(rooms_at + k * ROOM + ROOM / 2, &map_units, sides0 + 8 * k, x, (m.gram + 1) * SIDE + y);
+                tma_load_2d(rooms_at + k * ROOM, &map_units, sides0 + 8 * k, x, m.gram * SIDE + y);
+            };
+            const bool adds = !SYMMETRIC && !m.fine;
+            const auto lo_of = [&](int u) {
+                return reinterpret_cast<uint4 *>(o.work + (int64_t)(m.lo + ib * m.cb + jb0 + u / 2) * BLOCK_BYTES + lo_at(r0 + lane, 32 * (u & 1)));
+            };
+            uint4 ahead[4];
+            const auto ask = [&](int u) {
+                if (!adds || u >= units) return;
+                const uint4 *const at = lo_of(u);
+#pragma unroll
+                for (int e = 0; e < 4; e++) ahead[e] = __ldcg(at + 32 * e);
             };
             if (lane == 0) bulk_wait_read();
             __syncwarp();  // the rooms are free
+            ask(own);
             if (SPLIT) {
                 fetch(own);
             } else {
@@ -642,12 +658,14 @@ template <bool PAIR> struct Roles {
                         ok = false;
                         break;
                     }
-                } else if (u > 1) {  // the room's last contents have been taken away
+                } else if (m.fine && u > 1) {  // the room's last contents have been taken away
                     if (lane == 0) bulk_wait_read_but_one();
                     __syncwarp();
                 }
-                uint8_t *const room = rooms + k * ROOM;
-                const uint32_t room_at = rooms_at + k * ROOM;
+                // half a room where that is enough: each of a tile's units has its own
+                const uint32_t room_from = SPLIT ? 0u : (PHASE == GRAM || PHASE == APPLY) && !m.fine ? u * (ROOM / 2) : k * ROOM;
+                uint8_t *const room = rooms + room_from;
+                const uint32_t room_at = rooms_at + room_from;
                 const int x0 = 32 * (u & 1), y = row_of(u);
                 // this lane's row of 64 bytes: its piece e lies at e ^ (row / 2 & 3), as the TMA's swizzle has it
                 uint8_t *const mine = room + lane * 64;
@@ -689,13 +707,14 @@ template <bool PAIR> struct Roles {
                     }
                 } else {
                     float x[32];
+                    uint4 *const lo_to = lo_of(u);
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
 #pragma unroll
                         for (int i = 0; i < 8; i++) x[8 * e + i] = UNSCALE * __uint_as_float(v[8 * e + i]);
-                        if (reads) {
+                        if (adds) {
                             float l[8];
-                            unpack(*reinterpret_cast<const uint4 *>(mine + ROOM / 2 + piece(e)), l);
+                            unpack(ahead[e], l);
 #pragma unroll
                             for (int i = 0; i < 8; i++) x[8 * e + i] = fmaf(NS_A, l[i], x[8 * e + i]);
                         }
@@ -703,20 +722,24 @@ template <bool PAIR> struct Roles {
                             uint4 hi, lo;
                             split(reinterpret_cast<const float(&)[8]>(x[8 * e]), hi, lo);
                             *reinterpret_cast<uint4 *>(mine + piece(e)) = hi;
-                            *reinterpret_cast<uint4 *>(mine + ROOM / 2 + piece(e)) = lo;
+                            if (adds)
+                                lo_to[32 * e] = lo;
+                            else
+                                *reinterpret_cast<uint4 *>(mine + ROOM / 2 + piece(e)) = lo;
                         }
                     }
+                    if (PHASE == APPLY && !SPLIT) ask(u + 1);
                     if constexpr (PHASE == APPLY) {
                         fence_proxy_async();
                         __syncwarp();
                         if (lane == 0) {
                             tma_store_2d(&map_units, room_at, x0, hi_to * SIDE + y);
-                            tma_store_2d(&map_units, room_at + ROOM / 2, x0, m.lo * SIDE + y);
+                            if (m.fine) tma_store_2d(&map_units, room_at + ROOM / 2, x0, m.lo * SIDE + y);
                             bulk_commit();
                         }
                     } else {
                         finish(o, m, ib * SIDE + r0, jb0 * SIDE + 32 * u, x, params, reinterpret_cast<float *>(room));
-                        fence_proxy_async();  // the next load into the room comes after these reads
+                        if (!SPLIT) ask(u + 1);
                     }
                 }
                 __syncwarp();
