@@ -126,12 +126,16 @@ struct Load {
     double work[3];           // blocks of all sums, by product
     int64_t matrices;
     int widest, longest;      // the most tiles along a smaller side, and of one X'
+    int64_t wider;            // matrices whose smaller side has more than one block
+    int most_parts;           // of one matrix
 
     void add(const Matrix &m, int64_t count) {
         const int64_t s = symmetric_tiles(m, side) * count, f = full_tiles(m, side) * count;
         const int terms = m.fine ? 3 : 1, first = (m.tall ? m.rb : m.cb) * terms, others = m.sb * terms;
         const int wide = tiles_of(m.sb, side), most = (int)full_tiles(m, side);
         matrices += count;
+        if (!m.fine) wider += count;
+        if (m.parts > most_parts) most_parts = m.parts;
         if (wide > widest) widest = wide;
         if (most > longest) longest = most;
         symmetric += s, full += f;
@@ -139,6 +143,9 @@ struct Load {
         if (first > depth[0]) depth[0] = first;
         if (others > depth[1]) depth[1] = others;
     }
+    // Whether the steps are taken without X (muon_narrow.cuh). Beside other matrices the narrow ones go with those through
+    // their launches, at no cost.
+    bool narrow() const { return wider == 0; }
     // CTAs of the cluster that takes each matrix through all products in one launch, 0 where that is not done: every
     // matrix has one tile of A and no more than two of X' a CTA (128 x 4,000, with four, took 138 us in place of the launches'
     // 121), and all clusters run at once.
@@ -161,7 +168,7 @@ struct Load {
         return sum;
     }
 };
-inline Load load_of(int side) { return Load{side, 0, 0, {0, 0}, {0., 0., 0.}, 0, 0, 0}; }
+inline Load load_of(int side) { return Load{side, 0, 0, {0, 0}, {0., 0., 0.}, 0, 0, 0, 0, 0}; }
 
 // What a plan begins with: sizes of its lists and where they start (bytes).
 struct Plan {

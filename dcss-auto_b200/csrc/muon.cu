@@ -16,7 +16,8 @@
 // has nothing F is a, and the pair is carried on as one; elsewhere F lo is not a lo, an error of hi's size, but
 // in directions that X has (0.16 % there, 0.2 % of a full-rank one). In a matrix with a side of at most 64, where few
 // roundings average out (up to 1 % in some), A and F are pairs too and a product takes all three terms: it is as good as
-// one in fp32, and its time is the launches' all the same.
+// one in fp32, and its time is the launches' all the same. Where all matrices are as narrow as that they take
+// another way (muon_narrow.cuh).
 //
 // The three products of all matrices are one launch each. A and F are symmetric: only the tiles on and below the
 // diagonal are computed and stored, and read transposed for those above. The epilogues hold the rest of the
@@ -192,6 +193,28 @@ __device__ __forceinline__ double block_sum(double s, double *shared) {
     return s;
 }
 
+// u at n elements of row i from column j on, and the momentum, which UPDATE brings up to date.
+template <bool UPDATE> __device__ __forceinline__ void momentum8(const Job &o, const Matrix &m, int i, int j, int n, float (&u)[8]) {
+    load8(m.grad, m.grad_type, i * m.pitch + j, n, u);
+    if (!m.momentum) return;
+    float *p = m.momentum + (int64_t)i * m.cols + j, v[8];
+    const bool wide = n == 8 && ((uintptr_t)p & 15) == 0;
+    load8(p, n, wide, v);
+    if (UPDATE) {
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] = fmaf(o.mu, v[k], u[k]);
+        if (wide) {
+            *(float4 *)p = make_float4(v[0], v[1], v[2], v[3]);
+            *(float4 *)(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+        } else
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+                if (k < n) p[k] = v[k];
+    }
+#pragma unroll
+    for (int k = 0; k < 8; k++) u[k] = o.nesterov ? fmaf(o.mu, v[k], u[k]) : v[k];
+}
+
 // FIRST: the new momentum and the sum of the squares of u (in fp64: squares of fp32 numbers neither overflow
 // nor vanish there). Else X = u / |u|, as hi + lo.
 template <bool FIRST> __global__ void __launch_bounds__(PREP) prepare_kernel(Job o) {
@@ -217,27 +240,7 @@ template <bool FIRST> __global__ void __launch_bounds__(PREP) prepare_kernel(Job
             const int e = threadIdx.x + PREP * q, row = e >> 3, col = (e & 7) * 8;
             const int i = ib * SIDE + row, j = jb * SIDE + col, n = i < m.rows ? min(8, max(0, m.cols - j)) : 0;
             float u[8] = {};
-            if (n) {
-                load8(m.grad, m.grad_type, i * m.pitch + j, n, u);
-                if (m.momentum) {
-                    float *p = m.momentum + (int64_t)i * m.cols + j, v[8];
-                    const bool wide = n == 8 && ((uintptr_t)p & 15) == 0;
-                    load8(p, n, wide, v);
-                    if (FIRST) {
-#pragma unroll
-                        for (int k = 0; k < 8; k++) v[k] = fmaf(o.mu, v[k], u[k]);
-                        if (wide) {
-                            *(float4 *)p = make_float4(v[0], v[1], v[2], v[3]);
-                            *(float4 *)(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
-                        } else
-#pragma unroll
-                            for (int k = 0; k < 8; k++)
-                                if (k < n) p[k] = v[k];
-                    }
-#pragma unroll
-                    for (int k = 0; k < 8; k++) u[k] = o.nesterov ? fmaf(o.mu, v[k], u[k]) : v[k];
-                }
-            }
+            if (n) momentum8<FIRST>(o, m, i, j, n, u);
             if (FIRST) {
 #pragma unroll
                 for (int k = 0; k < 8; k++) sum = fma((double)u[k], (double)u[k], sum);
@@ -891,6 +894,8 @@ __global__ void __launch_bounds__(THREADS, 1) small_kernel(const __grid_constant
     end(roles);
 }
 
+#include "muon_narrow.cuh"
+
 // ---------------------------------------------------------------- host side
 
 typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
@@ -941,6 +946,7 @@ static int allow_space() {
         if (cudaError_t e = cudaFuncSetAttribute(product_of(k & 3, k >> 2), cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES)) return (int)e;
     for (int k = 0; k < 2; k++)
         if (cudaError_t e = cudaFuncSetAttribute(small_of(k), cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES)) return (int)e;
+    if (cudaError_t e = cudaFuncSetAttribute(narrow::steps_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, narrow::STEP_BYTES)) return (int)e;
     if (dev < 64) ready |= 1ull << dev;
     return 0;
 }
@@ -948,20 +954,34 @@ static int allow_space() {
 static int launch(Job &o, int64_t parts, int64_t blocks, const Load &load, int steps, cudaStream_t s) {
     if (parts > INT32_MAX || load.symmetric > INT32_MAX || load.full > INT32_MAX) return D1_ERR_TOO_LARGE;
     o.count_symmetric = (int)load.symmetric, o.count_full = (int)load.full;
-    Maps maps;
-    if (const int e = make_maps(maps, o.work, blocks)) return e;
     if (const int e = allow_space()) return e;
+    o.steps = steps;
     cudaLaunchAttribute attr[2];
     cudaLaunchConfig_t cfg = pdl_config(dim3((unsigned)parts), dim3(PREP), 0, s, attr);
     cfg.numAttrs = 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    if (load.narrow()) {
+        const int together = load.most_parts > narrow::FEW ? narrow::TOGETHER : 1;
+        cfg.blockDim = dim3(narrow::THREADS_SUM);
+        if (cudaError_t e = cudaLaunchKernelEx(&cfg, narrow::sums_kernel, o)) return (int)e;
+        cudaLaunchConfig_t mid = cfg;
+        mid.gridDim = dim3((unsigned)(load.matrices * together));
+        mid.dynamicSmemBytes = narrow::STEP_BYTES;
+        mid.numAttrs = 2;
+        attr[1].val.clusterDim.x = together;
+        if (cudaError_t e = cudaLaunchKernelEx(&mid, narrow::steps_kernel, o)) return (int)e;
+        cfg.blockDim = dim3(narrow::THREADS_APPLY);
+        cfg.numAttrs = 1;
+        return (int)cudaLaunchKernelEx(&cfg, narrow::apply_kernel, o);
+    }
+    Maps maps;
+    if (const int e = make_maps(maps, o.work, blocks)) return e;
     if (cudaError_t e = cudaLaunchKernelEx(&cfg, prepare_kernel<true>, o)) return (int)e;
     cfg.numAttrs = 1;
     if (cudaError_t e = cudaLaunchKernelEx(&cfg, prepare_kernel<false>, o)) return (int)e;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.blockDim = dim3(THREADS);
     cfg.dynamicSmemBytes = SMEM_BYTES;
-    o.steps = steps;
     if (const int together = load.small_together()) {
         cfg.gridDim = dim3((unsigned)(load.matrices * together));
         cfg.numAttrs = 2;

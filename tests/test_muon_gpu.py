@@ -112,6 +112,49 @@ def test_small_ones_together(batch, size):
     assert muon_error() == 0
 
 
+@pytest.mark.parametrize('steps', [1, 2, 5, 7])
+@pytest.mark.parametrize('batch, size', [(1, (1, 8)), (1, (64, 520)), (3, (7, 513)), (17, (64, 1100)), (1, (40, 20001)), (2, (16500, 33)), (300, (24, 48)), (5, (600, 64)),
+                                         (2, (8, 9))])
+def test_narrow_ones(batch, size, steps):
+    """A side of at most 64. Between the sums and the result all is fp64 (11.9 a step on 2^-53 is nothing); Q X is fp32: 64 terms' rounding, 2^-21 if
+    all were alike, of |Q| |X|, which is at most 3.44 a step (485) times the result where X hardly has a direction: 2^-12. Up to 7 steps (5,700)
+    the matrices of full rank here have no such direction, and those of low rank have it in fp32's last bits only, 2^-24 each."""
+    from d1.muon import orthogonalize
+    for kind in ('full', 'low') if steps <= 5 else ('full',):
+        x = matrix(batch, *size, kind=kind)
+        y = orthogonalize(x, steps=steps, out=torch.empty(x.shape, dtype=torch.float16, device='cuda'))
+        assert distance(y, exact(x, steps)) <= 2.0 ** -12 + OUT[y.dtype]
+        assert torch.equal(orthogonalize(x, steps=steps, out=torch.empty_like(y)), y)
+
+
+@pytest.mark.parametrize('scale', [1e-38, 1e-20, 1e19, 1e38])
+def test_scales_of_narrow_ones(scale):
+    from d1.muon import orthogonalize
+    for size in ((30, 150), (1000, 30)):
+        x = matrix(*size).clamp(-3, 3)
+        assert distance(orthogonalize(x * scale), exact((x * scale).double())) <= 2.0 ** -12 + OUT[torch.bfloat16]
+
+
+def test_zeros_and_infinities_in_narrow_ones():
+    from d1.muon import orthogonalize
+    for size in ((60, 90), (900, 60)):
+        x = matrix(4, *size)
+        x[0] = 0
+        x[1, 3, 4] = float('nan')
+        x[2, 5, 6] = float('inf')
+        y = orthogonalize(x)
+        assert (y[0] == 0).all() and y[1].isnan().any() and y[2].isnan().any() and torch.equal(y[3], orthogonalize(x[3]))
+
+
+NARROW = [(32, 90), (64, 288), (900, 12), (3, 28, 700), (1, 50), (50, 1), (5, 5), (1300, 61)]  # all taken without X
+
+
+@pytest.mark.parametrize('nesterov', [True, False])
+@pytest.mark.parametrize('grad', [torch.float32, torch.bfloat16])
+def test_step_of_narrow_ones(grad, nesterov):
+    test_step(grad, nesterov, NARROW)
+
+
 @pytest.mark.parametrize('size', [(2048, 2500), (2500, 2048), (1300, 5000)])
 def test_large(size):
     """Sizes that pairs of CTAs take together, whole tiles and ragged ones."""
