@@ -110,11 +110,12 @@ D1_MUON_BOTH int64_t full_tiles(const Matrix &m, int side) { return (int64_t)til
 
 // CTAs that share the sum of `depth` blocks of each of a few tiles: as many as there is room for, while it saves ten
 // blocks' time (the exchange of the parts costs some five).
+inline int room(int n) { return n == 8 ? 112 : n == 4 ? 128 : 148; }  // what clusters of n CTAs find room for at once
 inline bool saves(int depth, int parts) { return depth - depth / parts >= 10; }
 inline int parts_for(int64_t tiles, int depth) {
     int parts = 1;
     for (int n = 2; n <= 8; n *= 2)
-        if (tiles * n <= (n == 8 ? 112 : n == 4 ? 128 : 148) && saves(depth, n)) parts = n;  // what clusters find room for at once
+        if (tiles * n <= room(n) && saves(depth, n)) parts = n;
     return parts;
 }
 
@@ -127,7 +128,7 @@ struct Load {
     int64_t matrices;
     int widest, longest;      // the most tiles along a smaller side, and of one X'
     int64_t wider;            // matrices whose smaller side has more than one block
-    int most_parts;           // of one matrix
+    int most_parts, most_eights;  // of one matrix; of a smaller side, in eights
 
     void add(const Matrix &m, int64_t count) {
         const int64_t s = symmetric_tiles(m, side) * count, f = full_tiles(m, side) * count;
@@ -136,6 +137,8 @@ struct Load {
         matrices += count;
         if (!m.fine) wider += count;
         if (m.parts > most_parts) most_parts = m.parts;
+        const int eights = ((m.tall ? m.cols : m.rows) + 7) / 8;
+        if (eights > most_eights) most_eights = eights;
         if (wide > widest) widest = wide;
         if (most > longest) longest = most;
         symmetric += s, full += f;
@@ -144,8 +147,21 @@ struct Load {
         if (others > depth[1]) depth[1] = others;
     }
     // Whether the steps are taken without X (muon_narrow.cuh). Beside other matrices the narrow ones go with those through
-    // their launches, at no cost.
+    // their launches.
     bool narrow() const { return wider == 0; }
+    // Blocks of a cluster for each matrix, n at most, so that all clusters run at once.
+    int clusters(int n) const {
+        while (n > 1 && matrices * n > room(n)) n /= 2;
+        return n;
+    }
+    // Blocks of the cluster that takes a narrow matrix through everything in one launch, 0 where that is not done: a block has two
+    // of its blocks of X at most.
+    int whole_together() const {
+        int n = 1;
+        while (n < 8 && n < most_parts) n *= 2;
+        n = clusters(n);
+        return most_parts <= 2 * n ? n : 0;
+    }
     // CTAs of the cluster that takes each matrix through all products in one launch, 0 where that is not done: every
     // matrix has one tile of A and no more than two of X' a CTA (128 x 4,000, with four, took 138 us in place of the launches'
     // 121), and all clusters run at once.
@@ -153,7 +169,7 @@ struct Load {
         if (side != 2 || widest > 1) return 0;
         int n = 1;
         while (n < 8 && (n < longest || (!saves(depth[0], n) && saves(depth[0], 2 * n)))) n *= 2;
-        while (n > 1 && matrices * n > (n == 8 ? 112 : n == 4 ? 128 : 148)) n /= 2;
+        n = clusters(n);
         return matrices * n <= 148 && longest <= 2 * n ? n : 0;
     }
     // A block of 64 of the sum takes a pair of CTAs 0.43 us for a tile of 256 x 256, a CTA 0.5 us for one of 128 x 128 (both measured with the
@@ -168,7 +184,7 @@ struct Load {
         return sum;
     }
 };
-inline Load load_of(int side) { return Load{side, 0, 0, {0, 0}, {0., 0., 0.}, 0, 0, 0, 0, 0}; }
+inline Load load_of(int side) { return Load{side, 0, 0, {0, 0}, {0., 0., 0.}, 0, 0, 0, 0, 0, 0}; }
 
 // What a plan begins with: sizes of its lists and where they start (bytes).
 struct Plan {

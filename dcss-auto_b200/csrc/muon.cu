@@ -26,7 +26,7 @@
 //
 // Measured (one B200). 8,192 x 8,192 bf16: 9.97 ms, 1.3 PFLOP/s while the products run (a library product sustains 1.38
 // under the power limit). 72 matrices of 12 layers of 1,024, with masters, momentum and copies: 3.89 ms (floor 1.64). The conv policy's six:
-// 147 us, 17 launches. A pair of CTAs takes 0.43 us for a block of 64 of the sum of its 256 x 256 tile: 32 KB into shared memory and 48 KB read
+// 145 us, 17 launches. A pair of CTAs takes 0.43 us for a block of 64 of the sum of its 256 x 256 tile: 32 KB into shared memory and 48 KB read
 // for 512 cycles of the tensor pipe, 640 cycles at 128 bytes each, which bound it.
 #include <cuda.h>
 #include <math.h>
@@ -72,6 +72,7 @@ struct Job {
     double lr;
     int from;   // which hi is read
     int steps;
+    int adders;  // narrow matrices: blocks that add the sums of one
 };
 
 __device__ __forceinline__ Matrix matrix_of(const Job &o, int m) {
@@ -851,7 +852,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
 
 // All products of small matrices (one tile of A each) in one launch: a cluster takes a matrix through all steps, its CTAs share
 // the tiles of X' and, where it is long, the sum of A. A barrier of the cluster stands where the launches' ends stand otherwise:
-// 64 x 64 68 us in place of 87, 8 x 100 x 800 91 in place of 111. (What is left are the first loads of each product, a microsecond,
+// 8 x 100 x 800 91 us in place of 111. (What is left are the first loads of each product, a microsecond,
 // and instructions: every product's code comes from the far instruction cache each time.)
 template <bool DIVIDED>
 __global__ void __launch_bounds__(THREADS, 1) small_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ CUtensorMap map_units, const __grid_constant__ Job o) {
@@ -946,7 +947,8 @@ static int allow_space() {
         if (cudaError_t e = cudaFuncSetAttribute(product_of(k & 3, k >> 2), cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES)) return (int)e;
     for (int k = 0; k < 2; k++)
         if (cudaError_t e = cudaFuncSetAttribute(small_of(k), cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES)) return (int)e;
-    if (cudaError_t e = cudaFuncSetAttribute(narrow::steps_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, narrow::STEP_BYTES)) return (int)e;
+    if (cudaError_t e = cudaFuncSetAttribute(narrow::steps_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, narrow::step_bytes(8))) return (int)e;
+    if (cudaError_t e = cudaFuncSetAttribute(narrow::whole_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, narrow::whole_bytes(8))) return (int)e;
     if (dev < 64) ready |= 1ull << dev;
     return 0;
 }
@@ -962,14 +964,22 @@ static int launch(Job &o, int64_t parts, int64_t blocks, const Load &load, int s
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     if (load.narrow()) {
-        const int together = load.most_parts > narrow::FEW ? narrow::TOGETHER : 1;
-        cfg.blockDim = dim3(narrow::THREADS_SUM);
-        if (cudaError_t e = cudaLaunchKernelEx(&cfg, narrow::sums_kernel, o)) return (int)e;
         cudaLaunchConfig_t mid = cfg;
-        mid.gridDim = dim3((unsigned)(load.matrices * together));
-        mid.dynamicSmemBytes = narrow::STEP_BYTES;
+        mid.blockDim = cfg.blockDim = dim3(narrow::THREADS_SUM);
+        if (const int n = load.whole_together()) {
+            mid.gridDim = dim3((unsigned)(load.matrices * n));
+            mid.dynamicSmemBytes = narrow::whole_bytes(load.most_eights);
+            mid.attrs = attr + 1, mid.numAttrs = 1;
+            attr[1].val.clusterDim.x = n;
+            return (int)cudaLaunchKernelEx(&mid, narrow::whole_kernel, o);
+        }
+        o.adders = (int)std::max<int64_t>(narrow::FEW, 2 * SMS / load.matrices);
+        if (cudaError_t e = cudaLaunchKernelEx(&cfg, narrow::sums_kernel, o)) return (int)e;
+        const int n = std::min(load.most_parts, o.adders) > narrow::FEW ? load.clusters(8) : 1;
+        mid.gridDim = dim3((unsigned)(load.matrices * n));
+        mid.dynamicSmemBytes = narrow::step_bytes(load.most_eights);
         mid.numAttrs = 2;
-        attr[1].val.clusterDim.x = together;
+        attr[1].val.clusterDim.x = n;
         if (cudaError_t e = cudaLaunchKernelEx(&mid, narrow::steps_kernel, o)) return (int)e;
         cfg.blockDim = dim3(narrow::THREADS_APPLY);
         cfg.numAttrs = 1;

@@ -813,7 +813,7 @@ int d1_muon_plan(const D1MuonTensor *tensors, int ntensors, float *momentum, voi
  *   X = u / |u|_F, and `steps` (1 to 64) times X = 3.4445 X - 4.7750 (X X^T) X + 2.0315 (X X^T)^2 X
  *   p = p (1 - lr decay) - lr 0.2 sqrt(max(rows, cols)) X
  * An update of zeros leaves X zero. Products are fp16 with fp32 sums, X is held
- * to 22 bits. host_plan and device_plan are the two copies of the plan; work is
+ * to 22 bits (where a side is at most 64 they are as good as fp32 ones). host_plan and device_plan are the two copies of the plan; work is
  * 128-byte aligned. Calls that share work or state must not overlap. */
 int d1_muon(const void *host_plan, const void *device_plan, double lr, double momentum, int nesterov, int steps, void *work, void *stream);
 /* The orthogonalisation by itself: y[k] = X after `steps` steps from u = x[k], for

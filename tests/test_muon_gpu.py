@@ -11,7 +11,7 @@ that is off by 1e-4 crosses a border every fifth time, and the roundings are no 
 sums in fp32 instead of fp64, moves by 1e-7, 2e-6, 2e-4, 8e-4 and 1.6e-3 in steps one to five of 128 x 128). What is left is that both are within
 NS of the exact result: 2 NS.
 
-Matrices with a side of at most 64 take products of pairs of fp16: operands of 22 bits, sums in fp32 (a term of 2^-23 for each
+Matrices with a side of at most 64 take, beside wider ones, products of pairs of fp16: operands of 22 bits, sums in fp32 (a term of 2^-23 for each
 of up to 16 partial sums of a long row), under 2^-18 a step, and five steps with factors of at most 4: 2^-12.
 """
 import pytest
@@ -114,7 +114,7 @@ def test_small_ones_together(batch, size):
 
 @pytest.mark.parametrize('steps', [1, 2, 5, 7])
 @pytest.mark.parametrize('batch, size', [(1, (1, 8)), (1, (64, 520)), (3, (7, 513)), (17, (64, 1100)), (1, (40, 20001)), (2, (16500, 33)), (300, (24, 48)), (5, (600, 64)),
-                                         (2, (8, 9))])
+                                         (2, (8, 9)), (50, (60, 500)), (40, (30, 700)), (1, (9, 1024)), (1, (1025, 10)), (30, (64, 4096))])
 def test_narrow_ones(batch, size, steps):
     """A side of at most 64. Between the sums and the result all is fp64 (11.9 a step on 2^-53 is nothing); Q X is fp32: 64 terms' rounding, 2^-21 if
     all were alike, of |Q| |X|, which is at most 3.44 a step (485) times the result where X hardly has a direction: 2^-12. Up to 7 steps (5,700)

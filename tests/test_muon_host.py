@@ -72,6 +72,24 @@ int main() {
                 if (!n && symmetric_tiles(m, 2) == 1 && full_tiles(m, 2) <= 2 && count <= 148) return 17;
                 if (n && count == 1 && m.cb <= 10 && m.rb <= 2 && n < 8 && n < full_tiles(m, 2)) return 18;
             }
+    for (int64_t rows : {1, 8, 9, 64})
+        for (int64_t cols : {1, 64, 500, 513, 1024, 1025, 20000})
+            for (int64_t count : {1, 14, 15, 33, 149, 100000}) {
+                Load load = load_of(2);
+                Matrix m;
+                int64_t block = 0, part = 0;
+                place(m, cols, rows, block, part);
+                load.add(m, count);
+                if (!load.narrow() || load.most_parts != m.parts || load.most_eights != (int)((rows < cols ? rows : cols) + 7) / 8) return 19;
+                const int n = load.whole_together(), c = load.clusters(8);
+                if (n && ((n & (n - 1)) || n > 8 || m.parts > 2 * n || (n > 1 && count * n > room(n)))) return 20;
+                if (!n && (m.parts <= 2 || (count == 1 && cols <= 1024))) return 21;
+                if (c < 1 || c > 8 || (c > 1 && count * c > room(c))) return 22;
+                Matrix wide;
+                place(wide, 65, 65, block, part);
+                load.add(wide, 1);
+                if (load.narrow()) return 23;
+            }
     for (int64_t n : {64, 1000, 8192}) {
         Load small = load_of(2), large = load_of(4);
         Matrix m;
