@@ -146,6 +146,75 @@ def test_zeros_and_infinities_in_narrow_ones():
         assert (y[0] == 0).all() and y[1].isnan().any() and y[2].isnan().any() and torch.equal(y[3], orthogonalize(x[3]))
 
 
+def test_stacks_and_pitches_of_narrow_ones():
+    from d1.muon import orthogonalize
+    for size in ((20, 1100), (1100, 20), (33, 70)):
+        m, n = size
+        x = matrix(2, 3, *size)
+        y = orthogonalize(x)
+        assert distance(y, exact(x)) <= 2.0 ** -12 + OUT[y.dtype]
+        for i in range(2):
+            for j in range(3):
+                assert torch.equal(y[i, j], orthogonalize(x[i, j]))
+        wide = torch.zeros(2, 3, m + 10, n + 31, device='cuda')
+        wide[..., 5:5 + m, 3:3 + n] = x
+        assert torch.equal(orthogonalize(wide[..., 5:5 + m, 3:3 + n]), y)
+        assert torch.equal(orthogonalize(x[:1, :1].expand(2, 3, m, n)), y[:1, :1].expand(2, 3, m, n))
+
+
+def test_unaligned_narrow_tensors():
+    from d1.muon import Muon, orthogonalize
+    for size in ((12, 40), (60, 8), (16, 1200), (1200, 16), (64, 64)):
+        n = size[0] * size[1]
+        mk = lambda dtype, k: torch.zeros(n + 8, device='cuda', dtype=dtype)[k:k + n].view(size)
+        p, g, c = mk(torch.float32, 1), mk(torch.bfloat16, 3), mk(torch.bfloat16, 1)
+        q, h, d = (t.clone() for t in (p, g, c))
+        for t in (p, q):
+            t.copy_(matrix(*size))
+        for t in (g, h):
+            t.copy_(matrix(*size, seed=3))
+        for args in ((p, g, c), (q, h, d)):
+            Muon([args[0]], [args[1]], copies=[args[2]], lr=0.1).step()
+        assert torch.equal(p, q) and torch.equal(c, d) and torch.equal(c, p.to(torch.bfloat16))
+        assert torch.equal(orthogonalize(g, out=c), orthogonalize(h))
+
+
+def test_graphs_and_streams_of_narrow_ones():
+    from d1.muon import orthogonalize
+    for shapes in ([(28, 512), (12, 90), (64, 64)], [(28, 2512), (12, 90)]):   # one launch, three
+        a, pa, ga, ca = optimizer(shapes, lr=0.01)
+        b, pb, gb, cb = optimizer(shapes, lr=0.01)
+        a.step(), b.step()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            a.step()
+        for k in range(3):
+            for g, h in zip(ga, gb):
+                g.mul_(0.9).add_(1e-4 * k)
+                h.copy_(g)
+            graph.replay()
+            b.step()
+        assert all(torch.equal(p, q) for p, q in zip(pa + ca, pb + cb)) and torch.equal(a.momentum, b.momentum)
+    for size in ((30, 200), (2000, 30)):
+        x, z = matrix(*size), matrix(*size, seed=4)
+        want, wanted = orthogonalize(x), orthogonalize(z)
+        held, graphs, outs = z.clone(), [], []
+        for _ in range(2):
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1]):
+                outs.append(orthogonalize(held))
+        held.copy_(x)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        for _ in range(3):
+            for g in graphs:
+                g.replay()
+            with torch.cuda.stream(side):
+                eager = orthogonalize(z)
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want) for o in outs) and torch.equal(eager, wanted)
+
+
 NARROW = [(32, 90), (64, 288), (900, 12), (3, 28, 700), (1, 50), (50, 1), (5, 5), (1300, 61)]  # all taken without X
 
 
