@@ -147,7 +147,7 @@ struct Load {
         if (others > depth[1]) depth[1] = others;
     }
     // Whether the steps are taken without X (muon_narrow.cuh). Beside other matrices the narrow ones go with those through
-    // their launches.
+    // their launches at no cost (the conv policy's six take 140 us in one graph, its two wide ones 141 without the four narrow ones).
     bool narrow() const { return wider == 0; }
     // Blocks of a cluster for each matrix, n at most, so that all clusters run at once.
     int clusters(int n) const {
