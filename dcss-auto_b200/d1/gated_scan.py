@@ -63,37 +63,40 @@ def _pitch(shape, strides, name):
     return pitch
 
 
-def _flags(reset, x):
+def _flags(reset, shape, dev):
     """(address, step pitch, sequence pitch) of the resets."""
     if reset is None:
         return None, 0, 0
-    if x.dim() == 3 and reset.dtype in _FLAGS and reset.shape == (x.shape[0], x.shape[1]) and reset.device == x.device:
-        return reset.data_ptr(), *reset.stride()
-    if reset.dtype not in _FLAGS or reset.shape != x.shape[:-1] or reset.device != x.device:
-        raise ValueError(f'reset must be a bool or uint8 tensor {tuple(x.shape[:-1])} on {x.device}, not '
+    flags = shape[:-1]
+    if reset.dtype not in _FLAGS or reset.shape != flags or reset.device != dev:
+        raise ValueError(f'reset must be a bool or uint8 tensor {tuple(flags)} on {dev}, not '
                          f'{reset.dtype} {tuple(reset.shape)} on {reset.device}')
-    return reset.data_ptr(), reset.stride(0), _pitch(reset.shape[1:], reset.stride()[1:], 'reset')
+    if len(flags) == 2:
+        return reset.data_ptr(), *reset.stride()
+    return reset.data_ptr(), reset.stride(0), _pitch(flags[1:], reset.stride()[1:], 'reset')
 
 
-def _same(t, x, name):
-    if t.shape != x.shape or t.dtype is not x.dtype or t.device != x.device:
-        raise ValueError(f'{name} must be {x.dtype} {tuple(x.shape)} on {x.device}, not {t.dtype} {tuple(t.shape)} on {t.device}')
+def _same(t, shape, dtype, dev, name):
+    if t.shape != shape or t.dtype is not dtype or t.device != dev:
+        raise ValueError(f'{name} must be {dtype} {tuple(shape)} on {dev}, not {t.dtype} {tuple(t.shape)} on {t.device}')
     return _steps(t, name)
 
 
 def _sizes(x, form):
+    """(type, form, x's address and pitches, (T, B, D), (shape, dtype, device))."""
     kind, code = type_of(x, 'x'), FORMS.get(form)
     if code is None:
         raise ValueError(f"form must be 'average' or 'sum', not {form!r}")
-    ax = _steps(x, 'x')
-    T, D = x.shape[0], x.shape[-1]
+    ax, shape = _steps(x, 'x'), x.shape
+    D = shape[-1]
     if D < 1 or D > 2 ** 31 - 1:
         raise ValueError(f'x has {D} channels')
-    B = x.shape[1] if x.dim() == 3 else x.shape[1:-1].numel()
-    return kind, code, ax, T, B, D
+    sizes = tuple(shape) if len(shape) == 3 else (shape[0], shape[1:-1].numel(), D)
+    return kind, code, ax, sizes, (shape, x.dtype, x.device)
 
 
-def _work(T, B, D, device):
+def _work(sizes, device):
+    T, B, D = sizes
     if T <= 32:  # not cut into chunks
         return None
     size = library().d1_gated_scan_work_bytes(T, B, D)
@@ -131,14 +134,13 @@ def gated_scan(x, gate, h0=None, reset=None, form='average'):
 
 
 def _gated_scan(x, gate, h0, reset, form):
-    kind, code, ax, T, B, D = _sizes(x, form)
-    ag, dev = _same(gate, x, 'gate'), x.device
-    start = vector(h0, B * D, F32, dev, 'h0')
-    flags = _flags(reset, x)
+    kind, code, ax, sizes, as_x = _sizes(x, form)
+    shape, _, dev = as_x
+    ag, start, flags = _same(gate, *as_x, 'gate'), vector(h0, sizes[1] * sizes[2], F32, dev, 'h0'), _flags(reset, shape, dev)
     y = empty_like(x)
-    last = torch.empty_like(h0) if h0 is not None and h0.shape == x.shape[1:] else empty_f32(dev, *x.shape[1:])
-    work = _work(T, B, D, dev)
-    check(library().d1_gated_scan(*ax, *ag, kind, code, T, B, D, start, *flags, y.data_ptr(), last.data_ptr(),
+    last = torch.empty_like(h0) if h0 is not None and h0.shape == shape[1:] else empty_f32(dev, *shape[1:])
+    work = _work(sizes, dev)
+    check(library().d1_gated_scan(*ax, *ag, kind, code, *sizes, start, *flags, y.data_ptr(), last.data_ptr(),
                                   None if work is None else work.data_ptr(), stream_of(x)), 'd1_gated_scan')
     return y, last
 
@@ -146,13 +148,14 @@ def _gated_scan(x, gate, h0, reset, form):
 def gated_scan_backward(dy, x, gate, y, h0=None, reset=None, dlast=None, form='average'):
     """(dx, dgate, dh0) of gated_scan from the gradients of y (x's shape and type) and of
     last (float32, None: zeros). h0, reset and form are the forward pass's."""
-    kind, code, ax, T, B, D = _sizes(x, form)
-    ag, ay, ad, dev = _same(gate, x, 'gate'), _same(y, x, 'y'), _same(dy, x, 'dy'), x.device
-    first, end = vector(h0, B * D, F32, dev, 'h0'), vector(dlast, B * D, F32, dev, 'dlast')
-    flags = _flags(reset, x)
-    dx, dgate, dh0 = empty_like(x), empty_like(x), empty_f32(dev, *x.shape[1:])
-    work = _work(T, B, D, dev)
-    check(library().d1_gated_scan_backward(*ad, *ax, *ag, *ay, kind, code, T, B, D, first, end, *flags, dx.data_ptr(),
+    kind, code, ax, sizes, as_x = _sizes(x, form)
+    shape, _, dev = as_x
+    ag, ay, ad = _same(gate, *as_x, 'gate'), _same(y, *as_x, 'y'), _same(dy, *as_x, 'dy')
+    first, end = vector(h0, sizes[1] * sizes[2], F32, dev, 'h0'), vector(dlast, sizes[1] * sizes[2], F32, dev, 'dlast')
+    flags = _flags(reset, shape, dev)
+    dx, dgate, dh0 = empty_like(x), empty_like(x), empty_f32(dev, *shape[1:])
+    work = _work(sizes, dev)
+    check(library().d1_gated_scan_backward(*ad, *ax, *ag, *ay, kind, code, *sizes, first, end, *flags, dx.data_ptr(),
                                            dgate.data_ptr(), dh0.data_ptr(), None if work is None else work.data_ptr(),
                                            stream_of(x)), 'd1_gated_scan_backward')
     return dx, dgate, dh0
