@@ -178,7 +178,7 @@ __device__ __forceinline__ void take_steps(const Job &o, const Matrix &m, const 
             // F = polynomial of a a;  next = F q (in the first step q is F);  g = F a;  a = g F
             const bool poly = k ? p == 0 : p == 1, last = k + 1 == o.steps && p == 1;
             const int x = poly ? a : p == 3 ? g : f, y = poly ? a : p == 1 ? q : p == 2 ? a : f, to = poly ? f : p == 1 ? next : p == 2 ? g : a;
-lower.with_count([&](auto n) {
+            lower.with_count([&](auto n) {
                 constexpr int N = decltype(n)::value;
                 double2 c[3] = {};
                 lower.add<N>(c, space, x, y, 2 * side);
@@ -264,8 +264,7 @@ template <int THREADS> __device__ __forceinline__ void apply(const Job &o, const
                     store4((__half *)m.out + at, v);
             } else
                 for (int c = 0; c < 4 && col + c < m.cols; c++) {
-                    float x = v[0];
-                    x = c == 1 ? v[1] : c == 2 ? v[2] : c == 3 ? v[3] : x;
+                    float x = c == 0 ? v[0] : c == 1 ? v[1] : c == 2 ? v[2] : v[3];
                     if (m.param) m.param[at + c] = x = fmaf(rate, x, m.param[at + c] * keep);
                     if (m.out && m.out_type == D1_TYPE_BF16)
                         ((__nv_bfloat16 *)m.out)[at + c] = __float2bfloat16_rn(x);
