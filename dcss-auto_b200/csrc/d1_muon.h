@@ -155,12 +155,13 @@ struct Load {
         return n;
     }
     // Blocks of the cluster that takes a narrow matrix through everything in one launch, 0 where that is not done: a block has two
-    // of its blocks of X at most.
+    // of its blocks of X at most, one in the largest clusters of wider ones (three launches and one: 8 x 1,000 13.5 and 12.6 us,
+    // 100 x 60 x 120 55 and 48, but 48 x 1,000 30.7 and 32.0, 64 x 1,000 46 and 52).
     int whole_together() const {
         int n = 1;
         while (n < 8 && n < most_parts) n *= 2;
         n = clusters(n);
-        return most_parts <= 2 * n ? n : 0;
+        return most_parts <= (n == 8 && most_eights > 4 ? n : 2 * n) ? n : 0;
     }
     // CTAs of the cluster that takes each matrix through all products in one launch, 0 where that is not done: every
     // matrix has one tile of A and no more than two of X' a CTA (128 x 4,000, with four, took 138 us in place of the launches'

@@ -8,13 +8,13 @@
 // multiplied by a^2 = 11.9 a step where A_k should vanish, 2^-24 by 20,000 before the last of five. So A, F and Q are fp64 (the
 // fp64 form of mma.sync: tcgen05 has none), Q X is fp32. |u| is the root of the trace of u u^T, and A_0 is divided by the trace.
 //
-// Up to 16 blocks of X a matrix, a cluster does all of it in one launch, and its first block takes the steps. Longer ones have one launch for
+// Up to 8 or 16 blocks of X a matrix, a cluster does all of it in one launch, and its first block takes the steps. Longer ones have one launch for
 // momentum and A_0, one for the steps (a block a matrix) and one for the result. The sums of A_0 are a partial result of 18 KB of fp64 for
 // each block of threads; where they are many a cluster adds them (128 are 2.4 MB, 19 us at an SM's 64 bytes a cycle), always in
 // the same order.
 //
 // Measured (one B200, bf16, five steps; in brackets through the products of muon.cu). 1 x 8: 9 us (65). 28 x 512: 16 (80).
-// 64 x 64: 41 (68). 64 x 8,192: 51 (164). 16 x 64 x 4,096: 92 (215). With a side of 64 the steps are 33 of it: 17 products of 2,900 cycles,
+// 64 x 64: 41 (68). 64 x 8,192: 50 (164). 16 x 64 x 4,096: 91 (215). With a side of 64 the steps are 33 of it: 17 products of 2,900 cycles,
 // 2,300 of them the fp64 rate's (64 products and sums a cycle), the rest the way through shared memory.
 #pragma once
 

@@ -83,7 +83,7 @@ int main() {
                 if (!load.narrow() || load.most_parts != m.parts || load.most_eights != (int)((rows < cols ? rows : cols) + 7) / 8) return 19;
                 const int n = load.whole_together(), c = load.clusters(8);
                 if (n && ((n & (n - 1)) || n > 8 || m.parts > 2 * n || (n > 1 && count * n > room(n)))) return 20;
-                if (!n && (m.parts <= 2 || (count == 1 && cols <= 1024))) return 21;
+                if (!n && (m.parts <= 2 || (count == 1 && cols <= (rows <= 32 ? 1024 : 512)))) return 21;
                 if (c < 1 || c > 8 || (c > 1 && count * c > room(c))) return 22;
                 Matrix wide;
                 place(wide, 65, 65, block, part);
