@@ -37,7 +37,8 @@ struct Matrix {
     int sb;               // blocks along the smaller side
     int tall;             // rows > cols: the Gram matrix is X^T X
     int hi[2], lo, gram, quad;  // first blocks
-    int fine;             // small: A and B are pairs too (the second one a block after the first), and products take all three terms
+    int lo2;              // where a product writes lo when it reads the first one; the same where each tile reads its own only
+    int fine;             // A and F are pairs too (lo sb * sb blocks after hi), and products take all three terms
     int part0, parts;     // partial sums of the norm
     int grad_type, out_type;
     float rate, keep_decay;  // 0.2 sqrt(max(rows, cols)); the weight decay
@@ -56,32 +57,37 @@ struct Part {
 D1_MUON_BOTH int blocks_of(int64_t n) { return (int)((n + SIDE - 1) / SIDE); }
 D1_MUON_BOTH int tiles_of(int blocks, int side) { return (blocks + side - 1) / side; }
 
-// Blocks of A, or of B. With one block along the smaller side it is a pair.
-D1_MUON_BOTH int64_t gram_blocks(int64_t sb) { return sb == 1 ? 2 : sb * sb; }
+// Whether all products take three terms: where the caller asks for it, and with one block along the smaller side.
+D1_MUON_BOTH bool is_fine(int64_t sb, bool precise) { return precise || sb == 1; }
+// Blocks of A, or of F: a pair where it is fine.
+D1_MUON_BOTH int64_t gram_blocks(int64_t sb, bool precise) { return is_fine(sb, precise) ? 2 * sb * sb : sb * sb; }
+// Blocks of X: hi twice and lo, which a product of pairs may read and write in one place where a tile has all of the sum.
+D1_MUON_BOTH int64_t x_blocks(int64_t n, int64_t sb, bool precise) { return precise && sb > 1 ? 4 * n : 3 * n; }
 
 // Sizes, blocks (from `block` on) and parts (from `part` on) of a matrix; moves both on.
-inline void place(Matrix &m, int64_t rows, int64_t cols, int64_t &block, int64_t &part) {
+inline void place(Matrix &m, int64_t rows, int64_t cols, int64_t &block, int64_t &part, bool precise = false) {
     m.rows = (int)rows, m.cols = (int)cols;
     m.rb = blocks_of(rows), m.cb = blocks_of(cols);
     m.tall = rows > cols;
     m.sb = m.tall ? m.cb : m.rb;
-    m.fine = m.sb == 1;
-    const int64_t n = (int64_t)m.rb * m.cb, s = gram_blocks(m.sb);
+    m.fine = is_fine(m.sb, precise);
+    const int64_t n = (int64_t)m.rb * m.cb, s = gram_blocks(m.sb, precise), x = x_blocks(n, m.sb, precise);
     m.hi[0] = (int)block;
     m.hi[1] = (int)(block + n);
     m.lo = (int)(block + 2 * n);
-    m.gram = (int)(block + 3 * n);
-    m.quad = (int)(block + 3 * n + s);
-    block += 3 * n + 2 * s;
+    m.lo2 = x > 3 * n ? (int)(block + 3 * n) : m.lo;
+    m.gram = (int)(block + x);
+    m.quad = (int)(block + x + s);
+    block += x + 2 * s;
     m.part0 = (int)part;
     m.parts = (int)(n < MOST_PARTS ? n : MOST_PARTS);
     part += m.parts;
 }
 // Blocks that place() takes; -1 for a matrix that is out of range.
-inline int64_t blocks_needed(int64_t rows, int64_t cols) {
+inline int64_t blocks_needed(int64_t rows, int64_t cols, bool precise = false) {
     if (rows < 1 || cols < 1 || rows > ((int64_t)1 << 21) || cols > ((int64_t)1 << 21)) return -1;
     const int64_t rb = blocks_of(rows), cb = blocks_of(cols), sb = rows > cols ? cb : rb;
-    return 3 * rb * cb + 2 * gram_blocks(sb);
+    return x_blocks(rb * cb, sb, precise) + 2 * gram_blocks(sb, precise);
 }
 
 // Tile t of a symmetric matrix of tiles: row i >= column j, row after row. (In 32 bits and from a root, because the kernels
@@ -135,7 +141,7 @@ struct Load {
         const int terms = m.fine ? 3 : 1, first = (m.tall ? m.rb : m.cb) * terms, others = m.sb * terms;
         const int wide = tiles_of(m.sb, side), most = (int)full_tiles(m, side);
         matrices += count;
-        if (!m.fine) wider += count;
+        if (m.sb > 1) wider += count;
         if (m.parts > most_parts) most_parts = m.parts;
         const int eights = ((m.tall ? m.cols : m.rows) + 7) / 8;
         if (eights > most_eights) most_eights = eights;
@@ -178,7 +184,7 @@ struct Load {
     double microseconds() const {
         double sum = side == 4 ? 8. : 0.;
         for (int k = 0; k < 3; k++) {
-            const int parts = side == 4 ? 1 : parts_for(k < 2 ? symmetric : full, depth[k > 0]);
+            const int parts = side == 4 || k == 2 ? 1 : parts_for(symmetric, depth[k > 0]);
             const double even = work[k] / (side == 4 ? 74 : 148), longest = (double)depth[k > 0] / parts;
             sum += (side == 4 ? 0.43 : 0.5) * (even > longest ? even : longest);
         }

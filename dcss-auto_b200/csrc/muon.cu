@@ -14,9 +14,11 @@
 // whatever rounding puts there: of a gradient of low rank the result would be noise to a large part (simulated, rank 32 of
 // 512: 3 % of its norm in fp16, 22 % in bf16). So X is held as a pair hi + lo of fp16, 22 bits, and X' = F hi + a lo: where X
 // has nothing F is a, and the pair is carried on as one; elsewhere F lo is not a lo, an error of hi's size, but
-// in directions that X has (0.16 % there, 0.2 % of a full-rank one). In a matrix with a side of at most 64, where few
-// roundings average out (up to 1 % in some), A and F are pairs too and a product takes all three terms: it is as good as
-// one in fp32, and its time is the launches' all the same. Where all matrices are as narrow as that they take
+// in directions that X has (0.16 % there, 0.2 % of a full-rank one). That is a bf16 result's own rounding (0.17 %), but eight times an
+// fp16 one's: where the caller asks for it (`precise`), A and F are pairs too and a product takes all three terms, as good as one in
+// fp32 for up to three times the products' time (8,192 x 8,192 28.6 ms in place of 9.6, 7 x 1,777 x 1,003 908 us in place of 475, 512 x 512 247
+// in place of 167, all in one run). So it is in a matrix with a side of at most 64, where few
+// roundings average out (up to 1 % in some), and where its time is the launches' all the same. Where all matrices are as narrow as that they take
 // another way (muon_narrow.cuh).
 //
 // The three products of all matrices are one launch each. A and F are symmetric: only the tiles on and below the
@@ -81,7 +83,7 @@ __device__ __forceinline__ Matrix matrix_of(const Job &o, int m) {
     x.grad = (const char *)x.grad + m * o.grad_step;
     x.out = (char *)x.out + m * o.out_step;
     const int b = m * o.block_step;
-    x.hi[0] += b, x.hi[1] += b, x.lo += b, x.gram += b, x.quad += b;
+    x.hi[0] += b, x.hi[1] += b, x.lo += b, x.lo2 += b, x.gram += b, x.quad += b;
     x.part0 += m * x.parts;
     return x;
 }
@@ -280,13 +282,13 @@ struct Operands {
     int a_lo, b_lo;    // from a hi block to its lo block
 };
 __device__ __forceinline__ Operands operands(const Matrix &m, int phase, int from) {
-    const int hi = from ? m.hi[1] : m.hi[0], x_lo = m.lo - hi, terms = m.fine ? 3 : 1;
+    const int hi = from ? m.hi[1] : m.hi[0], x_lo = (from ? m.lo2 : m.lo) - hi, f_lo = m.sb * m.sb, terms = m.fine ? 3 : 1;
     if (phase == GRAM)
         return m.tall ? Operands{hi, 1, m.cb, hi, 1, m.cb, m.sb, m.sb, m.rb, true, true, false, false, terms, x_lo, x_lo}
                       : Operands{hi, m.cb, 1, hi, m.cb, 1, m.sb, m.sb, m.cb, false, false, false, false, terms, x_lo, x_lo};
-    if (phase == QUAD) return Operands{m.gram, m.sb, 1, m.gram, m.sb, 1, m.sb, m.sb, m.sb, false, false, true, true, terms, 1, 1};
-    return m.tall ? Operands{hi, m.cb, 1, m.quad, m.sb, 1, m.rb, m.cb, m.sb, false, false, false, true, terms, x_lo, 1}
-                  : Operands{m.quad, m.sb, 1, hi, 1, m.cb, m.rb, m.cb, m.sb, false, true, true, false, terms, 1, x_lo};
+    if (phase == QUAD) return Operands{m.gram, m.sb, 1, m.gram, m.sb, 1, m.sb, m.sb, m.sb, false, false, true, true, terms, f_lo, f_lo};
+    return m.tall ? Operands{hi, m.cb, 1, m.quad, m.sb, 1, m.rb, m.cb, m.sb, false, false, false, true, terms, x_lo, f_lo}
+                  : Operands{m.quad, m.sb, 1, hi, 1, m.cb, m.rb, m.cb, m.sb, false, true, true, false, terms, f_lo, x_lo};
 }
 
 // Where part r of `parts` of a product's sum begins.
@@ -558,7 +560,7 @@ template <bool PAIR> struct Roles {
         for (; ok && list.take(m, tile); local++) {
             const Operands p = operands(m, PHASE, from);
             const int b = local & 1, ib = tile.i * SIDES + 2 * rank + (q >> 1), r0 = 32 * (q & 1);
-            const int hi_to = from ? m.hi[0] : m.hi[1];
+            const int hi_to = from ? m.hi[0] : m.hi[1], lo_to_block = from ? m.lo : m.lo2;
             const int jb0 = tile.j * SIDES + half * (SIDES / 2);
             // unit u: columns 32 (u & 1) .. + 31 of block (ib, jb0 + u / 2); all warps' lanes agree on how many there are
             const int units = ib < p.ni ? max(0, min(UNITS, 2 * (p.nj - jb0))) : 0;
@@ -573,7 +575,7 @@ template <bool PAIR> struct Roles {
                 if (lane) return;
                 const int x = 32 * (u & 1), y = row_of(u);
                 mbar_expect_tx(sides0 + 8 * k, m.fine ? ROOM : ROOM / 2);
-                if (m.fine) tma_load_2d(rooms_at + k * ROOM + ROOM / 2, &map_units, sides0 + 8 * k, x, (m.gram + 1) * SIDE + y);
+                if (m.fine) tma_load_2d(rooms_at + k * ROOM + ROOM / 2, &map_units, sides0 + 8 * k, x, (m.gram + m.sb * m.sb) * SIDE + y);
                 tma_load_2d(rooms_at + k * ROOM, &map_units, sides0 + 8 * k, x, m.gram * SIDE + y);
             };
             const bool adds = !SYMMETRIC && !m.fine;
@@ -706,7 +708,7 @@ template <bool PAIR> struct Roles {
                     if (lane == 0) {
                         const int to = PHASE == GRAM ? m.gram : m.quad;
                         tma_store_2d(&map_units, room_at, x0, to * SIDE + y);
-                        if (m.fine) tma_store_2d(&map_units, room_at + ROOM / 2, x0, (to + 1) * SIDE + y);
+                        if (m.fine) tma_store_2d(&map_units, room_at + ROOM / 2, x0, (to + m.sb * m.sb) * SIDE + y);
                         bulk_commit();
                     }
                 } else {
@@ -738,7 +740,7 @@ template <bool PAIR> struct Roles {
                         __syncwarp();
                         if (lane == 0) {
                             tma_store_2d(&map_units, room_at, x0, hi_to * SIDE + y);
-                            if (m.fine) tma_store_2d(&map_units, room_at + ROOM / 2, x0, m.lo * SIDE + y);
+                            if (m.fine) tma_store_2d(&map_units, room_at + ROOM / 2, x0, lo_to_block * SIDE + y);
                             bulk_commit();
                         }
                     } else {
@@ -1001,7 +1003,7 @@ static int launch(Job &o, int64_t parts, int64_t blocks, const Load &load, int s
     for (int k = 0; k < steps; k++, o.from ^= 1)
         for (int phase = 0; phase < 3; phase++) {
             const int tiles = phase < 2 ? o.count_symmetric : o.count_full;
-            const int split = load.side == 4 ? 1 : parts_for(tiles, load.depth[phase > 0]);
+            const int split = load.side == 4 || phase == 2 ? 1 : parts_for(tiles, load.depth[phase > 0]);
             const int together = load.side == 4 ? 2 : split, most = SMS / together, n = tiles < most ? tiles : most;
             cfg.gridDim = dim3((unsigned)(n * together));
             cfg.numAttrs = together > 1 ? 2 : 1;
@@ -1025,13 +1027,13 @@ static int plan(const D1MuonTensor *tensors, int n, float *momentum, Plan &head,
     int64_t block = 0, part = 0;
     for (int t = 0; t < n; t++) {
         const D1MuonTensor &d = tensors[t];
-        const int64_t need = blocks_needed(d.rows, d.cols);
+        const int64_t need = blocks_needed(d.rows, d.cols, d.precise != 0);
         if (need < 0 || d.count < 0 || d.count > MOST_BLOCKS) return D1_ERR_BAD_ARGUMENT;
         if (need * d.count + block > MOST_BLOCKS) return D1_ERR_TOO_LARGE;
         if (!d.count) continue;
         Matrix m;
         int64_t from = block, from_part = part;
-        place(m, d.rows, d.cols, from, from_part);
+        place(m, d.rows, d.cols, from, from_part, d.precise != 0);
         block += (from - block) * d.count, part += (from_part - part) * d.count;
         head.matrices += d.count;
         small.add(m, d.count);
@@ -1059,7 +1061,7 @@ static int plan(const D1MuonTensor *tensors, int n, float *momentum, Plan &head,
         const int64_t size = d.rows * d.cols, grad_size = d.grad_type == D1_TYPE_F32 ? 4 : 2;
         for (int64_t c = 0; c < d.count; c++, k++) {
             Matrix m{};
-            place(m, d.rows, d.cols, block, part);
+            place(m, d.rows, d.cols, block, part, d.precise != 0);
             m.param = d.param + c * size;
             m.grad = (const char *)d.grad + c * size * grad_size;
             m.out = d.copy ? (char *)d.copy + c * size * 2 : nullptr;
@@ -1145,26 +1147,26 @@ extern "C" int d1_muon(const void *host_plan, const void *device_plan, double lr
 }
 
 // The stack's one matrix, its blocks and parts; false when it is out of range.
-static bool stack(int64_t count, int64_t rows, int64_t cols, Matrix &m, int64_t &blocks, int64_t &parts) {
-    const int64_t need = blocks_needed(rows, cols);
+static bool stack(int64_t count, int64_t rows, int64_t cols, bool precise, Matrix &m, int64_t &blocks, int64_t &parts) {
+    const int64_t need = blocks_needed(rows, cols, precise);
     if (need < 0 || count < 0 || count > MOST_BLOCKS || need * count > MOST_BLOCKS) return false;
     m = Matrix{};
     blocks = parts = 0;
-    place(m, rows, cols, blocks, parts);
+    place(m, rows, cols, blocks, parts, precise);
     return true;
 }
 
-extern "C" int64_t d1_orthogonalize_work_bytes(int64_t count, int64_t rows, int64_t cols) {
+static int64_t stack_bytes(int64_t count, int64_t rows, int64_t cols, bool precise) {
     Matrix m;
     int64_t blocks, parts;
-    return stack(count, rows, cols, m, blocks, parts) ? bytes_of(count * blocks, count * parts) : -1;
+    return stack(count, rows, cols, precise, m, blocks, parts) ? bytes_of(count * blocks, count * parts) : -1;
 }
 
-extern "C" int d1_orthogonalize(const void *x, int64_t ldx, int64_t x_step, int type, int64_t count, int64_t rows, int64_t cols, void *y, int y_type,
-                                int steps, void *work, void *stream) {
+static int orthogonalize(const void *x, int64_t ldx, int64_t x_step, int type, int64_t count, int64_t rows, int64_t cols, void *y, int y_type, int steps,
+                         bool precise, void *work, void *stream) {
     Matrix m;
     int64_t blocks, parts;
-    if (!d1::type_ok(type) || (y_type != D1_TYPE_BF16 && y_type != D1_TYPE_F16) || !stack(count, rows, cols, m, blocks, parts) || steps < 1 ||
+    if (!d1::type_ok(type) || (y_type != D1_TYPE_BF16 && y_type != D1_TYPE_F16) || !stack(count, rows, cols, precise, m, blocks, parts) || steps < 1 ||
         steps > 64 || (count && (!x || !y || !work)) || ldx < 0 || x_step < 0 || ldx > ((int64_t)1 << 42) || x_step > ((int64_t)1 << 42) ||
         !d1::element_aligned(x, type) || !d1::aligned_to(2, y) || !d1::aligned_to(128, work))
         return D1_ERR_BAD_ARGUMENT;
@@ -1190,6 +1192,17 @@ extern "C" int d1_orthogonalize(const void *x, int64_t ldx, int64_t x_step, int 
     o.work = (uint8_t *)work;
     o.partials = (double *)(o.work + work_blocks_bytes(count * blocks));
     return launch(o, count * parts, count * blocks, load, steps, (cudaStream_t)stream);
+}
+
+extern "C" int64_t d1_orthogonalize_work_bytes(int64_t count, int64_t rows, int64_t cols) { return stack_bytes(count, rows, cols, false); }
+extern "C" int d1_orthogonalize(const void *x, int64_t ldx, int64_t x_step, int type, int64_t count, int64_t rows, int64_t cols, void *y, int y_type,
+                                int steps, void *work, void *stream) {
+    return orthogonalize(x, ldx, x_step, type, count, rows, cols, y, y_type, steps, false, work, stream);
+}
+extern "C" int64_t d1_orthogonalize_precise_work_bytes(int64_t count, int64_t rows, int64_t cols) { return stack_bytes(count, rows, cols, true); }
+extern "C" int d1_orthogonalize_precise(const void *x, int64_t ldx, int64_t x_step, int type, int64_t count, int64_t rows, int64_t cols, void *y,
+                                        int y_type, int steps, void *work, void *stream) {
+    return orthogonalize(x, ldx, x_step, type, count, rows, cols, y, y_type, steps, true, work, stream);
 }
 
 // Last error recorded by a wait that ran out (0 = none); clears it.

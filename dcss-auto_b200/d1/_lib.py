@@ -112,13 +112,15 @@ SIGNATURES = {
     'd1_muon': [_P, _P, _D, _D, _I, _I, _P, _P],
     'd1_orthogonalize_work_bytes': [_I64, _I64, _I64],
     'd1_orthogonalize': [_P, _I64, _I64, _I, _I64, _I64, _I64, _P, _I, _I, _P, _P],
+    'd1_orthogonalize_precise_work_bytes': [_I64, _I64, _I64],
+    'd1_orthogonalize_precise': [_P, _I64, _I64, _I, _I64, _I64, _I64, _P, _I, _I, _P, _P],
     'd1_muon_error': [],
     'd1_adamw_work_bytes': [],
     'd1_adamw': [_P, _I, _I64, _I, _P, _P, _P, _P, _D, _D, _D, _D, _D, _P, _U64, _P, _P, _P],
 }
 
 RETURNS = {k: _I64 for k in ('d1_gated_scan_work_bytes', 'd1_policy_loss_work_bytes', 'd1_muon_plan_bytes', 'd1_muon_work_bytes',
-                             'd1_orthogonalize_work_bytes')}
+                             'd1_orthogonalize_work_bytes', 'd1_orthogonalize_precise_work_bytes')}
 
 _LIB = None
 

@@ -19,8 +19,8 @@ its storage for the optimizer's life (the step has their addresses).
 
 The products are fp16 with fp32 sums and X is held to 22 bits between them, so that a
 gradient of low rank comes out as exact as one of full rank (to 3e-3 of the result's norm; matrices with a
-side of at most 64 to 2e-4). The
-momentum is float32, flat over the tensors, each starting at a multiple of 128 elements
+side of at most 64 to 2e-4). precise=True takes products as good as fp32 ones, up to three times their time: X to 2e-4 for
+any size. The momentum is float32, flat over the tensors, each starting at a multiple of 128 elements
 (`offsets`); momentum_of(i) gives a tensor's in its shape. A step may be captured in a CUDA graph.
 Steps of one optimizer share its work buffer: run them on one stream, or ordered.
 """
@@ -39,7 +39,7 @@ MAX_STEPS = 64
 
 class _Tensor(C.Structure):
     _fields_ = [('param', C.c_void_p), ('grad', C.c_void_p), ('copy', C.c_void_p), ('count', C.c_int64), ('rows', C.c_int64),
-                ('cols', C.c_int64), ('decay', C.c_double), ('grad_type', C.c_int), ('reserved', C.c_int)]
+                ('cols', C.c_int64), ('decay', C.c_double), ('grad_type', C.c_int), ('precise', C.c_int)]
 
 
 def _steps_ok(steps):
@@ -48,7 +48,7 @@ def _steps_ok(steps):
 
 
 class Muon:
-    def __init__(self, params, grads, lr=3e-4, momentum=0.95, nesterov=True, weight_decay=0.01, steps=5, copies=None):
+    def __init__(self, params, grads, lr=3e-4, momentum=0.95, nesterov=True, weight_decay=0.01, steps=5, copies=None, precise=False):
         params, grads = list(params), list(grads)
         if not params or len(grads) != len(params):
             raise ValueError(f'{len(params)} parameters and {len(grads)} gradients')
@@ -71,7 +71,7 @@ class Muon:
                                [(f'copies[{i}]', c) for i, c in enumerate(copies) if c is not None])
         self.params, self.copies, self.decay = params, copies, decay
         self._leaves = [p for p in params if p.requires_grad]
-        self.lr, self.mu, self.nesterov, self.steps = lr, momentum, nesterov, steps
+        self.lr, self.mu, self.nesterov, self.steps, self.precise = lr, momentum, nesterov, steps, bool(precise)
         padded = [(p.numel() + 127) // 128 * 128 for p in params]
         self.offsets = [sum(padded[:i]) for i in range(len(padded))]
         self.momentum = torch.zeros(sum(padded), dtype=F32, device=self.device)
@@ -93,7 +93,7 @@ class Muon:
             _outside(g, i, self._written)
             rows, cols = p.shape[-2:]
             table[i] = _Tensor(p.data_ptr(), g.data_ptr(), None if c is None else c.data_ptr(), p.numel() // (rows * cols), rows, cols,
-                               self.decay[i], kind, 0)
+                               self.decay[i], kind, self.precise)
         size = self.lib.d1_muon_plan_bytes(table, len(grads))
         if size < 0:
             raise ValueError('the parameters are out of range (2^21 rows or columns, 2^36 elements of work)')
@@ -132,11 +132,13 @@ class Muon:
         self.momentum.copy_(m)
 
 
-def orthogonalize(x, steps=5, out=None):
+def orthogonalize(x, steps=5, out=None, precise=None):
     """x's directions with singular values brought near 1, matrix by matrix of [..., m, n]: bfloat16 or
     float16 as x is, bfloat16 of a float32 one (the products have 16 bits). Rows are contiguous, of one pitch, and
     the matrices of a stack one pitch apart. `out`: a contiguous tensor for the result (bfloat16 or float16), which
-    shares no memory with x."""
+    shares no memory with x. precise: products as good as fp32 ones, up to three times their time; None: for a float16 result, whose
+    own rounding the others' error (up to 3e-3 of the norm, a bfloat16 result's rounding) would pass. The result has no
+    gradient."""
     kind, dev = type_of(x, 'x'), x.device
     if x.dim() < 2:
         raise ValueError(f'x needs two dimensions, not {tuple(x.shape)}')
@@ -153,12 +155,16 @@ def orthogonalize(x, steps=5, out=None):
     elif out.dtype not in (BF16, torch.float16) or out.shape != x.shape or out.device != dev or not out.is_contiguous():
         raise ValueError(f'out must be a contiguous bfloat16 or float16 tensor {tuple(x.shape)} on {dev}')
     lib = library()
-    size = lib.d1_orthogonalize_work_bytes(count, rows, cols)
+    if precise is None:
+        precise = out.dtype is torch.float16
+    call, room = ((lib.d1_orthogonalize_precise, lib.d1_orthogonalize_precise_work_bytes) if precise else
+                  (lib.d1_orthogonalize, lib.d1_orthogonalize_work_bytes))
+    size = room(count, rows, cols)
     if size < 0:
         raise ValueError(f'{count} matrices of {rows} x {cols} are out of range')
     work = torch.empty(size, dtype=torch.uint8, device=dev)
-    check(lib.d1_orthogonalize(x.data_ptr(), x.stride(-2), between, kind, count, rows, cols, out.data_ptr(), type_of(out, 'out'), steps,
-                               work.data_ptr(), stream_of(x)), 'd1_orthogonalize')
+    check(call(x.data_ptr(), x.stride(-2), between, kind, count, rows, cols, out.data_ptr(), type_of(out, 'out'), steps, work.data_ptr(),
+               stream_of(x)), 'd1_orthogonalize')
     return out
 
 

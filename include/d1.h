@@ -790,15 +790,15 @@ int d1_policy_loss(const float *logp, int64_t ld_logp, const float *old_logp, in
 
 /* One parameter tensor of d1_muon: `count` matrices of rows x cols (at most 2^21 each)
  * fp32 elements behind one another at param, their gradients (fp32 or bf16), the bf16
- * compute copy that each step refreshes (or NULL), decay = the weight decay. param
- * and copy overlap no other param, copy or gradient. */
+ * compute copy that each step refreshes (or NULL), decay = the weight decay. precise: 0, or
+ * 1 for products as good as fp32 ones (d1_muon). param and copy overlap no other param, copy or gradient. */
 typedef struct {
     float *param;
     const void *grad;
     void *copy;
     int64_t count, rows, cols;
     double decay;
-    int grad_type, reserved;
+    int grad_type, precise;
 } D1MuonTensor;
 /* Bytes of the plan and of the work buffer for these tensors (a HOST array); -1 when
  * they are out of range or hold no matrix. Both are worked out on the host. */
@@ -813,8 +813,8 @@ int d1_muon_plan(const D1MuonTensor *tensors, int ntensors, float *momentum, voi
  *   X = u / |u|_F, and `steps` (1 to 64) times X = 3.4445 X - 4.7750 (X X^T) X + 2.0315 (X X^T)^2 X
  *   p = p (1 - lr decay) - lr 0.2 sqrt(max(rows, cols)) X
  * An update of zeros leaves X zero. Products are fp16 with fp32 sums, X is held
- * to 22 bits (where a side is at most 64 they are as good as fp32 ones). host_plan and device_plan are the two copies of the plan; work is
- * 128-byte aligned. Calls that share work or state must not overlap. */
+ * to 22 bits: 3e-3 of X's norm in five steps. Where a tensor is `precise`, or a side is at most 64, they are as good as fp32
+ * ones. host_plan and device_plan are the two copies of the plan; work is 128-byte aligned. Calls that share work or state must not overlap. */
 int d1_muon(const void *host_plan, const void *device_plan, double lr, double momentum, int nesterov, int steps, void *work, void *stream);
 /* The orthogonalisation by itself: y[k] = X after `steps` steps from u = x[k], for
  * `count` matrices of type `type` with row pitch ldx, x_step elements from one to the
@@ -823,6 +823,11 @@ int d1_muon(const void *host_plan, const void *device_plan, double lr, double mo
 int64_t d1_orthogonalize_work_bytes(int64_t count, int64_t rows, int64_t cols);
 int d1_orthogonalize(const void *x, int64_t ldx, int64_t x_step, int type, int64_t count, int64_t rows, int64_t cols, void *y, int y_type,
                      int steps, void *work, void *stream);
+/* The same with products as good as fp32 ones (up to three times the time where both sides are above 64), as an fp16 result has
+ * the bits for, and with a work buffer of its own size. */
+int64_t d1_orthogonalize_precise_work_bytes(int64_t count, int64_t rows, int64_t cols);
+int d1_orthogonalize_precise(const void *x, int64_t ldx, int64_t x_step, int type, int64_t count, int64_t rows, int64_t cols, void *y, int y_type,
+                             int steps, void *work, void *stream);
 /* Last error recorded by a wait of the products that ran out (0: none); clears it. */
 int d1_muon_error(void);
 
