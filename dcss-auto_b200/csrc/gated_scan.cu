@@ -16,7 +16,8 @@
 // half a rounding step of dg.
 //
 // Both directions are the map s -> a s + b, whose composition over a chunk of
-// steps is again such a map (P, Q). With enough channels one thread walks each
+// steps is again such a map (P, Q); decays of the sum form may pass 1, and their product fp32 where no state does: there P is a
+// number and a power of 2. With enough channels one thread walks each
 // of them through the whole time, a few steps' loads ahead of the arithmetic.
 // With few channels the time is cut into chunks: one launch reduces each chunk
 // to its (P, Q), a second runs over the chunks, a third walks all of them side
@@ -24,7 +25,8 @@
 //
 // Measured (one B200; floor: each operand once at 6.56 TB/s). 128 steps of 4,096 x 512 channels bf16: 247 us, the floor's
 // rate; 64 steps backward 268 (93 %). 131,072 steps of 256 channels 69 us (floor 31): 31 for the reduction, 33 for the walk, the
-// rest the launch between them. 50,021 x 3 x 111 fp32 backward 103 to 110 us (51). One step of 64 x 256: 1.9 us.
+// rest the launch between them; 82 in the sum form (70 without the powers). 50,021 x 3 x 111 fp32 backward, sum form, 110 us (51; 105 without).
+// One step of 64 x 256: 1.9 us.
 //
 // A reset replaces the state: a product with 0 would keep an infinity.
 #include <type_traits>
@@ -41,6 +43,7 @@ constexpr int MOST_CHUNKS = CARRY_RUNS * CARRY_EACH;
 // P of a chunk with a reset in it: the state before it does not reach its end (decays
 // are not negative, and one that has underflowed to 0 still lets an infinity through).
 constexpr float CUT = -1.f;
+constexpr int MOST_POWER = 1 << 26;  // of P; past this on either side it overflows or removes every state
 
 // A [T, B, D] operand with contiguous channels: strides in elements.
 template <class T> struct Span {
@@ -57,6 +60,7 @@ template <class T> struct Args {
     const float *h0;               // backward: the first step's state (NULL: zeros)
     float *last;                   // last forward, dh0 backward (may be NULL)
     float2 *carry;                 // [chunks][B * D]: (P, Q), then (state before the chunk, -)
+    int *power;                    // [chunks][B * D], sum form: the power of 2 that goes with P
     int64_t T_, B, D, lanes;       // lanes = B * D / V
     int64_t size;                  // steps of a chunk
     int chunks;
@@ -70,6 +74,15 @@ __device__ __forceinline__ float2 gates(float g) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x));
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(1.f + e));
     return make_float2(e * w, w);
+}
+
+// x = x 2^k, 1 <= x < 2, where x is positive and normal; the power is added to `power`.
+__device__ __forceinline__ void take_power(float &x, int &power) {
+    const uint32_t bits = __float_as_uint(x);
+    if (bits - 0x00800000u < 0x7f000000u) {
+        power += (int)(bits >> 23) - 127;
+        x = __uint_as_float((bits & 0x007fffffu) | 0x3f800000u);
+    }
 }
 
 // V elements as they lie in memory: words, so that a step under way takes no more registers than its bytes.
@@ -168,6 +181,7 @@ __global__ void __launch_bounds__(THREADS, blocks_of(V, BACK, PART)) scan_kernel
     }
     w.out = a.out + first * C + c, w.sout = SIGN * C;
     float s[V], prod[V];
+    int power[V];  // (sum form)
     // Resets: where a warp has one sequence and one chunk its lanes look at 32 steps at a time.
     const bool shared = a.reset && a.lanes % 32 == 0 && per % 32 == 0;
     const uint8_t *reset = a.reset ? a.reset + b * a.reset_b + (first + (shared ? SIGN * (int)(threadIdx.x & 31) : 0)) * a.reset_t : nullptr;
@@ -224,7 +238,10 @@ __global__ void __launch_bounds__(THREADS, blocks_of(V, BACK, PART)) scan_kernel
                 }
                 s[v] = cut ? 0.f : f.x * D;
             }
-            if constexpr (PART == 0) prod[v] = cut || prod[v] < 0.f ? CUT : prod[v] * f.x;
+            if constexpr (PART == 0) {
+                if constexpr (SUM) take_power(f.x, power[v]);
+                prod[v] = cut || prod[v] < 0.f ? CUT : prod[v] * f.x;
+            }
         }
         if constexpr (PART == 1) {
             Raw<T, V>::store(w.out, r);
@@ -232,6 +249,15 @@ __global__ void __launch_bounds__(THREADS, blocks_of(V, BACK, PART)) scan_kernel
             if constexpr (BACK) {
                 Raw<T, V>::store(w.dgate, dg);
                 w.dgate += w.sout;
+            }
+        }
+    };
+    const auto normalise = [&] {  // after U steps at most: below 2^(U + 1) till then
+        if constexpr (PART == 0 && SUM) {
+#pragma unroll
+            for (int v = 0; v < V; v++) {
+                take_power(prod[v], power[v]);
+                power[v] = max(-MOST_POWER, min(MOST_POWER, power[v]));
             }
         }
     };
@@ -252,6 +278,7 @@ __global__ void __launch_bounds__(THREADS, blocks_of(V, BACK, PART)) scan_kernel
     const auto compute = [&](const Step<T, V>(&of)[U], uint32_t cuts) {
 #pragma unroll
         for (int u = 0; u < U; u++) advance(of[u], cuts >> u & 1, false);
+        normalise();
     };
     if (groups) cp = fetch(p, 0);
     // The launches before this one read what it has read so far, and wrote none of it (the first of them began when all
@@ -260,6 +287,7 @@ __global__ void __launch_bounds__(THREADS, blocks_of(V, BACK, PART)) scan_kernel
 #pragma unroll
     for (int v = 0; v < V; v++) {
         prod[v] = 1.f;
+        power[v] = 0;
         s[v] = 0.f;
         if constexpr (PART == 1) s[v] = a.chunks > 1 ? a.carry[chunk * C + c + v].x : a.start ? a.start[c + v] : 0.f;
     }
@@ -277,50 +305,90 @@ __global__ void __launch_bounds__(THREADS, blocks_of(V, BACK, PART)) scan_kernel
         const bool earliest = BEFORE && i == n - 1 && first == n - 1;
         if (BEFORE && !earliest) w.load_before(p[0]);
         advance(p[0], cuts_of(i, 1) & 1, earliest);
+        normalise();
     }
 #pragma unroll
     for (int v = 0; v < V; v++) {
-        if constexpr (PART == 0)
+        if constexpr (PART == 0) {
             a.carry[chunk * C + c + v] = make_float2(prod[v], s[v]);
-        else if (a.last && chunk == a.chunks - 1)
+            if constexpr (SUM) a.power[chunk * C + c + v] = power[v];
+        } else if (a.last && chunk == a.chunks - 1)
             a.last[c + v] = s[v];
     }
 }
 
-// The map of one piece and then another.
-__device__ __forceinline__ float2 after(float2 first, float2 then) {
-    return make_float2(first.x < 0.f || then.x < 0.f ? CUT : first.x * then.x, then.x < 0.f ? then.y : fmaf(then.x, first.y, then.y));
+// The map of a piece of the time: s -> p 2^power s + q.
+template <bool SUM> struct Map {
+    float p = 1.f, q = 0.f;
+    int power = 0;  // (0 in the average form)
+};
+// Of a state through it: the power first, which a state of 0 bears whatever it is.
+template <bool SUM> __device__ __forceinline__ float through(const Map<SUM> &map, float s) {
+    return map.p < 0.f ? map.q : fmaf(map.p, SUM ? scalbnf(s, map.power) : s, map.q);
 }
-__device__ __forceinline__ float through(float2 map, float s) { return map.x < 0.f ? map.y : fmaf(map.x, s, map.y); }
+// Of one piece and then another.
+template <bool SUM> __device__ __forceinline__ Map<SUM> after(const Map<SUM> &first, const Map<SUM> &then) {
+    Map<SUM> both;
+    both.p = first.p < 0.f || then.p < 0.f ? CUT : first.p * then.p;
+    both.q = through(then, first.q);
+    if (SUM) both.power = first.power + then.power;
+    return both;
+}
+// After up to 16 joins of normalised ones.
+__device__ __forceinline__ void normalise(Map<true> &m) {
+    take_power(m.p, m.power);
+    m.power = max(-MOST_POWER, min(MOST_POWER, m.power));
+}
+__device__ __forceinline__ void normalise(Map<false> &) {}
 
 // The state before every chunk, in place of its (P, Q): eight channels a block, the chunks divided between 128
 // threads for each, which hold theirs and join them by doubling. (A warp for each of 32 runs of chunks, reading
 // them twice, took 26 us for 2,048 chunks of 256 channels: the latency of its loads.)
-__global__ void __launch_bounds__(CARRY_RUNS * CARRY_CHANNELS) carry_kernel(float2 *carry, const float *start, int64_t C, int chunks) {
+template <bool SUM>
+__global__ void __launch_bounds__(CARRY_RUNS * CARRY_CHANNELS) carry_kernel(float2 *carry, const int *power, const float *start, int64_t C, int chunks) {
     pdl_launch();
     pdl_wait();
     __shared__ float2 sums[CARRY_RUNS][CARRY_CHANNELS];
+    __shared__ int powers[SUM ? CARRY_RUNS : 1][CARRY_CHANNELS];
     const int run = threadIdx.x / CARRY_CHANNELS, lane = threadIdx.x % CARRY_CHANNELS;
     const int64_t c = (int64_t)blockIdx.x * CARRY_CHANNELS + lane;
     const int each = (chunks + CARRY_RUNS - 1) / CARRY_RUNS, lo = run * each;
-    float2 m[CARRY_EACH];
+    Map<SUM> m[CARRY_EACH];
 #pragma unroll
     for (int k = 0; k < CARRY_EACH; k++)
-        m[k] = k < each && lo + k < chunks && c < C ? carry[(lo + k) * C + c] : make_float2(1.f, 0.f);
-    float2 all = m[0];
+        if (k < each && lo + k < chunks && c < C) {
+            const float2 of = carry[(lo + k) * C + c];
+            m[k].p = of.x, m[k].q = of.y;
+            if constexpr (SUM) m[k].power = power[(lo + k) * C + c];
+        }
+    Map<SUM> all = m[0];
 #pragma unroll
     for (int k = 1; k < CARRY_EACH; k++) all = after(all, m[k]);
-    sums[run][lane] = all;
+    normalise(all);
+    const auto put = [&] {
+        sums[run][lane] = make_float2(all.p, all.q);
+        if constexpr (SUM) powers[run][lane] = all.power;
+    };
+    const auto get = [&](int r) {
+        Map<SUM> of;
+        of.p = sums[r][lane].x, of.q = sums[r][lane].y;
+        if constexpr (SUM) of.power = powers[r][lane];
+        return of;
+    };
+    put();
     __syncthreads();
 #pragma unroll
     for (int d = 1; d < CARRY_RUNS; d *= 2) {
-        const float2 before = run >= d ? sums[run - d][lane] : make_float2(1.f, 0.f);
+        Map<SUM> before;
+        if (run >= d) before = get(run - d);
         __syncthreads();
-        sums[run][lane] = all = after(before, all);
+        all = after(before, all);
+        normalise(all);
+        put();
         __syncthreads();
     }
     float s = start && c < C ? start[c] : 0.f;
-    if (run) s = through(sums[run - 1][lane], s);
+    if (run) s = through(get(run - 1), s);
 #pragma unroll
     for (int k = 0; k < CARRY_EACH; k++)
         if (k < each && lo + k < chunks && c < C) {
@@ -345,6 +413,7 @@ template <class T, int V, bool SUM, bool BACK> static int run(Args<T> &a, cudaSt
     a.chunks = (int)((a.T_ + a.size - 1) / a.size);
     if (a.size > INT32_MAX) return D1_ERR_TOO_LARGE;
     if (a.chunks > 1 && !a.carry) return D1_ERR_BAD_ARGUMENT;
+    a.power = (int *)(a.carry + a.chunks * a.B * a.D);
     const int64_t blocks = (a.lanes * a.chunks + THREADS - 1) / THREADS;
     if (blocks > INT32_MAX) return D1_ERR_TOO_LARGE;
     cudaLaunchAttribute attr;
@@ -357,7 +426,7 @@ template <class T, int V, bool SUM, bool BACK> static int run(Args<T> &a, cudaSt
         const int64_t C = a.B * a.D;
         mid.gridDim = dim3((unsigned)((C + CARRY_CHANNELS - 1) / CARRY_CHANNELS));
         mid.blockDim = dim3(CARRY_RUNS * CARRY_CHANNELS);
-        if (cudaError_t e = cudaLaunchKernelEx(&mid, carry_kernel, a.carry, a.start, C, a.chunks)) return (int)e;
+        if (cudaError_t e = cudaLaunchKernelEx(&mid, carry_kernel<SUM>, a.carry, a.power, a.start, C, a.chunks)) return (int)e;
     }
     return (int)cudaLaunchKernelEx(&cfg, scan_kernel<T, V, SUM, BACK, 1, U>, a);
 }
@@ -403,7 +472,7 @@ extern "C" int64_t d1_gated_scan_work_bytes(int64_t T, int64_t B, int64_t D) {
             const int chunks = chunks_of(T, B * D / V, blocks_of(V, back, 1));
             if (chunks > 1 && chunks > most) most = chunks;
         }
-    return 8 * most * B * D;
+    return 8 * ((3 * most + 1) / 2) * B * D;  // 8 bytes of (P, Q) and 4 of a power
 }
 
 extern "C" int d1_gated_scan(const void *x, int64_t x_t, int64_t x_b, const void *gate, int64_t gate_t, int64_t gate_b,

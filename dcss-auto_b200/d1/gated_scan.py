@@ -7,7 +7,7 @@
 Each of the D channels of each of the B sequences has a state of its own:
 
     form 'average':  a = sigmoid(gate)   h_t = a_t h_{t-1} + (1 - a_t) x_t
-    form 'sum':      a = exp(gate)       h_t = a_t h_{t-1} + x_t
+    form 'sum':      a = exp(gate)       h_t = a_t h_{t-1} + x_t     (a is float32: infinite for gates above 88.7)
 
 x and gate are float32, bfloat16 or float16 [T, ..., D], time first as the
 rollouts are, with contiguous channels and one pitch between sequences (a slice

@@ -740,7 +740,7 @@ int d1_adamw(const D1AdamWTensor *tensors, int ntensors, int64_t nblocks, int st
  * in the reference.
  * ====================================================================== */
 #define D1_SCAN_AVERAGE 0 /* a = sigmoid(gate), h_t = a_t h_{t-1} + (1 - a_t) x_t */
-#define D1_SCAN_SUM 1     /* a = e^gate,        h_t = a_t h_{t-1} + x_t */
+#define D1_SCAN_SUM 1     /* a = e^gate (f32),  h_t = a_t h_{t-1} + x_t */
 
 /* Bytes of the work buffer of d1_gated_scan and its backward pass (0: none
  * needed); -1 for sizes out of range. */
