@@ -18,8 +18,8 @@
 // fp16 one's: where the caller asks for it (`precise`), A and F are pairs too and a product takes all three terms, as good as one in
 // fp32 for up to three times the products' time (8,192 x 8,192 28.6 ms in place of 9.6, 7 x 1,777 x 1,003 908 us in place of 475, 512 x 512 247
 // in place of 167, all in one run). So it is in a matrix with a side of at most 64, where few
-// roundings average out (up to 1 % in some), and where its time is the launches' all the same. Where all matrices are as narrow as that they take
-// another way (muon_narrow.cuh).
+// roundings average out (up to 1 % in some), and where its time is the launches' all the same. Where all matrices are as narrow as that up to five
+// steps are taken another way (muon_narrow.cuh).
 //
 // The three products of all matrices are one launch each. A and F are symmetric: only the tiles on and below the
 // diagonal are computed and stored, and read transposed for those above. The epilogues hold the rest of the
@@ -965,7 +965,7 @@ static int launch(Job &o, int64_t parts, int64_t blocks, const Load &load, int s
     cfg.numAttrs = 0;
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    if (load.narrow()) {
+    if (load.narrow() && steps <= narrow::MOST_STEPS) {
         cudaLaunchConfig_t mid = cfg;
         mid.blockDim = cfg.blockDim = dim3(narrow::THREADS_SUM);
         if (const int n = load.whole_together()) {

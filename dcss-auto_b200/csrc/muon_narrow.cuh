@@ -6,7 +6,9 @@
 //
 // X is read twice instead of twice a step, and what lies between is 64 x 64 at most. Its price is precision: an error of A_0 is
 // multiplied by a^2 = 11.9 a step where A_k should vanish, 2^-24 by 20,000 before the last of five. So A, F and Q are fp64 (the
-// fp64 form of mma.sync: tcgen05 has none), Q X is fp32. |u| is the root of the trace of u u^T, and A_0 is divided by the trace.
+// fp64 form of mma.sync: tcgen05 has none), Q X is fp32. And its end are five steps: A_k may be a little below 0, where F_k pulls nothing back,
+// so that an error of 2^-56 of a matrix of low rank has passed 1 in 16 steps (and is NaN in 20); before that, fp32's rounding of X passes 2^-12 with
+// Q, a factor of 3.4 a step. More steps go through the products of muon.cu, which take A from X each time. |u| is the root of the trace of u u^T, and A_0 is divided by the trace.
 //
 // Up to 8 or 16 blocks of X a matrix, a cluster does all of it in one launch, and its first block takes the steps. Longer ones have one launch for
 // momentum and A_0, one for the steps (a block a matrix) and one for the result. The sums of A_0 are a partial result of 18 KB of fp64 for
@@ -24,6 +26,7 @@ constexpr int MOST = 64, TILES = 36, WARPS = 12, THREADS_SUM = 32 * WARPS, THREA
 constexpr int WIDTH = MOST + 4;  // fp64 of a row in shared memory: eight rows of four meet no bank twice
 constexpr int PART_BYTES = 3 * BLOCK_BYTES;
 constexpr int FEW = 8;  // partial sums that one block adds
+constexpr int MOST_STEPS = 5;
 
 static_assert(TILES * 64 * 8 <= PART_BYTES, "a part's sums lie in place of its blocks of X");
 
