@@ -34,6 +34,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <atomic>
 #include <new>
 #include <type_traits>
 
@@ -57,7 +58,10 @@ constexpr uint32_t WAIT_LIMIT = 1u << 22;
 constexpr float SCALE = 4096.f, UNSCALE = 1.f / 4096.f;  // of X, A and F in fp16
 constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
 
+// The last wait that ran out, on this device. While it stands no step changes a master: some of what it is made from is missing.
 __device__ int g_error;
+// The same in pinned host memory, of any device, where the caller sees it without a synchronisation (NULL: nowhere).
+static std::atomic<int *> told{nullptr};
 
 struct Job {
     const Matrix *matrices;  // NULL: a stack of `one`
@@ -75,7 +79,16 @@ struct Job {
     int from;   // which hi is read
     int steps;
     int adders;  // narrow matrices: blocks that add the sums of one
+    int *told;
 };
+
+__device__ __forceinline__ void fail(const Job &o, int code) {
+    atomicExch(&g_error, code);
+    if (o.told) {
+        *(volatile int *)o.told = code;
+        __threadfence_system();
+    }
+}
 
 __device__ __forceinline__ Matrix matrix_of(const Job &o, int m) {
     if (o.matrices) return o.matrices[m];
@@ -484,7 +497,7 @@ template <bool PAIR> struct Roles {
     // After the last product: what is under way lands before the block leaves.
     __device__ __forceinline__ void loaded() {
         if (!ok) {
-            atomicExch(&g_error, 1);
+            fail(o, 1);
             if (rank == 0)  // copies under way land before the block leaves
                 for (int i = in_flight; i < it; i++) mbar_wait(full0 + 8 * (i % STAGES), (uint32_t)(i / STAGES) & 1u, WAIT_LIMIT);
         } else  // and so do the last signals that a stage is free
@@ -501,7 +514,7 @@ template <bool PAIR> struct Roles {
             const int b = local & 1;
             const uint32_t acc = tmem + (uint32_t)(b * COLS);
             if (local >= 2 && !mbar_wait(acce0 + 8 * b, ((uint32_t)(local >> 1) & 1u) ^ 1u, WAIT_LIMIT)) {
-                atomicExch(&g_error, 2);
+                fail(o, 2);
                 ok = false;
                 break;
             }
@@ -510,7 +523,7 @@ template <bool PAIR> struct Roles {
             for (int n = begin, k = begin % p.nk; n < end; n++, it++) {
                 const int s = it % STAGES;
                 if (!mbar_wait(full0 + 8 * s, (uint32_t)(it / STAGES) & 1u, WAIT_LIMIT)) {
-                    atomicExch(&g_error, 3);
+                    fail(o, 3);
                     ok = false;
                     break;
                 }
@@ -554,6 +567,7 @@ template <bool PAIR> struct Roles {
         uint8_t *const area = smem + STAGES * STAGE_BYTES;
         uint8_t *const rooms = area + (SPLIT ? (index + own) / parts * parts : (warp - 2) * 2) * ROOM;
         const uint32_t rooms_at = smem_u32(rooms), sides0 = sides_at + 16 * (warp - 2);
+        const bool failed = PHASE == STEP && __any_sync(0xffffffffu, *(volatile int *)&g_error);
         bool met = false;
         Matrix m;
         Tile tile;
@@ -605,7 +619,7 @@ template <bool PAIR> struct Roles {
                     if (i < m.rows && j0 + j < m.cols) asm volatile("prefetch.global.L2 [%0];" ::"l"(m.param + (int64_t)i * m.cols + j0 + j));
             }
             if (!mbar_wait(accf0 + 8 * b, (uint32_t)(local >> 1) & 1u, WAIT_LIMIT)) {
-                atomicExch(&g_error, 4);
+                fail(o, 4);
                 ok = false;
                 break;
             }
@@ -660,7 +674,7 @@ template <bool PAIR> struct Roles {
                     pending &= ~(1u << k);
                     turns ^= 1u << k;
                     if (!mbar_wait(sides0 + 8 * k, (turns >> k & 1u) ^ 1u, WAIT_LIMIT)) {
-                        atomicExch(&g_error, 5);
+                        fail(o, 5);
                         ok = false;
                         break;
                     }
@@ -744,7 +758,7 @@ template <bool PAIR> struct Roles {
                             bulk_commit();
                         }
                     } else {
-                        finish(o, m, ib * SIDE + r0, jb0 * SIDE + 32 * u, x, params, reinterpret_cast<float *>(room));
+                        if (!failed || !m.param) finish(o, m, ib * SIDE + r0, jb0 * SIDE + 32 * u, x, params, reinterpret_cast<float *>(room));
                         if (!SPLIT) ask(u + 1);
                     }
                 }
@@ -960,6 +974,7 @@ static int launch(Job &o, int64_t parts, int64_t blocks, const Load &load, int s
     o.count_symmetric = (int)load.symmetric, o.count_full = (int)load.full;
     if (const int e = allow_space()) return e;
     o.steps = steps;
+    o.told = told;
     cudaLaunchAttribute attr[2];
     cudaLaunchConfig_t cfg = pdl_config(dim3((unsigned)parts), dim3(PREP), 0, s, attr);
     cfg.numAttrs = 0;
@@ -1210,5 +1225,16 @@ extern "C" int d1_muon_error(void) {
     int h = 0, z = 0;
     if (cudaMemcpyFromSymbol(&h, g_error, sizeof(int)) != cudaSuccess) return -1;
     if (h) cudaMemcpyToSymbol(g_error, &z, sizeof(int));
+    if (int *const p = told) *p = 0;
     return h;
+}
+extern "C" int d1_muon_error_flag(int *flag) {
+    if (!d1::aligned_to(4, flag)) return D1_ERR_BAD_ARGUMENT;
+    told = flag;
+    return 0;
+}
+extern "C" int d1_muon_set_error(int code) {
+    if (cudaError_t e = cudaMemcpyToSymbol(g_error, &code, sizeof(int))) return (int)e;
+    if (int *const p = told) *p = code;
+    return 0;
 }

@@ -114,7 +114,7 @@ SIGNATURES = {
     'd1_orthogonalize': [_P, _I64, _I64, _I, _I64, _I64, _I64, _P, _I, _I, _P, _P],
     'd1_orthogonalize_precise_work_bytes': [_I64, _I64, _I64],
     'd1_orthogonalize_precise': [_P, _I64, _I64, _I, _I64, _I64, _I64, _P, _I, _I, _P, _P],
-    'd1_muon_error': [],
+    'd1_muon_error': [], 'd1_muon_error_flag': [_P], 'd1_muon_set_error': [_I],
     'd1_adamw_work_bytes': [],
     'd1_adamw': [_P, _I, _I64, _I, _P, _P, _P, _P, _D, _D, _D, _D, _D, _P, _U64, _P, _P, _P],
 }

@@ -23,13 +23,14 @@ side of at most 64 to 2e-4). precise=True takes products as good as fp32 ones, u
 any size. Each further step makes the directions that a gradient does not have 3.4 times as large: from some twelve on a gradient of low
 rank has them too, as in any arithmetic of 32 bits. The momentum is float32, flat over the tensors, each starting at a multiple of 128 elements
 (`offsets`); momentum_of(i) gives a tensor's in its shape. A step may be captured in a CUDA graph.
-Steps of one optimizer share its work buffer: run them on one stream, or ordered.
+Steps of one optimizer share its work buffer: run them on one stream, or ordered. A step that failed is seen by the next
+one, which raises, or by check().
 """
 import ctypes as C
 
 import torch
 
-from ._lib import check, library, stream_of
+from ._lib import D1Error, check, library, stream_of
 from ._rows import type_of
 from .adamw import GRAD_TYPES, _outside, _spans
 from .gated_scan import _pitch
@@ -41,6 +42,23 @@ MAX_STEPS = 64
 class _Tensor(C.Structure):
     _fields_ = [('param', C.c_void_p), ('grad', C.c_void_p), ('copy', C.c_void_p), ('count', C.c_int64), ('rows', C.c_int64),
                 ('cols', C.c_int64), ('decay', C.c_double), ('grad_type', C.c_int), ('precise', C.c_int)]
+
+
+_told = None   # a pinned int that a failed call sets, looked at before the next one
+
+
+def _watch():
+    """Raises if a call before this one is known to have failed."""
+    global _told
+    if _told is None:
+        if torch.cuda.is_current_stream_capturing():   # (no time to allocate)
+            return
+        flag = torch.zeros(1, dtype=torch.int32).pin_memory()
+        check(library().d1_muon_error_flag(flag.data_ptr()), 'd1_muon_error_flag')
+        _told = C.c_int.from_address(flag.data_ptr()), flag
+    if _told[0].value:
+        raise D1Error(f'a wait of an earlier Muon step or orthogonalisation ran out (error {_told[0].value}): what it wrote is incomplete, '
+                      'the parameters of a step may be too. muon_error() clears it')
 
 
 def _steps_ok(steps):
@@ -107,11 +125,22 @@ class Muon:
         self._plan.copy_(torch.frombuffer(bytearray(host), dtype=torch.uint8))
 
     def step(self, lr=None):
-        """One step, in place. lr: this step's learning rate (default: self.lr)."""
+        """One step, in place. lr: this step's learning rate (default: self.lr). Raises D1Error where an earlier step is
+        known to have failed (see check())."""
+        _watch()
         check(self.lib.d1_muon(self._host, self._plan.data_ptr(), self.lr if lr is None else lr, self.mu, int(self.nesterov),
                                self.steps, self._work.data_ptr(), stream_of(self.momentum)), 'd1_muon')
         if self._leaves:  # torch then refuses a backward pass through what the step has overwritten
             torch.autograd.graph.increment_version(self._leaves)
+
+    def check(self):
+        """Raise if a wait inside the steps so far ran out (a GPU that others held for seconds): such a step leaves
+        the matrices that go through the products as they were, but for those it had already updated. Synchronises the
+        device and clears the error."""
+        torch.cuda.synchronize(self.device)
+        code = muon_error()
+        if code:
+            raise D1Error(f'a wait inside Muon ran out (error {code}): the parameters may be updated in part')
 
     def momentum_of(self, i):
         """The momentum of parameter i in its shape (a view)."""
@@ -156,6 +185,7 @@ def orthogonalize(x, steps=5, out=None, precise=None):
     elif out.dtype not in (BF16, torch.float16) or out.shape != x.shape or out.device != dev or not out.is_contiguous():
         raise ValueError(f'out must be a contiguous bfloat16 or float16 tensor {tuple(x.shape)} on {dev}')
     lib = library()
+    _watch()
     if precise is None:
         precise = out.dtype is torch.float16
     call, room = ((lib.d1_orthogonalize_precise, lib.d1_orthogonalize_precise_work_bytes) if precise else
@@ -170,4 +200,5 @@ def orthogonalize(x, steps=5, out=None, precise=None):
 
 
 def muon_error():
+    """The last error of a wait that ran out, on the current device (0: none); clears it."""
     return library().d1_muon_error()

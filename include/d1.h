@@ -828,8 +828,14 @@ int d1_orthogonalize(const void *x, int64_t ldx, int64_t x_step, int type, int64
 int64_t d1_orthogonalize_precise_work_bytes(int64_t count, int64_t rows, int64_t cols);
 int d1_orthogonalize_precise(const void *x, int64_t ldx, int64_t x_step, int type, int64_t count, int64_t rows, int64_t cols, void *y, int y_type,
                              int steps, void *work, void *stream);
-/* Last error recorded by a wait of the products that ran out (0: none); clears it. */
+/* Last error recorded on the current device by a wait of the products that ran out (0: none); clears it. While it stands the
+ * steps of matrices that take the products leave param and copy as they are. */
 int d1_muon_error(void);
+/* A pinned host int that a wait that ran out sets too (NULL: none), so that a caller sees it without a
+ * synchronisation; calls from now on, and graphs captured from now on, write to it. d1_muon_error clears it. */
+int d1_muon_error_flag(int *flag);
+/* Records an error as such a wait does: for tests of what a caller does about it. */
+int d1_muon_set_error(int code);
 
 #ifdef __cplusplus
 }
