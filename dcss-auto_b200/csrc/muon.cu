@@ -439,7 +439,8 @@ __device__ __forceinline__ void finish(const Job &o, const Matrix &m, int i0, in
 // A tile is 128 x 128 elements, or 256 x 256 of a PAIR. SPLIT: a cluster of 2, 4 or 8 CTAs takes a tile of 128 x 128 together, each
 // a part of the sum. Each then owns some of the tile's sixteen units of 32 x 32: the others' parts of them come to its shared
 // memory, and it adds them in the order of the parts. It is for products of few tiles with long sums: X X^T of 512 x 3136
-// has ten, of 49 blocks each.
+// has ten, of 49 blocks each. Single products X' have too many tiles for it wherever their sums are long enough; those of pairs from 4 x 4 blocks on
+// (189 of 100,000 shapes up to 200 x 600) are left whole too.
 template <bool PAIR> struct Roles {
     static constexpr int SIDES = PAIR ? 4 : 2, COLS = SIDES * SIDE;  // blocks along a tile; columns of an accumulator
 
@@ -559,6 +560,7 @@ template <bool PAIR> struct Roles {
     // Warp w holds rows 32 (w % 4) .. + 31 of this CTA's 128, in one half of the columns.
     template <int PHASE, bool SPLIT, class List> __device__ __forceinline__ void store(List &list, int from) {
         constexpr bool SYMMETRIC = symmetric(PHASE);
+        static_assert(SYMMETRIC || !SPLIT);
         const int q = warp & 3, half = (warp - 2) >> 2;
         constexpr int UNITS = COLS / 2 / 32;
         // SPLIT: unit `own` of this warp, if any, is this CTA's; `parts` rooms stand behind one another for it, one
@@ -605,7 +607,7 @@ template <bool PAIR> struct Roles {
             };
             if (lane == 0) bulk_wait_read();
             __syncwarp();  // the rooms are free
-            ask(own);
+            ask(0);
             if (SPLIT) {
                 fetch(own);
             } else {
@@ -748,7 +750,7 @@ template <bool PAIR> struct Roles {
                                 *reinterpret_cast<uint4 *>(mine + ROOM / 2 + piece(e)) = lo;
                         }
                     }
-                    if (PHASE == APPLY && !SPLIT) ask(u + 1);
+                    if (PHASE == APPLY) ask(u + 1);
                     if constexpr (PHASE == APPLY) {
                         fence_proxy_async();
                         __syncwarp();
@@ -759,7 +761,7 @@ template <bool PAIR> struct Roles {
                         }
                     } else {
                         if (!failed || !m.param) finish(o, m, ib * SIDE + r0, jb0 * SIDE + 32 * u, x, params, reinterpret_cast<float *>(room));
-                        if (!SPLIT) ask(u + 1);
+                        ask(u + 1);
                     }
                 }
                 __syncwarp();
@@ -949,7 +951,7 @@ static Product product_of(int phase, int mode) {
     static const Product all[3][4] = {
         {product_kernel<GRAM, SINGLES>, product_kernel<QUAD, SINGLES>, product_kernel<APPLY, SINGLES>, product_kernel<STEP, SINGLES>},
         {product_kernel<GRAM, PAIRS>, product_kernel<QUAD, PAIRS>, product_kernel<APPLY, PAIRS>, product_kernel<STEP, PAIRS>},
-        {product_kernel<GRAM, SPLITS>, product_kernel<QUAD, SPLITS>, product_kernel<APPLY, SPLITS>, product_kernel<STEP, SPLITS>}};
+        {product_kernel<GRAM, SPLITS>, product_kernel<QUAD, SPLITS>, nullptr, nullptr}};  // X' is not divided
     return all[mode][phase];
 }
 typedef Product Small;
@@ -960,7 +962,8 @@ static int allow_space() {
     if (cudaError_t e = cudaGetDevice(&dev)) return (int)e;
     if (dev < 64 && ((ready >> dev) & 1)) return 0;
     for (int k = 0; k < 12; k++)
-        if (cudaError_t e = cudaFuncSetAttribute(product_of(k & 3, k >> 2), cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES)) return (int)e;
+        if (const Product p = product_of(k & 3, k >> 2))
+            if (cudaError_t e = cudaFuncSetAttribute(p, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES)) return (int)e;
     for (int k = 0; k < 2; k++)
         if (cudaError_t e = cudaFuncSetAttribute(small_of(k), cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES)) return (int)e;
     if (cudaError_t e = cudaFuncSetAttribute(narrow::steps_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, narrow::step_bytes(8))) return (int)e;

@@ -81,3 +81,30 @@ def test_plans(lib):
         n = len(shapes)
         assert lib.d1_muon_work_bytes(p, n) - lib.d1_muon_work_bytes(t, n) == 8192 * more
         assert lib.d1_muon_plan_bytes(p, n) > 0
+
+
+DIVIDED = r"""
+#include <cstdio>
+#include "d1_muon.h"
+using namespace d1::muon;
+int main() {
+    for (int rb = 1; rb <= 200; rb++)
+        for (int cb = rb; cb <= 600; cb++) {
+            Matrix m;
+            int64_t block = 0, part = 0;
+            place(m, rb * 64, cb * 64, block, part);
+            Load load = load_of(2);
+            load.add(m, 1);
+            if (parts_for(load.full, load.depth[1]) > 1) return 1;
+        }
+    std::puts("ok");
+}
+"""
+
+
+def test_single_products_apply_is_never_divided(tmp_path):
+    """There is no kernel for it: no shape has few enough tiles of X' and long enough sums."""
+    source = tmp_path / 'divided.cpp'
+    source.write_text(DIVIDED)
+    subprocess.run(['g++', '-std=c++17', '-O1', '-I', str(CSRC), str(source), '-o', str(tmp_path / 'divided')], check=True)
+    assert subprocess.run([str(tmp_path / 'divided')], capture_output=True, text=True).stdout == 'ok\n'
