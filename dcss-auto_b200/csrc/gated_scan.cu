@@ -66,12 +66,17 @@ template <class T> struct Args {
     int chunks;
 };
 
-// (a, 1 - a) of the average form from E = e^g, as E / (1 + E) and 1 / (1 + E): both are right to a few
-// roundings at every g, neither is a difference from 1. E is capped where 1 / E would vanish (a NaN passes).
+// (a, 1 - a) of the average form from E = e^g, as E / (1 + E) and 1 / (1 + E): neither is a difference from 1. E = 2^x with x = g log2(e)
+// rounded, times 1 + (g - x ln 2), which that rounding left out (up to 60 * 2^-24 for large g): right to a few roundings wherever it is a
+// normal number. Below, E and a are 0; where 1 / E would vanish E is 2^126, so that 1 - a is 2^-126 at least (a NaN passes).
 __device__ __forceinline__ float2 gates(float g) {
-    float x = g * 1.4426950408889634f, e, w;
-    asm("min.NaN.f32 %0, %1, 0f42FC0000;" : "=f"(x) : "f"(x));  // 126
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x));
+    constexpr float LN2 = 0.6931471805599453f, REST = (float)(0.69314718055994530942 - (double)LN2);
+    const float x = g * 1.4426950408889634f;
+    float e, w, most;
+    asm("min.NaN.f32 %0, %1, 0f42FC0000;" : "=f"(most) : "f"(x));  // 126
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(most));
+    const float left = fmaf(-x, REST, fmaf(-x, LN2, g));
+    if (fabsf(x) < 126.f) e = fmaf(e, left, e);
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(1.f + e));
     return make_float2(e * w, w);
 }
