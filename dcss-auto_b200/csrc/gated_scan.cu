@@ -29,6 +29,7 @@
 // One step of 64 x 256: 1.9 us.
 //
 // A reset replaces the state: a product with 0 would keep an infinity.
+#include <initializer_list>
 #include <type_traits>
 
 #include "d1_common.cuh"
@@ -450,19 +451,32 @@ template <class T, bool BACK> static int any(Args<T> a, int form, void *work, cu
     return wide ? run<T, V, false, BACK>(a, s) : run<T, 1, false, BACK>(a, s);
 }
 
-// Whether sizes and strides are in range: D, B, T >= 0 and all offsets within 62 bits.
+// Whether sizes are in range: D, B, T >= 0 and all offsets of contiguous tensors within 62 bits.
 static bool shape_ok(int64_t T, int64_t B, int64_t D) {
     return T >= 0 && B >= 0 && D >= 1 && T <= ((int64_t)1 << 40) && B <= ((int64_t)1 << 40) && D <= INT32_MAX &&
            (B == 0 || D <= ((int64_t)1 << 42) / B) && (T == 0 || B * D <= ((int64_t)1 << 58) / T);
 }
 
-// Whether the contiguous result at q meets the range of a [T, B, D] operand.
-static bool meets(const void *q, const void *p, int64_t st, int64_t sb, int64_t T, int64_t B, int64_t D, int size) {
-    if (!q || !p || T < 1 || B < 1) return false;
-    const uintptr_t a = (uintptr_t)q, b = (uintptr_t)p;
-    return a < b + (uintptr_t)(((T - 1) * st + (B - 1) * sb + D) * size) && b < a + (uintptr_t)(T * B * D * size);
+// Whether the strides of a [T, B, D] operand are: its last element lies within 60 bits of its first.
+static bool strides_ok(int64_t st, int64_t sb, int64_t T, int64_t B) {
+    constexpr int64_t MOST = (int64_t)1 << 59;
+    return st >= 0 && sb >= 0 && (T < 2 || st <= MOST / (T - 1)) && (B < 2 || sb <= MOST / (B - 1));
 }
-static bool stride_ok(int64_t s) { return s >= 0 && s <= ((int64_t)1 << 42); }
+// The bytes from the first to the last that an operand (or a result) has.
+struct Range {
+    uintptr_t from, to;
+};
+static Range range_of(const void *p, int64_t st, int64_t sb, int64_t T, int64_t B, int64_t D, int size) {
+    const uintptr_t at = (uintptr_t)p;
+    return {at, p && T > 0 && B > 0 ? at + (uintptr_t)(((T - 1) * st + (B - 1) * sb + D) * size) : at};
+}
+static Range range_of(const void *p, int64_t count, int size) { return range_of(p, 0, 0, 1, 1, count, size); }
+static bool meet(const Range &a, const Range &b) { return a.from < b.to && b.from < a.to && a.from < a.to && b.from < b.to; }
+static bool meet_any(const Range &a, std::initializer_list<Range> others) {
+    for (const Range &b : others)
+        if (meet(a, b)) return true;
+    return false;
+}
 
 }  // namespace gs
 }  // namespace d1
@@ -485,17 +499,19 @@ extern "C" int d1_gated_scan(const void *x, int64_t x_t, int64_t x_b, const void
                              int64_t reset_t, int64_t reset_b, void *y, float *last, void *work, void *stream) {
     using namespace d1;
     if (!type_ok(type) || (form != D1_SCAN_AVERAGE && form != D1_SCAN_SUM) || !gs::shape_ok(T, B, D) ||
-        (T && B && (!x || !gate || !y)) || !gs::stride_ok(x_t) || !gs::stride_ok(x_b) || !gs::stride_ok(gate_t) ||
-        !gs::stride_ok(gate_b) || !gs::stride_ok(reset_t) || !gs::stride_ok(reset_b) || !element_aligned(x, type) ||
-        !element_aligned(gate, type) || !element_aligned(y, type) || !aligned_to(4, h0, last))
+        (T && B && (!x || !gate || !y)) || !gs::strides_ok(x_t, x_b, T, B) || !gs::strides_ok(gate_t, gate_b, T, B) ||
+        !gs::strides_ok(reset_t, reset_b, T, B) || !element_aligned(x, type) || !element_aligned(gate, type) || !element_aligned(y, type) || !aligned_to(4, h0, last))
         return D1_ERR_BAD_ARGUMENT;
     const int size = type == D1_TYPE_F32 ? 4 : 2;
-    if (gs::meets(y, x, x_t, x_b, T, B, D, size) || gs::meets(y, gate, gate_t, gate_b, T, B, D, size))
+    const gs::Range xs = gs::range_of(x, x_t, x_b, T, B, D, size), gates = gs::range_of(gate, gate_t, gate_b, T, B, D, size),
+                    resets = gs::range_of(reset, reset_t, reset_b, T, B, 1, 1), ys = gs::range_of(y, T * B * D, size),
+                    h0s = gs::range_of(h0, B * D, 4), lasts = gs::range_of(last, B * D, 4);
+    if (gs::meet_any(ys, {xs, gates, resets, h0s, lasts}) || gs::meet_any(lasts, {xs, gates, resets}) || (last != h0 && gs::meet(lasts, h0s)))
         return D1_ERR_BAD_ARGUMENT;
     const cudaStream_t s = (cudaStream_t)stream;
     if (B == 0) return 0;
     if (T == 0) {  // the state is what it was
-        if (!last) return 0;
+        if (!last || last == h0) return 0;
         return (int)(h0 ? cudaMemcpyAsync(last, h0, (size_t)(B * D) * 4, cudaMemcpyDeviceToDevice, s)
                         : cudaMemsetAsync(last, 0, (size_t)(B * D) * 4, s));
     }
@@ -520,24 +536,26 @@ extern "C" int d1_gated_scan_backward(const void *dy, int64_t dy_t, int64_t dy_b
                                       void *dgate, float *dh0, void *work, void *stream) {
     using namespace d1;
     if (!type_ok(type) || (form != D1_SCAN_AVERAGE && form != D1_SCAN_SUM) || !gs::shape_ok(T, B, D) ||
-        (T && B && (!dy || !x || !gate || !y || !dx || !dgate)) || !gs::stride_ok(x_t) || !gs::stride_ok(x_b) ||
-        !gs::stride_ok(gate_t) || !gs::stride_ok(gate_b) || !gs::stride_ok(y_t) || !gs::stride_ok(y_b) ||
-        !gs::stride_ok(dy_t) || !gs::stride_ok(dy_b) || !gs::stride_ok(reset_t) || !gs::stride_ok(reset_b) ||
+        (T && B && (!dy || !x || !gate || !y || !dx || !dgate)) || !gs::strides_ok(x_t, x_b, T, B) ||
+        !gs::strides_ok(gate_t, gate_b, T, B) || !gs::strides_ok(y_t, y_b, T, B) || !gs::strides_ok(dy_t, dy_b, T, B) ||
+        !gs::strides_ok(reset_t, reset_b, T, B) ||
         !element_aligned(x, type) || !element_aligned(gate, type) || !element_aligned(y, type) ||
         !element_aligned(dy, type) || !element_aligned(dx, type) || !element_aligned(dgate, type) ||
         !aligned_to(4, h0, dlast, dh0))
         return D1_ERR_BAD_ARGUMENT;
     const int size = type == D1_TYPE_F32 ? 4 : 2;
-    void *const results[2] = {dx, dgate};
-    for (void *q : results)
-        if (gs::meets(q, x, x_t, x_b, T, B, D, size) || gs::meets(q, gate, gate_t, gate_b, T, B, D, size) ||
-            gs::meets(q, y, y_t, y_b, T, B, D, size) || gs::meets(q, dy, dy_t, dy_b, T, B, D, size))
-            return D1_ERR_BAD_ARGUMENT;
-    if (gs::meets(dx, dgate, B * D, D, T, B, D, size)) return D1_ERR_BAD_ARGUMENT;
+    const gs::Range xs = gs::range_of(x, x_t, x_b, T, B, D, size), gates = gs::range_of(gate, gate_t, gate_b, T, B, D, size),
+                    ys = gs::range_of(y, y_t, y_b, T, B, D, size), dys = gs::range_of(dy, dy_t, dy_b, T, B, D, size),
+                    resets = gs::range_of(reset, reset_t, reset_b, T, B, 1, 1), h0s = gs::range_of(h0, B * D, 4), dlasts = gs::range_of(dlast, B * D, 4),
+                    dxs = gs::range_of(dx, T * B * D, size), dgates = gs::range_of(dgate, T * B * D, size), dh0s = gs::range_of(dh0, B * D, 4);
+    for (const gs::Range &q : {dxs, dgates})
+        if (gs::meet_any(q, {xs, gates, ys, dys, resets, h0s, dlasts, dh0s})) return D1_ERR_BAD_ARGUMENT;
+    if (gs::meet(dxs, dgates) || gs::meet_any(dh0s, {xs, gates, ys, dys, resets, h0s}) || (dh0 != dlast && gs::meet(dh0s, dlasts)))
+        return D1_ERR_BAD_ARGUMENT;
     const cudaStream_t s = (cudaStream_t)stream;
     if (B == 0) return 0;
     if (T == 0) {
-        if (!dh0) return 0;
+        if (!dh0 || dh0 == dlast) return 0;
         return (int)(dlast ? cudaMemcpyAsync(dh0, dlast, (size_t)(B * D) * 4, cudaMemcpyDeviceToDevice, s)
                            : cudaMemsetAsync(dh0, 0, (size_t)(B * D) * 4, s));
     }

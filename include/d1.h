@@ -750,16 +750,16 @@ int64_t d1_gated_scan_work_bytes(int64_t T, int64_t B, int64_t D);
  * channels; step t and sequence b lie t * x_t + b * x_b elements on. Where
  * reset[t * reset_t + b * reset_b] (bytes; NULL: nowhere) is not 0, an episode begins
  * at t: the state before it counts for nothing. States are f32; y (contiguous
- * [T, B, D], type `type`) is rounded once and shares no memory with the range
- * of x or gate; last (f32 [B, D]; NULL: not wanted; it may be h0 itself) is the state
- * after step T - 1, h0 when T is 0. work: 8-byte aligned, of the size above. */
+ * [T, B, D], type `type`) is rounded once; last (f32 [B, D]; NULL: not wanted) is the state
+ * after step T - 1, h0 when T is 0. Neither shares memory with the range of an operand or
+ * the other, but last may be h0 itself. work: 8-byte aligned, of the size above. */
 int d1_gated_scan(const void *x, int64_t x_t, int64_t x_b, const void *gate, int64_t gate_t, int64_t gate_b, int type,
                   int form, int64_t T, int64_t B, int64_t D, const float *h0, const uint8_t *reset, int64_t reset_t,
                   int64_t reset_b, void *y, float *last, void *work, void *stream);
 /* The gradients of d1_gated_scan from dy (type `type`) and dlast (f32 [B, D];
  * NULL: zeros): dx and dgate (contiguous, type `type`), dh0 (f32 [B, D]; NULL: not
- * wanted; it may be dlast itself). y is what the forward pass gave. dx and dgate share no memory with
- * the range of an input. */
+ * wanted). y is what the forward pass gave. None of them shares memory with the range of an operand or
+ * with another one, but dh0 may be dlast itself. */
 int d1_gated_scan_backward(const void *dy, int64_t dy_t, int64_t dy_b, const void *x, int64_t x_t, int64_t x_b,
                            const void *gate, int64_t gate_t, int64_t gate_b, const void *y, int64_t y_t, int64_t y_b,
                            int type, int form, int64_t T, int64_t B, int64_t D, const float *h0, const float *dlast,
