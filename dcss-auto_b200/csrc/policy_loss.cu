@@ -39,7 +39,7 @@ constexpr int SMALL = 32768, SMALL_THREADS = 512, SMALL_ROWS = 2048, MOST_TOGETH
 constexpr int PIECE = 4096, LONG = 16384;  // tokens of a row too long for one warp that a warp counts; of such a row
 constexpr int TEAM = 4;  // warps that count a row of more than 1,024 tokens
 
-struct Rows {  // fp32 [rows, length]: element (r, i) at p[r * ld + i * step]
+struct Rows {  // fp32 [rows, length]: element (r, i) at p[r * ld + i]
     const float *p;
     int64_t ld;
 };
@@ -90,12 +90,14 @@ __device__ __forceinline__ float token(const Args &a, float logp, float old, flo
         over = wide > a.over, under = wide < a.under;
     }
     const bool cut = (over && adv > 0.f) || (under && adv < 0.f);
-    s.t[0] -= w * ((cut ? (over ? a.most : a.least) : r) * adv);
-    float g = cut ? 0.f : -adv * r;
+    // an advantage or a coefficient of 0 is 0 beside a finite difference whose power passes fp32
+    const float gain = adv == 0.f && delta < INFINITY ? 0.f : r * adv;
+    s.t[0] -= w * (cut ? (over ? a.most : a.least) * adv : gain);
+    float g = cut ? 0.f : -gain;
     if (a.ref.p) {
         const float d = ref - logp, grown = __expf(d), k = beyond_linear(d, grown);
         s.t[1] += w * k;
-        g = fmaf(-a.kl, fabsf(d) < 0.5f ? d + k : grown - 1.f, g);  // e^d - 1
+        if (a.kl != 0.f) g = fmaf(-a.kl, fabsf(d) < 0.5f ? d + k : grown - 1.f, g);  // e^d - 1
     }
     if (a.entropy.p) s.t[2] += w * h;
     if (cut) s.t[3] += w;
@@ -204,7 +206,7 @@ template <int N> __device__ __forceinline__ void join(double (&total)[TERMS], do
 }
 
 __device__ __forceinline__ void finish(const Args &a, const double (&t)[TERMS]) {
-    if (a.loss) *a.loss = (float)(t[0] + (double)a.kl * t[1] - (double)a.ent * t[2]);
+    if (a.loss) *a.loss = (float)(t[0] + (a.kl != 0.f ? (double)a.kl * t[1] : 0.) - (a.ent != 0.f ? (double)a.ent * t[2] : 0.));
     if (a.stats)
         for (int k = 0; k < TERMS; k++) a.stats[k] = (float)t[k];
 }

@@ -13,7 +13,8 @@ dimensions have one row pitch; advantage has that shape, or one number for each 
 [...]. mask (bool or uint8) marks the tokens that count: the others are never looked
 at, whatever they hold. mean='token' takes the mean over all tokens that count,
 'row' over the rows that have any of each row's mean. A batch without a token that
-counts has a loss of 0 and gradients of 0. The log-probabilities are float32
+counts has a loss of 0 and gradients of 0. ratio and e^d are float32, infinite past a
+difference of 88.7; beside one an advantage or a coefficient of 0 still takes no part. The log-probabilities are float32
 because their differences are close to 0, where 16 bits would leave no ratio.
 
 The gradient comes with the loss, in one pass: each token's needs nothing that the
