@@ -83,7 +83,7 @@ struct Sums {
 
 // One token of weight w: its share of the five terms (times w) and its gradient.
 __device__ __forceinline__ float token(const Args &a, float logp, float old, float adv, float ref, float h, float w, Sums &s) {
-    const float delta = logp - old, r = __expf(delta);
+    const float delta = logp - old, r = expf(delta);
     bool over = delta > a.over32, under = delta < a.under32;
     if (delta == a.over32 || delta == a.under32) {  // rounding is monotonic: only here may the exact difference lie on the other side
         const double wide = (double)logp - (double)old;
@@ -95,7 +95,7 @@ __device__ __forceinline__ float token(const Args &a, float logp, float old, flo
     s.t[0] -= w * (cut ? (over ? a.most : a.least) * adv : gain);
     float g = cut ? 0.f : -gain;
     if (a.ref.p) {
-        const float d = ref - logp, grown = __expf(d), k = beyond_linear(d, grown);
+        const float d = ref - logp, grown = expf(d), k = beyond_linear(d, grown);
         s.t[1] += w * k;
         if (a.kl != 0.f) g = fmaf(-a.kl, fabsf(d) < 0.5f ? d + k : grown - 1.f, g);  // e^d - 1
     }
