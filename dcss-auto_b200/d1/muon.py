@@ -138,7 +138,8 @@ class Muon:
         the matrices that go through the products as they were, but for those it had already updated. Synchronises the
         device and clears the error."""
         torch.cuda.synchronize(self.device)
-        code = muon_error()
+        with torch.cuda.device(self.device):
+            code = muon_error()
         if code:
             raise D1Error(f'a wait inside Muon ran out (error {code}): the parameters may be updated in part')
 
