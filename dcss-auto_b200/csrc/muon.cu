@@ -575,6 +575,7 @@ template <bool PAIR> struct Roles {
         Tile tile;
         for (; ok && list.take(m, tile); local++) {
             const Operands p = operands(m, PHASE, from);
+            if (failed && m.param) m.rows = 0;  // the epilogue finds no row to update
             const int b = local & 1, ib = tile.i * SIDES + 2 * rank + (q >> 1), r0 = 32 * (q & 1);
             const int hi_to = from ? m.hi[0] : m.hi[1], lo_to_block = from ? m.lo : m.lo2;
             const int jb0 = tile.j * SIDES + half * (SIDES / 2);
@@ -760,7 +761,7 @@ template <bool PAIR> struct Roles {
                             bulk_commit();
                         }
                     } else {
-                        if (!failed || !m.param) finish(o, m, ib * SIDE + r0, jb0 * SIDE + 32 * u, x, params, reinterpret_cast<float *>(room));
+                        finish(o, m, ib * SIDE + r0, jb0 * SIDE + 32 * u, x, params, reinterpret_cast<float *>(room));
                         ask(u + 1);
                     }
                 }
