@@ -23,8 +23,8 @@
 // to its (P, Q), a second runs over the chunks, a third walks all of them side
 // by side from their true states. The order of all sums is fixed.
 //
-// Measured (one B200; floor: each operand once at 6.56 TB/s). 128 steps of 4,096 x 512 channels bf16: 247 us, the floor's
-// rate; 64 steps backward 268 (93 %). 131,072 steps of 256 channels 69 us (floor 31): 31 for the reduction, 33 for the walk, the
+// Measured (one B200; floor: each operand once at 6.56 TB/s). 128 steps of 4,096 x 512 channels bf16: 252 us (98 % of the floor's
+// rate); 64 steps backward 272 (92 %). 131,072 steps of 256 channels 75 us (floor 31): 34 for the reduction, 35 for the walk, the
 // rest the launch between them; 82 in the sum form (70 without the powers). 50,021 x 3 x 111 fp32 backward, sum form, 110 us (51; 105 without).
 // One step of 64 x 256: 1.9 us.
 //

@@ -16,8 +16,8 @@
 // has nothing F is a, and the pair is carried on as one; elsewhere F lo is not a lo, an error of hi's size, but
 // in directions that X has (0.16 % there, 0.2 % of a full-rank one). That is a bf16 result's own rounding (0.17 %), but eight times an
 // fp16 one's: where the caller asks for it (`precise`), A and F are pairs too and a product takes all three terms, as good as one in
-// fp32 for up to three times the products' time (8,192 x 8,192 28.6 ms in place of 9.6, 7 x 1,777 x 1,003 908 us in place of 475, 512 x 512 247
-// in place of 167, all in one run). So it is in a matrix with a side of at most 64, where few
+// fp32 for up to three times the products' time (8,192 x 8,192 28.6 ms in place of 10.0, 7 x 1,777 x 1,003 770 us in place of 371, 512 x 512 182
+// in place of 123, the conv policy's six 224 in place of 145). So it is in a matrix with a side of at most 64, where few
 // roundings average out (up to 1 % in some), and where its time is the launches' all the same. Where all matrices are as narrow as that up to five
 // steps are taken another way (muon_narrow.cuh).
 //
@@ -26,7 +26,7 @@
 // formulas, the last one the step itself. All operands are blocks of 64 x 64 elements (d1_muon.h) that the TMA
 // swizzles on its way to shared memory, as K-major operands or as MN-major ones: X is never transposed.
 //
-// Measured (one B200). 8,192 x 8,192 bf16: 9.97 ms, 1.3 PFLOP/s while the products run (a library product sustains 1.38
+// Measured (one B200). 8,192 x 8,192 bf16: 10.0 ms, 1.3 PFLOP/s while the products run (a library product sustains 1.38
 // under the power limit). 72 matrices of 12 layers of 1,024, with masters, momentum and copies: 3.89 ms (floor 1.64). The conv policy's six:
 // 145 us, 17 launches. A pair of CTAs takes 0.43 us for a block of 64 of the sum of its 256 x 256 tile: 32 KB into shared memory and 48 KB read
 // for 512 cycles of the tensor pipe, 640 cycles at 128 bytes each, which bound it.

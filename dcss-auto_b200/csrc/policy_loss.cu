@@ -22,7 +22,7 @@
 // blocks that are done, by which the last one knows that it is to add the blocks' sums.
 //
 // Measured (one B200): 16,384 tokens 4.2 us (one block in place of eight: 10.5), 512 x 4,099 tokens by rows with a mask and the KL
-// term 18 us (floor 5.4 at 6.56 TB/s), 128 x 65,536 with every term 46.6 us (37.1; 80 instructions a token fill half of the issue slots
+// term 20 us (floor 5.4 at 6.56 TB/s), 128 x 65,536 with every term 46.6 us (37.1; 80 instructions a token fill half of the issue slots
 // meanwhile).
 #include <math.h>
 
