@@ -460,7 +460,7 @@ static bool shape_ok(int64_t T, int64_t B, int64_t D) {
 // Whether the strides of a [T, B, D] operand are: its last element lies within 60 bits of its first.
 static bool strides_ok(int64_t st, int64_t sb, int64_t T, int64_t B) {
     constexpr int64_t MOST = (int64_t)1 << 59;
-    return st >= 0 && sb >= 0 && (T < 2 || st <= MOST / (T - 1)) && (B < 2 || sb <= MOST / (B - 1));
+    return st >= 0 && sb >= 0 && st <= MOST / (T < 2 ? 1 : T - 1) && sb <= MOST / (B < 2 ? 1 : B - 1);
 }
 // The bytes from the first to the last that an operand (or a result) has.
 struct Range {

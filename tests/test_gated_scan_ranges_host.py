@@ -41,3 +41,11 @@ def test_strides(lib):  # noqa: F811
         assert lib.d1_gated_scan_backward(*backward(**dict(BACK, T=T, B=1, D=1, dx=1 << 50, dgate=1 << 52, work=11 * P, **{k: 1 << 42}))) == BAD, k
     for k in ('xb', 'gb', 'rb'):
         assert lib.d1_gated_scan(*forward(**dict(FAR, T=1, B=T, D=1, y=1 << 50, **{k: 1 << 42}))) == BAD, k
+
+
+def test_strides_of_one_step(lib):  # noqa: F811
+    """Where there is one step or sequence its stride is not used, but one past 59 bits is refused all the same."""
+    for k in ('xt', 'gt', 'rt'):
+        assert lib.d1_gated_scan(*forward(**dict(FAR, T=1, **{k: 1 << 62}))) == BAD, k
+    for k in ('xb', 'gb', 'rb'):
+        assert lib.d1_gated_scan(*forward(**dict(FAR, B=1, **{k: 1 << 62}))) == BAD, k
