@@ -53,7 +53,7 @@ def _watch():
     if _told is None:
         if torch.cuda.is_current_stream_capturing():   # (no time to allocate)
             return
-        flag = torch.zeros(1, dtype=torch.int32).pin_memory()
+        flag = torch.zeros(1, dtype=torch.int32, device='cpu', pin_memory=True)
         check(library().d1_muon_error_flag(flag.data_ptr()), 'd1_muon_error_flag')
         _told = C.c_int.from_address(flag.data_ptr()), flag
     if _told[0].value:

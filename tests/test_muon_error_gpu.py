@@ -96,3 +96,16 @@ def test_first_call_in_a_capture():
     root = pathlib.Path(__file__).resolve().parents[1] / 'dcss-auto_b200'
     r = subprocess.run([sys.executable, '-c', code], capture_output=True, text=True, env={**__import__('os').environ, 'PYTHONPATH': str(root)}, timeout=300)
     assert r.stdout == 'ok\n', r.stderr
+
+
+def test_with_another_default_device():
+    """The word in host memory is one whatever torch's default device is, in a process whose first call that is."""
+    import os
+    import pathlib
+    import subprocess
+    import sys
+    code = ('import torch\nfrom d1.muon import orthogonalize\ntorch.set_default_device("cuda")\nx = torch.randn(100, 80)\ny = orthogonalize(x)\n'
+            'assert torch.equal(y, orthogonalize(x))\nprint("ok")')
+    root = pathlib.Path(__file__).resolve().parents[1] / 'dcss-auto_b200'
+    r = subprocess.run([sys.executable, '-c', code], capture_output=True, text=True, env={**os.environ, 'PYTHONPATH': str(root)}, timeout=300)
+    assert r.stdout == 'ok\n', r.stderr
